@@ -71,6 +71,20 @@ SIGNATURES = {
     "akv_paged_attn_status": (_i, [_p, C.POINTER(C.c_int), _p]),
     "akv_debug_set_handoff_spin_limit": (_i, [_i]),
     "akv_debug_read_probe": (_i, [_p, _sz, _p, _p]),
+    "akv_dense_chunk_attn_workspace_bytes": (_sz, [_i]),
+    "akv_dense_chunk_attn": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                  _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i,
+                                  _i, _i64, _i, _i, _i, _i, _i64, _i64, _i, _i, _f, _p, _sz, _p]),
+    "akv_paged_chunk_attn_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "akv_paged_chunk_attn": (_i, [_p, _i, _i64, _i64,
+                                  _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                  _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                  _p, _i, _i64, _p, _i, _p, _i, _p, _p, _i, _p, _i64, _i64, _i,
+                                  _i, _i64, _i, _i, _i, _i, _i64, _i64, _i, _f, _p, _sz, _p]),
+    "akv_rope_append": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i,
+                             _p, _i, _i64, _p, _i64, _i, C.POINTER(C.c_int), _i, _i, _p, _i,
+                             _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i,
+                             _i64, _i, _i, _i, _i, _i64, _p]),
     "akv_hybrid_encode": (_i, [_p, _i, _i64, _i64, _p, _p, _i64, _p]),
     "akv_hybrid_encode_paged": (_i, [_p, _i, _i64, _i, _i64, _i64, _p, _i, _p,
                                      _p, _i64, _i64, _i64, _i, _i64, _p]),
@@ -265,6 +279,22 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_ALREADY = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current one (kernels are launched on the current device's streams)."""
+    return _HERE_ALREADY if device.index is None or torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def attn_status(workspace: Optional[torch.Tensor]) -> int:

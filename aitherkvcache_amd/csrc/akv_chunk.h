@@ -1,0 +1,177 @@
+// Attention of a chunk of new tokens over a paged cache: arguments, and how the work of a call is cut.
+//
+// Sequence i brings n_i query tokens, the newest of its ctx_i tokens: token j of them stands at position ctx_i - n_i + j and sees
+// the keys at its own position and before.  The query heads of a kv head meet the same keys, so the rows of a tile are (token,
+// query head) pairs of one kv head, token-major, as many whole tokens as fit; their keys reach from `lo` (0, or what the window of
+// the tile's first token leaves) to the position of the tile's last token.
+//
+// The tiles of a sequence, of all sequences, once for every kv head, lie end to end on one axis, each as long as it has units (runs of
+// keys); workgroup g of G takes the units [g F / G, (g + 1) F / G) of that axis.  So every workgroup has the same number of units,
+// however the lengths are spread and whatever the causal edge leaves of a tile, and few rows over many keys are split by themselves.  A
+// tile that lies in one range is finished there; the pieces of one that does not go to memory and are joined by ck_merge_kernel
+// in the order of the axis.  All of it is derived on the device: no call waits for a length.
+#pragma once
+#include "akv_attn_common.h"
+
+#define CK_SEQS 256               // sequences whose starts and lengths are held in LDS (more are read from memory)
+#define CK_NARROW_ROWS 64         // a sequence of at most so many rows a kv head goes to the narrow kernel
+
+struct ck_record {                // what a workgroup leaves of the tile that begins in its range and ends in another
+  int64_t end;                    // one past the tile's last unit
+  int64_t total;                  // F
+  int32_t valid, head, token, tokens;
+};
+
+struct ck_args {
+  const void* q; int64_t qs_tok, qs_head;        // queries (packed: rotated, float16), strides in elements
+  const float* qfac;                             // packed: factor of a row [T][QH]
+  const uint8_t* k; int64_t k_blk, k_pos, k_head;          // bytes
+  const uint8_t* v; int64_t v_blk, v_pos, v_head;
+  const float* kn; int64_t kn_blk, kn_pos, kn_head;        // packed: norms, elements
+  const float* vn; int64_t vn_blk, vn_pos, vn_head;
+  const float* centroids;
+  const void* tables; int64_t bt_stride;
+  const void* lens;
+  const void* starts;
+  int tables_it, lens_it, starts_it;
+  void* out; int64_t os_tok, os_head;            // packed: float32, in the order of the packed groups
+  float* part; float2* part_ml; ck_record* rec;
+  int S, T, QH, KVH, G, HS, GC;                  // G query heads a kv head, in HS groups of GC
+  int block_size; uint32_t bs_recip;
+  int64_t max_blocks, num_blocks;
+  int window;                                    // 0: none
+  int kind;                                      // sequences of this launch: 0 all, 1 those of few rows, 2 the others
+  int tail;                                      // rows behind the last sequence are zeroed
+  float scale2;                                  // score scale x log2 e
+};
+
+struct ck_seq { int q0, n, ctx; };               // first query row, query tokens, tokens
+
+template <int THREADS> struct ck_lengths {       // starts and lengths of the batch
+  int start[CK_SEQS + 1];
+  int ctx[CK_SEQS];
+  int sum[THREADS / 64];
+  int total;
+  int found[2];
+};
+
+__device__ __forceinline__ int ck_clamp(int64_t v, int64_t hi) { return (int)(v < 0 ? 0 : v > hi ? hi : v); }
+__device__ __forceinline__ int ck_start_of(const ck_args& a, int i) { return ck_clamp(akv_load_index(a.starts, a.starts_it, i), a.T); }
+__device__ __forceinline__ int ck_ctx_of(const ck_args& a, int i) {
+  const int64_t cap = a.max_blocks * a.block_size;
+  return ck_clamp(akv_load_index(a.lens, a.lens_it, i), cap < 0x7fff0000 ? cap : 0x7fff0000);
+}
+
+template <int THREADS> __device__ __forceinline__ void ck_load_lengths(const ck_args& a, ck_lengths<THREADS>& L) {
+  if (a.S <= CK_SEQS) {
+    for (int i = threadIdx.x; i <= a.S; i += THREADS) L.start[i] = ck_start_of(a, i);
+    for (int i = threadIdx.x; i < a.S; i += THREADS) L.ctx[i] = ck_ctx_of(a, i);
+  }
+  __syncthreads();
+}
+
+// Sequence i; i == S: the rows behind the last one, which see nothing.
+template <int THREADS> __device__ __forceinline__ ck_seq ck_sequence(const ck_args& a, const ck_lengths<THREADS>& L, int i) {
+  const bool held = a.S <= CK_SEQS;
+  ck_seq s;
+  s.q0 = held ? L.start[i] : ck_start_of(a, i);
+  if (i == a.S) {
+    s.n = a.tail && a.kind != 2 ? a.T - s.q0 : 0;
+    s.ctx = 0;
+    return s;
+  }
+  const int q1 = held ? L.start[i + 1] : ck_start_of(a, i + 1);
+  s.n = q1 > s.q0 ? q1 - s.q0 : 0;
+  s.ctx = held ? L.ctx[i] : ck_ctx_of(a, i);
+  if (a.kind != 0 && ((int64_t)s.n * a.G <= CK_NARROW_ROWS) != (a.kind == 1)) s.n = 0;
+  return s;
+}
+
+// keys [lo, hi) of tile j, TM tokens a tile; a tile has at least one unit of N keys
+struct ck_range { int first, units, hi; };
+template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, const ck_seq& s, int j, int TM) {
+  const int t0 = j * TM, t1 = t0 + TM < s.n ? t0 + TM : s.n;
+  ck_range r;
+  r.hi = s.ctx - s.n + t1;
+  if (r.hi < 0) r.hi = 0;
+  int lo = 0;
+  if (a.window > 0) {
+    lo = s.ctx - s.n + t0 - a.window + 1;
+    if (lo < 0) lo = 0;
+  }
+  r.first = lo / N;
+  r.units = (r.hi + N - 1) / N - r.first;
+  if (r.units < 1) r.units = 1;
+  return r;
+}
+
+// Tiles are numbered with gaps: tile j of sequence i is floor(start_i / TM) + i + j, which no two tiles share.
+__device__ __forceinline__ int ck_tile_numbers(const ck_args& a, int TM) { return a.T / TM + a.S + 1; }
+template <int THREADS, int N>
+__device__ __forceinline__ int ck_units_of(const ck_args& a, const ck_lengths<THREADS>& L, int x, int TM, int& seq, int& tile) {
+  int lo = 0, hi = a.S + 1;                 // the last i with floor(start_i / TM) + i <= x
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int s = a.S <= CK_SEQS ? L.start[mid] : ck_start_of(a, mid);
+    if (s / TM + mid <= x) lo = mid; else hi = mid;
+  }
+  const ck_seq s = ck_sequence(a, L, lo);
+  seq = lo;
+  tile = x - (s.q0 / TM + lo);
+  if (tile < 0 || (int64_t)tile * TM >= s.n) return 0;
+  return ck_keys<N>(a, s, tile, TM).units;
+}
+
+__device__ __forceinline__ int ck_wave_scan(int v) { return akv_wave_inclusive_scan(v); }
+
+// units of one kv head, in every thread
+template <int THREADS, int N> __device__ __forceinline__ int ck_total(const ck_args& a, ck_lengths<THREADS>& L, int TM) {
+  int sum = 0, seq, tile;
+  const int numbers = ck_tile_numbers(a, TM);
+  for (int x = threadIdx.x; x < numbers; x += THREADS) sum += ck_units_of<THREADS, N>(a, L, x, TM, seq, tile);
+  sum = akv_wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) L.sum[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) all += L.sum[w];
+  __syncthreads();
+  return all;
+}
+
+// the tile that holds unit `at` (< total): its sequence, number and first unit
+template <int THREADS, int N>
+__device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L, int TM, int at, int& seq, int& tile, int& first) {
+  const int numbers = ck_tile_numbers(a, TM);
+  int base = 0;
+  for (int x0 = 0;; x0 += THREADS) {
+    const int x = x0 + (int)threadIdx.x;
+    int sq = 0, tl = 0;
+    const int u = x < numbers ? ck_units_of<THREADS, N>(a, L, x, TM, sq, tl) : 0;
+    const int inc = ck_wave_scan(u);
+    if ((threadIdx.x & 63) == 63) L.sum[threadIdx.x >> 6] = inc;
+    __syncthreads();
+    int before = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      const int s = L.sum[w];
+      if (w < (int)(threadIdx.x >> 6)) before += s;
+      all += s;
+    }
+    const int b = before + inc - u;
+    if (u > 0 && at >= b && at < b + u) {
+      L.found[0] = sq;
+      L.found[1] = tl;
+      L.total = b;
+    }
+    __syncthreads();
+    base += all;
+    if (at < base || x0 + THREADS >= numbers) break;      // (the second never before the first: at < total)
+  }
+  seq = __builtin_amdgcn_readfirstlane(L.found[0]);
+  tile = __builtin_amdgcn_readfirstlane(L.found[1]);
+  first = __builtin_amdgcn_readfirstlane(L.total);
+}
+
+// first unit of workgroup g's range
+__device__ __forceinline__ int64_t ck_begin(int64_t total, int g, int G) { return total * g / G; }

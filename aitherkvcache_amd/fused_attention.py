@@ -152,6 +152,63 @@ class TQPagedAttention:
             ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
         return out if out.dtype == query.dtype else out.to(query.dtype)
 
+    def forward_chunk(self, query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc,
+                      block_size: int = 16, num_kv_heads: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                      max_query_len: Optional[int] = None) -> torch.Tensor:
+        """Causal attention of a chunk of new tokens a sequence (a draft to verify, a prompt that goes on) over the packed cache,
+        which holds the chunk's own tokens already; a chunk of one token is forward().
+
+        query           [num_tokens, num_query_heads, head_dim] float16 / bfloat16, the chunks of all sequences one after the other
+        query_start_loc [num_seqs + 1]: sequence i owns query rows query_start_loc[i] .. query_start_loc[i + 1] - 1, the newest of
+                        its context_lens[i] tokens; token j of n stands at position context_len - n + j and sees the
+                        keys up to there (none: zeros)
+        out             where the result goes (shape and type of query; rows behind the last sequence are left as they were);
+                        without it a new tensor, zero in such rows
+        max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result does not
+
+        Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector."""
+        from .chunk_attention import _check_out, check_chunk, check_query
+        if self._block_selector is not None:
+            raise ValueError("forward_chunk does not run the block selector")
+        tq = self._tq
+        if tq.rotation is not self.rotation:
+            self.rotation = tq.rotation
+        check_query(query)
+        if k_packed.dim() != 4 or v_packed.dim() != 4 or k_norms.dim() != 3 or v_norms.dim() != 3:
+            raise ValueError("expected caches [blocks, block_size, heads, bytes] and norms [blocks, block_size, heads]")
+        dev = _lib.require_gpu(query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc, out)
+        num_tokens, num_q_heads, d = query.shape
+        if d != self.head_dim or num_q_heads != self.num_query_heads:
+            raise ValueError(f"query shape {tuple(query.shape)} does not match heads={self.num_query_heads}, head_dim={self.head_dim}")
+        if num_kv_heads is None:
+            num_kv_heads = k_packed.shape[2]
+        for name, t in (("k_packed", k_packed), ("v_packed", v_packed)):
+            if t.dtype != torch.uint8 or t.stride(-1) != 1 or t.shape[-1] < self.packed_dim:
+                raise ValueError(f"{name} must be uint8 with contiguous rows of >= {self.packed_dim} bytes")
+        _lib.check_caches(block_size, num_kv_heads, k_packed, k_norms, v_packed, v_norms)
+        num_seqs, q, bt, lens, starts = check_chunk(query, num_kv_heads, block_tables, context_lens, query_start_loc)
+        k_norms = k_norms if k_norms.dtype == torch.float32 else k_norms.float()
+        v_norms = v_norms if v_norms.dtype == torch.float32 else v_norms.float()
+        if out is not None:
+            _check_out("out", out, query)
+        result = out if out is not None else torch.empty((num_tokens, num_q_heads, d), dtype=query.dtype, device=dev)
+        L = _lib.lib()
+        ws = torch.empty(L.akv_paged_chunk_attn_workspace_bytes(num_tokens, num_q_heads, d), dtype=torch.uint8, device=dev)
+        blocks = min(k_packed.shape[0], k_norms.shape[0], v_packed.shape[0], v_norms.shape[0])
+        with _lib.on_device(dev):
+            _lib.check(L.akv_paged_chunk_attn(
+                q.data_ptr(), _lib.dtype_code(q), q.stride(0), q.stride(1),
+                k_packed.data_ptr(), k_packed.stride(0), k_packed.stride(1), k_packed.stride(2),
+                k_norms.data_ptr(), k_norms.stride(0), k_norms.stride(1), k_norms.stride(2),
+                v_packed.data_ptr(), v_packed.stride(0), v_packed.stride(1), v_packed.stride(2),
+                v_norms.data_ptr(), v_norms.stride(0), v_norms.stride(1), v_norms.stride(2),
+                bt.data_ptr(), _lib.itype_code(bt), bt.stride(0), lens.data_ptr(), _lib.itype_code(lens),
+                starts.data_ptr(), _lib.itype_code(starts), tq.prepared_rotation().ptr, self.centroids.data_ptr(), self.bits,
+                result.data_ptr(), result.stride(0), result.stride(1), int(out is None),
+                num_seqs, num_tokens, num_q_heads, num_kv_heads, d, block_size, blocks, bt.shape[1],
+                max_query_len or 0, self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
+        return result
+
     def last_call_status(self) -> int:
         """0 when the most recent forward() / forward_no_alloc() ran clean; bit 0 set when it failed on the device (its
         outputs are NaN).  Synchronises the stream."""

@@ -250,6 +250,78 @@ int akv_debug_set_handoff_spin_limit(int polls);
 int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * A chunk of new tokens over a paged cache (no counterpart in the reference, whose prefill path calls its
+ * engine's dense kernel, aither_kvcache/vllm/backend.py:1200-1236).
+ *
+ * Sequence i of a call owns the query rows [query_starts[i], query_starts[i + 1]), the newest n_i of its
+ * context_lens[i] tokens (which the cache holds already): its token j stands at position context_lens[i] - n_i + j and
+ * attends to the keys at its own position and before.  A row without a key (its position is negative) is zero.
+ *   query        [num_tokens][num_q_heads][d] float16 or bfloat16, strides qs_tok / qs_head (last dim contiguous)
+ *   query_starts [num_seqs + 1], non-decreasing, in [0, num_tokens] (clamped there)
+ *   out          like query, its type; rows at or behind query_starts[num_seqs] are zeroed where zero_tail is not 0
+ *                and left as they were otherwise
+ *   block_tables, context_lens, num_blocks as in akv_paged_attn: entries at or beyond ceil(ctx / block_size) are never
+ *                read, entries inside are clamped into the cache
+ *   max_query_len the longest chunk, as far as the caller knows it (0: not): which kernels are launched goes by it,
+ *                results do not
+ * d is 64, 128 or 256; any number of query heads a kv head, any block size.  The values of a chunk's own tokens are expected to
+ * be finite (a weight of zero is multiplied with them); rows of the cache past a context may hold anything.
+ *
+ * akv_dense_chunk_attn: over a cache [num_blocks][block_size][num_kv_heads][d] of the query's type (element
+ * strides, rows at multiples of 16 bytes); window > 0: a token sees the newest `window` keys only (its own included).
+ * akv_paged_chunk_attn: over the packed cache of akv_paged_attn (rows at multiples of 4 bytes), scores and values of all
+ * tokens, the chunk's own included, as decoded from it.
+ * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must
+ * not overlap in time.
+ * ------------------------------------------------------------------------------- */
+size_t akv_dense_chunk_attn_workspace_bytes(int d);
+int akv_dense_chunk_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
+                         const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
+                         const void* value_cache, int64_t vs_blk, int64_t vs_pos, int64_t vs_head,
+                         const void* block_tables, int bt_itype, int64_t bt_stride,
+                         const void* context_lens, int cl_itype, const void* query_starts, int qs_itype,
+                         void* out, int64_t os_tok, int64_t os_head, int zero_tail,
+                         int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d,
+                         int block_size, int64_t num_blocks, int64_t max_blocks_per_seq, int window,
+                         int max_query_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t akv_paged_chunk_attn_workspace_bytes(int64_t num_tokens, int num_q_heads, int d);
+int akv_paged_chunk_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
+                         const uint8_t* k_packed, int64_t kps_blk, int64_t kps_pos, int64_t kps_head,
+                         const float* k_norms, int64_t kns_blk, int64_t kns_pos, int64_t kns_head,
+                         const uint8_t* v_packed, int64_t vps_blk, int64_t vps_pos, int64_t vps_head,
+                         const float* v_norms, int64_t vns_blk, int64_t vns_pos, int64_t vns_head,
+                         const void* block_tables, int bt_itype, int64_t bt_stride,
+                         const void* context_lens, int cl_itype, const void* query_starts, int qs_itype,
+                         const void* rot_prep, const float* centroids, int bits,
+                         void* out, int64_t os_tok, int64_t os_head, int zero_tail,
+                         int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d,
+                         int block_size, int64_t num_blocks, int64_t max_blocks_per_seq,
+                         int max_query_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Rotary positions and the append to an uncompressed paged cache in one launch (no counterpart in the
+ * reference, which scatters unrotated rows with torch indexing, aither_kvcache/vllm/backend.py:1247-1272).
+ * Queries go to query_out (which may be query itself), keys to key_cache, both with the pairs of their first rotary_dim
+ * coordinates turned; values go to value_cache.  Arithmetic in float32, one rounding to the type of the destination.
+ *   query, key, value [num_tokens][heads][d] of x_dtype (num_q_heads may be 0: no queries; num_kv_heads may be 0: no cache)
+ *   pair p < rotary_dim / 2: coordinates p and p + rotary_dim / 2, or 2 p and 2 p + 1 where interleaved is not 0
+ *   cos_sin      [cos_sin_rows][rotary_dim] float32: cosines of the pairs, then sines
+ *   positions    [num_axes][num_tokens] (pos_axis_stride elements from axis to axis), clamped into the table; axis i turns
+ *                the next sections[i] pairs (host array of num_axes, unused for one axis)
+ *   slot_mapping [num_tokens]: block x block_size + place; negative slots and blocks >= num_blocks are skipped.  The slots of a call
+ *                must differ: of tokens that share one, either may end up in it, coordinate by coordinate
+ * d and rotary_dim (0: nothing turns, positions and table unused) are multiples of 16.
+ * ------------------------------------------------------------------------------- */
+int akv_rope_append(const void* query, int64_t qs_tok, int64_t qs_head, void* query_out, int64_t qo_tok, int64_t qo_head,
+                    const void* key, int64_t ks_tok, int64_t ks_head, const void* value, int64_t vs_tok, int64_t vs_head,
+                    int x_dtype, const void* positions, int pos_itype, int64_t pos_axis_stride,
+                    const float* cos_sin, int64_t cos_sin_rows, int rotary_dim, const int* sections, int num_axes,
+                    int interleaved, const void* slot_mapping, int slot_itype,
+                    void* key_cache, int64_t kc_blk, int64_t kc_pos, int64_t kc_head,
+                    void* value_cache, int64_t vc_blk, int64_t vc_pos, int64_t vc_head, int cache_dtype,
+                    int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size, int64_t num_blocks, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * HybridTurboQuant, mode tq35 with calibrate_uniform() groups (dims 0..63 at 3-bit MSE,
  * dims 64..127 at 2-bit MSE, each with a 1-bit QJL residual sketch and fp16 norms inside
  * the 64-byte row) -- aither_kvcache/hybrid_quantizer.py:616-779 (encode), :785-933 (decode).
