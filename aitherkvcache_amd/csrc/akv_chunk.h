@@ -34,7 +34,7 @@ struct ck_args {
   const void* lens;
   const void* starts;
   int tables_it, lens_it, starts_it;
-  void* out; int64_t os_tok, os_head;            // packed: float32, in the order of the packed groups
+  void* out; int64_t os_tok, os_head;            // packed: float32
   float* part; float2* part_ml; ck_record* rec;
   int S, T, QH, KVH, G, HS, GC;                  // G query heads a kv head, in HS groups of GC
   int block_size; uint32_t bs_recip;

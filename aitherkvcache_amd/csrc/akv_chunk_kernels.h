@@ -18,6 +18,7 @@
 #pragma once
 #include "akv_chunk.h"
 #include "akv_device_once.h"
+#include <type_traits>
 
 typedef _Float16 ck_half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 ck_bf8 __attribute__((ext_vector_type(8)));
@@ -32,7 +33,7 @@ typedef __attribute__((address_space(3))) ck_u4 ck_lds_u4;
 #define CK_BF16 1                 // 2, 3, 4: packed codes of so many bits
 
 // Smallest value norm that counts (its inverse, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
-// frame of the exponents, as if its logarithm were 0, and its key is taken out of the product (ck_drop).  Norms of one sequence may
+// frame of the exponents, as if its logarithm were 0, and its value is zero.  Norms of one sequence may
 // lie 2^120 apart: weights are float32 until the sum of the softmax has taken them.
 #define CK_TINY 0x1p-90f
 
@@ -63,7 +64,7 @@ template <int KIND> struct ck_math {
 template <int BITS> struct ck_table {
   static constexpr int N = BITS == 4 ? 4 : BITS == 3 ? 2 : 1;
   uint32_t lo[N], hi[N];
-  float up;                 // the levels are in units of 1 / up ... value = level x unit
+  float up;                 // value = level x up, a power of two
   __device__ __forceinline__ void load(const float* __restrict__ centroids) {
     float c[1 << BITS], m = 0.f;
 #pragma unroll
@@ -134,74 +135,128 @@ template <int BITS, int W> __device__ __forceinline__ ck_u4 ck_levels(const ck_t
   r[0] = r0; r[1] = r1; r[2] = r2; r[3] = r3;
   return r;
 }
-// place of coordinate c (of eight) in such a group, and the coordinate at a place
-template <int BITS> __host__ __device__ constexpr int ck_place(int c) { return BITS == 4 ? (c >> 1) + 4 * (c & 1) : (c & 4) + 3 - (c & 3); }
+// coordinate at place p of such a group
 template <int BITS> __host__ __device__ constexpr int ck_coord(int p) { return BITS == 4 ? 2 * (p & 3) + (p >> 2) : (p & 4) + 3 - (p & 3); }
 
-// ---- one step of the softmax ----------------------------------------------------------------------------------------
-// A row's running state; l is the sum over the lane's own keys (the halves are added at the end).
-struct ck_row { float m, l; };
-// Scores s of NT tiles of 32 keys to weights, in place; returns what the sums so far have to be multiplied with.  Dense: s is a raw product
-// and m a maximum of such, c = scale x log2 e.  Packed: s are exponents already (norms in them), c = 1, `inv` the inverse value norms.
-template <int NT, bool PACKED>
-__device__ __forceinline__ float ck_softmax(ck_f16v (&s)[NT], ck_row& r, float c, const float* __restrict__ inv) {
-  float mx = s[0][0];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-  mx = fmaxf(mx, akv_lane_xor<32>(mx));
-  const float mn = fmaxf(r.m, mx);
-  const float ref = mn == -INFINITY ? 0.f : mn * c;
-  const float alpha = ck_exp2(fmaf(r.m, c, -ref));
-  r.m = mn;
-  float l = 0.f;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float w = ck_exp2(PACKED ? s[t][i] - ref : fmaf(s[t][i], c, -ref));
-      s[t][i] = w;
-      if constexpr (!PACKED) l += w;
-    }
-  if constexpr (PACKED) {
-    const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float4 v = *(const float4*)(inv + 32 * t + 8 * b + 4 * h);
-        l = fmaf(s[t][4 * b], v.x, l); l = fmaf(s[t][4 * b + 1], v.y, l);
-        l = fmaf(s[t][4 * b + 2], v.z, l); l = fmaf(s[t][4 * b + 3], v.w, l);
+// The same from a table in LDS, levels in their own order: of two codes (4 bits: a byte; 3 bits: six), or of the four of a byte.
+template <int BITS> struct ck_lut {
+  static constexpr int ENTRIES = BITS == 3 ? 64 : 256, WORDS = BITS == 2 ? 2 : 1;
+  uint32_t level[ENTRIES * WORDS];
+  // by `threads` threads; the unit of the levels is that of ck_table
+  __device__ __forceinline__ void fill(const float* __restrict__ centroids, int tid, int threads, float unit) {
+    const float down = 1.f / unit;
+    auto one = [&](int code) { return (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)(centroids[code] * down)); };
+    constexpr int M = (1 << BITS) - 1;
+    for (int i = tid; i < ENTRIES; i += threads) {
+      if constexpr (BITS == 2) {
+        level[2 * i] = one(i >> 6) | one((i >> 4) & 3) << 16;
+        level[2 * i + 1] = one((i >> 2) & 3) | one(i & 3) << 16;
+      } else {
+        level[i] = one(i >> BITS) | one(i & M) << 16;
       }
+    }
   }
-  r.l = fmaf(r.l, alpha, l);
-  return alpha;
+  // group g (eight coordinates) of a run of codes that starts at word 0 of `w`
+  template <int W> __device__ __forceinline__ ck_u4 group(const uint32_t (&w)[W], int g) const {
+    const unsigned char* t = (const unsigned char*)level;
+    ck_u4 r;
+    if constexpr (BITS == 4) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) r[b] = *(const uint32_t*)(t + (b == 0 ? (w[g] << 2) & 0x3fcu : (w[g] >> (8 * b - 2)) & 0x3fcu));
+    } else if constexpr (BITS == 3) {
+      const int b = 3 * g, i = b >> 2, o = b & 3;
+      const uint32_t sel = (uint32_t)(o + 2) | (uint32_t)(o + 1) << 8 | (uint32_t)o << 16 | 0x0c000000u;
+      const uint32_t x = __builtin_amdgcn_perm(i + 1 < W ? w[i + 1 < W ? i + 1 : 0] : 0u, w[i], sel);      // 24 bits, the first coordinate on top
+      r[0] = *(const uint32_t*)(t + ((x >> 16) & 0xfcu));
+      r[1] = *(const uint32_t*)(t + ((x >> 10) & 0xfcu));
+      r[2] = *(const uint32_t*)(t + ((x >> 4) & 0xfcu));
+      r[3] = *(const uint32_t*)(t + ((x << 2) & 0xfcu));
+    } else {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int sh = 16 * (g & 1) + 8 * b;
+        const ck_u2 v = *(const ck_u2*)(t + (sh < 3 ? (w[g >> 1] << 3) & 0x7f8u : (w[g >> 1] >> (sh - 3)) & 0x7f8u));
+        r[2 * b] = v[0];
+        r[2 * b + 1] = v[1];
+      }
+    }
+    return r;
+  }
+};
+
+// ---- one step of the softmax ----------------------------------------------------------------------------------------
+// A row's running state: weights are 2^(exponent - m), and l is their sum over the lane's own keys (the halves are added at the end).  m is
+// not the maximum so far but lies at most CK_FRAME below it: the sums are rescaled only when a row's maximum has outgrown that, and weights of
+// up to 2^CK_FRAME lose nothing, as their rounding is relative.
+#define CK_FRAME 8.f
+struct ck_row { float m, l; };
+// largest of NT tiles of 32 products, over both halves
+template <int NT> __device__ __forceinline__ float ck_max(const ck_f16v (&s)[NT]) {
+  float a = s[0][0], b = s[0][1];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = t == 0 ? 2 : 0; i < 16; i += 2) {
+      a = fmaxf(a, s[t][i]);
+      b = fmaxf(b, s[t][i + 1]);
+    }
+  a = fmaxf(a, b);
+  return fmaxf(a, akv_lane_xor<32>(a));
 }
-// products to exponents: norms of 32 NT keys from LDS, f = the row's factor
-template <int NT>
-__device__ __forceinline__ void ck_norms(ck_f16v (&s)[NT], float f, const float* __restrict__ kn, const float* __restrict__ lg) {
+// Whether some row's largest exponent has outgrown its frame; `alpha` is then what the row's sums are multiplied with.
+__device__ __forceinline__ bool ck_outgrown(ck_row& r, float mx, float& alpha) {
+  const bool grown = mx > r.m + CK_FRAME;
+  if (!__ballot(grown)) return false;
+  const float m = grown ? mx : r.m;
+  alpha = grown ? ck_exp2(r.m - m) : 1.f;
+  r.m = m;
+  r.l *= alpha;
+  return true;
+}
+// Products (packed: exponents) to weights, in place; c = scale x log2 e.
+template <int NT, bool PACKED>
+__device__ __forceinline__ void ck_weights(ck_f16v (&s)[NT], ck_row& r, float c, const float* __restrict__ inv) {
+  const float ref = r.m == -INFINITY ? 0.f : r.m;
   const int h = (threadIdx.x & 63) >> 5;
+  float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = ck_exp2(PACKED ? s[t][4 * b + e] - ref : fmaf(s[t][4 * b + e], c, -ref));
+      if constexpr (PACKED) {
+        const float4 v = *(const float4*)(inv + 32 * t + 8 * b + 4 * h);
+        l0 = fmaf(w[0], v.x, l0); l1 = fmaf(w[1], v.y, l1);
+        l0 = fmaf(w[2], v.z, l0); l1 = fmaf(w[3], v.w, l1);
+      } else {
+        l0 += w[0]; l1 += w[1];
+        l0 += w[2]; l1 += w[3];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[t][4 * b + e] = w[e];
+    }
+  r.l += l0 + l1;
+}
+// Products to exponents: s x (key norm x unit of the levels) + log2 of the value norm, norms of 32 NT keys from LDS.  f: what the row was
+// scaled with, 1 but for rows far from the usual size.
+template <int NT>
+__device__ __forceinline__ void ck_norms(ck_f16v (&s)[NT], float f, bool scaled, const float* __restrict__ kn, const float* __restrict__ lg) {
+  const int h = (threadIdx.x & 63) >> 5;
+  if (scaled) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s[t] *= f;
+  }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const float4 k = *(const float4*)(kn + 32 * t + 8 * b + 4 * h), g = *(const float4*)(lg + 32 * t + 8 * b + 4 * h);
-      s[t][4 * b] = fmaf(s[t][4 * b] * k.x, f, g.x);
-      s[t][4 * b + 1] = fmaf(s[t][4 * b + 1] * k.y, f, g.y);
-      s[t][4 * b + 2] = fmaf(s[t][4 * b + 2] * k.z, f, g.z);
-      s[t][4 * b + 3] = fmaf(s[t][4 * b + 3] * k.w, f, g.w);
-    }
-}
-// weights of keys whose value norm counts as nothing
-template <int NT> __device__ __forceinline__ void ck_drop(ck_f16v (&s)[NT], const float* __restrict__ keep) {
-  const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const float4 k = *(const float4*)(keep + 32 * t + 8 * b + 4 * h);
-      s[t][4 * b] *= k.x; s[t][4 * b + 1] *= k.y; s[t][4 * b + 2] *= k.z; s[t][4 * b + 3] *= k.w;
+      s[t][4 * b] = fmaf(s[t][4 * b], k.x, g.x);
+      s[t][4 * b + 1] = fmaf(s[t][4 * b + 1], k.y, g.y);
+      s[t][4 * b + 2] = fmaf(s[t][4 * b + 2], k.z, g.z);
+      s[t][4 * b + 3] = fmaf(s[t][4 * b + 3], k.w, g.w);
     }
 }
 // keys that the row at position `pos` does not see: from `base` on, NT x 32 of them
@@ -296,7 +351,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
   __shared__ __align__(16) unsigned char lds[P::LDS];
   __shared__ ck_lengths<256> L;
   __shared__ float ml[4][64][2];
-  __shared__ __align__(16) float nrm[PACKED ? 4 : 1][4][32];     // per wavefront: key norms, log2 and inverse of value norms, whether they count
+  __shared__ __align__(16) float nrm[PACKED ? 4 : 1][3][32];     // per wavefront: key norms, log2 and inverse of value norms
+  __shared__ ck_lut<BITS> lut;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
   const int G = gridDim.x;
@@ -315,8 +371,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
   ck_find<256, P::N>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
   int64_t tile_at = (int64_t)head * per_head + first;        // the tile's first unit on the axis
 
+  // keys: levels by byte permutes in registers, values: from a table in LDS; each alone would fill the vector unit, or LDS
   ck_table<BITS> table;
-  if constexpr (PACKED) table.load(a.centroids);
+  if constexpr (PACKED) {
+    table.load(a.centroids);
+    lut.fill(a.centroids, tid, 256, table.up);
+  }
 
   for (;;) {
     const ck_seq s = ck_sequence(a, L, seq);
@@ -335,9 +395,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
       for (int ks = 0; ks < KS; ++ks) {
         const int grp = PACKED ? KS * h + ks : 2 * ks + h;
         q[ks] = row.valid ? *(const ck_u4*)(p + 8 * grp) : (ck_u4){0u, 0u, 0u, 0u};
+        if constexpr (PACKED) {      // in the order of ck_levels
+          const ck_u4 x = q[ks];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c0 = ck_coord<BITS>(2 * i), c1 = ck_coord<BITS>(2 * i + 1);
+            const uint32_t sel = (c0 & 1 ? 0x0302u : 0x0100u) | (c1 & 1 ? 0x07060000u : 0x05040000u);
+            q[ks][i] = __builtin_amdgcn_perm(x[c1 / 2], x[c0 / 2], sel);
+          }
+        }
       }
-      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] * table.up : 0.f;
+      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
     }
+    const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     ck_f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = (ck_f16v)(0.f);
@@ -381,20 +451,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
       // ---- values to LDS, products of keys and rows
       ck_f16v sc[1];
       sc[0] = (ck_f16v)(0.f);
-      bool drop = false;
       if constexpr (PACKED) {
+        const uint32_t keep = vn < CK_TINY ? 0u : 0xffffffffu;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          *(ck_u4*)(vl + col * P::PITCH + 16 * (KS * h + ks)) = ck_levels<BITS>(table, vw, ks);
+          *(ck_u4*)(vl + col * P::PITCH + 16 * (KS * h + ks)) = lut.group(vw, ks) & keep;
           sc[0] = M::mfma(ck_levels<BITS>(table, kw, ks), q[ks], sc[0]);
         }
-        drop = __ballot(vn < CK_TINY) != 0;
         if (h == 0) {
           const float v = vn < CK_TINY ? 1.f : vn;
-          nrm[wave][0][col] = kn;
+          nrm[wave][0][col] = kn * table.up;
           nrm[wave][1][col] = __log2f(v);
           nrm[wave][2][col] = 1.f / v;
-          nrm[wave][3][col] = vn < CK_TINY ? 0.f : 1.f;
         }
       } else {
 #pragma unroll
@@ -410,15 +478,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
       }
       akv_wave_sync();
       if (base < keys.hi) {
-        if constexpr (PACKED) ck_norms(sc, fac, nrm[wave][0], nrm[wave][1]);
+        if constexpr (PACKED) ck_norms(sc, fac, scaled, nrm[wave][0], nrm[wave][1]);
         if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
-        const float alpha = ck_softmax<1, PACKED>(sc, st, PACKED ? 1.f : a.scale2, PACKED ? nrm[wave][2] : nullptr);
-        if constexpr (PACKED)
-          if (drop) ck_drop(sc, nrm[wave][3]);
-        if (__ballot(alpha != 1.f)) {
+        float alpha;
+        if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
 #pragma unroll
           for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
+        ck_weights<1, PACKED>(sc, st, a.scale2, PACKED ? nrm[wave][2] : nullptr);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           ck_u4 p;
@@ -446,11 +513,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
     float m = ml[0][lane][0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][lane][0]);
-    const float c = PACKED ? 1.f : a.scale2, ref = m == -INFINITY ? 0.f : m * c;
+    const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) l += ml[w][lane][1] * ck_exp2(fmaf(ml[w][lane][0], c, -ref));
-    const float mine = ck_exp2(fmaf(st.m, c, -ref));
+    for (int w = 0; w < 4; ++w) l += ml[w][lane][1] * ck_exp2(ml[w][lane][0] - ref);
+    const float mine = ck_exp2(st.m - ref);
     float4* merge = (float4*)lds;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -495,38 +562,54 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
 }
 
 // ---- many rows a sequence -----------------------------------------------------------------------------------------------------
-// A tile is 32 rows a wavefront, a unit 64 keys, which the wavefronts of the workgroup share in LDS, in two buffers: while one is multiplied the
-// next is requested into registers.  Matrix cores and the vector work of the softmax bound it.
+// A tile is 32 rows a wavefront, a unit N keys, which the wavefronts of the workgroup share in LDS.  Work goes by steps of 32
+// keys: while the weights of step x are computed (vector unit) the products of step x + 1 are (matrix cores), their operands read during the
+// value products of step x - 1; then the values of step x are multiplied, their operands read during the first half.  The two units take
+// turns instruction by instruction: left to two wavefronts a SIMD with both in blocks, they overlapped by a quarter (mean of 16
+// products and 16 weights 1417 clocks, in turns 1071).  Keys of unit u + 2 and values of u + 1 are on their way during unit u.
+//
+// Rows lie in LDS without padding, their pieces of sixteen bytes in an order that depends on the row, piece c at place c ^ f(row): sixteen
+// lanes that read one piece of sixteen keys, and 32 that read four coordinates each of four values, meet all 64 banks once
+// (245 and 216 bytes a clock; rows padded by 32 bytes gave 128 and 126).
 template <int D, int KIND> struct ck_wide {
-  static constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES, N = 64;
+  static constexpr int WAVES = D == 128 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES, N = D == 256 ? 32 : 64, STEPS = N / 32;
+  static constexpr int PER_CU = D == 64 ? 2 : 1;                      // workgroups a CU
+  static constexpr int PER_SIMD = D == 256 ? 1 : 2;     // wavefronts a SIMD
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8;
-  static constexpr int PITCH = 2 * D + 32;
-  static constexpr int TILE = N * PITCH;
-  static constexpr int NORMS = KIND >= 2 ? 4 * N * 4 : 0;
-  static constexpr int BUF = 2 * TILE + NORMS;
-  static constexpr int LDS = 2 * BUF;
+  static constexpr int ROW = 2 * D, TILE = N * ROW;
+  static constexpr int KRING = 3, VRING = 2, RING = 4;                // units of keys, of values, of places and norms
+  static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + VRING * TILE, NORM0 = PLACE0 + RING * N * 16;
+  static constexpr int LDS = NORM0 + (KIND >= 2 ? RING * N * 16 : 0);
+  static __device__ __forceinline__ int fk(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int fv(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : 5 * (r & 3); }
 };
+// Sixteen bytes a lane from `src` into LDS at `at` + 16 x lane.  (The compiler does not see the request: who reads waits by
+// ck_landed() and a barrier.  The wait states stand behind m0.)
+__device__ __forceinline__ void ck_request(const uint8_t* src, uint32_t at) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(at) : "memory");
+}
+__device__ __forceinline__ void ck_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <int D, int KIND>
-__global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), D == 256 ? 1 : 2) void ck_wide_kernel(ck_args a) {
+__global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER_SIMD)) void ck_wide_kernel(ck_args a) {
   typedef ck_wide<D, KIND> P;
   typedef ck_math<KIND> M;
   constexpr bool PACKED = M::packed;
   constexpr int BITS = PACKED ? KIND : 4;
   constexpr int KS = P::KS, DT = P::DT, N = P::N, T = P::THREADS;
-  constexpr int CPR = D / 8;                                  // dense: pieces of 16 bytes a row
-  constexpr int NP = N * CPR / T;                             // pieces of K, and of V, a thread
-  constexpr int TPR = D / 32, TASKS = N * TPR, NT = (TASKS + T - 1) / T;      // packed: 32 codes a task
-  extern __shared__ __align__(16) unsigned char lds[];
+  constexpr int CPR = D / 8;                                  // pieces of 16 bytes a row
+  constexpr int RPI = 64 / CPR, NP = N / RPI / P::WAVES;      // dense: rows a request, requests a wavefront
+  constexpr int TPR = D / 32, TASKS = N * TPR, NT = 2 * TASKS / T;      // packed: 32 codes a task, keys' then values'
+  static_assert(NT * T == 2 * TASKS && NP * RPI * P::WAVES == N, "whole tasks and requests");
+  extern __shared__ __align__(1024) unsigned char lds[];
   __shared__ ck_lengths<T> L;
-  __shared__ int64_t place_blk[2][N];
-  __shared__ int place_pos[2][N];
-  __shared__ int drops[2];                                    // packed: value norms of the unit that count as nothing
+  __shared__ ck_lut<BITS> lut;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
   const int G = gridDim.x;
   const int g = G % 8 == 0 ? (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
   const int TM = P::ROWS / a.GC;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   ck_load_lengths(a, L);
   const int per_head = ck_total<T, N>(a, L, TM);
@@ -540,14 +623,29 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), D == 256 ? 1 : 2) void
   ck_find<T, N>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
   int64_t tile_at = (int64_t)head * per_head + first;
 
-  ck_table<BITS> table;
-  if constexpr (PACKED) table.load(a.centroids);
+  float unit = 1.f;                // of the levels
+  if constexpr (PACKED) {
+    ck_table<BITS> table;
+    table.load(a.centroids);
+    unit = table.up;
+    lut.fill(a.centroids, tid, T, unit);
+  }
+  // where the lane reads its operands: a piece of a key, four coordinates of a value
+  uint32_t k_at[KS], v_at[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) k_at[ks] = lds0 + P::K0 + col * P::ROW + 16 * ((2 * ks + h) ^ P::fk(col));
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int r = 4 * h + (lane & 15) / 4, c = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    v_at[dt] = lds0 + P::V0 + r * P::ROW + 16 * (c ^ P::fv(r)) + 8 * (lane & 1);
+  }
 
   for (;;) {
     const ck_seq s = ck_sequence(a, L, seq);
     const ck_range keys = ck_keys<N>(a, s, tile, TM);
     const int t0 = tile * TM, t1 = min(s.n, t0 + TM);
-    const int u0 = (int)(at - tile_at), u1 = (int)min((int64_t)keys.units, end - tile_at), steps = u1 - u0;
+    const int u0 = (int)(at - tile_at), u1 = (int)min((int64_t)keys.units, end - tile_at);
+    const int units = keys.hi > 0 ? u1 - u0 : 0;
     const ck_lane row = ck_row_of(a, s, t0, t1, head, 32 * wave + col);
     const int kvh = head / a.HS;
     // positions of the wavefront's rows
@@ -559,156 +657,206 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), D == 256 ? 1 : 2) void
       const uint16_t* p = (const uint16_t*)a.q + (int64_t)row.token * a.qs_tok + (int64_t)row.head * a.qs_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) q[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
-      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] * table.up : 0.f;
+      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
     }
+    const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     ck_f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = (ck_f16v)(0.f);
     ck_row st = {-INFINITY, 0.f};
 
     const int base0 = (keys.first + u0) * N;
-    ck_u4 kd[PACKED ? 1 : NP], vd[PACKED ? 1 : NP];
-    uint32_t kw[PACKED ? NT : 1][BITS], vw[PACKED ? NT : 1][BITS];
-    float kn = 0.f, vn = 1.f;
-    // places of a unit's keys, by the first threads
-    auto look = [&](int u) { return ck_key(a, seq, base0 + u * N + tid, tid < N && u < steps && base0 + u * N + tid < keys.hi); };
-    auto note = [&](int u, const ck_place_of& p) {
+    // Places of a unit's keys, a thread each (all wavefronts alike): the table's entry is requested, and what the rows of keys and
+    // values lie at is written a unit later.  A key behind the last one has the last one's place: what is read for it is masked, and its
+    // value is as finite as that one's.
+    struct entry { uint32_t lo, hi; };
+    const int wide_id = a.tables_it == AKV_I64;
+    auto key_of = [&](int u) { return min(base0 + u * N + (tid & (N - 1)), keys.hi - 1); };
+    auto look = [&](int u) {
+      uint32_t rem;
+      const int64_t i = (int64_t)seq * a.bt_stride + akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, rem);
+      const uint32_t* p = (const uint32_t*)a.tables + (i << wide_id);
+      return entry{p[0], p[wide_id]};
+    };
+    float kn = 0.f, vn = 1.f;      // packed: norms of the unit noted last
+    auto note = [&](int u, const entry& e) {
+      uint32_t pos;
+      akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, pos);
+      const int64_t blk = akv_clamp_block(wide_id ? (int64_t)((uint64_t)e.hi << 32 | e.lo) : (int64_t)(int32_t)e.lo, a.num_blocks);
       if (tid < N) {
-        place_blk[u & 1][tid] = p.blk;
-        place_pos[u & 1][tid] = p.pos;
+        int64_t* place = (int64_t*)(lds + P::PLACE0) + (u & (P::RING - 1)) * 2 * N;
+        place[tid] = blk * a.k_blk + pos * a.k_pos + kvh * a.k_head;
+        place[N + tid] = blk * a.v_blk + pos * a.v_pos + kvh * a.v_head;
       }
-    };
-    auto request = [&](int u) {
-      const int b = u & 1, limit = keys.hi - (base0 + u * N);
       if constexpr (PACKED) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const int task = tid + T * i, r = task / TPR, part = task % TPR;
-          if (task < TASKS && r < limit) {
-            const int64_t blk = place_blk[b][r];
-            const int pos = place_pos[b][r];
-            ck_load_words(kw[i], a.k + blk * a.k_blk + pos * a.k_pos + kvh * a.k_head + 4 * BITS * part);
-            ck_load_words(vw[i], a.v + blk * a.v_blk + pos * a.v_pos + kvh * a.v_head + 4 * BITS * part);
-          } else {
-#pragma unroll
-            for (int j = 0; j < BITS; ++j) kw[i][j] = vw[i][j] = 0u;
-          }
-        }
-        kn = 0.f;
-        vn = 1.f;
-        if (tid < N && tid < limit) {
-          const int64_t blk = place_blk[b][tid];
-          const int pos = place_pos[b][tid];
-          kn = a.kn[blk * a.kn_blk + pos * a.kn_pos + kvh * a.kn_head];
-          vn = a.vn[blk * a.vn_blk + pos * a.vn_pos + kvh * a.vn_head];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int c = tid + T * i, r = c / CPR, part = c % CPR;
-          if (r < limit) {
-            const int64_t blk = place_blk[b][r];
-            const int pos = place_pos[b][r];
-            kd[i] = *(const ck_u4*)(a.k + blk * a.k_blk + pos * a.k_pos + kvh * a.k_head + 16 * part);
-            vd[i] = *(const ck_u4*)(a.v + blk * a.v_blk + pos * a.v_pos + kvh * a.v_head + 16 * part);
-          } else {
-            kd[i] = vd[i] = (ck_u4){0u, 0u, 0u, 0u};
-          }
-        }
+        kn = a.kn[blk * a.kn_blk + pos * a.kn_pos + kvh * a.kn_head];
+        vn = a.vn[blk * a.vn_blk + pos * a.vn_pos + kvh * a.vn_head];
       }
     };
-    auto put = [&](int u) {
-      unsigned char* kt = lds + (u & 1) * P::BUF;
-      unsigned char* vt = kt + P::TILE;
-      if constexpr (PACKED) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const int task = tid + T * i, r = task / TPR, part = task % TPR;
-          if (TASKS % T == 0 || task < TASKS) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              *(ck_u4*)(kt + r * P::PITCH + 64 * part + 16 * j) = ck_levels<BITS>(table, kw[i], j);
-              *(ck_u4*)(vt + r * P::PITCH + 64 * part + 16 * j) = ck_levels<BITS>(table, vw[i], j);
-            }
-          }
-        }
-        if (tid < N) {
-          float* nr = (float*)(vt + P::TILE);
-          const float v = vn < CK_TINY ? 1.f : vn;
-          nr[tid] = kn;
-          nr[N + tid] = __log2f(v);
-          nr[2 * N + tid] = 1.f / v;
-          nr[3 * N + tid] = vn < CK_TINY ? 0.f : 1.f;
-          const int drop = __ballot(vn < CK_TINY) != 0;      // (the N threads are the first wavefront)
-          if (tid == 0) drops[u & 1] = drop;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int c = tid + T * i, r = c / CPR, part = c % CPR;
-          *(ck_u4*)(kt + r * P::PITCH + 16 * part) = kd[i];
-          *(ck_u4*)(vt + r * P::PITCH + 16 * part) = vd[i];
-        }
+    auto note_norms = [&](int u) {
+      if (PACKED && tid < N) {
+        float* nr = (float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
+        const float v = vn < CK_TINY ? 1.f : vn;
+        nr[tid] = kn * unit;
+        nr[N + tid] = __log2f(v);
+        nr[2 * N + tid] = 1.f / v;
+        ((uint32_t*)nr)[3 * N + tid] = vn < CK_TINY ? 0u : 0xffffffffu;
       }
     };
+    // dense: keys of one unit, values of another on their way to LDS
+    auto request = [&](int uk, int k_slot, bool k_there, int uv, bool v_there) {
+      const int64_t* pk = (const int64_t*)(lds + P::PLACE0) + (uk & (P::RING - 1)) * 2 * N;
+      const int64_t* pv = (const int64_t*)(lds + P::PLACE0) + (uv & (P::RING - 1)) * 2 * N + N;
+      int64_t ok[NP], ov[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int r = (wave * NP + i) * RPI + lane / CPR;
+        ok[i] = pk[r] + 16 * ((lane % CPR) ^ P::fk(r));
+        ov[i] = pv[r] + 16 * ((lane % CPR) ^ P::fv(r));
+      }
+      const uint32_t k_to = lds0 + P::K0 + k_slot * P::TILE + wave * NP * RPI * P::ROW, v_to = lds0 + P::V0 + (uv & 1) * P::TILE + wave * NP * RPI * P::ROW;
+      if (k_there) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) ck_request(a.k + ok[i], __builtin_amdgcn_readfirstlane(k_to + i * 1024));
+      }
+      if (v_there) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) ck_request(a.v + ov[i], __builtin_amdgcn_readfirstlane(v_to + i * 1024));
+      }
+    };
+    // packed: codes of the keys of one unit and the values of another to registers, and from there to LDS; a value whose norm counts as
+    // nothing is zero
+    uint32_t words[PACKED ? NT : 1][BITS];
+    auto fetch = [&](int uk, int uv) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int task = tid + T * i, v = task / TASKS, r = task % TASKS / TPR, part = task % TPR;
+        const int64_t* place = (const int64_t*)(lds + P::PLACE0) + ((v ? uv : uk) & (P::RING - 1)) * 2 * N + v * N;
+        ck_load_words(words[i], (v ? a.v : a.k) + place[r] + 4 * BITS * part);
+      }
+    };
+    auto put = [&](int k_slot, int uv) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int task = tid + T * i, v = task / TASKS, r = task % TASKS / TPR, part = task % TPR;
+        unsigned char* to = lds + (v ? P::V0 + (uv & 1) * P::TILE : P::K0 + k_slot * P::TILE) + r * P::ROW;
+        const int f = v ? P::fv(r) : P::fk(r);
+        uint32_t keep = 0xffffffffu;
+        if (v) keep = ((const uint32_t*)(lds + P::NORM0))[(uv & (P::RING - 1)) * 4 * N + 3 * N + r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(ck_u4*)(to + 16 * ((4 * part + j) ^ f)) = lut.group(words[i], j) & keep;
+      }
+    };
+
     __syncthreads();               // (LDS of the tile before has been read)
-    note(0, look(0));
-    note(1, look(1));
-    __syncthreads();
-    request(0);
-    put(0);
-    __syncthreads();
-    for (int u = 0; u < steps; ++u) {
-      const int base = base0 + u * N;
-      ck_place_of ahead = {0, 0};
-      if (u + 1 < steps) {
-        request(u + 1);
-        ahead = look(u + 2);
+    if (units > 0) {
+      const entry e0 = look(0), e1 = look(1), e2 = look(2);
+      note(0, e0);
+      note_norms(0);
+      note(1, e1);
+      note_norms(1);
+      note(2, e2);
+      note_norms(2);
+      __syncthreads();
+      if constexpr (PACKED) {
+        fetch(0, 0);
+        put(0, 0);
+        fetch(1, 0);
+        put(1, 0);
+      } else {
+        request(0, 0, true, 0, true);
+        request(1, 1, units > 1, 0, false);
+        ck_landed();
       }
-      if (base <= pos_last && !(a.window > 0 && base + N - 1 <= pos_first - a.window)) {
-        const unsigned char* kt = lds + (u & 1) * P::BUF;
-        unsigned char* vt = (unsigned char*)kt + P::TILE;
-        const float* nr = (const float*)(vt + P::TILE);
-        ck_f16v sc[2];
+    }
+    __syncthreads();
+    ck_u4 kf[KS];
+    ck_f16v sc[1];
+    auto read_keys = [&](uint32_t from) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          sc[t] = (ck_f16v)(0.f);
+      for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const ck_lds_u4*)(uintptr_t)(k_at[ks] + from);
+    };
+    // bytes from a step's keys to the next but one's: within the unit, or into the ring's next
+    int k_slot = 0;                // of unit u
+    if (units > 0) {
+      read_keys(0);
+      sc[0] = (ck_f16v)(0.f);
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) sc[t] = M::mfma(*(const ck_u4*)(kt + (32 * t + col) * P::PITCH + 16 * (2 * ks + h)), q[ks], sc[t]);
-        }
-        if constexpr (PACKED) ck_norms(sc, fac, nr, nr + N);
-        if (base + N - 1 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
-        const float alpha = ck_softmax<2, PACKED>(sc, st, PACKED ? 1.f : a.scale2, PACKED ? nr + 2 * N : nullptr);
-        if constexpr (PACKED)
-          if (drops[u & 1]) ck_drop(sc, nr + 3 * N);
-        if (__ballot(alpha != 1.f)) {
+      for (int ks = 0; ks < KS; ++ks) sc[0] = M::mfma(kf[ks], q[ks], sc[0]);
+      read_keys(P::STEPS > 1 ? 32 * P::ROW : P::TILE);
+    }
+    for (int u = 0; u < units; ++u) {
+      const int k_next = k_slot == 2 ? 0 : k_slot + 1, k_after = k_next == 2 ? 0 : k_next + 1;
+      // ---- on their way: places of unit u + 3, keys of u + 2, values of u + 1
+      const entry ahead = look(u + 3);
+      if constexpr (PACKED) fetch(u + 2, u + 1);
+      else request(u + 2, k_after, u + 2 < units, u + 1, u + 1 < units);
+      const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
+      const uint32_t v_from = (u & 1) * P::TILE;
+#pragma unroll
+      for (int t = 0; t < P::STEPS; ++t) {
+        const int base = base0 + u * N + 32 * t;
+        if constexpr (PACKED) ck_norms(sc, fac, scaled, nr + 32 * t, nr + N + 32 * t);
+        if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
+        float alpha;
+        if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
 #pragma unroll
           for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
+        // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
+        ck_f16v next = (ck_f16v)(0.f);
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          ck_u4 p;
+        for (int ks = 0; ks < KS; ++ks) next = M::mfma(kf[ks], q[ks], next);
+        ck_u2 vf[2][DT][2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = M::pair(sc[kb / 2][8 * (kb & 1) + 2 * i], sc[kb / 2][8 * (kb & 1) + 2 * i + 1]);
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            unsigned char* at_v = vt + (16 * kb + 4 * h + (lane & 15) / 4) * P::PITCH + 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-            const ck_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)at_v);
-            const ck_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)(at_v + 8 * P::PITCH));
-            const ck_u2 xu = __builtin_bit_cast(ck_u2, x), yu = __builtin_bit_cast(ck_u2, y);
-            o[dt] = M::mfma((ck_u4){xu[0], xu[1], yu[0], yu[1]}, p, o[dt]);
-          }
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)     // keys 16 kb + 8 e + 4 h .. + 3, coordinate 32 dt + lane % 32
+              vf[kb][dt][e] = __builtin_bit_cast(ck_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)(uintptr_t)(v_at[dt] + v_from + (32 * t + 16 * kb + 8 * e) * P::ROW)));
+        ck_weights<1, PACKED>(sc, st, a.scale2, PACKED ? nr + 2 * N + 32 * t : nullptr);
+        ck_u4 p[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[kb][i] = M::pair(sc[0][8 * kb + 2 * i], sc[0][8 * kb + 2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                      // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / KS + (PACKED ? 1 : 0), 0);         // LDS read
+          __builtin_amdgcn_sched_group_barrier(0x402, (PACKED ? 64 : 56) / KS + 1, 0);            // vector and transcendental
         }
+        // ---- values, and the keys of the step after the next to registers
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            o[dt] = M::mfma((ck_u4){vf[kb][dt][0][0], vf[kb][dt][0][1], vf[kb][dt][1][0], vf[kb][dt][1][1]}, p[kb], o[dt]);
+        read_keys(P::STEPS == 1 ? k_after * P::TILE : k_next * P::TILE + t * 32 * P::ROW);
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, KS / (2 * DT), 0);
+        }
+        sc[0] = next;
       }
-      if (u + 1 < steps) put(u + 1);
-      if (u + 2 < steps) note(u + 2, ahead);
+      // ---- what was requested is there
+      if constexpr (PACKED) {
+        put(k_after, u + 1);
+        note_norms(u + 2);
+      } else {
+        ck_landed();
+      }
+      note(u + 3, ahead);
+      k_slot = k_next;
       __syncthreads();
     }
 
     st.l += akv_lane_xor<32>(st.l);
     const bool whole = u0 == 0 && u1 == keys.units;
     if (whole) {
-      const float f = ck_finish<KIND>(st.l, PACKED ? table.up : 1.f);
+      const float f = ck_finish<KIND>(st.l, unit);
       if (row.valid) {
 #pragma unroll
         for (int c = 0; c < P::QUADS; ++c)
@@ -745,15 +893,14 @@ __global__ __launch_bounds__(256) void ck_merge_kernel(ck_args a, int G) {
   const ck_record rec = a.rec[g];
   if (!rec.valid) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
-  const float c = ck_math<KIND>::packed ? 1.f : a.scale2;
   float m = -INFINITY, l = 0.f;
   float4 x[MINE];
 #pragma unroll
   for (int i = 0; i < MINE; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](int64_t slot) {
     const float2 e = a.part_ml[(slot * WAVES + part) * 64 + lane];
-    const float mn = fmaxf(m, e.x), ref = mn == -INFINITY ? 0.f : mn * c;
-    const float f0 = ck_exp2(fmaf(m, c, -ref)), f1 = ck_exp2(fmaf(e.x, c, -ref));
+    const float mn = fmaxf(m, e.x), ref = mn == -INFINITY ? 0.f : mn;
+    const float f0 = ck_exp2(m - ref), f1 = ck_exp2(e.x - ref);
     l = l * f0 + e.y * f1;
     m = mn;
 #pragma unroll
@@ -793,7 +940,7 @@ static inline int ck_groups(int per_cu) {
 }
 struct ck_scratch { size_t rec, ml, part, bytes; };
 static inline ck_scratch ck_scratch_layout(int D) {
-  const size_t g = (size_t)ck_groups(2), slots = 2 * g * 4;          // (the wide kernel's: four times the narrow one's)
+  const size_t g = (size_t)ck_groups(2), slots = 2 * (size_t)ck_groups(2) * 8;
   ck_scratch w;
   w.rec = 0;
   w.ml = akv_align256(g * sizeof(ck_record));
@@ -838,7 +985,7 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
       return AKV_OK;
     });
     if (rc) return rc;
-    const int G = ck_groups(D == 256 ? 1 : 2);
+    const int G = ck_groups(W::PER_CU);
     ck_wide_kernel<D, KIND><<<G, W::THREADS, W::LDS, stream>>>(n);
     AKV_LAUNCH_CHECK("ck_wide_kernel");
     ck_merge_kernel<D, KIND, W::WAVES><<<dim3(G, W::WAVES), 256, 0, stream>>>(n, G);

@@ -28,16 +28,16 @@ static int ck_run(ck_args a, int dtype, const void* prep, void* out, int64_t os_
   const dim3 grid((unsigned)(tiles < most ? tiles : most), D / 64);
   const void* q = a.q;
   const int64_t qs_tok = a.qs_tok, qs_head = a.qs_head;
-  if (dtype == AKV_F16) ck_rotate_kernel<D, AKV_F16, BITS, true, AKV_F16><<<grid, 256, 0, stream>>>(q, qs_tok, qs_head, rows, a.QH, pi, ps, qr, 0, 0, fac, a.scale2, a.starts, a.starts_it, a.S, a.tail);
-  else ck_rotate_kernel<D, AKV_BF16, BITS, true, AKV_F16><<<grid, 256, 0, stream>>>(q, qs_tok, qs_head, rows, a.QH, pi, ps, qr, 0, 0, fac, a.scale2, a.starts, a.starts_it, a.S, a.tail);
+  if (dtype == AKV_F16) ck_rotate_kernel<D, AKV_F16, true, AKV_F16><<<grid, 256, 0, stream>>>(q, qs_tok, qs_head, rows, a.QH, pi, ps, qr, 0, 0, fac, a.scale2, a.starts, a.starts_it, a.S, a.tail);
+  else ck_rotate_kernel<D, AKV_BF16, true, AKV_F16><<<grid, 256, 0, stream>>>(q, qs_tok, qs_head, rows, a.QH, pi, ps, qr, 0, 0, fac, a.scale2, a.starts, a.starts_it, a.S, a.tail);
   AKV_LAUNCH_CHECK("ck_rotate_kernel");
   a.q = qr; a.qs_tok = (int64_t)a.QH * D; a.qs_head = D; a.qfac = fac;
   a.out = turned; a.os_tok = (int64_t)a.QH * D; a.os_head = D;
   const int rc = ck_launch<D, BITS>(a, most_new, (char*)workspace + w.scratch, stream);
   if (rc) return rc;
   const float* pit = pi + (size_t)D * D;
-  if (dtype == AKV_F16) ck_rotate_kernel<D, AKV_F32, BITS, false, AKV_F16><<<grid, 256, 0, stream>>>(turned, a.os_tok, a.os_head, rows, a.QH, pit, ps, out, os_tok, os_head, nullptr, 0.f, a.starts, a.starts_it, a.S, a.tail);
-  else ck_rotate_kernel<D, AKV_F32, BITS, false, AKV_BF16><<<grid, 256, 0, stream>>>(turned, a.os_tok, a.os_head, rows, a.QH, pit, ps, out, os_tok, os_head, nullptr, 0.f, a.starts, a.starts_it, a.S, a.tail);
+  if (dtype == AKV_F16) ck_rotate_kernel<D, AKV_F32, false, AKV_F16><<<grid, 256, 0, stream>>>(turned, a.os_tok, a.os_head, rows, a.QH, pit, ps, out, os_tok, os_head, nullptr, 0.f, a.starts, a.starts_it, a.S, a.tail);
+  else ck_rotate_kernel<D, AKV_F32, false, AKV_BF16><<<grid, 256, 0, stream>>>(turned, a.os_tok, a.os_head, rows, a.QH, pit, ps, out, os_tok, os_head, nullptr, 0.f, a.starts, a.starts_it, a.S, a.tail);
   AKV_LAUNCH_CHECK("ck_rotate_kernel");
   return AKV_OK;
 }

@@ -4,9 +4,10 @@
 #include "akv_attn_rows.h"
 
 // ---- packed: rotations of queries and outputs ---------------------------------------------------------------------------------
-// Rows of `in` (any strides) times the matrix, 16 rows a step; workgroup (b, slice): 64 outputs.  IN_PLACES: the row's coordinates lie in
-// the order of the packed groups.
-template <int D, int XDT, int BITS, bool QUERY, int ODT>
+// Rows of `in` (any strides) times the matrix, 16 rows a step; workgroup (b, slice): 64 outputs.  QUERY: to float16, times the scale of the
+// scores and log2 e; `fac` is what a row has to be multiplied with still, 1 unless its largest coordinate is far from 1 (then the row
+// is stored with that between 2^5 and 2^6).
+template <int D, int XDT, bool QUERY, int ODT>
 __global__ __launch_bounds__(256) void ck_rotate_kernel(const void* __restrict__ in, int64_t is_tok, int64_t is_head, int64_t rows, int QH,
                                                         const float* __restrict__ matrix, const akv_prep_scale* __restrict__ scale,
                                                         void* __restrict__ out, int64_t os_tok, int64_t os_head, float* __restrict__ fac, float qscale,
@@ -41,8 +42,7 @@ __global__ __launch_bounds__(256) void ck_rotate_kernel(const void* __restrict__
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       float v = x[i] * sc;
-      int d = 64 * (i >> 2) + 4 * part + (i & 3);
-      if constexpr (!QUERY) d = (d & ~7) + ck_coord<BITS>(d & 7);
+      const int d = 64 * (i >> 2) + 4 * part + (i & 3);
 #pragma unroll
       for (int j = 0; j < TERMS; ++j) {
         const _Float16 t = (_Float16)(j == 2 ? v * AR_THIRD : v);
@@ -51,8 +51,10 @@ __global__ __launch_bounds__(256) void ck_rotate_kernel(const void* __restrict__
       }
     }
     if (part == 0) {
-      r.unscale[row] = un;
-      if (QUERY && slice == 0 && n < rows) fac[n] = un * AR_M_SCALE * qscale;
+      // queries: the usual sizes go as they are (the factor is in the row), the others scaled
+      const bool usual = mx * qscale >= 0x1p-8f && mx * qscale <= 0x1p8f;
+      r.unscale[row] = !QUERY ? un : usual ? un * qscale : 1.f / AR_M_SCALE;
+      if (QUERY && slice == 0 && n < rows) fac[n] = usual ? 1.f : un * AR_M_SCALE * qscale;
     }
     __syncthreads();
     const ar_float4 y = m.times(r);
@@ -60,9 +62,11 @@ __global__ __launch_bounds__(256) void ck_rotate_kernel(const void* __restrict__
     const int64_t no = tile * 16 + rr;
     if (no < limit) {
       if constexpr (QUERY) {
-        uint16_t* dst = (uint16_t*)out + no * D + (d0 & ~7);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dst[ck_place<BITS>((d0 & 7) + e)] = __builtin_bit_cast(unsigned short, (_Float16)(y[e] * (1.f / AR_M_SCALE)));
+        const float f = r.unscale[rr];
+        ck_u2 v;
+        v[0] = ck_math<CK_F16>::pair(y[0] * f, y[1] * f);
+        v[1] = ck_math<CK_F16>::pair(y[2] * f, y[3] * f);
+        *(ck_u2*)((uint16_t*)out + no * D + d0) = v;
       } else {
         const float f = r.unscale[rr];
         const int64_t t = no / QH, o = t * os_tok + (no - t * QH) * os_head + d0;
