@@ -5,9 +5,10 @@
 // query head) pairs of one kv head, token-major, as many whole tokens as fit; their keys reach from `lo` (0, or what the window of
 // the tile's first token leaves) to the position of the tile's last token.
 //
-// The tiles of a sequence, of all sequences, once for every kv head, lie end to end on one axis, each as long as it has units (runs of
-// keys); workgroup g of G takes the units [g F / G, (g + 1) F / G) of that axis.  So every workgroup has the same number of units,
-// however the lengths are spread and whatever the causal edge leaves of a tile, and few rows over many keys are split by themselves.  A
+// The tiles of a sequence, of all sequences, once for every kv head, lie end to end on one axis, each as long as its units (runs of
+// keys) and START more, what a tile costs besides: rows, first keys, results.  Workgroup g of G takes what lies in [g F / G, (g + 1) F / G)
+// of that axis.  So every workgroup has as much to do, however the lengths are spread and whatever the causal edge leaves of a
+// tile, and few rows over many keys are split by themselves.  A
 // tile that lies in one range is finished there; the pieces of one that does not go to memory and are joined by ck_merge_kernel
 // in the order of the axis.  All of it is derived on the device: no call waits for a length.
 #pragma once
@@ -17,7 +18,7 @@
 #define CK_NARROW_ROWS 64         // a sequence of at most so many rows a kv head goes to the narrow kernel
 
 struct ck_record {                // what a workgroup leaves of the tile that begins in its range and ends in another
-  int64_t end;                    // one past the tile's last unit
+  int64_t end;                    // one past the tile on the axis
   int64_t total;                  // F
   int32_t valid, head, token, tokens;
 };
@@ -107,7 +108,7 @@ template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, c
 
 // Tiles are numbered with gaps: tile j of sequence i is floor(start_i / TM) + i + j, which no two tiles share.
 __device__ __forceinline__ int ck_tile_numbers(const ck_args& a, int TM) { return a.T / TM + a.S + 1; }
-template <int THREADS, int N>
+template <int THREADS, int N, int START>
 __device__ __forceinline__ int ck_units_of(const ck_args& a, const ck_lengths<THREADS>& L, int x, int TM, int& seq, int& tile) {
   int lo = 0, hi = a.S + 1;                 // the last i with floor(start_i / TM) + i <= x
   while (hi - lo > 1) {
@@ -119,16 +120,16 @@ __device__ __forceinline__ int ck_units_of(const ck_args& a, const ck_lengths<TH
   seq = lo;
   tile = x - (s.q0 / TM + lo);
   if (tile < 0 || (int64_t)tile * TM >= s.n) return 0;
-  return ck_keys<N>(a, s, tile, TM).units;
+  return ck_keys<N>(a, s, tile, TM).units + START;
 }
 
 __device__ __forceinline__ int ck_wave_scan(int v) { return akv_wave_inclusive_scan(v); }
 
-// units of one kv head, in every thread
-template <int THREADS, int N> __device__ __forceinline__ int ck_total(const ck_args& a, ck_lengths<THREADS>& L, int TM) {
+// length of one kv head's part of the axis, in every thread
+template <int THREADS, int N, int START> __device__ __forceinline__ int ck_total(const ck_args& a, ck_lengths<THREADS>& L, int TM) {
   int sum = 0, seq, tile;
   const int numbers = ck_tile_numbers(a, TM);
-  for (int x = threadIdx.x; x < numbers; x += THREADS) sum += ck_units_of<THREADS, N>(a, L, x, TM, seq, tile);
+  for (int x = threadIdx.x; x < numbers; x += THREADS) sum += ck_units_of<THREADS, N, START>(a, L, x, TM, seq, tile);
   sum = akv_wave_sum(sum);
   if ((threadIdx.x & 63) == 0) L.sum[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -139,15 +140,15 @@ template <int THREADS, int N> __device__ __forceinline__ int ck_total(const ck_a
   return all;
 }
 
-// the tile that holds unit `at` (< total): its sequence, number and first unit
-template <int THREADS, int N>
+// the tile that holds `at` (< total): its sequence, number and place on the axis
+template <int THREADS, int N, int START>
 __device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L, int TM, int at, int& seq, int& tile, int& first) {
   const int numbers = ck_tile_numbers(a, TM);
   int base = 0;
   for (int x0 = 0;; x0 += THREADS) {
     const int x = x0 + (int)threadIdx.x;
     int sq = 0, tl = 0;
-    const int u = x < numbers ? ck_units_of<THREADS, N>(a, L, x, TM, sq, tl) : 0;
+    const int u = x < numbers ? ck_units_of<THREADS, N, START>(a, L, x, TM, sq, tl) : 0;
     const int inc = ck_wave_scan(u);
     if ((threadIdx.x & 63) == 63) L.sum[threadIdx.x >> 6] = inc;
     __syncthreads();
@@ -173,5 +174,5 @@ __device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L
   first = __builtin_amdgcn_readfirstlane(L.total);
 }
 
-// first unit of workgroup g's range
+// where workgroup g's range begins
 __device__ __forceinline__ int64_t ck_begin(int64_t total, int g, int G) { return total * g / G; }

@@ -332,7 +332,7 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 // operand, values through its own part of LDS; what the four hold of the tile is added at the end of the tile or range.  No barrier
 // inside.  Reading the cache bounds it.
 template <int D, int KIND> struct ck_narrow {
-  static constexpr int ROWS = 32, N = 128, THREADS = 256;
+  static constexpr int ROWS = 32, N = 128, THREADS = 256, START = 2;
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8;
   static constexpr int PITCH = 2 * D + 32;                            // bytes of a value row in LDS: eight rows meet all banks
   static constexpr int V_BYTES = 32 * PITCH;
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
   const int TM = P::ROWS / a.GC;
 
   ck_load_lengths(a, L);
-  const int per_head = ck_total<256, P::N>(a, L, TM);
+  const int per_head = ck_total<256, P::N, P::START>(a, L, TM);
   const int heads = a.KVH * a.HS;
   const int64_t total = (int64_t)per_head * heads;
   int64_t at = ck_begin(total, g, G);
@@ -368,8 +368,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
   int head = (int)(at / per_head), seq, tile, first;
-  ck_find<256, P::N>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
-  int64_t tile_at = (int64_t)head * per_head + first;        // the tile's first unit on the axis
+  ck_find<256, P::N, P::START>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
+  int64_t tile_at = (int64_t)head * per_head + first;        // the tile's place on the axis
 
   // keys: levels by byte permutes in registers, values: from a table in LDS; each alone would fill the vector unit, or LDS
   ck_table<BITS> table;
@@ -382,7 +382,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
     const ck_seq s = ck_sequence(a, L, seq);
     const ck_range keys = ck_keys<P::N>(a, s, tile, TM);
     const int t0 = tile * TM, t1 = min(s.n, t0 + TM);
-    const int u0 = (int)(at - tile_at), u1 = (int)min((int64_t)keys.units, end - tile_at);
+    const int64_t tile_end = tile_at + P::START + keys.units;
+    const int u0 = max(0, (int)(at - tile_at) - P::START), u1 = min(keys.units, (int)min((int64_t)0x7fffffff, end - tile_at) - P::START);
+    if (u1 <= 0) return;           // (nothing but the start of the tile: it begins in the next range)
     const ck_lane row = ck_row_of(a, s, t0, t1, head, col);
     const int kvh = head / a.HS;
     const int pos_first = s.ctx - s.n + t0, pos_last = s.ctx - s.n + t1 - 1;
@@ -545,12 +547,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
     }
     if (!whole && wave == 0) {
       a.part_ml[slot * 64 + lane] = make_float2(m, l);
-      if (u0 == 0 && lane == 0) a.rec[g] = {tile_at + keys.units, total, 1, head, s.q0 + t0, t1 - t0};
+      if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
     }
     // ---- on to the next tile
-    at = tile_at + u1;
+    at = tile_at = tile_end;
     if (at >= end) return;
-    tile_at += keys.units;
     ++tile;
     int n = s.n;
     while ((int64_t)tile * TM >= n) {
@@ -572,13 +573,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
 // lanes that read one piece of sixteen keys, and 32 that read four coordinates each of four values, meet all 64 banks once
 // (245 and 216 bytes a clock; rows padded by 32 bytes gave 128 and 126).
 template <int D, int KIND> struct ck_wide {
+  static constexpr bool AHEAD = D == 64 || (D == 128 && KIND < 2);    // registers for the keys of the step after the next
   static constexpr int WAVES = D == 128 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES, N = D == 256 ? 32 : 64, STEPS = N / 32;
-  static constexpr int PER_CU = D == 64 ? 2 : 1;                      // workgroups a CU
-  static constexpr int PER_SIMD = D == 256 ? 1 : 2;     // wavefronts a SIMD
+  static constexpr int START = 192 / N;                               // (what a tile costs besides its units, in units)
+  static constexpr int PER_CU = D == 256 || WAVES == 8 ? 1 : 2;       // workgroups a CU
+  static constexpr int PER_SIMD = D == 256 ? 1 : 2;                   // wavefronts a SIMD
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8;
   static constexpr int ROW = 2 * D, TILE = N * ROW;
-  static constexpr int KRING = 3, VRING = 2, RING = 4;                // units of keys, of values, of places and norms
-  static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + VRING * TILE, NORM0 = PLACE0 + RING * N * 16;
+  // Units of keys held: of those read during a unit, and the one that is written (a unit on with AHEAD, or where a unit is a step)
+  static constexpr int KRING = AHEAD || STEPS == 1 ? 2 : 3;
+  static constexpr int UNROLL = KIND >= 2 && D == 128 ? 1 : STEPS;
+  static constexpr int RING = 4;                                      // units whose places and norms are held
+  static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
   static constexpr int LDS = NORM0 + (KIND >= 2 ? RING * N * 16 : 0);
   static __device__ __forceinline__ int fk(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
   static __device__ __forceinline__ int fv(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : 5 * (r & 3); }
@@ -612,7 +618,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   ck_load_lengths(a, L);
-  const int per_head = ck_total<T, N>(a, L, TM);
+  const int per_head = ck_total<T, N, P::START>(a, L, TM);
   const int heads = a.KVH * a.HS;
   const int64_t total = (int64_t)per_head * heads;
   int64_t at = ck_begin(total, g, G);
@@ -620,7 +626,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
   int head = (int)(at / per_head), seq, tile, first;
-  ck_find<T, N>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
+  ck_find<T, N, P::START>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
   int64_t tile_at = (int64_t)head * per_head + first;
 
   float unit = 1.f;                // of the levels
@@ -644,34 +650,27 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     const ck_seq s = ck_sequence(a, L, seq);
     const ck_range keys = ck_keys<N>(a, s, tile, TM);
     const int t0 = tile * TM, t1 = min(s.n, t0 + TM);
-    const int u0 = (int)(at - tile_at), u1 = (int)min((int64_t)keys.units, end - tile_at);
+    const int64_t tile_end = tile_at + P::START + keys.units;
+    const int u0 = max(0, (int)(at - tile_at) - P::START), u1 = min(keys.units, (int)min((int64_t)0x7fffffff, end - tile_at) - P::START);
+    if (u1 <= 0) return;           // (nothing but the start of the tile: it begins in the next range)
     const int units = keys.hi > 0 ? u1 - u0 : 0;
     const ck_lane row = ck_row_of(a, s, t0, t1, head, 32 * wave + col);
     const int kvh = head / a.HS;
     // positions of the wavefront's rows
     const int w0 = t0 + 32 * wave / a.GC, w1 = min(t1, t0 + (32 * wave + 31) / a.GC + 1);
     const int pos_first = s.ctx - s.n + w0, pos_last = w0 < t1 ? s.ctx - s.n + w1 - 1 : -1;
-    ck_u4 q[KS];
-    float fac = 1.f;
-    {
-      const uint16_t* p = (const uint16_t*)a.q + (int64_t)row.token * a.qs_tok + (int64_t)row.head * a.qs_head;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) q[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
-      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
-    }
-    const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     ck_f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = (ck_f16v)(0.f);
     ck_row st = {-INFINITY, 0.f};
 
     const int base0 = (keys.first + u0) * N;
-    // Places of a unit's keys, a thread each (all wavefronts alike): the table's entry is requested, and what the rows of keys and
+    // Places of a unit's keys, by one wavefront, a lane a key: the table's entry is requested, and what the rows of keys and
     // values lie at is written a unit later.  A key behind the last one has the last one's place: what is read for it is masked, and its
     // value is as finite as that one's.
     struct entry { uint32_t lo, hi; };
     const int wide_id = a.tables_it == AKV_I64;
-    auto key_of = [&](int u) { return min(base0 + u * N + (tid & (N - 1)), keys.hi - 1); };
+    auto key_of = [&](int u) { return min(base0 + u * N + (lane & (N - 1)), keys.hi - 1); };
     auto look = [&](int u) {
       uint32_t rem;
       const int64_t i = (int64_t)seq * a.bt_stride + akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, rem);
@@ -683,24 +682,23 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       uint32_t pos;
       akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, pos);
       const int64_t blk = akv_clamp_block(wide_id ? (int64_t)((uint64_t)e.hi << 32 | e.lo) : (int64_t)(int32_t)e.lo, a.num_blocks);
-      if (tid < N) {
-        int64_t* place = (int64_t*)(lds + P::PLACE0) + (u & (P::RING - 1)) * 2 * N;
-        place[tid] = blk * a.k_blk + pos * a.k_pos + kvh * a.k_head;
-        place[N + tid] = blk * a.v_blk + pos * a.v_pos + kvh * a.v_head;
-      }
+      int64_t* place = (int64_t*)(lds + P::PLACE0) + (u & (P::RING - 1)) * 2 * N;
+      place[lane & (N - 1)] = blk * a.k_blk + pos * a.k_pos + kvh * a.k_head;
+      place[N + (lane & (N - 1))] = blk * a.v_blk + pos * a.v_pos + kvh * a.v_head;
       if constexpr (PACKED) {
         kn = a.kn[blk * a.kn_blk + pos * a.kn_pos + kvh * a.kn_head];
         vn = a.vn[blk * a.vn_blk + pos * a.vn_pos + kvh * a.vn_head];
       }
     };
     auto note_norms = [&](int u) {
-      if (PACKED && tid < N) {
+      if constexpr (PACKED) {
         float* nr = (float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
         const float v = vn < CK_TINY ? 1.f : vn;
-        nr[tid] = kn * unit;
-        nr[N + tid] = __log2f(v);
-        nr[2 * N + tid] = 1.f / v;
-        ((uint32_t*)nr)[3 * N + tid] = vn < CK_TINY ? 0u : 0xffffffffu;
+        const int key = lane & (N - 1);
+        nr[key] = kn * unit;
+        nr[N + key] = __log2f(v);
+        nr[2 * N + key] = 1.f / v;
+        ((uint32_t*)nr)[3 * N + key] = vn < CK_TINY ? 0u : 0xffffffffu;
       }
     };
     // dense: keys of one unit, values of another on their way to LDS
@@ -748,27 +746,43 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       }
     };
 
+    // (the rows of the tile are requested behind the first keys and values)
+    ck_u4 q[KS];
+    float fac = 1.f;
+    auto rows = [&]() {
+      const uint16_t* p = (const uint16_t*)a.q + (int64_t)row.token * a.qs_tok + (int64_t)row.head * a.qs_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) q[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
+      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
+    };
     __syncthreads();               // (LDS of the tile before has been read)
     if (units > 0) {
-      const entry e0 = look(0), e1 = look(1), e2 = look(2);
-      note(0, e0);
-      note_norms(0);
-      note(1, e1);
-      note_norms(1);
-      note(2, e2);
-      note_norms(2);
+      if (wave == 0) {
+        const entry e0 = look(0), e1 = look(1), e2 = look(2);
+        note(0, e0);
+        note_norms(0);
+        note(1, e1);
+        note_norms(1);
+        note(2, e2);
+        note_norms(2);
+      }
       __syncthreads();
       if constexpr (PACKED) {
         fetch(0, 0);
+        rows();
         put(0, 0);
         fetch(1, 0);
         put(1, 0);
       } else {
         request(0, 0, true, 0, true);
         request(1, 1, units > 1, 0, false);
+        rows();
         ck_landed();
       }
+    } else {
+      rows();
     }
+    const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     __syncthreads();
     ck_u4 kf[KS];
     ck_f16v sc[1];
@@ -776,24 +790,26 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const ck_lds_u4*)(uintptr_t)(k_at[ks] + from);
     };
-    // bytes from a step's keys to the next but one's: within the unit, or into the ring's next
-    int k_slot = 0;                // of unit u
     if (units > 0) {
       read_keys(0);
       sc[0] = (ck_f16v)(0.f);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sc[0] = M::mfma(kf[ks], q[ks], sc[0]);
-      read_keys(P::STEPS > 1 ? 32 * P::ROW : P::TILE);
+      if (P::AHEAD) read_keys(32 * P::ROW);
+      __syncthreads();             // (unit 2's keys may go where these were)
     }
+    int k_slot = 0;                // of unit u
     for (int u = 0; u < units; ++u) {
-      const int k_next = k_slot == 2 ? 0 : k_slot + 1, k_after = k_next == 2 ? 0 : k_next + 1;
-      // ---- on their way: places of unit u + 3, keys of u + 2, values of u + 1
-      const entry ahead = look(u + 3);
+      // ---- on their way: places of unit u + 3 (the wavefronts take turns), keys of u + 2, values of u + 1
+      const bool mine = wave == (u & (P::WAVES - 1));
+      const int k_next = P::KRING == 2 ? k_slot ^ 1 : k_slot == 2 ? 0 : k_slot + 1, k_after = P::KRING == 2 ? k_slot : k_next == 2 ? 0 : k_next + 1;
+      entry ahead;
+      if (mine) ahead = look(u + 3);
       if constexpr (PACKED) fetch(u + 2, u + 1);
       else request(u + 2, k_after, u + 2 < units, u + 1, u + 1 < units);
       const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
       const uint32_t v_from = (u & 1) * P::TILE;
-#pragma unroll
+#pragma unroll (P::UNROLL)
       for (int t = 0; t < P::STEPS; ++t) {
         const int base = base0 + u * N + 32 * t;
         if constexpr (PACKED) ck_norms(sc, fac, scaled, nr + 32 * t, nr + N + 32 * t);
@@ -804,6 +820,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
           for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
         // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
+        if (!P::AHEAD) read_keys(t + 1 < P::STEPS ? k_slot * P::TILE + (t + 1) * 32 * P::ROW : k_next * P::TILE);
         ck_f16v next = (ck_f16v)(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) next = M::mfma(kf[ks], q[ks], next);
@@ -821,10 +838,12 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[kb][i] = M::pair(sc[0][8 * kb + 2 * i], sc[0][8 * kb + 2 * i + 1]);
+        constexpr int READS = 4 * DT + (P::AHEAD ? 0 : KS) + (PACKED ? 4 : 0), FIRST = P::AHEAD ? 0 : 4;
+        if (FIRST > 0) __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                      // MFMA
-          __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT / KS + (PACKED ? 1 : 0), 0);         // LDS read
+          __builtin_amdgcn_sched_group_barrier(0x100, (READS - FIRST + KS - 1) / KS, 0);          // LDS read
           __builtin_amdgcn_sched_group_barrier(0x402, (PACKED ? 64 : 56) / KS + 1, 0);            // vector and transcendental
         }
         // ---- values, and the keys of the step after the next to registers
@@ -833,22 +852,22 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
             o[dt] = M::mfma((ck_u4){vf[kb][dt][0][0], vf[kb][dt][0][1], vf[kb][dt][1][0], vf[kb][dt][1][1]}, p[kb], o[dt]);
-        read_keys(P::STEPS == 1 ? k_after * P::TILE : k_next * P::TILE + t * 32 * P::ROW);
+        if (P::AHEAD) read_keys(k_next * P::TILE + t * 32 * P::ROW);
 #pragma unroll
         for (int i = 0; i < 2 * DT; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, KS / (2 * DT), 0);
+          if (P::AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, KS / (2 * DT), 0);
         }
         sc[0] = next;
       }
       // ---- what was requested is there
       if constexpr (PACKED) {
         put(k_after, u + 1);
-        note_norms(u + 2);
+        if (u > 0 && wave == ((u - 1) & (P::WAVES - 1))) note_norms(u + 2);        // (requested a unit ago, by the same wavefront)
       } else {
         ck_landed();
       }
-      note(u + 3, ahead);
+      if (mine) note(u + 3, ahead);
       k_slot = k_next;
       __syncthreads();
     }
@@ -868,11 +887,10 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       for (int c = 0; c < P::QUADS; ++c)
         ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)], o[c / 4][4 * (c & 3) + 1], o[c / 4][4 * (c & 3) + 2], o[c / 4][4 * (c & 3) + 3]);
       a.part_ml[slot * 64 + lane] = make_float2(st.m, st.l);
-      if (u0 == 0 && tid == 0) a.rec[g] = {tile_at + keys.units, total, 1, head, s.q0 + t0, t1 - t0};
+      if (u0 == 0 && tid == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
     }
-    at = tile_at + u1;
+    at = tile_at = tile_end;
     if (at >= end) return;
-    tile_at += keys.units;
     ++tile;
     int n = s.n;
     while ((int64_t)tile * TM >= n) {

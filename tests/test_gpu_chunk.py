@@ -266,6 +266,18 @@ def test_packed_long_context_is_split(dev):
     check(p.run(), *p.reference())
 
 
+@pytest.mark.parametrize("d,bits", [(64, 4), (128, 4), (128, 3), (128, 2), (256, 4)])
+def test_packed_many_keys_a_workgroup(dev, d, bits):
+    """Ranges of some twenty units and several tiles."""
+    p = Packed(Batch([(700, 2900), (333, 6001)], 16, dev, 7), d, bits, 16, 2, BF, dev, 38)
+    check(p.run(), *p.reference())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_dense_many_keys_a_workgroup(dev, d):
+    run_dense(Batch([(900, 3100), (333, 6001)], 16, dev, 8), d, 32, 4, BF, dev, 24)
+
+
 @pytest.mark.parametrize("lens", [[(3, 200)], [(90, 200)]], ids=["few", "many"])
 def test_packed_norms_of_any_size(dev, lens):
     """Value norms from 0 over 2^-60 to 2^60 of each other: the largest weights times norms decide, and the others are not lost
