@@ -29,6 +29,9 @@ typedef uint32_t ck_u2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) ck_s4 ck_lds_s4;
 typedef __attribute__((address_space(3))) ck_u4 ck_lds_u4;
 
+#ifndef CK_UNROLL
+#define CK_UNROLL (KIND >= 2 ? 1 : STEPS)
+#endif
 #define CK_F16 0
 #define CK_BF16 1                 // 2, 3, 4: packed codes of so many bits
 
@@ -239,15 +242,10 @@ __device__ __forceinline__ void ck_weights(ck_f16v (&s)[NT], ck_row& r, float c,
     }
   r.l += l0 + l1;
 }
-// Products to exponents: s x (key norm x unit of the levels) + log2 of the value norm, norms of 32 NT keys from LDS.  f: what the row was
-// scaled with, 1 but for rows far from the usual size.
+// Products to exponents: s x (key norm x unit of the levels) + log2 of the value norm, norms of 32 NT keys from LDS.
 template <int NT>
-__device__ __forceinline__ void ck_norms(ck_f16v (&s)[NT], float f, bool scaled, const float* __restrict__ kn, const float* __restrict__ lg) {
+__device__ __forceinline__ void ck_norms(ck_f16v (&s)[NT], const float* __restrict__ kn, const float* __restrict__ lg) {
   const int h = (threadIdx.x & 63) >> 5;
-  if (scaled) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) s[t] *= f;
-  }
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -480,7 +478,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
       }
       akv_wave_sync();
       if (base < keys.hi) {
-        if constexpr (PACKED) ck_norms(sc, fac, scaled, nrm[wave][0], nrm[wave][1]);
+        if (scaled) sc[0] *= fac;        // (a row far from the usual size)
+        if constexpr (PACKED) ck_norms(sc, nrm[wave][0], nrm[wave][1]);
         if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
         float alpha;
         if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
@@ -582,8 +581,8 @@ template <int D, int KIND> struct ck_wide {
   static constexpr int ROW = 2 * D, TILE = N * ROW;
   // Units of keys held: of those read during a unit, and the one that is written (a unit on with AHEAD, or where a unit is a step)
   static constexpr int KRING = AHEAD || STEPS == 1 ? 2 : 3;
-  static constexpr int UNROLL = KIND >= 2 && D == 128 ? 1 : STEPS;
-  static constexpr int RING = 4;                                      // units whose places and norms are held
+  static constexpr int UNROLL = CK_UNROLL;
+  static constexpr int RING = 2 * WAVES;                              // units whose places and norms are held
   static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
   static constexpr int LDS = NORM0 + (KIND >= 2 ? RING * N * 16 : 0);
   static __device__ __forceinline__ int fk(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
@@ -666,8 +665,9 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 
     const int base0 = (keys.first + u0) * N;
     // Places of a unit's keys, by one wavefront, a lane a key: the table's entry is requested, and what the rows of keys and
-    // values lie at is written a unit later.  A key behind the last one has the last one's place: what is read for it is masked, and its
-    // value is as finite as that one's.
+    // values lie at is written a unit later.  Every wavefront does so for one unit of the next WAVES, all at the same time: one that did
+    // it for the others would be what they wait for.  A key behind the last one has the last one's place: what is read for it is masked,
+    // and its value is as finite as that one's.
     struct entry { uint32_t lo, hi; };
     const int wide_id = a.tables_it == AKV_I64;
     auto key_of = [&](int u) { return min(base0 + u * N + (lane & (N - 1)), keys.hi - 1); };
@@ -757,15 +757,8 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     };
     __syncthreads();               // (LDS of the tile before has been read)
     if (units > 0) {
-      if (wave == 0) {
-        const entry e0 = look(0), e1 = look(1), e2 = look(2);
-        note(0, e0);
-        note_norms(0);
-        note(1, e1);
-        note_norms(1);
-        note(2, e2);
-        note_norms(2);
-      }
+      note(wave, look(wave));
+      note_norms(wave);
       __syncthreads();
       if constexpr (PACKED) {
         fetch(0, 0);
@@ -782,6 +775,9 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     } else {
       rows();
     }
+    // (the rows are there: without a use here the compiler waits for them in the loop, and so for what flies then)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(q[ks]));
     const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     __syncthreads();
     ck_u4 kf[KS];
@@ -797,28 +793,27 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       for (int ks = 0; ks < KS; ++ks) sc[0] = M::mfma(kf[ks], q[ks], sc[0]);
       if (P::AHEAD) read_keys(32 * P::ROW);
       __syncthreads();             // (unit 2's keys may go where these were)
+      const float* nr = (const float*)(lds + P::NORM0);
+      if (scaled) sc[0] *= fac;
+      if constexpr (PACKED) ck_norms(sc, nr, nr + N);
+      if (base0 + 31 > pos_first || (a.window > 0 && base0 <= pos_last - a.window)) ck_mask(sc, base0, row.pos, a.window);
+      float alpha;
+      ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha);      // (nothing to rescale yet)
     }
     int k_slot = 0;                // of unit u
+    entry ahead = {0u, 0u};
     for (int u = 0; u < units; ++u) {
-      // ---- on their way: places of unit u + 3 (the wavefronts take turns), keys of u + 2, values of u + 1
-      const bool mine = wave == (u & (P::WAVES - 1));
+      // ---- on their way: places of the WAVES units behind the WAVES that this one belongs to, keys of u + 2, values of u + 1
+      const int turn = u & (P::WAVES - 1);
+      if (turn == 1) note(u - 1 + P::WAVES + wave, ahead);
+      if (turn == 0) ahead = look(u + P::WAVES + wave);
       const int k_next = P::KRING == 2 ? k_slot ^ 1 : k_slot == 2 ? 0 : k_slot + 1, k_after = P::KRING == 2 ? k_slot : k_next == 2 ? 0 : k_next + 1;
-      entry ahead;
-      if (mine) ahead = look(u + 3);
       if constexpr (PACKED) fetch(u + 2, u + 1);
       else request(u + 2, k_after, u + 2 < units, u + 1, u + 1 < units);
       const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
       const uint32_t v_from = (u & 1) * P::TILE;
 #pragma unroll (P::UNROLL)
       for (int t = 0; t < P::STEPS; ++t) {
-        const int base = base0 + u * N + 32 * t;
-        if constexpr (PACKED) ck_norms(sc, fac, scaled, nr + 32 * t, nr + N + 32 * t);
-        if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
-        float alpha;
-        if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
-#pragma unroll
-          for (int i = 0; i < DT; ++i) o[i] *= alpha;
-        }
         // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
         if (!P::AHEAD) read_keys(t + 1 < P::STEPS ? k_slot * P::TILE + (t + 1) * 32 * P::ROW : k_next * P::TILE);
         ck_f16v next = (ck_f16v)(0.f);
@@ -846,28 +841,49 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
           __builtin_amdgcn_sched_group_barrier(0x100, (READS - FIRST + KS - 1) / KS, 0);          // LDS read
           __builtin_amdgcn_sched_group_barrier(0x402, (PACKED ? 64 : 56) / KS + 1, 0);            // vector and transcendental
         }
-        // ---- values, and the keys of the step after the next to registers
+        // (the weights stay on this side of the branch: behind it they would have no products to run beside)
+        asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(st.l));
+        // ---- what the next step's rows do not see
+        const int base = base0 + u * N + 32 * (t + 1);
+        const float* nn = t + 1 < P::STEPS ? nr + 32 * (t + 1) : (const float*)(lds + P::NORM0) + ((u + 1) & (P::RING - 1)) * 4 * N;
+        sc[0] = next;
+        if (scaled) sc[0] *= fac;
+        const bool hidden = base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window);
+        if (hidden) {
+          if constexpr (PACKED) ck_norms(sc, nn, nn + N);
+          ck_mask(sc, base, row.pos, a.window);
+        }
+        // ---- values, the keys of the step after the next to registers, and the largest of the next step's scores
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
             o[dt] = M::mfma((ck_u4){vf[kb][dt][0][0], vf[kb][dt][0][1], vf[kb][dt][1][0], vf[kb][dt][1][1]}, p[kb], o[dt]);
         if (P::AHEAD) read_keys(k_next * P::TILE + t * 32 * P::ROW);
+        if constexpr (PACKED) {
+          // (masked scores are infinite: norms may come on top of them once more only where there are none yet)
+          if (!hidden) ck_norms(sc, nn, nn + N);
+        }
+        const float mx = ck_max(sc) * (PACKED ? 1.f : a.scale2);
 #pragma unroll
         for (int i = 0; i < 2 * DT; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          if (P::AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, KS / (2 * DT), 0);
+          if (P::AHEAD || PACKED) __builtin_amdgcn_sched_group_barrier(0x100, (P::AHEAD ? KS / (2 * DT) : 0) + (PACKED ? 1 : 0), 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (PACKED ? 32 : 16) / (2 * DT) + 1, 0);
         }
-        sc[0] = next;
+        float alpha;
+        if ((t + 1 < P::STEPS || u + 1 < units) && ck_outgrown(st, mx, alpha)) {
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[i] *= alpha;
+        }
       }
       // ---- what was requested is there
       if constexpr (PACKED) {
         put(k_after, u + 1);
-        if (u > 0 && wave == ((u - 1) & (P::WAVES - 1))) note_norms(u + 2);        // (requested a unit ago, by the same wavefront)
+        if (turn == 1) note_norms(u - 1 + P::WAVES + wave);
       } else {
         ck_landed();
       }
-      if (mine) note(u + 3, ahead);
       k_slot = k_next;
       __syncthreads();
     }
