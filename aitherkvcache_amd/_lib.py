@@ -75,7 +75,7 @@ SIGNATURES = {
     "akv_dense_chunk_attn": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                   _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i,
                                   _i, _i64, _i, _i, _i, _i, _i64, _i64, _i, _i, _f, _p, _sz, _p]),
-    "akv_paged_chunk_attn_workspace_bytes": (_sz, [_i64, _i, _i]),
+    "akv_paged_chunk_attn_workspace_bytes": (_sz, [_i]),
     "akv_paged_chunk_attn": (_i, [_p, _i, _i64, _i64,
                                   _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                   _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,

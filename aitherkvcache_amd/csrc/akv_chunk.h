@@ -14,6 +14,41 @@
 #pragma once
 #include "akv_attn_common.h"
 
+typedef _Float16 ck_half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 ck_bf8 __attribute__((ext_vector_type(8)));
+typedef short ck_s4 __attribute__((ext_vector_type(4)));
+typedef float ck_f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t ck_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ck_u2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) ck_s4 ck_lds_s4;
+typedef __attribute__((address_space(3))) ck_u4 ck_lds_u4;
+
+#define CK_F16 0
+#define CK_BF16 1                 // 2, 3, 4: packed codes of so many bits
+
+
+__device__ __forceinline__ float ck_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int KIND> struct ck_math {
+  static constexpr bool packed = KIND >= 2;
+  static __device__ __forceinline__ ck_f16v mfma(ck_u4 a, ck_u4 b, ck_f16v c) {
+    if constexpr (KIND == CK_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ck_bf8, a), __builtin_bit_cast(ck_bf8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ck_half8, a), __builtin_bit_cast(ck_half8, b), c, 0, 0, 0);
+  }
+  // two weights in [0, 1] to the type of the values (one rounding, to nearest)
+  static __device__ __forceinline__ uint32_t pair(float x, float y) {
+    if constexpr (KIND == CK_BF16) {
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      b2 r = {(__bf16)x, (__bf16)y};
+      return __builtin_bit_cast(uint32_t, r);
+    } else {
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      h2 r = {(_Float16)x, (_Float16)y};
+      return __builtin_bit_cast(uint32_t, r);
+    }
+  }
+};
+
 #define CK_SEQS 256               // sequences whose starts and lengths are held in LDS (more are read from memory)
 #define CK_NARROW_ROWS 64         // a sequence of at most so many rows a kv head goes to the narrow kernel
 
@@ -24,8 +59,10 @@ struct ck_record {                // what a workgroup leaves of the tile that be
 };
 
 struct ck_args {
-  const void* q; int64_t qs_tok, qs_head;        // queries (packed: rotated, float16), strides in elements
-  const float* qfac;                             // packed: factor of a row [T][QH]
+  const void* q; int64_t qs_tok, qs_head;        // queries, strides in elements
+  const uint4 *turn_in, *turn_out;               // packed: the rotation's tables, and their scale
+  const akv_prep_scale* turn_scale;
+  int dtype;                                     // packed: type of queries and outputs
   const uint8_t* k; int64_t k_blk, k_pos, k_head;          // bytes
   const uint8_t* v; int64_t v_blk, v_pos, v_head;
   const float* kn; int64_t kn_blk, kn_pos, kn_head;        // packed: norms, elements
@@ -35,7 +72,8 @@ struct ck_args {
   const void* lens;
   const void* starts;
   int tables_it, lens_it, starts_it;
-  void* out; int64_t os_tok, os_head;            // packed: float32
+  void* out; int64_t os_tok, os_head;
+  int kv_alike;                                  // keys and values lie alike, and so do their norms
   float* part; float2* part_ml; ck_record* rec;
   int S, T, QH, KVH, G, HS, GC;                  // G query heads a kv head, in HS groups of GC
   int block_size; uint32_t bs_recip;

@@ -30,6 +30,7 @@ extern "C" int akv_dense_chunk_attn(const void* query, int dtype, int64_t qs_tok
   a.S = num_seqs; a.T = (int)num_tokens; a.QH = num_q_heads; a.KVH = num_kv_heads; a.G = num_q_heads / num_kv_heads;
   a.block_size = block_size; a.bs_recip = ck_reciprocal(block_size);
   a.max_blocks = num_blocks > 0 ? max_blocks_per_seq : 0; a.num_blocks = num_blocks;
+  a.kv_alike = ks_blk == vs_blk && ks_pos == vs_pos && ks_head == vs_head;
   a.window = window; a.tail = zero_tail; a.scale2 = scale * 1.44269504088896341f;
   const hipStream_t s = (hipStream_t)stream;
 #define CK_CASE(DIM) if (d == DIM) return dtype == AKV_F16 ? ck_launch<DIM, CK_F16>(a, max_query_len, workspace, s) : ck_launch<DIM, CK_BF16>(a, max_query_len, workspace, s);

@@ -16,164 +16,103 @@
 // exponent, w = 2^(s + log2 v - M), with M the running maximum of s + log2 v, so weights stay in [0, 1] for norms of any size,
 // and the sum of the softmax takes w / v.
 #pragma once
-#include "akv_chunk.h"
+#include "akv_chunk_rotate.h"
 #include "akv_device_once.h"
 #include <type_traits>
-
-typedef _Float16 ck_half8 __attribute__((ext_vector_type(8)));
-typedef __bf16 ck_bf8 __attribute__((ext_vector_type(8)));
-typedef short ck_s4 __attribute__((ext_vector_type(4)));
-typedef float ck_f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t ck_u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t ck_u2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) ck_s4 ck_lds_s4;
-typedef __attribute__((address_space(3))) ck_u4 ck_lds_u4;
-
-#ifndef CK_UNROLL
-#define CK_UNROLL (KIND >= 2 ? 1 : STEPS)
-#endif
-#define CK_F16 0
-#define CK_BF16 1                 // 2, 3, 4: packed codes of so many bits
 
 // Smallest value norm that counts (its inverse, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
 // frame of the exponents, as if its logarithm were 0, and its value is zero.  Norms of one sequence may
 // lie 2^120 apart: weights are float32 until the sum of the softmax has taken them.
 #define CK_TINY 0x1p-90f
 
-__device__ __forceinline__ float ck_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-template <int KIND> struct ck_math {
-  static constexpr bool packed = KIND >= 2;
-  static __device__ __forceinline__ ck_f16v mfma(ck_u4 a, ck_u4 b, ck_f16v c) {
-    if constexpr (KIND == CK_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(ck_bf8, a), __builtin_bit_cast(ck_bf8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ck_half8, a), __builtin_bit_cast(ck_half8, b), c, 0, 0, 0);
-  }
-  // two weights in [0, 1] to the type of the values (one rounding, to nearest)
-  static __device__ __forceinline__ uint32_t pair(float x, float y) {
-    if constexpr (KIND == CK_BF16) {
-      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-      b2 r = {(__bf16)x, (__bf16)y};
-      return __builtin_bit_cast(uint32_t, r);
-    } else {
-      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-      h2 r = {(_Float16)x, (_Float16)y};
-      return __builtin_bit_cast(uint32_t, r);
-    }
-  }
-};
-
 // ---- packed codes -> float16 levels -----------------------------------------------------------------------------
-// The codebook as bytes: low and high bytes of the levels of codes 0..3, 4..7, 8..11, 12..15, for v_perm.
-template <int BITS> struct ck_table {
-  static constexpr int N = BITS == 4 ? 4 : BITS == 3 ? 2 : 1;
-  uint32_t lo[N], hi[N];
-  float up;                 // value = level x up, a power of two
-  __device__ __forceinline__ void load(const float* __restrict__ centroids) {
-    float c[1 << BITS], m = 0.f;
+// Value of the levels' last place, so to say: a level is a float16 number times this.  Any unit would do (scores take it with the key's norm,
+// outputs in the end); of 64 between two powers of two every wavefront picks the one whose float16 levels are nearest to the
+// codebook, the same everywhere: 16 levels are then off by a third of what a power of two leaves, 2^-13.6 of themselves instead of 2^-12.
+template <int BITS> __device__ __forceinline__ float ck_unit(const float* __restrict__ centroids) {
+  const int lane = threadIdx.x & 63;
+  float c[1 << BITS], m = 0.f;
 #pragma unroll
-    for (int i = 0; i < (1 << BITS); ++i) {
-      c[i] = centroids[i];
-      m = fmaxf(m, fabsf(c[i]));
-    }
-    const uint32_t e = akv_row_exponent(m);
-    const float down = akv_row_scale(e);
-    up = akv_row_unscale(e);
+  for (int i = 0; i < (1 << BITS); ++i) {
+    c[i] = centroids[i];
+    m = fmaxf(m, fabsf(c[i]));
+  }
+  // the largest to [16, 32) x (1 .. 2): levels down to 2^-18 of it are normal numbers
+  const float down = akv_row_scale(akv_row_exponent(m)) * (16.f + 0.25f * lane);
+  float off = 0.f;
 #pragma unroll
-    for (int w = 0; w < N; ++w) {
-      lo[w] = hi[w] = 0u;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const uint32_t h = __builtin_bit_cast(unsigned short, (_Float16)(c[4 * w + b] * down));
-        lo[w] |= (h & 255u) << (8 * b);
-        hi[w] |= (h >> 8) << (8 * b);
-      }
-    }
+  for (int i = 0; i < (1 << BITS); ++i) {
+    const float x = c[i] * down, e = (float)(_Float16)x - x;
+    off = fmaf(e, e, off);
   }
-  // four codes, a byte each, to two words of two levels
-  __device__ __forceinline__ void four(uint32_t sel, uint32_t& w0, uint32_t& w1) const {
-    uint32_t l, h;
-    if constexpr (BITS == 4) {
-      const uint32_t s = sel & 0x07070707u, t = (sel >> 3) & 0x01010101u, m = (t << 8) - t;
-      const uint32_t l0 = __builtin_amdgcn_perm(lo[1], lo[0], s), l1 = __builtin_amdgcn_perm(lo[3], lo[2], s);
-      const uint32_t h0 = __builtin_amdgcn_perm(hi[1], hi[0], s), h1 = __builtin_amdgcn_perm(hi[3], hi[2], s);
-      l = (l1 & m) | (l0 & ~m);
-      h = (h1 & m) | (h0 & ~m);
-    } else if constexpr (BITS == 3) {
-      l = __builtin_amdgcn_perm(lo[1], lo[0], sel);
-      h = __builtin_amdgcn_perm(hi[1], hi[0], sel);
-    } else {
-      l = __builtin_amdgcn_perm(0u, lo[0], sel);
-      h = __builtin_amdgcn_perm(0u, hi[0], sel);
-    }
-    w0 = __builtin_amdgcn_perm(h, l, 0x05010400u);
-    w1 = __builtin_amdgcn_perm(h, l, 0x07030602u);
-  }
-};
-// Group g (eight coordinates) of a run of codes that starts at word 0 of `w`, as eight levels in the order ck_order.
-template <int BITS, int W> __device__ __forceinline__ ck_u4 ck_levels(const ck_table<BITS>& t, const uint32_t (&w)[W], int g) {
-  uint32_t s0, s1;
-  if constexpr (BITS == 4) {
-    s0 = (w[g] >> 4) & 0x0f0f0f0fu;
-    s1 = w[g] & 0x0f0f0f0fu;
-  } else if constexpr (BITS == 3) {
-    // 24 bits, the first coordinate on top: bytes 3g, 3g + 1, 3g + 2
-    const int b = 3 * g, i = b >> 2, o = b & 3;
-    const uint32_t sel = (uint32_t)(o + 2) | (uint32_t)(o + 1) << 8 | (uint32_t)o << 16 | 0x0c000000u;
-    const uint32_t x = __builtin_amdgcn_perm(i + 1 < W ? w[i + 1 < W ? i + 1 : 0] : 0u, w[i], sel);
-    const uint32_t a = x >> 12, c = x & 0xfffu;
-    const uint32_t a2 = (a | a << 10) & 0x003f003fu, c2 = (c | c << 10) & 0x003f003fu;
-    s0 = (a2 | a2 << 5) & 0x07070707u;
-    s1 = (c2 | c2 << 5) & 0x07070707u;
-  } else {
-    const uint32_t x = g & 1 ? w[g >> 1] >> 16 : w[g >> 1];
-    const uint32_t a = x & 0xffu, c = (x >> 8) & 0xffu;
-    const uint32_t a2 = (a | a << 12) & 0x000f000fu, c2 = (c | c << 12) & 0x000f000fu;
-    s0 = (a2 | a2 << 6) & 0x03030303u;
-    s1 = (c2 | c2 << 6) & 0x03030303u;
-  }
-  ck_u4 r;
-  uint32_t r0, r1, r2, r3;
-  t.four(s0, r0, r1);
-  t.four(s1, r2, r3);
-  r[0] = r0; r[1] = r1; r[2] = r2; r[3] = r3;
-  return r;
+  off *= __builtin_amdgcn_rcpf((16.f + 0.25f * lane) * (16.f + 0.25f * lane));
+  // the least, of equal ones the first; a codebook that is not finite leaves the first
+  uint32_t key = off < INFINITY ? (__float_as_uint(off) & ~63u) | (uint32_t)lane : 0x7f800000u | (uint32_t)lane;
+  key = min(key, akv_lane_xor_u32<32>(key)); key = min(key, akv_lane_xor_u32<16>(key)); key = min(key, akv_lane_xor_u32<8>(key));
+  key = min(key, akv_lane_xor_u32<4>(key)); key = min(key, akv_lane_xor_u32<2>(key)); key = min(key, akv_lane_xor_u32<1>(key));
+  const float best = 16.f + 0.25f * (float)(__builtin_amdgcn_readfirstlane((int)(key & 63u)));
+  return akv_row_unscale(akv_row_exponent(m)) / best;
 }
-// coordinate at place p of such a group
-template <int BITS> __host__ __device__ constexpr int ck_coord(int p) { return BITS == 4 ? 2 * (p & 3) + (p >> 2) : (p & 4) + 3 - (p & 3); }
-
-// The same from a table in LDS, levels in their own order: of two codes (4 bits: a byte; 3 bits: six), or of the four of a byte.
-template <int BITS> struct ck_lut {
-  static constexpr int ENTRIES = BITS == 3 ? 64 : 256, WORDS = BITS == 2 ? 2 : 1;
-  uint32_t level[ENTRIES * WORDS];
-  // by `threads` threads; the unit of the levels is that of ck_table
+// Levels from a table in LDS, of two codes at a time (four where a byte holds them).  COPIES of 64: every lane has its own, so that no two
+// meet a bank (a shared table of 256 entries cost 9 clocks a look-up: lanes meet banks, codes in the middle are frequent).
+template <int BITS, int COPIES> struct ck_lut {
+  static constexpr bool OWN = COPIES == 64;
+  static constexpr int ENTRIES = BITS == 3 ? 64 : OWN && BITS == 2 ? 16 : 256, WORDS = BITS == 2 && !OWN ? 2 : 1;
+  uint32_t level[ENTRIES * WORDS * COPIES];
   __device__ __forceinline__ void fill(const float* __restrict__ centroids, int tid, int threads, float unit) {
-    const float down = 1.f / unit;
-    auto one = [&](int code) { return (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)(centroids[code] * down)); };
     constexpr int M = (1 << BITS) - 1;
-    for (int i = tid; i < ENTRIES; i += threads) {
-      if constexpr (BITS == 2) {
-        level[2 * i] = one(i >> 6) | one((i >> 4) & 3) << 16;
-        level[2 * i + 1] = one((i >> 2) & 3) | one(i & 3) << 16;
-      } else {
-        level[i] = one(i >> BITS) | one(i & M) << 16;
+    // (a lane a level, looked up across the wavefront: every entry would wait for memory otherwise)
+    const uint32_t mine = __builtin_bit_cast(unsigned short, (_Float16)(centroids[tid & M] * (1.f / unit)));
+    auto one = [&](int code) { return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * code, (int)mine); };
+    if constexpr (OWN) {
+      // sixteen lanes an entry, sixteen bytes each
+      for (int i = tid / 16; i < ENTRIES; i += threads / 16) {
+        const uint32_t v = one(i >> BITS) | one(i & M) << 16;
+        *(ck_u4*)(level + i * 64 + 4 * (tid & 15)) = (ck_u4){v, v, v, v};
+      }
+    } else {
+      for (int i = tid; i < ENTRIES; i += threads) {
+        if constexpr (BITS == 2) {
+          level[2 * i] = one(i >> 6) | one((i >> 4) & 3) << 16;
+          level[2 * i + 1] = one((i >> 2) & 3) | one(i & 3) << 16;
+        } else {
+          level[i] = one(i >> BITS) | one(i & M) << 16;
+        }
       }
     }
   }
   // group g (eight coordinates) of a run of codes that starts at word 0 of `w`
   template <int W> __device__ __forceinline__ ck_u4 group(const uint32_t (&w)[W], int g) const {
     const unsigned char* t = (const unsigned char*)level;
+    const uint32_t mine = 4 * (threadIdx.x & 63);
+    // (a lane's own table begins where LDS does: the sum of entry and lane is the address)
+    auto own = [](uint32_t at) { return *(const __attribute__((address_space(3))) uint32_t*)(uintptr_t)at; };
     ck_u4 r;
     if constexpr (BITS == 4) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) r[b] = *(const uint32_t*)(t + (b == 0 ? (w[g] << 2) & 0x3fcu : (w[g] >> (8 * b - 2)) & 0x3fcu));
+      for (int b = 0; b < 4; ++b) {
+        if constexpr (OWN) r[b] = own(__builtin_amdgcn_perm(w[g], mine, 0x0c0c0000u | (uint32_t)(4 + b) << 8));
+        else r[b] = *(const uint32_t*)(t + (b == 0 ? (w[g] << 2) & 0x3fcu : (w[g] >> (8 * b - 2)) & 0x3fcu));
+      }
     } else if constexpr (BITS == 3) {
       const int b = 3 * g, i = b >> 2, o = b & 3;
       const uint32_t sel = (uint32_t)(o + 2) | (uint32_t)(o + 1) << 8 | (uint32_t)o << 16 | 0x0c000000u;
       const uint32_t x = __builtin_amdgcn_perm(i + 1 < W ? w[i + 1 < W ? i + 1 : 0] : 0u, w[i], sel);      // 24 bits, the first coordinate on top
-      r[0] = *(const uint32_t*)(t + ((x >> 16) & 0xfcu));
-      r[1] = *(const uint32_t*)(t + ((x >> 10) & 0xfcu));
-      r[2] = *(const uint32_t*)(t + ((x >> 4) & 0xfcu));
-      r[3] = *(const uint32_t*)(t + ((x << 2) & 0xfcu));
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        constexpr int up = OWN ? 8 : 2;
+        const int sh = 18 - 6 * p;
+        const uint32_t v = (sh >= up ? x >> (sh - up) : x << (up - sh)) & (63u << up);
+        if constexpr (OWN) r[p] = own(v | mine);
+        else r[p] = *(const uint32_t*)(t + v);
+      }
+    } else if constexpr (OWN) {
+      // nibbles: of a byte the upper first
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int sh = 16 * (g & 1) + 8 * (p >> 1) + 4 * (1 - (p & 1));
+        r[p] = own(((sh >= 8 ? w[g >> 1] >> (sh - 8) : w[g >> 1] << (8 - sh)) & 0xf00u) | mine);
+      }
     } else {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -285,37 +224,82 @@ __device__ __forceinline__ ck_lane ck_row_of(const ck_args& a, const ck_seq& s, 
   r.pos = r.valid ? s.ctx - s.n + t0 + j : -1;
   return r;
 }
-// quad c of a row's outputs: coordinates 32 (c / 4) + 8 (c % 4) + 4 h .. + 3, finished
-template <int D, int KIND>
+// quad c of a row's outputs: coordinates 8 c + 4 h .. + 3, finished
+template <int KIND>
 __device__ __forceinline__ void ck_store(const ck_args& a, int token, int head, int c, float x, float y, float z, float w) {
   const int d = 8 * c + 4 * ((threadIdx.x & 63) >> 5);
-  if constexpr (ck_math<KIND>::packed) {
-    *(float4*)((float*)a.out + (int64_t)token * a.os_tok + (int64_t)head * a.os_head + d) = make_float4(x, y, z, w);
+  ck_u2 v;
+  if (ck_math<KIND>::packed && a.dtype == AKV_BF16) {
+    v[0] = ck_math<CK_BF16>::pair(x, y);
+    v[1] = ck_math<CK_BF16>::pair(z, w);
   } else {
-    ck_u2 v;
     v[0] = ck_math<KIND>::pair(x, y);
     v[1] = ck_math<KIND>::pair(z, w);
-    *(ck_u2*)((uint16_t*)a.out + (int64_t)token * a.os_tok + (int64_t)head * a.os_head + d) = v;
   }
+  *(ck_u2*)((uint16_t*)a.out + (int64_t)token * a.os_tok + (int64_t)head * a.os_head + d) = v;
 }
 // what the sums of a row are multiplied with in the end
-template <int KIND> __device__ __forceinline__ float ck_finish(float l, float unit) { return l == 0.f ? 0.f : (ck_math<KIND>::packed ? unit / l : 1.f / l); }
+__device__ __forceinline__ float ck_finish(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// bytes of a cache row of D coordinates
-template <int D, int KIND> constexpr int ck_row_bytes() { return KIND >= 2 ? D * KIND / 8 : 2 * D; }
-
-// byte or element offsets of a key: its block (clamped into the cache) and place there
-struct ck_place_of { int64_t blk; int pos; };
-__device__ __forceinline__ ck_place_of ck_key(const ck_args& a, int seq, int key, bool there) {
-  ck_place_of p = {0, 0};
-  if (there) {
-    uint32_t rem;
-    const uint32_t b = akv_div32((uint32_t)key, (uint32_t)a.block_size, a.bs_recip, rem);
-    p.blk = akv_clamp_block(akv_load_index(a.tables, a.tables_it, (int64_t)seq * a.bt_stride + b), a.num_blocks);
-    p.pos = (int)rem;
+// Results of 32 rows whose coordinates are spread over the W wavefronts of a workgroup, QW quads each, times f.  Packed rows go
+// through `rows` (LDS, 32 x (D + 4) floats, which has been read by others) and are turned back.
+template <int D, int KIND, int W, int QW>
+__device__ __forceinline__ void ck_results(const ck_args& a, const float4 (&x)[QW], float f, bool valid, int token, int head, float* __restrict__ rows) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+  if constexpr (!ck_math<KIND>::packed) {
+    if (valid) {
+#pragma unroll
+      for (int i = 0; i < QW; ++i) ck_store<KIND>(a, token, head, QW * wave + i, x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f);
+    }
+  } else {
+    constexpr int ROW = D + 4, KS = D / 16, DT = D / 32;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QW; ++i) *(float4*)(rows + col * ROW + 8 * (QW * wave + i) + 4 * h) = make_float4(x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f);
+    __syncthreads();
+    if (wave < DT) {
+      float v[KS][8];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const float4 y = *(const float4*)(rows + col * ROW + 16 * ks + 8 * p + 4 * h);
+          v[ks][4 * p] = y.x; v[ks][4 * p + 1] = y.y; v[ks][4 * p + 2] = y.z; v[ks][4 * p + 3] = y.w;
+        }
+      ck_u4 hi[KS], lo[KS];
+      const float un = ck_result_operand<D>([&](int ks, int j) { return v[ks][j]; }, hi, lo) * a.turn_scale->up * (1.f / CK_TURN);
+#pragma unroll
+      for (int dt = wave; dt < DT; dt += W) {
+        const ck_f16v y = ck_turn<D>(a.turn_out, dt, hi, lo);
+        if (valid) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) ck_store<KIND>(a, token, head, 4 * dt + b, y[4 * b] * un, y[4 * b + 1] * un, y[4 * b + 2] * un, y[4 * b + 3] * un);
+        }
+      }
+    }
   }
+}
+
+
+// A key's entry in the block table, as it is requested (both words of a 64-bit one), and the key's place in the cache from it: the block is clamped
+// into the cache.  (Taken apart so that nothing waits for the entry where it is requested.)
+struct ck_entry { uint32_t lo, hi; };
+__device__ __forceinline__ ck_entry ck_look(const ck_args& a, int seq, int key) {
+  uint32_t rem;
+  const int wide = a.tables_it == AKV_I64;
+  const int64_t i = (int64_t)seq * a.bt_stride + akv_div32((uint32_t)key, (uint32_t)a.block_size, a.bs_recip, rem);
+  const uint32_t* p = (const uint32_t*)a.tables + (i << wide);
+  return {p[0], p[wide]};
+}
+struct ck_place { uint32_t blk, pos; };
+__device__ __forceinline__ ck_place ck_place_of(const ck_args& a, int key, ck_entry e) {
+  ck_place p;
+  akv_div32((uint32_t)key, (uint32_t)a.block_size, a.bs_recip, p.pos);
+  const int64_t id = a.tables_it == AKV_I64 ? (int64_t)((uint64_t)e.hi << 32 | e.lo) : (int64_t)(int32_t)e.lo;
+  p.blk = (uint32_t)akv_clamp_block(id, a.num_blocks);
   return p;
 }
+__device__ __forceinline__ int64_t ck_offset(ck_place p, int64_t blk, int64_t pos) { return (int64_t)p.blk * blk + (int64_t)p.pos * pos; }
 
 template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W], const uint8_t* __restrict__ p) {
   // rows lie at multiples of four bytes
@@ -326,31 +310,43 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 }
 
 // ---- few rows a sequence ---------------------------------------------------------------------------------------------------
-// A tile is 32 rows, a unit 128 keys: each of the four wavefronts takes 32 of them on its own, keys straight from memory into the
-// operand, values through its own part of LDS; what the four hold of the tile is added at the end of the tile or range.  No barrier
-// inside.  Reading the cache bounds it.
+// A tile is 32 rows, a unit 32 keys a wavefront: each takes its own, keys straight from memory into the operand, values through its
+// part of LDS (sixteen bytes c of value t lie at c ^ f(t), which 16 rows written and 4 read at a time meet all banks with); what the
+// wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Reading the cache bounds it, and for packed rows the
+// vector unit: some 300 instructions for 32 keys.
 template <int D, int KIND> struct ck_narrow {
-  static constexpr int ROWS = 32, N = 128, THREADS = 256, START = 2;
-  static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8;
-  static constexpr int PITCH = 2 * D + 32;                            // bytes of a value row in LDS: eight rows meet all banks
-  static constexpr int V_BYTES = 32 * PITCH;
-  static constexpr int MERGE_BYTES = 4 * QUADS * 64 * 16;             // the sums of four wavefronts
-  static constexpr int LDS = 4 * V_BYTES > MERGE_BYTES ? 4 * V_BYTES : MERGE_BYTES;
+  static constexpr bool PACKED = KIND >= 2;
+  static constexpr int WAVES = PACKED && D < 256 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32, N = 32 * WAVES, START = 3;
+  static constexpr int PER_CU = PACKED || D == 256 ? 1 : 2;
+  static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8, QW = QUADS / WAVES;
+  static constexpr int V_BYTES = 32 * 2 * D, ROW = D + 4;            // (of a value; floats of a row that is turned)
+  // sums of the wavefronts: the upper half's are added to the lower's first where not all fit
+  static constexpr int LEFT = WAVES == 8 || D == 256 ? WAVES / 2 : WAVES;
+  static constexpr int MERGE = LEFT * QUADS * 1024, TURN = 32 * ROW * 4;
+  static constexpr int V0 = PACKED ? (int)sizeof(ck_lut<PACKED ? KIND : 4, 64>) : 0;
+  static constexpr int AREA = MERGE > WAVES * V_BYTES ? MERGE : WAVES * V_BYTES, Q0 = V0 + (AREA > TURN ? AREA : TURN);
+  static constexpr bool Q_LDS = PACKED && D < 256;                   // rows as operands in LDS: registers hold the keys on their way
+  static constexpr int ML0 = Q0 + (Q_LDS ? 2 * KS * 1024 : 0), NRM0 = ML0 + WAVES * 512, UNDO0 = NRM0 + (PACKED ? WAVES * 3 * 128 : 0), L0 = UNDO0 + 128;
+  static constexpr int LDS = L0 + (int)sizeof(ck_lengths<THREADS>);      // (nothing is static: the table of levels begins at 0)
+  static __device__ __forceinline__ int f(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3); }
 };
 
 template <int D, int KIND>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_args a) {
+__global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) void ck_narrow_kernel(ck_args a) {
   typedef ck_narrow<D, KIND> P;
   typedef ck_math<KIND> M;
   constexpr bool PACKED = M::packed;
   constexpr int BITS = PACKED ? KIND : 4;
-  constexpr int KS = P::KS, DT = P::DT;
+  constexpr int KS = P::KS, DT = P::DT, W = P::WAVES, T = P::THREADS;
   constexpr int HW = D * BITS / 64;                // packed: words of half a row
-  __shared__ __align__(16) unsigned char lds[P::LDS];
-  __shared__ ck_lengths<256> L;
-  __shared__ float ml[4][64][2];
-  __shared__ __align__(16) float nrm[PACKED ? 4 : 1][3][32];     // per wavefront: key norms, log2 and inverse of value norms
-  __shared__ ck_lut<BITS> lut;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  ck_lengths<T>& L = *(ck_lengths<T>*)(lds + P::L0);
+  float (*const ml)[64][2] = (float (*)[64][2])(lds + P::ML0);
+  float (*const nrm)[3][32] = (float (*)[3][32])(lds + P::NRM0);     // packed, per wavefront: key norms, log2 and inverse of value norms
+  float* const undo = (float*)(lds + P::UNDO0);    // packed: what undoes the scale of a row of queries
+  typedef ck_lut<BITS, 64> lut_type;
+  const lut_type& lut = *(const lut_type*)lds;
+  unsigned char* const area = lds + P::V0;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
   const int G = gridDim.x;
@@ -358,23 +354,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
   const int TM = P::ROWS / a.GC;
 
   ck_load_lengths(a, L);
-  const int per_head = ck_total<256, P::N, P::START>(a, L, TM);
-  const int heads = a.KVH * a.HS;
-  const int64_t total = (int64_t)per_head * heads;
-  int64_t at = ck_begin(total, g, G);
-  const int64_t end = ck_begin(total, g + 1, G);
+  const int64_t total = ck_total<T, P::N, P::START>(a, L, TM);
+  // Ranges of one kv head's part of the axis, each taken by as many workgroups as there are heads, side by side on one die: they read the
+  // same lines of the cache at the same time.  (A packed row is half a line or less, a norm a thirty-second of one; with the heads one
+  // after the other on the axis, cut anywhere, a verification of 350 MB fetched 830.)
+  const int heads = a.KVH * a.HS, head = g % heads, R = G / heads;
+  int64_t at = ck_begin(total, g / heads, R);
+  const int64_t end = ck_begin(total, g / heads + 1, R);
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
-  int head = (int)(at / per_head), seq, tile, first;
-  ck_find<256, P::N, P::START>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
-  int64_t tile_at = (int64_t)head * per_head + first;        // the tile's place on the axis
+  int seq, tile, first;
+  ck_find<T, P::N, P::START>(a, L, TM, (int)at, seq, tile, first);
+  int64_t tile_at = first;             // the tile's place on the axis
 
-  // keys: levels by byte permutes in registers, values: from a table in LDS; each alone would fill the vector unit, or LDS
-  ck_table<BITS> table;
-  if constexpr (PACKED) {
-    table.load(a.centroids);
-    lut.fill(a.centroids, tid, 256, table.up);
-  }
+  float unit = 1.f, turned = 0.f;      // of the levels; what undoes the matrix's scale, times the scale of the scores
+  bool filled = false;
 
   for (;;) {
     const ck_seq s = ck_sequence(a, L, seq);
@@ -386,167 +380,276 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
     const ck_lane row = ck_row_of(a, s, t0, t1, head, col);
     const int kvh = head / a.HS;
     const int pos_first = s.ctx - s.n + t0, pos_last = s.ctx - s.n + t1 - 1;
-    // the rows: columns of the operand
-    ck_u4 q[KS];
+
+    // ---- 32 keys of the wavefront, a lane its half of one (behind the last key: the last one, masked)
+    const int base0 = (keys.first + u0) * P::N + 32 * wave;
+    const int steps = keys.hi > base0 ? min(u1 - u0, (keys.hi - base0 + P::N - 1) / P::N) : 0;
+    auto key_of = [&](int u) { return min(base0 + u * P::N + col, keys.hi - 1); };
+    ck_u4 kd[PACKED ? 1 : KS], vd[PACKED ? 1 : KS];
+    struct codes { uint32_t k[PACKED ? HW : 1], v[PACKED ? HW : 1]; float kn, vn; };
+    codes even, odd;               // packed: those of two units (in turns, so that nothing in flight is ever moved)
+    const uint8_t *const k_base = a.k + kvh * a.k_head + (PACKED ? 4 * HW : 16) * h, *const v_base = a.v + kvh * a.v_head + (PACKED ? 4 * HW : 16) * h;
+    // (the entry after this unit's is requested first: what waits for it must not wait for the keys as well)
+    ck_entry ahead = {0u, 0u};
+    auto request = [&](int u, codes& w) {
+      const ck_place p = ck_place_of(a, key_of(u), ahead);
+      ahead = ck_look(a, seq, key_of(u + 1));
+      const int64_t ko = ck_offset(p, a.k_blk, a.k_pos), vo = a.kv_alike ? ko : ck_offset(p, a.v_blk, a.v_pos);
+      if constexpr (PACKED) {
+        ck_load_words(w.k, k_base + ko);
+        ck_load_words(w.v, v_base + vo);
+        const int64_t kno = ck_offset(p, a.kn_blk, a.kn_pos), vno = a.kv_alike ? kno : ck_offset(p, a.vn_blk, a.vn_pos);
+        w.kn = a.kn[kno + kvh * a.kn_head];
+        w.vn = a.vn[vno + kvh * a.vn_head];
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          kd[ks] = *(const ck_u4*)(k_base + ko + 32 * ks);
+          vd[ks] = *(const ck_u4*)(v_base + vo + 32 * ks);
+        }
+      }
+    };
+    if (steps > 0) {
+      ahead = ck_look(a, seq, key_of(0));
+      request(0, even);
+      if constexpr (PACKED) request(1, odd);
+    }
+
+    // ---- the rows: columns of the operand
+    ck_u4 q[P::Q_LDS ? 1 : KS], ql[PACKED && !P::Q_LDS ? KS : 1];      // packed: two terms
+    ck_u4* const q_lds = (ck_u4*)(lds + P::Q0) + lane;
     float fac = 1.f;
     {
       const uint16_t* p = (const uint16_t*)a.q + (int64_t)row.token * a.qs_tok + (int64_t)row.head * a.qs_head;
+      if constexpr (PACKED) {
+        float* rows = (float*)area;
+        ck_u4 x[KS];
+        float un = 1.f;
+        if (wave < DT) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int grp = PACKED ? KS * h + ks : 2 * ks + h;
-        q[ks] = row.valid ? *(const ck_u4*)(p + 8 * grp) : (ck_u4){0u, 0u, 0u, 0u};
-        if constexpr (PACKED) {      // in the order of ck_levels
-          const ck_u4 x = q[ks];
+          for (int ks = 0; ks < KS; ++ks) x[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
+          un = ck_query_operand<D>(x, a.dtype);
+        }
+        if (!filled) {
+          unit = ck_unit<BITS>(a.centroids);
+          turned = a.turn_scale->up * (1.f / CK_TURN) * a.scale2;
+        }
+        __syncthreads();           // (the area has been read)
+        if (wave < DT) {
+          if (wave == 0) undo[col] = un;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c0 = ck_coord<BITS>(2 * i), c1 = ck_coord<BITS>(2 * i + 1);
-            const uint32_t sel = (c0 & 1 ? 0x0302u : 0x0100u) | (c1 & 1 ? 0x07060000u : 0x05040000u);
-            q[ks][i] = __builtin_amdgcn_perm(x[c1 / 2], x[c0 / 2], sel);
+          for (int dt = wave; dt < DT; dt += W) {
+            const ck_f16v y = ck_turn<D>(a.turn_in, dt, x);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) *(float4*)(rows + col * P::ROW + 32 * dt + 8 * b + 4 * h) = make_float4(y[4 * b], y[4 * b + 1], y[4 * b + 2], y[4 * b + 3]);
           }
         }
+        if (!filled) {
+          ((lut_type*)lds)->fill(a.centroids, tid, T, unit);
+          filled = true;
+        }
+        __syncthreads();
+        // half h of a row: coordinates D / 2 h ..
+        const float* from = rows + col * P::ROW + D / 2 * h;
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float4 u = *(const float4*)(from + 4 * i);
+          m = fmaxf(fmaxf(m, fmaxf(fabsf(u.x), fabsf(u.y))), fmaxf(fabsf(u.z), fabsf(u.w)));
+        }
+        m = fmaxf(m, akv_lane_xor<32>(m));
+        const float f = ck_query_scale(m, undo[col] * turned, fac);
+        auto piece = [&](int ks, ck_u4& hi, ck_u4& lo) {
+          typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+          const float4 u = *(const float4*)(from + 8 * ks), v = *(const float4*)(from + 8 * ks + 4);
+          const float y[8] = {u.x * f, u.y * f, u.z * f, u.w * f, v.x * f, v.y * f, v.z * f, v.w * f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            hi[i] = M::pair(y[2 * i], y[2 * i + 1]);
+            const h2 t = __builtin_bit_cast(h2, (uint32_t)hi[i]);
+            lo[i] = M::pair(y[2 * i] - (float)t[0], y[2 * i + 1] - (float)t[1]);
+          }
+        };
+        if constexpr (P::Q_LDS) {
+          if (wave < KS) {         // (a piece a wavefront; all read all of them)
+            static_assert(KS <= W, "a piece a wavefront");
+            ck_u4 hi, lo;
+            piece(wave, hi, lo);
+            q_lds[64 * wave] = hi;
+            q_lds[64 * (KS + wave)] = lo;
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) piece(ks, q[ks], ql[ks]);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) q[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(q[ks]));
       }
-      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
     }
     const bool scaled = PACKED && __ballot(fac != 1.f) != 0;
     ck_f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = (ck_f16v)(0.f);
     ck_row st = {-INFINITY, 0.f};
-
-    // 32 keys of the wavefront, a lane its half of one
-    const int base0 = (keys.first + u0) * P::N + 32 * wave, steps = u1 - u0;
-    ck_place_of at0 = ck_key(a, seq, base0 + col, steps > 0 && base0 + col < keys.hi);
-    ck_u4 kd[PACKED ? 1 : KS], vd[PACKED ? 1 : KS];
-    uint32_t kw[PACKED ? HW : 1], vw[PACKED ? HW : 1];
-    float kn = 0.f, vn = 0.f;
-    auto request = [&](const ck_place_of& p, bool there) {
-      if constexpr (PACKED) {
-        if (there) {
-          ck_load_words(kw, a.k + p.blk * a.k_blk + p.pos * a.k_pos + kvh * a.k_head + 4 * HW * h);
-          ck_load_words(vw, a.v + p.blk * a.v_blk + p.pos * a.v_pos + kvh * a.v_head + 4 * HW * h);
-          kn = a.kn[p.blk * a.kn_blk + p.pos * a.kn_pos + kvh * a.kn_head];
-          vn = a.vn[p.blk * a.vn_blk + p.pos * a.vn_pos + kvh * a.vn_head];
-        } else {
+    unsigned char* vl = area + wave * P::V_BYTES;
+    uint32_t v_at[DT];             // where the lane reads four coordinates of its value
 #pragma unroll
-          for (int i = 0; i < HW; ++i) kw[i] = vw[i] = 0u;
-          kn = 0.f;
-          vn = 1.f;
-        }
-      } else {
-        const uint8_t* k = a.k + p.blk * a.k_blk + p.pos * a.k_pos + kvh * a.k_head + 16 * h;
-        const uint8_t* v = a.v + p.blk * a.v_blk + p.pos * a.v_pos + kvh * a.v_head + 16 * h;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          kd[ks] = there ? *(const ck_u4*)(k + 32 * ks) : (ck_u4){0u, 0u, 0u, 0u};
-          vd[ks] = there ? *(const ck_u4*)(v + 32 * ks) : (ck_u4){0u, 0u, 0u, 0u};
-        }
-      }
-    };
-    request(at0, base0 + col < keys.hi);
-    ck_place_of next = ck_key(a, seq, base0 + P::N + col, steps > 1 && base0 + P::N + col < keys.hi);
-    unsigned char* vl = lds + wave * P::V_BYTES;
-    __syncthreads();               // (LDS of the tile before has been read)
-    for (int u = 0; u < steps; ++u) {
+    for (int dt = 0; dt < DT; ++dt) {
+      const int r = 4 * h + (lane & 15) / 4, c = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      v_at[dt] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)vl + r * 2 * D + 16 * (c ^ P::f(r)) + 8 * (lane & 1);
+    }
+    __syncthreads();               // (the area has been read)
+    auto unit_of = [&](int u, codes& w) {
       const int base = base0 + u * P::N;
       // ---- values to LDS, products of keys and rows
       ck_f16v sc[1];
       sc[0] = (ck_f16v)(0.f);
       if constexpr (PACKED) {
-        const uint32_t keep = vn < CK_TINY ? 0u : 0xffffffffu;
+        const uint32_t keep = w.vn < CK_TINY ? 0u : 0xffffffffu;
+        // look-ups of all keys, then of the values half at a time while the keys are multiplied
+        ck_u4 k[KS], v[KS / 2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          *(ck_u4*)(vl + col * P::PITCH + 16 * (KS * h + ks)) = lut.group(vw, ks) & keep;
-          sc[0] = M::mfma(ck_levels<BITS>(table, kw, ks), q[ks], sc[0]);
+        for (int ks = 0; ks < KS; ++ks) k[ks] = lut.group(w.k, ks);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) v[i] = lut.group(w.v, p * (KS / 2) + i);
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) {
+            const int ks = p * (KS / 2) + i;
+            if constexpr (P::Q_LDS) {
+              sc[0] = M::mfma(k[ks], q_lds[64 * (KS + ks)], sc[0]);
+              sc[0] = M::mfma(k[ks], q_lds[64 * ks], sc[0]);
+            } else {
+              sc[0] = M::mfma(k[ks], ql[ks], sc[0]);
+              sc[0] = M::mfma(k[ks], q[ks], sc[0]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) *(ck_u4*)(vl + col * 2 * D + 16 * ((KS * h + p * (KS / 2) + i) ^ P::f(col))) = v[i] & keep;
         }
         if (h == 0) {
-          const float v = vn < CK_TINY ? 1.f : vn;
-          nrm[wave][0][col] = kn * table.up;
+          const float v = w.vn < CK_TINY ? 1.f : w.vn;
+          nrm[wave][0][col] = w.kn * unit;
           nrm[wave][1][col] = __log2f(v);
           nrm[wave][2][col] = 1.f / v;
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          *(ck_u4*)(vl + col * P::PITCH + 16 * (2 * ks + h)) = vd[ks];
+          *(ck_u4*)(vl + col * 2 * D + 16 * ((2 * ks + h) ^ P::f(col))) = vd[ks];
           sc[0] = M::mfma(kd[ks], q[ks], sc[0]);
         }
       }
-      // ---- the next keys fly from here on
-      if (u + 1 < steps) {
-        request(next, base + P::N + col < keys.hi);
-        next = ck_key(a, seq, base + 2 * P::N + col, u + 2 < steps && base + 2 * P::N + col < keys.hi);
-      }
+      // ---- the next keys (packed: those two units on) fly from here on, and the entries of those behind them
+      constexpr int ON = PACKED ? 2 : 1;
+      if (u + ON < steps) request(u + ON, w);
       akv_wave_sync();
-      if (base < keys.hi) {
-        if (scaled) sc[0] *= fac;        // (a row far from the usual size)
-        if constexpr (PACKED) ck_norms(sc, nrm[wave][0], nrm[wave][1]);
-        if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
-        float alpha;
-        if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
+      // keys 16 kb + 8 e + 4 h .. + 3, coordinate 32 dt + lane % 32 (eight rows on, f differs in its bit 1)
+      auto value = [&](int kb, int dt, int e) {
+        return __builtin_bit_cast(ck_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)(uintptr_t)((v_at[dt] ^ (32u * e)) + (16 * kb + 8 * e) * 2 * D)));
+      };
+      constexpr bool V_AHEAD = D == 64;      // read while the weights are computed, as far as there are registers
+      ck_u2 vf[2][DT][2];
+      if constexpr (V_AHEAD) {
 #pragma unroll
-          for (int i = 0; i < DT; ++i) o[i] *= alpha;
-        }
-        ck_weights<1, PACKED>(sc, st, a.scale2, PACKED ? nrm[wave][2] : nullptr);
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          ck_u4 p;
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = M::pair(sc[0][8 * kb + 2 * i], sc[0][8 * kb + 2 * i + 1]);
+            for (int e = 0; e < 2; ++e) vf[kb][dt][e] = value(kb, dt, e);
+      }
+      if (scaled) sc[0] *= fac;        // (a row far from the usual size)
+      if constexpr (PACKED) ck_norms(sc, nrm[wave][0], nrm[wave][1]);
+      if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
+      float alpha;
+      if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            // keys 16 kb + 4 h .. + 3 and + 8, coordinate 32 dt + lane % 32
-            unsigned char* at_v = vl + (16 * kb + 4 * h + (lane & 15) / 4) * P::PITCH + 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-            const ck_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)at_v);
-            const ck_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ck_lds_s4*)(at_v + 8 * P::PITCH));
-            const ck_u2 xu = __builtin_bit_cast(ck_u2, x), yu = __builtin_bit_cast(ck_u2, y);
-            o[dt] = M::mfma((ck_u4){xu[0], xu[1], yu[0], yu[1]}, p, o[dt]);
-          }
+        for (int i = 0; i < DT; ++i) o[i] *= alpha;
+      }
+      ck_weights<1, PACKED>(sc, st, a.scale2, PACKED ? nrm[wave][2] : nullptr);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        ck_u4 p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = M::pair(sc[0][8 * kb + 2 * i], sc[0][8 * kb + 2 * i + 1]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const ck_u2 x = V_AHEAD ? vf[kb][dt][0] : value(kb, dt, 0), y = V_AHEAD ? vf[kb][dt][1] : value(kb, dt, 1);
+          o[dt] = M::mfma((ck_u4){x[0], x[1], y[0], y[1]}, p, o[dt]);
         }
       }
       akv_wave_sync();             // (the next values go where these are)
+    };
+    if constexpr (PACKED) {
+      for (int u = 0; u < steps; u += 2) {
+        unit_of(u, even);
+        if (u + 1 < steps) unit_of(u + 1, odd);
+      }
+    } else {
+      for (int u = 0; u < steps; ++u) unit_of(u, even);
     }
 
-    // ---- the four wavefronts' sums of the tile: wavefront w ends up with a quarter of the coordinates
+    // ---- the wavefronts' sums of the tile, each in the frame of all; a wavefront ends up with QW quads of the coordinates
     st.l += akv_lane_xor<32>(st.l);
     ml[wave][lane][0] = st.m;
     ml[wave][lane][1] = st.l;
     __syncthreads();
     float m = ml[0][lane][0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][lane][0]);
+    for (int w = 1; w < W; ++w) m = fmaxf(m, ml[w][lane][0]);
     const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) l += ml[w][lane][1] * ck_exp2(ml[w][lane][0] - ref);
-    const float mine = ck_exp2(st.m - ref);
-    float4* merge = (float4*)lds;
+    for (int w = 0; w < W; ++w) l += ml[w][lane][1] * ck_exp2(ml[w][lane][0] - ref);
+    const float mine = ck_exp2(st.m - ref) * unit;
+    float4* merge = (float4*)area;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt) o[dt] *= mine;
+    auto dump = [&](int w) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        merge[(wave * P::QUADS + 4 * dt + b) * 64 + lane] = make_float4(o[dt][4 * b] * mine, o[dt][4 * b + 1] * mine, o[dt][4 * b + 2] * mine, o[dt][4 * b + 3] * mine);
+      for (int c = 0; c < P::QUADS; ++c)
+        merge[(w * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)], o[c / 4][4 * (c & 3) + 1], o[c / 4][4 * (c & 3) + 2], o[c / 4][4 * (c & 3) + 3]);
+    };
+    if (P::LEFT < W) {
+      if (wave >= P::LEFT) dump(wave - P::LEFT);
+      __syncthreads();
+      if (wave < P::LEFT) {
+#pragma unroll
+        for (int c = 0; c < P::QUADS; ++c) {
+          const float4 y = merge[(wave * P::QUADS + c) * 64 + lane];
+          o[c / 4][4 * (c & 3)] += y.x; o[c / 4][4 * (c & 3) + 1] += y.y; o[c / 4][4 * (c & 3) + 2] += y.z; o[c / 4][4 * (c & 3) + 3] += y.w;
+        }
+      }
+      __syncthreads();
+    }
+    if (wave < P::LEFT) dump(wave);
     __syncthreads();
     const bool whole = u0 == 0 && u1 == keys.units;
-    const float f = ck_finish<KIND>(l, PACKED ? table.up : 1.f);
     const int64_t slot = 2 * (int64_t)g + (u0 == 0 ? 1 : 0);
+    float4 x[P::QW];
 #pragma unroll
-    for (int i = 0; i < P::QUADS / 4; ++i) {
-      const int cq = (P::QUADS / 4) * wave + i;
-      float4 x = merge[cq * 64 + lane];
+    for (int i = 0; i < P::QW; ++i) {
+      const int cq = P::QW * wave + i;
+      x[i] = merge[cq * 64 + lane];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) {
+      for (int w = 1; w < P::LEFT; ++w) {
         const float4 y = merge[(w * P::QUADS + cq) * 64 + lane];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
-      if (whole) {
-        if (row.valid) ck_store<D, KIND>(a, row.token, row.head, cq, x.x * f, x.y * f, x.z * f, x.w * f);
-      } else {
-        ((float4*)a.part)[(slot * P::QUADS + cq) * 64 + lane] = x;
+        x[i].x += y.x; x[i].y += y.y; x[i].z += y.z; x[i].w += y.w;
       }
     }
-    if (!whole && wave == 0) {
-      a.part_ml[slot * 64 + lane] = make_float2(m, l);
-      if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < P::QW; ++i) ((float4*)a.part)[(slot * P::QUADS + P::QW * wave + i) * 64 + lane] = x[i];
+      if (wave == 0) {
+        a.part_ml[slot * 64 + lane] = make_float2(m, l);
+        if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
+      }
+    } else {
+      ck_results<D, KIND, W, P::QW>(a, x, ck_finish(l), row.valid, row.token, row.head, (float*)area);
     }
     // ---- on to the next tile
     at = tile_at = tile_end;
@@ -555,8 +658,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void ck_narrow_kernel(ck_arg
     int n = s.n;
     while ((int64_t)tile * TM >= n) {
       tile = 0;
-      if (++seq > a.S) { seq = 0; ++head; }
-      n = ck_sequence(a, L, seq).n;
+      n = ck_sequence(a, L, ++seq).n;
     }
   }
 }
@@ -581,7 +683,7 @@ template <int D, int KIND> struct ck_wide {
   static constexpr int ROW = 2 * D, TILE = N * ROW;
   // Units of keys held: of those read during a unit, and the one that is written (a unit on with AHEAD, or where a unit is a step)
   static constexpr int KRING = AHEAD || STEPS == 1 ? 2 : 3;
-  static constexpr int UNROLL = CK_UNROLL;
+  static constexpr int UNROLL = KIND >= 2 ? 1 : STEPS;
   static constexpr int RING = 2 * WAVES;                              // units whose places and norms are held
   static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
   static constexpr int LDS = NORM0 + (KIND >= 2 ? RING * N * 16 : 0);
@@ -608,7 +710,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   static_assert(NT * T == 2 * TASKS && NP * RPI * P::WAVES == N, "whole tasks and requests");
   extern __shared__ __align__(1024) unsigned char lds[];
   __shared__ ck_lengths<T> L;
-  __shared__ ck_lut<BITS> lut;
+  __shared__ ck_lut<BITS, 1> lut;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
   const int G = gridDim.x;
@@ -630,9 +732,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 
   float unit = 1.f;                // of the levels
   if constexpr (PACKED) {
-    ck_table<BITS> table;
-    table.load(a.centroids);
-    unit = table.up;
+    unit = ck_unit<BITS>(a.centroids);
     lut.fill(a.centroids, tid, T, unit);
   }
   // where the lane reads its operands: a piece of a key, four coordinates of a value
@@ -668,26 +768,19 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     // values lie at is written a unit later.  Every wavefront does so for one unit of the next WAVES, all at the same time: one that did
     // it for the others would be what they wait for.  A key behind the last one has the last one's place: what is read for it is masked,
     // and its value is as finite as that one's.
-    struct entry { uint32_t lo, hi; };
-    const int wide_id = a.tables_it == AKV_I64;
     auto key_of = [&](int u) { return min(base0 + u * N + (lane & (N - 1)), keys.hi - 1); };
-    auto look = [&](int u) {
-      uint32_t rem;
-      const int64_t i = (int64_t)seq * a.bt_stride + akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, rem);
-      const uint32_t* p = (const uint32_t*)a.tables + (i << wide_id);
-      return entry{p[0], p[wide_id]};
-    };
+    auto look = [&](int u) { return ck_look(a, seq, key_of(u)); };
     float kn = 0.f, vn = 1.f;      // packed: norms of the unit noted last
-    auto note = [&](int u, const entry& e) {
-      uint32_t pos;
-      akv_div32((uint32_t)key_of(u), (uint32_t)a.block_size, a.bs_recip, pos);
-      const int64_t blk = akv_clamp_block(wide_id ? (int64_t)((uint64_t)e.hi << 32 | e.lo) : (int64_t)(int32_t)e.lo, a.num_blocks);
+    auto note = [&](int u, const ck_entry& e) {
+      const ck_place p = ck_place_of(a, key_of(u), e);
       int64_t* place = (int64_t*)(lds + P::PLACE0) + (u & (P::RING - 1)) * 2 * N;
-      place[lane & (N - 1)] = blk * a.k_blk + pos * a.k_pos + kvh * a.k_head;
-      place[N + (lane & (N - 1))] = blk * a.v_blk + pos * a.v_pos + kvh * a.v_head;
+      const int64_t k_at = ck_offset(p, a.k_blk, a.k_pos) + kvh * a.k_head;
+      place[lane & (N - 1)] = k_at;
+      place[N + (lane & (N - 1))] = a.kv_alike ? k_at : ck_offset(p, a.v_blk, a.v_pos) + kvh * a.v_head;
       if constexpr (PACKED) {
-        kn = a.kn[blk * a.kn_blk + pos * a.kn_pos + kvh * a.kn_head];
-        vn = a.vn[blk * a.vn_blk + pos * a.vn_pos + kvh * a.vn_head];
+        const int64_t n_at = ck_offset(p, a.kn_blk, a.kn_pos) + kvh * a.kn_head;
+        kn = a.kn[n_at];
+        vn = a.vn[a.kv_alike ? n_at : ck_offset(p, a.vn_blk, a.vn_pos) + kvh * a.vn_head];
       }
     };
     auto note_norms = [&](int u) {
@@ -742,7 +835,16 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         uint32_t keep = 0xffffffffu;
         if (v) keep = ((const uint32_t*)(lds + P::NORM0))[(uv & (P::RING - 1)) * 4 * N + 3 * N + r];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *(ck_u4*)(to + 16 * ((4 * part + j) ^ f)) = lut.group(words[i], j) & keep;
+        for (int j = 0; j < 4; j += 2) {
+          ck_u4 x = lut.group(words[i], j), y = lut.group(words[i], j + 1);
+          if (!v) {                // keys: the order of the turned rows
+            const ck_u4 z = x;
+            x = (ck_u4){z[0], z[1], y[0], y[1]};
+            y = (ck_u4){z[2], z[3], y[2], y[3]};
+          }
+          *(ck_u4*)(to + 16 * ((4 * part + j) ^ f)) = x & keep;
+          *(ck_u4*)(to + 16 * ((4 * part + j + 1) ^ f)) = y & keep;
+        }
       }
     };
 
@@ -753,7 +855,25 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       const uint16_t* p = (const uint16_t*)a.q + (int64_t)row.token * a.qs_tok + (int64_t)row.head * a.qs_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) q[ks] = row.valid ? *(const ck_u4*)(p + 8 * (2 * ks + h)) : (ck_u4){0u, 0u, 0u, 0u};
-      if constexpr (PACKED) fac = row.valid ? a.qfac[(int64_t)row.token * a.QH + row.head] : 1.f;
+    };
+    // packed: turned, by the lane's own products: the coordinates of a step come out as 4 h .. + 3 and 8 + 4 h .. + 3 of sixteen, the
+    // order that keys are put to LDS in
+    auto turn_rows = [&]() {
+      const float un = ck_query_operand<D>(q, a.dtype) * a.turn_scale->up * (1.f / CK_TURN) * a.scale2;
+      ck_f16v y[DT];
+      float m = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        y[dt] = ck_turn<D>(a.turn_in, dt, q);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(y[dt][i]));
+      }
+      m = fmaxf(m, akv_lane_xor<32>(m));
+      const float f = ck_query_scale(m, un, fac);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[ks][i] = M::pair(y[ks / 2][8 * (ks & 1) + 2 * i] * f, y[ks / 2][8 * (ks & 1) + 2 * i + 1] * f);
     };
     __syncthreads();               // (LDS of the tile before has been read)
     if (units > 0) {
@@ -765,6 +885,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         rows();
         put(0, 0);
         fetch(1, 0);
+        turn_rows();
         put(1, 0);
       } else {
         request(0, 0, true, 0, true);
@@ -774,6 +895,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       }
     } else {
       rows();
+      fac = 1.f;
     }
     // (the rows are there: without a use here the compiler waits for them in the loop, and so for what flies then)
 #pragma unroll
@@ -801,7 +923,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha);      // (nothing to rescale yet)
     }
     int k_slot = 0;                // of unit u
-    entry ahead = {0u, 0u};
+    ck_entry ahead = {0u, 0u};
     for (int u = 0; u < units; ++u) {
       // ---- on their way: places of the WAVES units behind the WAVES that this one belongs to, keys of u + 2, values of u + 1
       const int turn = u & (P::WAVES - 1);
@@ -890,18 +1012,30 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 
     st.l += akv_lane_xor<32>(st.l);
     const bool whole = u0 == 0 && u1 == keys.units;
-    if (whole) {
-      const float f = ck_finish<KIND>(st.l, unit);
+    if (whole && PACKED) {
+      const float f = ck_finish(st.l) * unit;
+      ck_u4 hi[KS], lo[KS];
+      const float un = ck_result_operand<D>([&](int ks, int j) { return o[ks / 2][8 * (ks & 1) + j] * f; }, hi, lo) * a.turn_scale->up * (1.f / CK_TURN);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const ck_f16v y = ck_turn<D>(a.turn_out, dt, hi, lo);
+        if (row.valid) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) ck_store<KIND>(a, row.token, row.head, 4 * dt + b, y[4 * b] * un, y[4 * b + 1] * un, y[4 * b + 2] * un, y[4 * b + 3] * un);
+        }
+      }
+    } else if (whole) {
+      const float f = ck_finish(st.l);
       if (row.valid) {
 #pragma unroll
         for (int c = 0; c < P::QUADS; ++c)
-          ck_store<D, KIND>(a, row.token, row.head, c, o[c / 4][4 * (c & 3)] * f, o[c / 4][4 * (c & 3) + 1] * f, o[c / 4][4 * (c & 3) + 2] * f, o[c / 4][4 * (c & 3) + 3] * f);
+          ck_store<KIND>(a, row.token, row.head, c, o[c / 4][4 * (c & 3)] * f, o[c / 4][4 * (c & 3) + 1] * f, o[c / 4][4 * (c & 3) + 2] * f, o[c / 4][4 * (c & 3) + 3] * f);
       }
     } else {
       const int64_t slot = (2 * (int64_t)g + (u0 == 0 ? 1 : 0)) * P::WAVES + wave;
 #pragma unroll
       for (int c = 0; c < P::QUADS; ++c)
-        ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)], o[c / 4][4 * (c & 3) + 1], o[c / 4][4 * (c & 3) + 2], o[c / 4][4 * (c & 3) + 3]);
+        ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)] * unit, o[c / 4][4 * (c & 3) + 1] * unit, o[c / 4][4 * (c & 3) + 2] * unit, o[c / 4][4 * (c & 3) + 3] * unit);
       a.part_ml[slot * 64 + lane] = make_float2(st.m, st.l);
       if (u0 == 0 && tid == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
     }
@@ -918,52 +1052,55 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 }
 
 // ---- the pieces of a tile that several ranges share --------------------------------------------------------------------------
-// Workgroup (g, w): the 32 rows w of the tile that begins in range g and does not end there; its other pieces are the first ones of the
-// ranges behind.
+// Workgroup (g, w): the 32 rows w of the tile that begins in workgroup g's range and does not end there; its other pieces are the first ones
+// of the ranges behind, which are `stride` workgroups apart.  Their maxima are looked through first, so that the sums of up to four pieces are on their way together.
 template <int D, int KIND, int WAVES>
-__global__ __launch_bounds__(256) void ck_merge_kernel(ck_args a, int G) {
+__global__ __launch_bounds__(256) void ck_merge_kernel(ck_args a, int G, int stride) {
   constexpr int QUADS = D / 8, MINE = QUADS / 4;
+  __shared__ __align__(16) float rows[ck_math<KIND>::packed ? 32 * (D + 4) : 1];
   const int g = blockIdx.x, part = blockIdx.y;
   const ck_record rec = a.rec[g];
   if (!rec.valid) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
+  // ranges first + 1 .. last hold a piece each, unless they are empty
+  const int R = G / stride, first = g / stride;
+  int last = first;
+  while (last + 1 < R && ck_begin(rec.total, last + 1, R) < rec.end) ++last;
+  auto slot_of = [&](int r) { return (2 * (int64_t)(r * stride + g % stride) + (r == first ? 1 : 0)) * WAVES + part; };
+  auto held = [&](int r) { return r == first || ck_begin(rec.total, r, R) < ck_begin(rec.total, r + 1, R); };
   float m = -INFINITY, l = 0.f;
+  for (int r = first; r <= last; ++r) m = fmaxf(m, held(r) ? a.part_ml[slot_of(r) * 64 + lane].x : -INFINITY);
+  const float ref = m == -INFINITY ? 0.f : m;
   float4 x[MINE];
 #pragma unroll
   for (int i = 0; i < MINE; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int64_t slot) {
-    const float2 e = a.part_ml[(slot * WAVES + part) * 64 + lane];
-    const float mn = fmaxf(m, e.x), ref = mn == -INFINITY ? 0.f : mn;
-    const float f0 = ck_exp2(m - ref), f1 = ck_exp2(e.x - ref);
-    l = l * f0 + e.y * f1;
-    m = mn;
+  for (int r = first; r <= last; r += 4) {
+    float2 e[4];
+    float4 y[4][MINE];
 #pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-      const float4 y = ((const float4*)a.part)[((slot * WAVES + part) * QUADS + MINE * wave + i) * 64 + lane];
-      x[i].x = x[i].x * f0 + y.x * f1; x[i].y = x[i].y * f0 + y.y * f1;
-      x[i].z = x[i].z * f0 + y.z * f1; x[i].w = x[i].w * f0 + y.w * f1;
+    for (int k = 0; k < 4; ++k) {
+      const bool there = r + k <= last && held(r + k);
+      const int64_t slot = slot_of(there ? r + k : first);
+      e[k] = a.part_ml[slot * 64 + lane];
+      if (!there) e[k].x = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) y[k][i] = ((const float4*)a.part)[(slot * QUADS + MINE * wave + i) * 64 + lane];
     }
-  };
-  add(2 * (int64_t)g + 1);
-  for (int r = g + 1; r < G; ++r) {
-    const int64_t b = ck_begin(rec.total, r, G), e = ck_begin(rec.total, r + 1, G);
-    if (b >= rec.end) break;
-    if (b < e) add(2 * (int64_t)r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!(r + k <= last && held(r + k))) continue;
+      const float f = ck_exp2(e[k].x - ref);
+      l = fmaf(e[k].y, f, l);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        x[i].x = fmaf(y[k][i].x, f, x[i].x); x[i].y = fmaf(y[k][i].y, f, x[i].y);
+        x[i].z = fmaf(y[k][i].z, f, x[i].z); x[i].w = fmaf(y[k][i].w, f, x[i].w);
+      }
+    }
   }
   const int row = 32 * part + col, j = row / a.GC, gq = (rec.head % a.HS) * a.GC + row - j * a.GC;
-  if (j >= rec.tokens || gq >= a.G) return;
-  float unit = 1.f;
-  if constexpr (ck_math<KIND>::packed) {
-    ck_table<KIND> t;
-    t.load(a.centroids);
-    unit = t.up;
-  }
-  const float f = ck_finish<KIND>(l, unit);
-#pragma unroll
-  for (int i = 0; i < MINE; ++i)
-    ck_store<D, KIND>(a, rec.token + j, (rec.head / a.HS) * a.G + gq, MINE * wave + i, x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f);
+  ck_results<D, KIND, 4, MINE>(a, x, ck_finish(l), j < rec.tokens && gq < a.G, rec.token + j, (rec.head / a.HS) * a.G + gq, rows);
 }
-
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
 // Scratch of the main kernels: a record a workgroup, and the pieces of two tiles (the sums of 32 rows, QUADS x 64 x 16 bytes, and their
@@ -972,12 +1109,13 @@ static inline int ck_groups(int per_cu) {
   const int cus = akv_cached_cu_count();
   return (cus > 0 ? cus : 256) * per_cu;
 }
+#define CK_GROUPS 4096            // workgroups of a launch at most
 struct ck_scratch { size_t rec, ml, part, bytes; };
 static inline ck_scratch ck_scratch_layout(int D) {
-  const size_t g = (size_t)ck_groups(2), slots = 2 * (size_t)ck_groups(2) * 8;
+  const size_t wide = 2 * (size_t)ck_groups(1) * 8, slots = wide > 2 * CK_GROUPS ? wide : 2 * CK_GROUPS;      // (either kernel's)
   ck_scratch w;
   w.rec = 0;
-  w.ml = akv_align256(g * sizeof(ck_record));
+  w.ml = akv_align256(CK_GROUPS * sizeof(ck_record));
   w.part = w.ml + akv_align256(slots * 64 * sizeof(float2));
   w.bytes = w.part + slots * (size_t)(D / 8) * 64 * 16;
   return w;
@@ -995,15 +1133,25 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
   // each takes its own, by the lengths on the device.
   const int64_t most = most_new > 0 && most_new < a.T ? most_new : a.T;
   const bool few = most * a.G <= CK_NARROW_ROWS, one = !few && a.S == 1;
+  int dev = 0;
+  AKV_HIP(hipGetDevice(&dev));
   if (!one) {
     ck_args n = a;
     n.kind = few ? 0 : 1;
     n.HS = (a.G + 31) / 32;
     n.GC = (a.G + n.HS - 1) / n.HS;
-    const int G = ck_groups(D == 256 ? 1 : 2);
-    ck_narrow_kernel<D, KIND><<<G, 256, 0, stream>>>(n);
+    typedef ck_narrow<D, KIND> P;
+    static akv_device_once once;
+    const int rc = once(dev, [&]() -> int {
+      AKV_HIP(hipFuncSetAttribute((const void*)ck_narrow_kernel<D, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
+      return AKV_OK;
+    });
+    if (rc) return rc;
+    const int heads = n.KVH * n.HS, ranges = ck_groups(P::PER_CU) / heads, G = heads * (ranges > 1 ? ranges : 1);
+    if (G > CK_GROUPS) return akv_fail(AKV_ERR_UNSUPPORTED, "more than %d kv heads", CK_GROUPS);
+    ck_narrow_kernel<D, KIND><<<G, P::THREADS, P::LDS, stream>>>(n);
     AKV_LAUNCH_CHECK("ck_narrow_kernel");
-    ck_merge_kernel<D, KIND, 1><<<dim3(G, 1), 256, 0, stream>>>(n, G);
+    ck_merge_kernel<D, KIND, 1><<<dim3(G, 1), 256, 0, stream>>>(n, G, heads);
     AKV_LAUNCH_CHECK("ck_merge_kernel");
   }
   if (!few) {
@@ -1012,8 +1160,6 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
     n.HS = (a.G + W::ROWS - 1) / W::ROWS;
     n.GC = (a.G + n.HS - 1) / n.HS;
     static akv_device_once once;
-    int dev = 0;
-    AKV_HIP(hipGetDevice(&dev));
     const int rc = once(dev, [&]() -> int {
       AKV_HIP(hipFuncSetAttribute((const void*)ck_wide_kernel<D, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, W::LDS));
       return AKV_OK;
@@ -1022,7 +1168,7 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
     const int G = ck_groups(W::PER_CU);
     ck_wide_kernel<D, KIND><<<G, W::THREADS, W::LDS, stream>>>(n);
     AKV_LAUNCH_CHECK("ck_wide_kernel");
-    ck_merge_kernel<D, KIND, W::WAVES><<<dim3(G, W::WAVES), 256, 0, stream>>>(n, G);
+    ck_merge_kernel<D, KIND, W::WAVES><<<dim3(G, W::WAVES), 256, 0, stream>>>(n, G, 1);
     AKV_LAUNCH_CHECK("ck_merge_kernel");
   }
   return AKV_OK;
@@ -1043,6 +1189,7 @@ static inline int ck_check_batch(const char* name, const void* query, int dtype,
   AKV_REQUIRE(S == 0 || max_blocks == 0 || num_blocks == 0 || tables, "%s: null pointer", name);
   if (dtype == AKV_F32) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: float32 queries are not supported; use float16 or bfloat16", name);
   if (D != 64 && D != 128 && D != 256) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: head_dim %d; kernels are built for 64, 128 and 256", name, D);
+  if (num_blocks > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^31 blocks", name);
   if (T > 0x3fffffff || S > 0x3fffffff || T * (int64_t)QH > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^31 rows", name);
   return AKV_OK;
 }

@@ -1,79 +1,102 @@
-// Rotations of a chunk's queries and outputs for attention over packed rows.
+// Rotations of a chunk's rows inside the kernels that attend: queries on the way in, results on the way out.
+//
+//   Y^T[n, row] = sum_k M[n, k] X[row, k]            v_mfma_f32_32x32x16_f16, A = 32 rows of the matrix, B = 32 rows of X
+//
+// The matrix (Pi for queries, Pi^T for results) is prepared as two float16 terms of its entries times 1024 (22 bits), in the order of
+// the operand: [hi, lo][n / 32][k / 16][64 lanes] sixteen bytes.  float16 queries are operands as they are; bfloat16 ones are scaled by
+// a power of two a row, which keeps what lies within 2^14 of the largest exact.  Results are scaled alike and split into two terms.
+// Per tile of 32 rows a rotation takes 2 (3 for results) x 32 products at head_dim 128, some 1 (1.5) us of a wavefront; kernels of their own
+// before and after took 6 + 6 us for small calls and 39 + 51 us for 65,000 rows, and the float32 rows between them.
 #pragma once
-#include "akv_chunk_kernels.h"
-#include "akv_attn_rows.h"
+#include "akv_chunk.h"
 
-// ---- packed: rotations of queries and outputs ---------------------------------------------------------------------------------
-// Rows of `in` (any strides) times the matrix, 16 rows a step; workgroup (b, slice): 64 outputs.  QUERY: to float16, times the scale of the
-// scores and log2 e; `fac` is what a row has to be multiplied with still, 1 unless its largest coordinate is far from 1 (then the row
-// is stored with that between 2^5 and 2^6).
-template <int D, int XDT, bool QUERY, int ODT>
-__global__ __launch_bounds__(256) void ck_rotate_kernel(const void* __restrict__ in, int64_t is_tok, int64_t is_head, int64_t rows, int QH,
-                                                        const float* __restrict__ matrix, const akv_prep_scale* __restrict__ scale,
-                                                        void* __restrict__ out, int64_t os_tok, int64_t os_head, float* __restrict__ fac, float qscale,
-                                                        const void* __restrict__ starts, int starts_it, int S, int tail) {
-  constexpr int TERMS = ar_terms<XDT>(), EPT = D / 16;
-  __shared__ ar_rows<D, TERMS> r;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slice = blockIdx.y, n0 = 64 * slice + 16 * wave;
-  const int row = tid >> 4, part = tid & 15;
-  ar_matrix<D> m;
-  m.load(matrix + (size_t)n0 * D, AR_M_SCALE * scale->down);
-  const float up = scale->up;
-  int64_t limit = rows;                 // rows behind the last sequence are left as they were
-  if (!QUERY && !tail) {
-    const int64_t last = akv_load_index(starts, starts_it, S) * QH;
-    limit = last < 0 ? 0 : last < rows ? last : rows;
+#define CK_TURN 1024.f
+// k of element j of a lane of half h in a step of sixteen: queries 8 h + j; results in the order in which the second product of attention
+// leaves them, 4 h + j and 8 + 4 h + j - 4
+__host__ __device__ constexpr int ck_result_k(int h, int j) { return 4 * h + (j & 3) + 8 * (j >> 2); }
+// (a pointer the compiler knows nothing of: it would keep the whole table in registers from one tile for the next)
+__device__ __forceinline__ const uint4* ck_turn_table(const uint4* table) {
+  asm volatile("" : "+s"(table));
+  return table;
+}
+__device__ __forceinline__ const uint4* ck_turn_at(const uint4* table, int D, int term, int dt, int ks) {
+  return table + (((size_t)term * (D / 32) + dt) * (D / 16) + ks) * 64 + (threadIdx.x & 63);
+}
+// Rows dt of M times rows held as operands: one term (queries) ...
+template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restrict__ all, int dt, const ck_u4 (&x)[D / 16]) {
+  const uint4* table = ck_turn_table(all);
+  ck_f16v y = (ck_f16v)(0.f);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const ck_u4 lo = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 1, dt, ks)), hi = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 0, dt, ks));
+    y = ck_math<CK_F16>::mfma(lo, x[ks], y);
+    y = ck_math<CK_F16>::mfma(hi, x[ks], y);
+    if ((ks & 3) == 3) __builtin_amdgcn_sched_barrier(0);      // (no more of the table than this in registers)
   }
-  for (int64_t tile = blockIdx.x; tile * 16 < rows; tile += gridDim.x) {
-    const int64_t n = tile * 16 + row;
-    float x[EPT];
-    const int64_t tok = n / QH, at = tok * is_tok + (n - tok * QH) * is_head;
-    float mx = 0.f;
+  return y;
+}
+// ... or two (results)
+template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restrict__ all, int dt, const ck_u4 (&x)[D / 16], const ck_u4 (&xl)[D / 16]) {
+  const uint4* table = ck_turn_table(all);
+  ck_f16v y = (ck_f16v)(0.f);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      x[i] = n < rows ? akv_elem<XDT>::load(in, at + 64 * (i >> 2) + 4 * part + (i & 3)) : 0.f;
-      mx = fmaxf(mx, fabsf(x[i]));
-    }
-    mx = fmaxf(mx, akv_lane_xor<1>(mx)); mx = fmaxf(mx, akv_lane_xor<2>(mx));
-    mx = fmaxf(mx, akv_lane_xor<4>(mx)); mx = fmaxf(mx, akv_lane_xor<8>(mx));
-    float un;
-    const float sc = ar_scale(mx, un);
-    un *= up;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      float v = x[i] * sc;
-      const int d = 64 * (i >> 2) + 4 * part + (i & 3);
-#pragma unroll
-      for (int j = 0; j < TERMS; ++j) {
-        const _Float16 t = (_Float16)(j == 2 ? v * AR_THIRD : v);
-        r.term[j][row][d] = t;
-        v -= (float)t;
-      }
-    }
-    if (part == 0) {
-      // queries: the usual sizes go as they are (the factor is in the row), the others scaled
-      const bool usual = mx * qscale >= 0x1p-8f && mx * qscale <= 0x1p8f;
-      r.unscale[row] = !QUERY ? un : usual ? un * qscale : 1.f / AR_M_SCALE;
-      if (QUERY && slice == 0 && n < rows) fac[n] = usual ? 1.f : un * AR_M_SCALE * qscale;
-    }
-    __syncthreads();
-    const ar_float4 y = m.times(r);
-    const int rr = lane & 15, d0 = n0 + 4 * (lane >> 4);
-    const int64_t no = tile * 16 + rr;
-    if (no < limit) {
-      if constexpr (QUERY) {
-        const float f = r.unscale[rr];
-        ck_u2 v;
-        v[0] = ck_math<CK_F16>::pair(y[0] * f, y[1] * f);
-        v[1] = ck_math<CK_F16>::pair(y[2] * f, y[3] * f);
-        *(ck_u2*)((uint16_t*)out + no * D + d0) = v;
-      } else {
-        const float f = r.unscale[rr];
-        const int64_t t = no / QH, o = t * os_tok + (no - t * QH) * os_head + d0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) akv_elem<ODT>::store(out, o + e, y[e] * f);
-      }
-    }
-    __syncthreads();
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const ck_u4 lo = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 1, dt, ks)), hi = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 0, dt, ks));
+    y = ck_math<CK_F16>::mfma(lo, x[ks], y);
+    y = ck_math<CK_F16>::mfma(hi, xl[ks], y);
+    y = ck_math<CK_F16>::mfma(hi, x[ks], y);
+    if ((ks & 3) == 3) __builtin_amdgcn_sched_barrier(0);
   }
+  return y;
+}
+// A row of queries (this lane's half of every sixteen coordinates) as operand; returns what undoes its scale.
+template <int D> __device__ __forceinline__ float ck_query_operand(ck_u4 (&x)[D / 16], int dtype) {
+  if (dtype == AKV_F16) return 1.f;
+  uint32_t m = 0u;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max((x[ks][i] << 16) & 0x7fff0000u, x[ks][i] & 0x7fff0000u));
+  m = max(m, akv_lane_xor_u32<32>(m));
+  const uint32_t e = akv_row_exponent(__uint_as_float(m));
+  const float sc = akv_row_scale(e);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[ks][i] = ck_math<CK_F16>::pair(__uint_as_float(x[ks][i] << 16) * sc, __uint_as_float(x[ks][i] & 0xffff0000u) * sc);
+  return akv_row_unscale(e);
+}
+// Scale of turned queries, by the row's largest: the usual sizes go as they are, times `f`, and need no factor later; others are brought to
+// [1, 2), and `later` is what their scores are multiplied with.
+__device__ __forceinline__ float ck_query_scale(float largest, float f, float& later) {
+  const float m = largest * f;
+  if (m >= 0x1p-8f && m <= 0x1p12f) {
+    later = 1.f;
+    return f;
+  }
+  const uint32_t e = akv_row_exponent(largest);
+  later = akv_row_unscale(e) * f;
+  return akv_row_scale(e);
+}
+// results of a row, times `f`, as two operands; returns what undoes their scale
+template <int D, class Get> __device__ __forceinline__ float ck_result_operand(Get get, ck_u4 (&hi)[D / 16], ck_u4 (&lo)[D / 16]) {
+  float m = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(get(ks, j)));
+  m = fmaxf(m, akv_lane_xor<32>(m));
+  const uint32_t e = akv_row_exponent(m);
+  const float sc = akv_row_scale(e);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = get(ks, 2 * i) * sc, y = get(ks, 2 * i + 1) * sc;
+      hi[ks][i] = ck_math<CK_F16>::pair(x, y);
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      const h2 h = __builtin_bit_cast(h2, (uint32_t)hi[ks][i]);
+      lo[ks][i] = ck_math<CK_F16>::pair(x - (float)h[0], y - (float)h[1]);
+    }
+  return akv_row_unscale(e);
 }

@@ -149,6 +149,7 @@ __global__ __launch_bounds__(1024) void akv_prepare_scale_kernel(const float4* _
 
 int akv_prepare_rotation_mfma(const float* rotation, int d, void* prep, hipStream_t stream);
 int akv_prepare_decode_mfma(const float* rotation, int d, void* prep, hipStream_t stream);
+int akv_prepare_chunk(int d, void* prep, hipStream_t stream);  // defined in akv_chunk_packed.hip
 int akv_prepare_decode_slices(const float* rotation, int d, void* prep, hipStream_t stream);
 int akv_decode_mfma_try(const akv_gen_args& a, bool blocks, int d, int bits, int out_dtype, const void* rot_prep,
                         hipStream_t stream);
@@ -174,7 +175,8 @@ extern "C" int akv_rotation_prepare(const float* rotation, int d, void* prep, si
     rc = akv_prepare_decode_mfma(rotation, d, prep, (hipStream_t)stream);
     if (rc) return rc;
   }
-  return akv_prepare_decode_slices(rotation, d, prep, (hipStream_t)stream);
+  const int rc = akv_prepare_decode_slices(rotation, d, prep, (hipStream_t)stream);
+  return rc ? rc : akv_prepare_chunk(d, prep, (hipStream_t)stream);
 }
 
 // ----------------------------------------------------------------------------------

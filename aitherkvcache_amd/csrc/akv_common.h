@@ -86,7 +86,8 @@ void akv_profile_stamp(hipStream_t s, hipEvent_t begin);
 //   [2*d*d, ...)    d = 128 only: float16 hi/lo operand tiles of the MFMA encode kernel (64 KB),
 //                   a flag word (256 B reserved), the same for the rotations of the attention kernels (64 KB)
 //   then            d = 64, 128, 256: float16 hi/lo slices of Pi^T, the operand of the MFMA decode kernel (4 d*d bytes),
-//                   and an akv_prep_scale
+//                   and an akv_prep_scale; then the same two terms of Pi and of Pi^T (8 d*d bytes) in the order in which the kernels of a
+//                   chunk's attention read them (akv_chunk_rotate.h)
 #define AKV_PREP_DECODE_OFFSET(d) ((size_t)2 * (d) * (d) * 4 + 65536 + 256)
 #define AKV_PREP_SLICES_OFFSET(d) ((size_t)2 * (d) * (d) * 4 + ((d) == 128 ? 2 * 65536 + 256 : 0))
 #define AKV_PREP_SCALE_OFFSET(d) (AKV_PREP_SLICES_OFFSET(d) + ((d) == 512 ? 0 : (size_t)4 * (d) * (d)))
@@ -96,8 +97,9 @@ struct akv_prep_scale {
   float down, up;      // 2^-k, 2^k
   int k;
 };
+#define AKV_PREP_CHUNK_OFFSET(d) ((AKV_PREP_SCALE_OFFSET(d) + sizeof(akv_prep_scale) + 255) & ~(size_t)255)
 static inline size_t akv_prep_floats(int d) {
-  const size_t reserved = (size_t)4 * d * d + 1024, used = (AKV_PREP_SCALE_OFFSET(d) + sizeof(akv_prep_scale) + 3) / 4;
+  const size_t reserved = (size_t)4 * d * d + 1024, used = (AKV_PREP_CHUNK_OFFSET(d) + (d == 512 ? 0 : (size_t)8 * d * d)) / 4;
   return reserved > used ? reserved : used;
 }
 

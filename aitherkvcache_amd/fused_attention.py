@@ -193,7 +193,7 @@ class TQPagedAttention:
             _check_out("out", out, query)
         result = out if out is not None else torch.empty((num_tokens, num_q_heads, d), dtype=query.dtype, device=dev)
         L = _lib.lib()
-        ws = torch.empty(L.akv_paged_chunk_attn_workspace_bytes(num_tokens, num_q_heads, d), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.akv_paged_chunk_attn_workspace_bytes(d), dtype=torch.uint8, device=dev)
         blocks = min(k_packed.shape[0], k_norms.shape[0], v_packed.shape[0], v_norms.shape[0])
         with _lib.on_device(dev):
             _lib.check(L.akv_paged_chunk_attn(

@@ -284,7 +284,7 @@ int akv_dense_chunk_attn(const void* query, int dtype, int64_t qs_tok, int64_t q
                          int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d,
                          int block_size, int64_t num_blocks, int64_t max_blocks_per_seq, int window,
                          int max_query_len, float scale, void* workspace, size_t workspace_bytes, void* stream);
-size_t akv_paged_chunk_attn_workspace_bytes(int64_t num_tokens, int num_q_heads, int d);
+size_t akv_paged_chunk_attn_workspace_bytes(int d);
 int akv_paged_chunk_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
                          const uint8_t* k_packed, int64_t kps_blk, int64_t kps_pos, int64_t kps_head,
                          const float* k_norms, int64_t kns_blk, int64_t kns_pos, int64_t kns_head,
