@@ -129,7 +129,9 @@ _lib: Optional[C.CDLL] = None
 _calls = None          # the binding of the hot calls (csrc/akv_binding.cpp), once the library is loaded
 _BOUND = ("akv_paged_attn_workspace_bytes", "akv_paged_attn", "akv_encode_paged_kv", "akv_hybrid_paged_attn_workspace_bytes",
           "akv_hybrid_paged_attn", "akv_hybrid25_paged_attn", "akv_hybrid_encode_paged_kv", "akv_hybrid25_encode_paged_kv",
-          "akv_decode_blocks_kv", "akv_tri_encode_paged_kv", "akv_tri_decode_workspace_bytes", "akv_tri_decode_paged")
+          "akv_decode_blocks_kv", "akv_tri_encode_paged_kv", "akv_tri_decode_workspace_bytes", "akv_tri_decode_paged",
+          "akv_rope_append", "akv_dense_chunk_attn_workspace_bytes", "akv_dense_chunk_attn", "akv_paged_chunk_attn_workspace_bytes",
+          "akv_paged_chunk_attn")
 
 
 def available() -> bool:
@@ -202,7 +204,7 @@ def calls():
         if not available():
             return _NoBinding()
         lib()
-    return _calls
+    return _NoBinding() if _calls is None else _calls
 
 
 class AkvError(RuntimeError):

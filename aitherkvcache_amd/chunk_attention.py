@@ -29,6 +29,13 @@ def _check_out(name: str, out: torch.Tensor, like: torch.Tensor) -> None:
         raise ValueError(f"{name} must be {like.dtype} of shape {tuple(like.shape)}, got {out.dtype} {tuple(out.shape)}")
 
 
+_INT_MAX = (1 << 31) - 1
+
+
+def _longest(max_query_len: Optional[int]) -> int:
+    return 0 if max_query_len is None else max(0, min(max_query_len, _INT_MAX))
+
+
 def check_query(query: torch.Tensor) -> None:
     if query.dim() != 3:
         raise ValueError(f"query must be [tokens, heads, head_dim], got shape {tuple(query.shape)}")
@@ -70,6 +77,10 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result does not
 
     Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256."""
+    result = _lib.calls().dense_chunk(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, scale, window, out,
+                                      max_query_len)
+    if result is not None:
+        return result if type(result) is not int else _lib.check(result)
     check_query(query)
     _check_rows("key_cache", key_cache, 4)
     _check_rows("value_cache", value_cache, 4)
@@ -93,8 +104,8 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
             value_cache.data_ptr(), value_cache.stride(0), value_cache.stride(1), value_cache.stride(2),
             bt.data_ptr(), _lib.itype_code(bt), bt.stride(0), lens.data_ptr(), _lib.itype_code(lens), starts.data_ptr(), _lib.itype_code(starts),
             result.data_ptr(), result.stride(0), result.stride(1), int(out is None),
-            num_seqs, num_tokens, num_q_heads, kv_heads, d, block_size, min(blocks, value_cache.shape[0]), bt.shape[1], window,
-            max_query_len or 0, 1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
+            num_seqs, num_tokens, num_q_heads, kv_heads, d, block_size, min(blocks, value_cache.shape[0]), bt.shape[1], min(window, _INT_MAX),
+            _longest(max_query_len), 1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
     return result
 
 
@@ -115,6 +126,10 @@ def rope_append(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.T
 
     Returns the rotated queries (None without queries).  Arithmetic in float32, one rounding to the type stored.  Positions
     outside the table are clamped into it.  head_dim and rotary_dim are multiples of 16."""
+    result = _lib.calls().rope_append(query, key, value, positions, cos_sin, slot_mapping, key_cache, value_cache, sections, interleaved,
+                                      query_out)
+    if result is not None:
+        return result if type(result) is not int else _lib.check(result)
     for name, t, dims in (("key", key, 3), ("value", value, 3), ("key_cache", key_cache, 4), ("value_cache", value_cache, 4)):
         if t.dim() != dims:
             raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")

@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
@@ -30,9 +31,14 @@ struct Library {
   decltype(&akv_tri_encode_paged_kv) tri_encode;
   decltype(&akv_tri_decode_workspace_bytes) tri_bytes;
   decltype(&akv_tri_decode_paged) tri_decode;
+  decltype(&akv_rope_append) rope_append;
+  decltype(&akv_dense_chunk_attn_workspace_bytes) dense_chunk_bytes;
+  decltype(&akv_dense_chunk_attn) dense_chunk;
+  decltype(&akv_paged_chunk_attn_workspace_bytes) paged_chunk_bytes;
+  decltype(&akv_paged_chunk_attn) paged_chunk;
 } g_lib;
 static_assert(std::is_same_v<decltype(&akv_hybrid_paged_attn), decltype(&akv_hybrid25_paged_attn)> && std::is_same_v<decltype(&akv_hybrid_encode_paged_kv), decltype(&akv_hybrid25_encode_paged_kv)>);
-constexpr int kFunctions = 12;
+constexpr int kFunctions = 17;
 PyObject* g_raw_stream = nullptr;      // torch's function: handle of the current stream of a device
 
 // the tensors of a call; ok() once all of them are plain device tensors of one device
@@ -321,6 +327,140 @@ PyObject* spectral_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return rc ? status(rc) : THPVariable_Wrap(std::move(out));
 }
 
+// ---- a chunk of new tokens: the three calls run on the current device only (on another one: the long way, which changes to it)
+bool here(const Tensors& ts) { return ts.ok() && c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index() == ts.device(); }
+bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+bool fits_int(int64_t v) { return v >= 0 && v <= INT_MAX; }
+// a cache [blocks, positions, heads, d] of t's type with contiguous rows
+bool dense_rows(const at::Tensor& t, at::ScalarType type) { return t.dim() == 4 && t.scalar_type() == type && t.stride(3) == 1; }
+
+// queries, tables, lengths and starts of a chunk as the kernels take them
+bool chunk_inputs(const at::Tensor& q, const at::Tensor& bt, const at::Tensor& cl, const at::Tensor& qs) {
+  if (q.dim() != 3 || !half_type(q) || q.size(0) == 0 || q.size(1) == 0 || q.stride(2) != 1 || (uintptr_t)q.const_data_ptr() % 16 || q.stride(0) % 8 || q.stride(1) % 8) return false;
+  if (bt.dim() != 2 || cl.dim() != 1 || qs.dim() != 1 || qs.numel() < 2 || !cl.is_contiguous() || !qs.is_contiguous() || bt.stride(1) != 1) return false;
+  const int64_t seqs = qs.numel() - 1;
+  return bt.size(0) >= seqs && cl.numel() >= seqs && index_code(bt) >= 0 && index_code(cl) >= 0 && index_code(qs) >= 0 && fits_int(seqs) && fits_int(q.size(0)) && fits_int(q.size(1));
+}
+// where the result goes: `given`, or a new tensor like q
+bool chunk_result(Tensors& ts, PyObject* given, const at::Tensor& q, at::Tensor& out) {
+  if (given == Py_None) return true;          // (allocated once everything else is known to be right)
+  out = ts.take(given);
+  return ts.ok() && out.dim() == 3 && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1;
+}
+PyObject* result_of(int rc, PyObject* given, at::Tensor&& out) {
+  if (rc) return status(rc);
+  if (given == Py_None) return THPVariable_Wrap(std::move(out));
+  Py_INCREF(given);
+  return given;
+}
+
+// (query, key cache, value cache, block_tables, context_lens, query_start_loc, scale or None, window, out or None, longest chunk or None)
+PyObject* dense_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t window, longest;
+  if (n != 10 || (a[6] != Py_None && !PyFloat_CheckExact(a[6])) || !integer(a[7], window) || !integer(a[9], longest, 0, true) || !fits_int(window) || !fits_int(longest)) Py_RETURN_NONE;
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &kc = ts.take(a[1]), &vc = ts.take(a[2]), &bt = ts.take(a[3]), &cl = ts.take(a[4]), &qs = ts.take(a[5]);
+  at::Tensor out;
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs) || !chunk_result(ts, a[8], q, out)) Py_RETURN_NONE;
+  const int64_t heads = q.size(1), d = q.size(2);
+  if (!dense_rows(kc, q.scalar_type()) || !dense_rows(vc, q.scalar_type()) || kc.sizes().slice(1) != vc.sizes().slice(1) || kc.size(3) != d || kc.size(2) == 0 || heads % kc.size(2) != 0 ||
+      !fits_int(kc.size(1)) || (d != 64 && d != 128 && d != 256))
+    Py_RETURN_NONE;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[8] == Py_None) out = at::empty(q.sizes(), q.options());
+  const at::Tensor ws = at::empty({(int64_t)g_lib.dense_chunk_bytes((int)d)}, q.options().dtype(at::kByte));
+  const float scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)PyFloat_AS_DOUBLE(a[6]);
+  const int rc = without_gil(g_lib.dense_chunk, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), kc.const_data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
+                             vc.const_data_ptr(), vc.stride(0), vc.stride(1), vc.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(), index_code(cl),
+                             qs.const_data_ptr(), index_code(qs), out.mutable_data_ptr(), out.stride(0), out.stride(1), (int)(a[8] == Py_None), (int)(qs.numel() - 1), q.size(0),
+                             (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1), std::min(kc.size(0), vc.size(0)), bt.size(1), (int)window, (int)longest, scale,
+                             ws.mutable_data_ptr(), (size_t)ws.numel(), stream);
+  return result_of(rc, a[8], std::move(out));
+}
+
+// (query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc, centroids, prepared rotation, kv heads or
+//  None, query heads, head size, bytes of a row, bits, block size, longest chunk or None, scale, out or None)
+PyObject* packed_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t v[8];
+  if (n != 19 || !PyFloat_CheckExact(a[17])) Py_RETURN_NONE;
+  for (int i = 0; i < 8; ++i)
+    if (!integer(a[9 + i], v[i], 0, i == 1 || i == 7)) Py_RETURN_NONE;
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &kp = ts.take(a[1]), &kn = ts.take(a[2]), &vp = ts.take(a[3]), &vn = ts.take(a[4]);
+  const at::Tensor &bt = ts.take(a[5]), &cl = ts.take(a[6]), &qs = ts.take(a[7]), &cen = ts.take(a[8]);
+  const int64_t heads = v[2], d = v[3], row = v[4], bits = v[5], block = v[6];
+  at::Tensor out;
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs) || !chunk_result(ts, a[18], q, out) || q.size(1) != heads || q.size(2) != d || kp.dim() != 4 || bits < 2 || bits > 4 ||
+      !floats(cen, 1 << bits) || !fits_int(block) || !fits_int(v[7]) || (d != 64 && d != 128 && d != 256))
+    Py_RETURN_NONE;
+  const int64_t kv_heads = a[10] == Py_None ? kp.size(2) : v[1];
+  if (kv_heads <= 0 || heads % kv_heads != 0 || !packed_rows(kp, row, block, kv_heads) || !packed_rows(vp, row, block, kv_heads) || !norm_rows(kn, block, kv_heads) || !norm_rows(vn, block, kv_heads))
+    Py_RETURN_NONE;
+  const int64_t blocks = std::min(std::min(kp.size(0), kn.size(0)), std::min(vp.size(0), vn.size(0)));
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[18] == Py_None) out = at::empty(q.sizes(), q.options());
+  const at::Tensor ws = at::empty({(int64_t)g_lib.paged_chunk_bytes((int)d)}, q.options().dtype(at::kByte));
+  const int rc = without_gil(g_lib.paged_chunk, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), (const uint8_t*)kp.const_data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
+                             (const float*)kn.const_data_ptr(), kn.stride(0), kn.stride(1), kn.stride(2), (const uint8_t*)vp.const_data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2),
+                             (const float*)vn.const_data_ptr(), vn.stride(0), vn.stride(1), vn.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(),
+                             index_code(cl), qs.const_data_ptr(), index_code(qs), (const void*)(uintptr_t)v[0], (const float*)cen.const_data_ptr(), (int)bits, out.mutable_data_ptr(),
+                             out.stride(0), out.stride(1), (int)(a[18] == Py_None), (int)(qs.numel() - 1), q.size(0), (int)heads, (int)kv_heads, (int)d, (int)block, blocks, bt.size(1),
+                             (int)v[7], (float)PyFloat_AS_DOUBLE(a[17]), ws.mutable_data_ptr(), (size_t)ws.numel(), stream);
+  return result_of(rc, a[18], std::move(out));
+}
+
+// (query or None, key, value, positions, table or None, slot_mapping, key cache, value cache, sections (tuple or list) or None,
+//  interleaved, query_out or None) -> the rotated queries, or a status where there are none
+PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !PyBool_Check(a[9])) Py_RETURN_NONE;
+  const bool has_q = a[0] != Py_None, turns = a[4] != Py_None;
+  if (!has_q && a[10] != Py_None) Py_RETURN_NONE;
+  int sections[4], axes = 1;
+  int64_t pairs = 0;
+  if (a[8] != Py_None) {
+    const bool tuple = PyTuple_CheckExact(a[8]);
+    if (!turns || (!tuple && !PyList_CheckExact(a[8]))) Py_RETURN_NONE;
+    const Py_ssize_t m = tuple ? PyTuple_GET_SIZE(a[8]) : PyList_GET_SIZE(a[8]);
+    if (m < 1 || m > 4) Py_RETURN_NONE;
+    axes = (int)m;
+    for (int i = 0; i < axes; ++i) {
+      int64_t v;
+      if (!integer(tuple ? PyTuple_GET_ITEM(a[8], i) : PyList_GET_ITEM(a[8], i), v) || !fits_int(v)) Py_RETURN_NONE;
+      sections[i] = (int)v;
+      pairs += v;
+    }
+  }
+  const bool sectioned = a[8] != Py_None;
+  static const at::Tensor none;
+  Tensors ts;
+  const at::Tensor &k = ts.take(a[1]), &v = ts.take(a[2]), &slots = ts.take(a[5]), &kc = ts.take(a[6]), &vc = ts.take(a[7]);
+  const at::Tensor &q = has_q ? ts.take(a[0]) : none, &pos = turns ? ts.take(a[3]) : none, &table = turns ? ts.take(a[4]) : none;
+  if (!ts.ok() || !here(ts) || k.dim() != 3 || k.size(0) == 0 || k.stride(2) != 1 || v.stride(v.dim() - 1) != 1 || v.sizes() != k.sizes() || float_code(k) < 0 ||
+      v.scalar_type() != k.scalar_type() || float_code(kc) < 0 || !dense_rows(kc, kc.scalar_type()) || !dense_rows(vc, kc.scalar_type()) || kc.sizes().slice(1) != vc.sizes().slice(1) ||
+      kc.size(2) != k.size(1) || kc.size(3) != k.size(2) || slots.dim() != 1 || slots.numel() < k.size(0) || !slots.is_contiguous() || index_code(slots) < 0)
+    Py_RETURN_NONE;
+  const int64_t tokens = k.size(0), d = k.size(2);
+  if (!fits_int(tokens) || !fits_int(k.size(1)) || !fits_int(d) || !fits_int(kc.size(1))) Py_RETURN_NONE;
+  at::Tensor out;
+  if (has_q && (q.dim() != 3 || q.size(0) != tokens || q.size(2) != d || !fits_int(q.size(1)) || q.stride(2) != 1 || q.scalar_type() != k.scalar_type() || !chunk_result(ts, a[10], q, out))) Py_RETURN_NONE;
+  if (turns && (table.dim() != 2 || table.scalar_type() != at::kFloat || !table.is_contiguous() || table.size(0) == 0 || !fits_int(table.size(1)) || index_code(pos) < 0 ||
+                (sectioned && pairs != table.size(1) / 2) || pos.dim() != (sectioned ? 2 : 1) || (sectioned && pos.size(0) != axes) || pos.size(pos.dim() - 1) < tokens || pos.stride(pos.dim() - 1) != 1))
+    Py_RETURN_NONE;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (has_q && a[10] == Py_None) out = at::empty(q.sizes(), q.options());
+  const int rc = without_gil(g_lib.rope_append, has_q ? q.const_data_ptr() : nullptr, has_q ? q.stride(0) : 0, has_q ? q.stride(1) : 0, has_q ? out.mutable_data_ptr() : nullptr,
+                             has_q ? out.stride(0) : 0, has_q ? out.stride(1) : 0, k.const_data_ptr(), k.stride(0), k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1),
+                             float_code(k), turns ? pos.const_data_ptr() : nullptr, turns ? index_code(pos) : 0, sectioned && axes > 1 ? pos.stride(0) : 0,
+                             turns ? (const float*)table.const_data_ptr() : nullptr, turns ? table.size(0) : 0, turns ? (int)table.size(1) : 0,
+                             sectioned ? (const int*)sections : nullptr, axes, (int)(a[9] == Py_True), slots.const_data_ptr(), index_code(slots), kc.mutable_data_ptr(),
+                             kc.stride(0), kc.stride(1), kc.stride(2), vc.mutable_data_ptr(), vc.stride(0), vc.stride(1), vc.stride(2), float_code(kc), tokens,
+                             has_q ? (int)q.size(1) : 0, (int)k.size(1), (int)d, (int)kc.size(1), std::min(kc.size(0), vc.size(0)), stream);
+  return has_q ? result_of(rc, a[10], std::move(out)) : status(rc);
+}
+
 // (raw stream function, addresses in the order of Library)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   static_assert(sizeof(Library) == kFunctions * sizeof(void*), "one address a member");
@@ -359,6 +499,9 @@ PyMethodDef kMethods[] = {
     {"decode_blocks", (PyCFunction)(void (*)(void))guarded<decode_blocks>, METH_FASTCALL, nullptr},
     {"spectral_encode", (PyCFunction)(void (*)(void))guarded<spectral_encode>, METH_FASTCALL, nullptr},
     {"spectral_attention", (PyCFunction)(void (*)(void))guarded<spectral_attention>, METH_FASTCALL, nullptr},
+    {"rope_append", (PyCFunction)(void (*)(void))guarded<rope_append>, METH_FASTCALL, nullptr},
+    {"dense_chunk", (PyCFunction)(void (*)(void))guarded<dense_chunk>, METH_FASTCALL, nullptr},
+    {"packed_chunk", (PyCFunction)(void (*)(void))guarded<packed_chunk>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -167,12 +167,18 @@ class TQPagedAttention:
         max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result does not
 
         Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector."""
-        from .chunk_attention import _check_out, check_chunk, check_query
+        from .chunk_attention import _check_out, _longest, check_chunk, check_query
         if self._block_selector is not None:
             raise ValueError("forward_chunk does not run the block selector")
         tq = self._tq
         if tq.rotation is not self.rotation:
             self.rotation = tq.rotation
+        if query.is_cuda:
+            result = _lib.calls().packed_chunk(query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc,
+                                               self.centroids, tq.prepared_rotation().ptr, num_kv_heads, self.num_query_heads, self.head_dim,
+                                               self.packed_dim, self.bits, block_size, max_query_len, self.scale, out)
+            if result is not None:
+                return result if type(result) is not int else _lib.check(result)
         check_query(query)
         if k_packed.dim() != 4 or v_packed.dim() != 4 or k_norms.dim() != 3 or v_norms.dim() != 3:
             raise ValueError("expected caches [blocks, block_size, heads, bytes] and norms [blocks, block_size, heads]")
@@ -206,7 +212,7 @@ class TQPagedAttention:
                 starts.data_ptr(), _lib.itype_code(starts), tq.prepared_rotation().ptr, self.centroids.data_ptr(), self.bits,
                 result.data_ptr(), result.stride(0), result.stride(1), int(out is None),
                 num_seqs, num_tokens, num_q_heads, num_kv_heads, d, block_size, blocks, bt.shape[1],
-                max_query_len or 0, self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
+                _longest(max_query_len), self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
         return result
 
     def last_call_status(self) -> int:
