@@ -278,3 +278,20 @@ def test_a_row_of_nan_stays_its_own(dev):
     for got, o, bound in ((akv.paged_chunk_attention(p.q, kc, vc, b.tables, b.ctx, b.starts), o1, b1), (p.run(), o2, b2)):
         assert not bool(got[b.tokens:].any())
         check(got[:b.tokens][clean], o[clean], bound[clean])
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [(BF, BF), (torch.float32, FP), (FP, torch.float32)])
+@pytest.mark.parametrize("sections", [None, (16, 24, 24), (15, 25, 24)])
+def test_rope_append_of_many_tokens(dev, dtype, cache_dtype, sections):
+    """More rows than the second-level caches hold; axes that take whole units of eight pairs, and others."""
+    tokens, heads, kv, d = 3001, 32, 8, 128
+    x = vectors(130, dev, dtype, tokens, heads + 2 * kv, d)
+    table = table_of(4000, d, dev)
+    g = torch.Generator(device=dev).manual_seed(1)
+    pos = torch.randint(0, 4000, (3, tokens) if sections else (tokens,), device=dev, generator=g)
+    slots = torch.randperm(200 * 16, device=dev, generator=g)[:tokens]
+    kc, vc = (torch.zeros(200, 16, kv, d, dtype=cache_dtype, device=dev) for _ in range(2))
+    got = akv.rope_append(x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:], pos, table, slots, kc, vc, sections=sections)
+    check_rope(got, *rope_reference(x[:, :heads], pos, table, sections, False))
+    check_rope(kc.flatten(0, 1)[slots], *rope_reference(x[:, heads:heads + kv], pos, table, sections, False))
+    assert torch.equal(vc.flatten(0, 1)[slots], x[:, heads + kv:].to(cache_dtype))
