@@ -9,8 +9,9 @@ resolves a registered backend by `getattr(module, name)` while its own configura
 still be half imported.  With vLLM importable they derive from its AttentionBackend and
 TritonAttentionImpl; without it they derive from small stand-ins that keep the constructor
 arguments, so the TurboQuant side (cache write, decode attention, block decompression) can run and
-be tested on its own -- whatever is vLLM's own job (attention over an uncompressed cache, the
-metadata builder) then raises with a message that says so.
+be tested on its own, prefill included, whose attention is then this package's paged_chunk_attention
+-- whatever is vLLM's own job (layers that are not compressed, the metadata builder) raises with a
+message that says so.
 
 What the impl does with the cache (PRIMARY mode: the tensor vLLM allocates IS the compressed cache,
 uint8 [num_blocks, 2, block_size, num_kv_heads, tq_dim]):
@@ -23,7 +24,8 @@ uint8 [num_blocks, 2, block_size, num_kv_heads, tq_dim]):
                        tq::decode_step / tq::hybrid_decode_step op.
   forward, prefill     the blocks the batch addresses are decompressed into a bf16 block buffer
                        (batch_decompress_active_blocks), the chunk's own rows are scattered in
-                       uncompressed, and vLLM's unified_attention runs on that buffer.
+                       uncompressed (rope_append without a rotation), and vLLM's unified_attention runs
+                       on that buffer, or paged_chunk_attention where there is no vLLM.
 
 In SHADOW mode vLLM's own cache stays authoritative and this impl keeps a compressed copy beside
 it (TQGPUCache); decode may be served from the copy (AITHER_TQ_FUSED=1).  The format comes from
@@ -112,6 +114,22 @@ def _vllm_unified_attention(impl, q, k_buf, v_buf, out, attn_metadata):
                       q_descale=None, k_descale=ones, v_descale=ones)
 
 
+def _dense_attention(impl, q, k_buf, v_buf, out, attn_metadata):
+    """vLLM's attention over the block buffer where vLLM is importable, paged_chunk_attention otherwise."""
+    try:
+        return _vllm_unified_attention(impl, q, k_buf, v_buf, out, attn_metadata)
+    except ImportError:
+        pass
+    from ..chunk_attention import paged_chunk_attention
+    if impl.alibi_slopes is not None or impl.logits_soft_cap:
+        raise NotImplementedError("ALiBi slopes and a soft cap of the scores need vLLM's attention; vLLM is not importable")
+    left, right = impl.sliding_window
+    if right > 0:
+        raise NotImplementedError(f"a window of {impl.sliding_window} is not causal")
+    paged_chunk_attention(q, k_buf, v_buf, attn_metadata.block_table, attn_metadata.seq_lens, attn_metadata.query_start_loc,
+                          scale=impl.scale, window=left + 1 if left >= 0 else 0, out=out, max_query_len=attn_metadata.max_query_len)
+
+
 # --------------------------------------------------------------------------------------------
 # backend class
 # --------------------------------------------------------------------------------------------
@@ -186,6 +204,7 @@ def _make_impl_class():
     except ImportError:
         base = _StandaloneImplBase
 
+    from ..chunk_attention import rope_append
     from ..fused_attention import TQPagedAttention
     from ..fused_kv_update import fused_encode_and_store, fused_kv_update_pair
     from ..hybrid_attention import HybridPagedAttention, hybrid_encode_and_store_pair
@@ -211,8 +230,8 @@ def _make_impl_class():
         _forward_count: ClassVar[int] = 0
         _INIT_AFTER_FORWARDS: ClassVar[int] = 2
         _MIN_BLOCKS_FOR_INIT: ClassVar[int] = 16
-        # attention over an uncompressed block buffer: vLLM's kernel; replaceable (tests, other engines)
-        _dense_paged_attention = staticmethod(_vllm_unified_attention)
+        # attention over an uncompressed block buffer: vLLM's kernel or this package's; replaceable (tests, other engines)
+        _dense_paged_attention = staticmethod(_dense_attention)
 
         @classmethod
         def reset_class_state(cls) -> None:
@@ -410,7 +429,7 @@ def _make_impl_class():
                                                attn_metadata.block_table, num_blocks,
                                                cls._primary_k_norms[li], cls._primary_v_norms[li])
             if key is not None and value is not None:
-                self._scatter_rows(key, value, k_buf, v_buf, attn_metadata.slot_mapping, block_size)
+                self._scatter_rows(key, value, k_buf, v_buf, attn_metadata.slot_mapping)
             n = attn_metadata.num_actual_tokens
             if query.dim() == 2:
                 query = query.view(query.shape[0], self.num_heads, self.head_size)
@@ -421,17 +440,11 @@ def _make_impl_class():
             return output
 
         @staticmethod
-        def _scatter_rows(key, value, k_buf, v_buf, slot_mapping, block_size) -> None:
+        def _scatter_rows(key, value, k_buf, v_buf, slot_mapping) -> None:
             """Rows of the current chunk into the block buffers at their slots; negative slots and
             slots beyond the buffer are left out (reference: backend.py:1247-1272)."""
             n = min(key.shape[0], slot_mapping.shape[0])
-            slots = slot_mapping[:n].long()
-            ok = (slots >= 0) & (slots < k_buf.shape[0] * block_size)
-            slots = torch.where(ok, slots, torch.zeros_like(slots))
-            src = torch.nonzero(ok).squeeze(-1)
-            bi, oi = slots[src] // block_size, slots[src] % block_size
-            k_buf[bi, oi] = key[:n][src].to(k_buf.dtype)
-            v_buf[bi, oi] = value[:n][src].to(v_buf.dtype)
+            rope_append(None, key[:n], value[:n], None, None, slot_mapping[:n], k_buf, v_buf)
 
         # SHADOW ---------------------------------------------------------------------------
         def _forward_shadow(self, layer, query, key, value, kv_cache, attn_metadata, output,
