@@ -212,5 +212,14 @@ __device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L
   first = __builtin_amdgcn_readfirstlane(L.total);
 }
 
-// where workgroup g's range begins
-__device__ __forceinline__ int64_t ck_begin(int64_t total, int g, int G) { return total * g / G; }
+// where workgroup g's range begins: floor(total g / G), G at most 2^15
+struct ck_share { int64_t whole; uint32_t rest; };
+__device__ __forceinline__ ck_share ck_share_of(int64_t total, int G) {
+  if (total <= 0xffffffffll) {
+    const uint32_t w = (uint32_t)total / (uint32_t)G;
+    return {(int64_t)w, (uint32_t)total - w * (uint32_t)G};
+  }
+  const int64_t w = total / G;
+  return {w, (uint32_t)(total - w * G)};
+}
+__device__ __forceinline__ int64_t ck_begin(const ck_share& s, int g, int G) { return s.whole * g + s.rest * (uint32_t)g / (uint32_t)G; }

@@ -243,8 +243,8 @@ __device__ __forceinline__ float ck_finish(float l) { return l == 0.f ? 0.f : 1.
 
 // Results of 32 rows whose coordinates are spread over the W wavefronts of a workgroup, QW quads each, times f.  Packed rows go
 // through `rows` (LDS, 32 x (D + 4) floats, which has been read by others) and are turned back.
-template <int D, int KIND, int W, int QW>
-__device__ __forceinline__ void ck_results(const ck_args& a, const float4 (&x)[QW], float f, bool valid, int token, int head, float* __restrict__ rows) {
+template <int D, int KIND, int W, int QW, class Matrix>
+__device__ __forceinline__ void ck_results(const ck_args& a, const float4 (&x)[QW], float f, const Matrix& matrix, bool valid, int token, int head, float* __restrict__ rows) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
   if constexpr (!ck_math<KIND>::packed) {
     if (valid) {
@@ -270,7 +270,7 @@ __device__ __forceinline__ void ck_results(const ck_args& a, const float4 (&x)[Q
       const float un = ck_result_operand<D>([&](int ks, int j) { return v[ks][j]; }, hi, lo) * a.turn_scale->up * (1.f / CK_TURN);
 #pragma unroll
       for (int dt = wave; dt < DT; dt += W) {
-        const ck_f16v y = ck_turn<D>(a.turn_out, dt, hi, lo);
+        const ck_f16v y = matrix.turn(dt, hi, lo);
         if (valid) {
 #pragma unroll
           for (int b = 0; b < 4; ++b) ck_store<KIND>(a, token, head, 4 * dt + b, y[4 * b] * un, y[4 * b + 1] * un, y[4 * b + 2] * un, y[4 * b + 3] * un);
@@ -359,8 +359,9 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
   // same lines of the cache at the same time.  (A packed row is half a line or less, a norm a thirty-second of one; with the heads one
   // after the other on the axis, cut anywhere, a verification of 350 MB fetched 830.)
   const int heads = a.KVH * a.HS, head = g % heads, R = G / heads;
-  int64_t at = ck_begin(total, g / heads, R);
-  const int64_t end = ck_begin(total, g / heads + 1, R);
+  const ck_share share = ck_share_of(total, R);
+  int64_t at = ck_begin(share, g / heads, R);
+  const int64_t end = ck_begin(share, g / heads + 1, R);
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
   int seq, tile, first;
@@ -649,7 +650,7 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
         if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
       }
     } else {
-      ck_results<D, KIND, W, P::QW>(a, x, ck_finish(l), row.valid, row.token, row.head, (float*)area);
+      ck_results<D, KIND, W, P::QW>(a, x, ck_finish(l), ck_turn_rows<D, false>(a.turn_out, wave), row.valid, row.token, row.head, (float*)area);
     }
     // ---- on to the next tile
     at = tile_at = tile_end;
@@ -722,8 +723,9 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   const int per_head = ck_total<T, N, P::START>(a, L, TM);
   const int heads = a.KVH * a.HS;
   const int64_t total = (int64_t)per_head * heads;
-  int64_t at = ck_begin(total, g, G);
-  const int64_t end = ck_begin(total, g + 1, G);
+  const ck_share share = ck_share_of(total, G);
+  int64_t at = ck_begin(share, g, G);
+  const int64_t end = ck_begin(share, g + 1, G);
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
   int head = (int)(at / per_head), seq, tile, first;
@@ -922,6 +924,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       float alpha;
       ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha);      // (nothing to rescale yet)
     }
+    const bool busy = 32 * wave < (t1 - t0) * a.GC;      // (a wavefront behind the tile's last row only brings keys and values)
     int k_slot = 0;                // of unit u
     ck_entry ahead = {0u, 0u};
     for (int u = 0; u < units; ++u) {
@@ -934,6 +937,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       else request(u + 2, k_after, u + 2 < units, u + 1, u + 1 < units);
       const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
       const uint32_t v_from = (u & 1) * P::TILE;
+      if (busy)
 #pragma unroll (P::UNROLL)
       for (int t = 0; t < P::STEPS; ++t) {
         // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
@@ -1033,10 +1037,12 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       }
     } else {
       const int64_t slot = (2 * (int64_t)g + (u0 == 0 ? 1 : 0)) * P::WAVES + wave;
+      if (busy) {
 #pragma unroll
-      for (int c = 0; c < P::QUADS; ++c)
-        ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)] * unit, o[c / 4][4 * (c & 3) + 1] * unit, o[c / 4][4 * (c & 3) + 2] * unit, o[c / 4][4 * (c & 3) + 3] * unit);
-      a.part_ml[slot * 64 + lane] = make_float2(st.m, st.l);
+        for (int c = 0; c < P::QUADS; ++c)
+          ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)] * unit, o[c / 4][4 * (c & 3) + 1] * unit, o[c / 4][4 * (c & 3) + 2] * unit, o[c / 4][4 * (c & 3) + 3] * unit);
+        a.part_ml[slot * 64 + lane] = make_float2(st.m, st.l);
+      }
       if (u0 == 0 && tid == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
     }
     at = tile_at = tile_end;
@@ -1055,40 +1061,50 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 // Workgroup (g, w): the 32 rows w of the tile that begins in workgroup g's range and does not end there; its other pieces are the first ones
 // of the ranges behind, which are `stride` workgroups apart.  Their maxima are looked through first, so that the sums of up to four pieces are on their way together.
 template <int D, int KIND, int WAVES>
-__global__ __launch_bounds__(256) void ck_merge_kernel(ck_args a, int G, int stride) {
+__global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_kernel(ck_args a, int G, int stride) {
   constexpr int QUADS = D / 8, MINE = QUADS / 4;
   __shared__ __align__(16) float rows[ck_math<KIND>::packed ? 32 * (D + 4) : 1];
   const int g = blockIdx.x, part = blockIdx.y;
   const ck_record rec = a.rec[g];
-  if (!rec.valid) return;
+  if (!rec.valid || 32 * part >= rec.tokens * a.GC) return;      // (rows behind the tile's last: nothing was left of them)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
+  ck_turn_rows<D, ck_math<KIND>::packed && D < 256 && WAVES == 1> matrix(a.turn_out, wave);
   // ranges first + 1 .. last hold a piece each, unless they are empty
   const int R = G / stride, first = g / stride;
-  int last = first;
-  while (last + 1 < R && ck_begin(rec.total, last + 1, R) < rec.end) ++last;
-  auto slot_of = [&](int r) { return (2 * (int64_t)(r * stride + g % stride) + (r == first ? 1 : 0)) * WAVES + part; };
-  auto held = [&](int r) { return r == first || ck_begin(rec.total, r, R) < ck_begin(rec.total, r + 1, R); };
+  const ck_share share = ck_share_of(rec.total, R);
+  int next = first + 1;
   float m = -INFINITY, l = 0.f;
-  for (int r = first; r <= last; ++r) m = fmaxf(m, held(r) ? a.part_ml[slot_of(r) * 64 + lane].x : -INFINITY);
-  const float ref = m == -INFINITY ? 0.f : m;
   float4 x[MINE];
 #pragma unroll
   for (int i = 0; i < MINE; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r = first; r <= last; r += 4) {
+  for (bool more = true, begun = false; more; begun = true) {
     float2 e[4];
     float4 y[4][MINE];
+    float top = m;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const bool there = r + k <= last && held(r + k);
-      const int64_t slot = slot_of(there ? r + k : first);
+      int r = begun || k > 0 ? R : first;
+      if (begun || k > 0) {
+        while (next < R && share.whole == 0 && ck_begin(share, next, R) == ck_begin(share, next + 1, R)) ++next;
+        if (next < R && ck_begin(share, next, R) < rec.end) r = next++;
+      }
+      const bool there = r < R;
+      more = there;
+      const int64_t slot = (2 * (int64_t)((there ? r : first) * stride + g % stride) + (!there || r == first ? 1 : 0)) * WAVES + part;
       e[k] = a.part_ml[slot * 64 + lane];
-      if (!there) e[k].x = -INFINITY;
 #pragma unroll
       for (int i = 0; i < MINE; ++i) y[k][i] = ((const float4*)a.part)[(slot * QUADS + MINE * wave + i) * 64 + lane];
+      if (!there) e[k] = make_float2(-INFINITY, 0.f);
     }
 #pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, e[k].x);
+    const float ref = top == -INFINITY ? 0.f : top, old = ck_exp2(m - ref);
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) { x[i].x *= old; x[i].y *= old; x[i].z *= old; x[i].w *= old; }
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (!(r + k <= last && held(r + k))) continue;
+      if (e[k].x == -INFINITY) continue;       // (no such piece, or nothing in it)
       const float f = ck_exp2(e[k].x - ref);
       l = fmaf(e[k].y, f, l);
 #pragma unroll
@@ -1097,9 +1113,10 @@ __global__ __launch_bounds__(256) void ck_merge_kernel(ck_args a, int G, int str
         x[i].z = fmaf(y[k][i].z, f, x[i].z); x[i].w = fmaf(y[k][i].w, f, x[i].w);
       }
     }
+    m = top;
   }
   const int row = 32 * part + col, j = row / a.GC, gq = (rec.head % a.HS) * a.GC + row - j * a.GC;
-  ck_results<D, KIND, 4, MINE>(a, x, ck_finish(l), j < rec.tokens && gq < a.G, rec.token + j, (rec.head / a.HS) * a.G + gq, rows);
+  ck_results<D, KIND, 4, MINE>(a, x, ck_finish(l), matrix, j < rec.tokens && gq < a.G, rec.token + j, (rec.head / a.HS) * a.G + gq, rows);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------

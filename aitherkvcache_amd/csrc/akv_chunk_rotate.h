@@ -49,6 +49,32 @@ template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restr
   }
   return y;
 }
+// Rows dt of the matrix for results: read where they are multiplied, or (HELD: D at most 128, a workgroup of four wavefronts with one dt each)
+// requested before the results are there.
+template <int D, bool HELD> struct ck_turn_rows {
+  const uint4* all;
+  uint4 x[HELD ? 2 * (D / 16) : 1];
+  __device__ __forceinline__ ck_turn_rows(const uint4* table, int dt) : all(table) {
+    if constexpr (HELD) {
+      if (dt < D / 32) {
+#pragma unroll
+        for (int i = 0; i < 2 * (D / 16); ++i) x[i] = *ck_turn_at(table, D, i & 1, dt, i >> 1);
+      }
+    }
+  }
+  __device__ __forceinline__ ck_f16v turn(int dt, const ck_u4 (&hi)[D / 16], const ck_u4 (&lo)[D / 16]) const {
+    if constexpr (!HELD) return ck_turn<D>(all, dt, hi, lo);
+    ck_f16v y = (ck_f16v)(0.f);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const ck_u4 m_hi = __builtin_bit_cast(ck_u4, x[HELD ? 2 * ks : 0]), m_lo = __builtin_bit_cast(ck_u4, x[HELD ? 2 * ks + 1 : 0]);
+      y = ck_math<CK_F16>::mfma(m_lo, hi[ks], y);
+      y = ck_math<CK_F16>::mfma(m_hi, lo[ks], y);
+      y = ck_math<CK_F16>::mfma(m_hi, hi[ks], y);
+    }
+    return y;
+  }
+};
 // A row of queries (this lane's half of every sixteen coordinates) as operand; returns what undoes its scale.
 template <int D> __device__ __forceinline__ float ck_query_operand(ck_u4 (&x)[D / 16], int dtype) {
   if (dtype == AKV_F16) return 1.f;
