@@ -669,13 +669,16 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
 // keys: while the weights of step x are computed (vector unit) the products of step x + 1 are (matrix cores), their operands read during the
 // value products of step x - 1; then the values of step x are multiplied, their operands read during the first half.  The two units take
 // turns instruction by instruction: left to two wavefronts a SIMD with both in blocks, they overlapped by a quarter (mean of 16
-// products and 16 weights 1417 clocks, in turns 1071).  Keys of unit u + 2 and values of u + 1 are on their way during unit u.
+// products and 16 weights 1417 clocks, in turns 1071).  Keys of unit u + 2 and values of u + 1 are on their way during unit u; packed ones
+// are put to LDS then, beside the value products, from codes that were requested a unit before (all at the end of a unit: 2000 rows over
+// 8000 keys, 32 heads, 445 us instead of 422).
 //
 // Rows lie in LDS without padding, their pieces of sixteen bytes in an order that depends on the row, piece c at place c ^ f(row): sixteen
 // lanes that read one piece of sixteen keys, and 32 that read four coordinates each of four values, meet all 64 banks once
 // (245 and 216 bytes a clock; rows padded by 32 bytes gave 128 and 126).
 template <int D, int KIND> struct ck_wide {
   static constexpr bool AHEAD = D == 64 || (D == 128 && KIND < 2);    // registers for the keys of the step after the next
+  static constexpr int EARLY = AHEAD ? D / 16 : KIND >= 2 && D < 256 ? D / 32 : 0;     // pieces of a step's keys that are read during the step before
   static constexpr int WAVES = D == 128 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES, N = D == 256 ? 32 : 64, STEPS = N / 32;
   static constexpr int START = 192 / N;                               // (what a tile costs besides its units, in units)
   static constexpr int PER_CU = D == 256 || WAVES == 8 ? 1 : 2;       // workgroups a CU
@@ -684,6 +687,7 @@ template <int D, int KIND> struct ck_wide {
   static constexpr int ROW = 2 * D, TILE = N * ROW;
   // Units of keys held: of those read during a unit, and the one that is written (a unit on with AHEAD, or where a unit is a step)
   static constexpr int KRING = AHEAD || STEPS == 1 ? 2 : 3;
+  static_assert(EARLY == 0 || STEPS == 2, "the step after the next lies in the next unit");
   static constexpr int UNROLL = KIND >= 2 ? 1 : STEPS;
   static constexpr int RING = 2 * WAVES;                              // units whose places and norms are held
   static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
@@ -819,35 +823,45 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     };
     // packed: codes of the keys of one unit and the values of another to registers, and from there to LDS; a value whose norm counts as
     // nothing is zero
-    uint32_t words[PACKED ? NT : 1][BITS];
-    auto fetch = [&](int uk, int uv) {
+    struct codes { uint32_t w[PACKED ? NT : 1][BITS]; };
+    codes words;
+    auto fetch = [&](int uk, int uv, codes& c) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int task = tid + T * i, v = task / TASKS, r = task % TASKS / TPR, part = task % TPR;
         const int64_t* place = (const int64_t*)(lds + P::PLACE0) + ((v ? uv : uk) & (P::RING - 1)) * 2 * N + v * N;
-        ck_load_words(words[i], (v ? a.v : a.k) + place[r] + 4 * BITS * part);
+        ck_load_words(c.w[i], (v ? a.v : a.k) + place[r] + 4 * BITS * part);
       }
     };
-    auto put = [&](int k_slot, int uv) {
+    // ... the part `step` of STEPS of them
+    auto put = [&](int k_slot, int uv, int step) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const int task = tid + T * i, v = task / TASKS, r = task % TASKS / TPR, part = task % TPR;
+        const int task = tid + T * i, v = (64 * wave + T * i) / TASKS, r = task % TASKS / TPR, part = task % TPR;
         unsigned char* to = lds + (v ? P::V0 + (uv & 1) * P::TILE : P::K0 + k_slot * P::TILE) + r * P::ROW;
         const int f = v ? P::fv(r) : P::fk(r);
-        uint32_t keep = 0xffffffffu;
-        if (v) keep = ((const uint32_t*)(lds + P::NORM0))[(uv & (P::RING - 1)) * 4 * N + 3 * N + r];
+        const uint32_t keep = ((const uint32_t*)(lds + P::NORM0))[(uv & (P::RING - 1)) * 4 * N + 3 * N + r] | (v ? 0u : 0xffffffffu);
+        // (the step is no constant: its sixteen codes are moved to the front)
+        uint32_t w[BITS];
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          ck_u4 x = lut.group(words[i], j), y = lut.group(words[i], j + 1);
-          if (!v) {                // keys: the order of the turned rows
-            const ck_u4 z = x;
-            x = (ck_u4){z[0], z[1], y[0], y[1]};
-            y = (ck_u4){z[2], z[3], y[2], y[3]};
-          }
-          *(ck_u4*)(to + 16 * ((4 * part + j) ^ f)) = x & keep;
-          *(ck_u4*)(to + 16 * ((4 * part + j + 1) ^ f)) = y & keep;
+        for (int b = 0; b < BITS; ++b) {
+          w[b] = words.w[i][b];
+          const uint32_t far = BITS == 3 ? (b == 0 ? __builtin_amdgcn_alignbyte(words.w[i][2], words.w[i][1], 2) : words.w[i][2] >> 16) : words.w[i][(b + BITS / 2) % BITS];
+          if (P::STEPS == 2 && step == 1 && b < (BITS + 1) / 2) w[b] = far;
+        }
+#pragma unroll
+        for (int n = 0; n < 4 / P::STEPS; n += 2) {
+          const int j = 2 * (P::STEPS == 2 ? step : 0) + n;
+          // (keys: the order of the turned rows; without branches, which the products could not be spread over)
+          const ck_u4 x = lut.group(w, n), y = lut.group(w, n + 1);
+          *(ck_u4*)(to + 16 * ((4 * part + j) ^ f)) = (ck_u4){x[0], x[1], v ? x[2] : y[0], v ? x[3] : y[1]} & keep;
+          *(ck_u4*)(to + 16 * ((4 * part + j + 1) ^ f)) = (ck_u4){v ? y[0] : x[2], v ? y[1] : x[3], y[2], y[3]} & keep;
         }
       }
+    };
+    auto put_all = [&](int k_slot, int uv) {
+#pragma unroll
+      for (int t = 0; t < P::STEPS; ++t) put(k_slot, uv, t);
     };
 
     // (the rows of the tile are requested behind the first keys and values)
@@ -877,18 +891,21 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[ks][i] = M::pair(y[ks / 2][8 * (ks & 1) + 2 * i] * f, y[ks / 2][8 * (ks & 1) + 2 * i + 1] * f);
     };
+    ck_entry ahead = {0u, 0u};
     __syncthreads();               // (LDS of the tile before has been read)
     if (units > 0) {
       note(wave, look(wave));
       note_norms(wave);
       __syncthreads();
+      ahead = look(P::WAVES + wave);
       if constexpr (PACKED) {
-        fetch(0, 0);
+        fetch(0, 0, words);
         rows();
-        put(0, 0);
-        fetch(1, 0);
+        put_all(0, 0);
+        fetch(1, 0, words);
         turn_rows();
-        put(1, 0);
+        put_all(1, 0);
+        fetch(2, 1, words);
       } else {
         request(0, 0, true, 0, true);
         request(1, 1, units > 1, 0, false);
@@ -906,16 +923,17 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     __syncthreads();
     ck_u4 kf[KS];
     ck_f16v sc[1];
-    auto read_keys = [&](uint32_t from) {
+    auto read_keys = [&](uint32_t from, int first, int last) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[ks] = *(const ck_lds_u4*)(uintptr_t)(k_at[ks] + from);
+      for (int ks = 0; ks < KS; ++ks)
+        if (ks >= first && ks < last) kf[ks] = *(const ck_lds_u4*)(uintptr_t)(k_at[ks] + from);
     };
     if (units > 0) {
-      read_keys(0);
+      read_keys(0, 0, KS);
       sc[0] = (ck_f16v)(0.f);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) sc[0] = M::mfma(kf[ks], q[ks], sc[0]);
-      if (P::AHEAD) read_keys(32 * P::ROW);
+      if (P::EARLY > 0) read_keys(32 * P::ROW, 0, P::EARLY);
       __syncthreads();             // (unit 2's keys may go where these were)
       const float* nr = (const float*)(lds + P::NORM0);
       if (scaled) sc[0] *= fac;
@@ -926,14 +944,17 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     }
     const bool busy = 32 * wave < (t1 - t0) * a.GC;      // (a wavefront behind the tile's last row only brings keys and values)
     int k_slot = 0;                // of unit u
-    ck_entry ahead = {0u, 0u};
     for (int u = 0; u < units; ++u) {
-      // ---- on their way: places of the WAVES units behind the WAVES that this one belongs to, keys of u + 2, values of u + 1
+      // ---- on their way: places of the WAVES units behind the WAVES that this one belongs to; keys of u + 2, values of u + 1 (packed:
+      // of units one further on, while the codes requested a unit ago are put to LDS beside the products).  Noted during unit k WAVES
+      // they are read from k WAVES + 1 on, up to three units ahead: WAVES is at least four.
+      static_assert(P::WAVES >= 4, "places are noted before they are read");
       const int turn = u & (P::WAVES - 1);
-      if (turn == 1) note(u - 1 + P::WAVES + wave, ahead);
-      if (turn == 0) ahead = look(u + P::WAVES + wave);
+      if (turn == 0) note(u + P::WAVES + wave, ahead);
+      if (turn == P::WAVES - 1) ahead = look(u + 1 + P::WAVES + wave);
       const int k_next = P::KRING == 2 ? k_slot ^ 1 : k_slot == 2 ? 0 : k_slot + 1, k_after = P::KRING == 2 ? k_slot : k_next == 2 ? 0 : k_next + 1;
-      if constexpr (PACKED) fetch(u + 2, u + 1);
+      codes flying;
+      if constexpr (PACKED) fetch(u + 3, u + 2, flying);
       else request(u + 2, k_after, u + 2 < units, u + 1, u + 1 < units);
       const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
       const uint32_t v_from = (u & 1) * P::TILE;
@@ -941,7 +962,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 #pragma unroll (P::UNROLL)
       for (int t = 0; t < P::STEPS; ++t) {
         // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
-        if (!P::AHEAD) read_keys(t + 1 < P::STEPS ? k_slot * P::TILE + (t + 1) * 32 * P::ROW : k_next * P::TILE);
+        if (!P::AHEAD) read_keys(t + 1 < P::STEPS ? k_slot * P::TILE + (t + 1) * 32 * P::ROW : k_next * P::TILE, P::EARLY, KS);
         ck_f16v next = (ck_f16v)(0.f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) next = M::mfma(kf[ks], q[ks], next);
@@ -959,7 +980,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[kb][i] = M::pair(sc[0][8 * kb + 2 * i], sc[0][8 * kb + 2 * i + 1]);
-        constexpr int READS = 4 * DT + (P::AHEAD ? 0 : KS) + (PACKED ? 4 : 0), FIRST = P::AHEAD ? 0 : 4;
+        constexpr int READS = 4 * DT + KS - P::EARLY + (PACKED ? 4 : 0), FIRST = P::AHEAD ? 0 : 4;
         if (FIRST > 0) __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -975,27 +996,31 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         sc[0] = next;
         if (scaled) sc[0] *= fac;
         const bool hidden = base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window);
-        if (hidden) {
-          if constexpr (PACKED) ck_norms(sc, nn, nn + N);
-          ck_mask(sc, base, row.pos, a.window);
-        }
-        // ---- values, the keys of the step after the next to registers, and the largest of the next step's scores
+        if (!PACKED && hidden) ck_mask(sc, base, row.pos, a.window);
+        // ---- values, the keys of the step after the next to registers, and the largest of the next step's scores (packed: their norms, and
+        // codes to LDS; without a branch, over which the products could not be spread)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
             o[dt] = M::mfma((ck_u4){vf[kb][dt][0][0], vf[kb][dt][0][1], vf[kb][dt][1][0], vf[kb][dt][1][1]}, p[kb], o[dt]);
-        if (P::AHEAD) read_keys(k_next * P::TILE + t * 32 * P::ROW);
+        if (P::AHEAD) read_keys(k_next * P::TILE + t * 32 * P::ROW, 0, KS);
+        else if (P::EARLY > 0) read_keys(k_next * P::TILE + t * 32 * P::ROW, 0, P::EARLY);
         if constexpr (PACKED) {
-          // (masked scores are infinite: norms may come on top of them once more only where there are none yet)
-          if (!hidden) ck_norms(sc, nn, nn + N);
+          ck_norms(sc, nn, nn + N);
+          put(k_after, u + 1, t);
         }
-        const float mx = ck_max(sc) * (PACKED ? 1.f : a.scale2);
+        constexpr int LOOK = PACKED ? 16 * NT / P::STEPS : 0;      // levels looked up
+        float mx = PACKED ? 0.f : ck_max(sc) * a.scale2;
 #pragma unroll
         for (int i = 0; i < 2 * DT; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          if (P::AHEAD || PACKED) __builtin_amdgcn_sched_group_barrier(0x100, (P::AHEAD ? KS / (2 * DT) : 0) + (PACKED ? 1 : 0), 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, (PACKED ? 32 : 16) / (2 * DT) + 1, 0);
+          if (P::EARLY > 0) __builtin_amdgcn_sched_group_barrier(0x100, (P::EARLY + (PACKED ? 10 : 0) + LOOK + 2 * DT - 1) / (2 * DT), 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (PACKED ? 32 + 4 * LOOK : 16) / (2 * DT) + 1, 0);
+        }
+        if constexpr (PACKED) {
+          if (hidden) ck_mask(sc, base, row.pos, a.window);
+          mx = ck_max(sc);
         }
         float alpha;
         if ((t + 1 < P::STEPS || u + 1 < units) && ck_outgrown(st, mx, alpha)) {
@@ -1005,8 +1030,9 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       }
       // ---- what was requested is there
       if constexpr (PACKED) {
-        put(k_after, u + 1);
-        if (turn == 1) note_norms(u - 1 + P::WAVES + wave);
+        if (!busy) put_all(k_after, u + 1);
+        if (turn == 0) note_norms(u + P::WAVES + wave);
+        words = flying;
       } else {
         ck_landed();
       }
