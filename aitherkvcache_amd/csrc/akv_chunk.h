@@ -54,9 +54,12 @@ template <int KIND> struct ck_math {
 
 struct ck_record {                // what a workgroup leaves of the tile that begins in its range and ends in another
   int64_t end;                    // one past the tile on the axis
-  int64_t total;                  // F
-  int32_t valid, head, token, tokens;
+  int64_t total;                  // length of the axis
+  int32_t valid, head, token, tokens;      // valid: CK_LEFT_ of the kernel, 0: none
+  int32_t base, count;            // the workgroups that share the axis
 };
+#define CK_LEFT_NARROW 1
+#define CK_LEFT_WIDE 2
 
 struct ck_args {
   const void* q; int64_t qs_tok, qs_head;        // queries, strides in elements

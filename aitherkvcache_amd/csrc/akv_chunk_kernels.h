@@ -317,7 +317,8 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 template <int D, int KIND> struct ck_narrow {
   static constexpr bool PACKED = KIND >= 2;
   static constexpr int WAVES = PACKED && D < 256 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32, N = 32 * WAVES, START = 3;
-  static constexpr int PER_CU = PACKED || D == 256 ? 1 : 2;
+  static constexpr int PER_CU = PACKED || D == 256 ? 1 : 2, PER_SIMD = D == 256 ? 1 : 2;
+  static constexpr int COST = PACKED ? 3 : D == 256 ? 5 : 2;         // of a unit, beside ck_wide's (2.7 us and 3.6 us of packed rows of 128)
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8, QW = QUADS / WAVES;
   static constexpr int V_BYTES = 32 * 2 * D, ROW = D + 4;            // (of a value; floats of a row that is turned)
   // sums of the wavefronts: the upper half's are added to the lower's first where not all fit
@@ -331,16 +332,16 @@ template <int D, int KIND> struct ck_narrow {
   static __device__ __forceinline__ int f(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3); }
 };
 
+// What workgroup g of G does (workgroups 0 .. G - 1 of the launch), with `slots` pieces a tile in the scratch; `total`: length of one kv head's part of
+// the axis.
 template <int D, int KIND>
-__global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) void ck_narrow_kernel(ck_args a) {
+__device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* const lds, ck_lengths<ck_narrow<D, KIND>::THREADS>& L, const int64_t total, const int g, const int G, const int slots) {
   typedef ck_narrow<D, KIND> P;
   typedef ck_math<KIND> M;
   constexpr bool PACKED = M::packed;
   constexpr int BITS = PACKED ? KIND : 4;
   constexpr int KS = P::KS, DT = P::DT, W = P::WAVES, T = P::THREADS;
   constexpr int HW = D * BITS / 64;                // packed: words of half a row
-  extern __shared__ __align__(1024) unsigned char lds[];
-  ck_lengths<T>& L = *(ck_lengths<T>*)(lds + P::L0);
   float (*const ml)[64][2] = (float (*)[64][2])(lds + P::ML0);
   float (*const nrm)[3][32] = (float (*)[3][32])(lds + P::NRM0);     // packed, per wavefront: key norms, log2 and inverse of value norms
   float* const undo = (float*)(lds + P::UNDO0);    // packed: what undoes the scale of a row of queries
@@ -349,12 +350,8 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
   unsigned char* const area = lds + P::V0;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
-  const int G = gridDim.x;
-  const int g = G % 8 == 0 ? (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
   const int TM = P::ROWS / a.GC;
 
-  ck_load_lengths(a, L);
-  const int64_t total = ck_total<T, P::N, P::START>(a, L, TM);
   // Ranges of one kv head's part of the axis, each taken by as many workgroups as there are heads, side by side on one die: they read the
   // same lines of the cache at the same time.  (A packed row is half a line or less, a norm a thirty-second of one; with the heads one
   // after the other on the axis, cut anywhere, a verification of 350 MB fetched 830.)
@@ -630,7 +627,7 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
     if (wave < P::LEFT) dump(wave);
     __syncthreads();
     const bool whole = u0 == 0 && u1 == keys.units;
-    const int64_t slot = 2 * (int64_t)g + (u0 == 0 ? 1 : 0);
+    const int64_t slot = (2 * (int64_t)g + (u0 == 0 ? 1 : 0)) * slots;
     float4 x[P::QW];
 #pragma unroll
     for (int i = 0; i < P::QW; ++i) {
@@ -647,7 +644,7 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), D == 256 ? 1 : 2) vo
       for (int i = 0; i < P::QW; ++i) ((float4*)a.part)[(slot * P::QUADS + P::QW * wave + i) * 64 + lane] = x[i];
       if (wave == 0) {
         a.part_ml[slot * 64 + lane] = make_float2(m, l);
-        if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
+        if (u0 == 0 && lane == 0) a.rec[g] = {tile_end, total, CK_LEFT_NARROW, head, s.q0 + t0, t1 - t0, 0, G};
       }
     } else {
       ck_results<D, KIND, W, P::QW>(a, x, ck_finish(l), ck_turn_rows<D, false>(a.turn_out, wave), row.valid, row.token, row.head, (float*)area);
@@ -690,8 +687,10 @@ template <int D, int KIND> struct ck_wide {
   static_assert(EARLY == 0 || STEPS == 2, "the step after the next lies in the next unit");
   static constexpr int UNROLL = KIND >= 2 ? 1 : STEPS;
   static constexpr int RING = 2 * WAVES;                              // units whose places and norms are held
+  static constexpr int COST = KIND >= 2 ? 4 : 2;
   static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
-  static constexpr int LDS = NORM0 + (KIND >= 2 ? RING * N * 16 : 0);
+  static constexpr int LUT0 = NORM0 + (KIND >= 2 ? RING * N * 16 : 0), L0 = LUT0 + (KIND >= 2 ? (int)sizeof(ck_lut<KIND >= 2 ? KIND : 4, 1>) : 0);
+  static constexpr int LDS = L0 + (int)sizeof(ck_lengths<THREADS>);
   static __device__ __forceinline__ int fk(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
   static __device__ __forceinline__ int fv(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : 5 * (r & 3); }
 };
@@ -702,8 +701,9 @@ __device__ __forceinline__ void ck_request(const uint8_t* src, uint32_t at) {
 }
 __device__ __forceinline__ void ck_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// What workgroup g of G does, number base + g of the launch; `per_head`: length of one kv head's part of the axis.
 template <int D, int KIND>
-__global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER_SIMD)) void ck_wide_kernel(ck_args a) {
+__device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* const lds, ck_lengths<ck_wide<D, KIND>::THREADS>& L, const int per_head, const int g, const int G, const int base) {
   typedef ck_wide<D, KIND> P;
   typedef ck_math<KIND> M;
   constexpr bool PACKED = M::packed;
@@ -713,24 +713,19 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   constexpr int RPI = 64 / CPR, NP = N / RPI / P::WAVES;      // dense: rows a request, requests a wavefront
   constexpr int TPR = D / 32, TASKS = N * TPR, NT = 2 * TASKS / T;      // packed: 32 codes a task, keys' then values'
   static_assert(NT * T == 2 * TASKS && NP * RPI * P::WAVES == N, "whole tasks and requests");
-  extern __shared__ __align__(1024) unsigned char lds[];
-  __shared__ ck_lengths<T> L;
-  __shared__ ck_lut<BITS, 1> lut;
+  typedef ck_lut<BITS, 1> lut_type;
+  lut_type& lut = *(lut_type*)(lds + P::LUT0);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
-  const int G = gridDim.x;
-  const int g = G % 8 == 0 ? (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8) : (int)blockIdx.x;
   const int TM = P::ROWS / a.GC;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
-  ck_load_lengths(a, L);
-  const int per_head = ck_total<T, N, P::START>(a, L, TM);
   const int heads = a.KVH * a.HS;
   const int64_t total = (int64_t)per_head * heads;
   const ck_share share = ck_share_of(total, G);
   int64_t at = ck_begin(share, g, G);
   const int64_t end = ck_begin(share, g + 1, G);
-  if (tid == 0) a.rec[g].valid = 0;
+  if (tid == 0) a.rec[base + g].valid = 0;
   if (at >= end) return;
   int head = (int)(at / per_head), seq, tile, first;
   ck_find<T, N, P::START>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
@@ -825,12 +820,15 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
     // nothing is zero
     struct codes { uint32_t w[PACKED ? NT : 1][BITS]; };
     codes words;
+    // (the wavefront's own choice of the two, and by value: taken from the arguments' memory it made every request a generic one, for which reads
+    // of LDS wait)
+    const uint8_t *const k_base = a.k, *const v_base = a.v;
     auto fetch = [&](int uk, int uv, codes& c) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const int task = tid + T * i, v = task / TASKS, r = task % TASKS / TPR, part = task % TPR;
+        const int task = tid + T * i, v = (64 * wave + T * i) / TASKS, r = task % TASKS / TPR, part = task % TPR;
         const int64_t* place = (const int64_t*)(lds + P::PLACE0) + ((v ? uv : uk) & (P::RING - 1)) * 2 * N + v * N;
-        ck_load_words(c.w[i], (v ? a.v : a.k) + place[r] + 4 * BITS * part);
+        ck_load_words(c.w[i], (v ? v_base : k_base) + place[r] + 4 * BITS * part);
       }
     };
     // ... the part `step` of STEPS of them
@@ -959,7 +957,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
       const float* nr = (const float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
       const uint32_t v_from = (u & 1) * P::TILE;
       if (busy)
-#pragma unroll (P::UNROLL)
+#pragma unroll P::UNROLL
       for (int t = 0; t < P::STEPS; ++t) {
         // ---- weights of these keys, products of the next 32 (behind the last: of whatever lies there, unused), values to registers
         if (!P::AHEAD) read_keys(t + 1 < P::STEPS ? k_slot * P::TILE + (t + 1) * 32 * P::ROW : k_next * P::TILE, P::EARLY, KS);
@@ -990,6 +988,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
         }
         // (the weights stay on this side of the branch: behind it they would have no products to run beside)
         asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(st.l));
+        if constexpr (PACKED) __builtin_amdgcn_sched_barrier(0);
         // ---- what the next step's rows do not see
         const int base = base0 + u * N + 32 * (t + 1);
         const float* nn = t + 1 < P::STEPS ? nr + 32 * (t + 1) : (const float*)(lds + P::NORM0) + ((u + 1) & (P::RING - 1)) * 4 * N;
@@ -1062,14 +1061,14 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
           ck_store<KIND>(a, row.token, row.head, c, o[c / 4][4 * (c & 3)] * f, o[c / 4][4 * (c & 3) + 1] * f, o[c / 4][4 * (c & 3) + 2] * f, o[c / 4][4 * (c & 3) + 3] * f);
       }
     } else {
-      const int64_t slot = (2 * (int64_t)g + (u0 == 0 ? 1 : 0)) * P::WAVES + wave;
+      const int64_t slot = (2 * (int64_t)(base + g) + (u0 == 0 ? 1 : 0)) * P::WAVES + wave;
       if (busy) {
 #pragma unroll
         for (int c = 0; c < P::QUADS; ++c)
           ((float4*)a.part)[(slot * P::QUADS + c) * 64 + lane] = make_float4(o[c / 4][4 * (c & 3)] * unit, o[c / 4][4 * (c & 3) + 1] * unit, o[c / 4][4 * (c & 3) + 2] * unit, o[c / 4][4 * (c & 3) + 3] * unit);
         a.part_ml[slot * 64 + lane] = make_float2(st.m, st.l);
       }
-      if (u0 == 0 && tid == 0) a.rec[g] = {tile_end, total, 1, head, s.q0 + t0, t1 - t0};
+      if (u0 == 0 && tid == 0) a.rec[base + g] = {tile_end, total, CK_LEFT_WIDE, head, s.q0 + t0, t1 - t0, base, G};
     }
     at = tile_at = tile_end;
     if (at >= end) return;
@@ -1083,16 +1082,75 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   }
 }
 
+// ---- kernels -------------------------------------------------------------------------------------------------------------------
+// Nothing in LDS is static: the narrow kernel's table of levels begins at 0, the lengths lie behind everything.
+template <class P> __device__ __forceinline__ ck_lengths<P::THREADS>& ck_lengths_at(unsigned char* lds, int at) { return *(ck_lengths<P::THREADS>*)(lds + at); }
+// Workgroups in the order in which they lie on the dies.
+__device__ __forceinline__ int ck_workgroup() {
+  const int G = gridDim.x, b = blockIdx.x;
+  return G % 8 == 0 ? b % 8 * (G / 8) + b / 8 : b;
+}
+template <int D, int KIND>
+__global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), (ck_narrow<D, KIND>::PER_SIMD)) void ck_narrow_kernel(ck_args a) {
+  typedef ck_narrow<D, KIND> P;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  auto& L = ck_lengths_at<P>(lds, P::L0);
+  ck_load_lengths(a, L);
+  const int64_t total = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
+  ck_narrow_work<D, KIND>(a, lds, L, total, ck_workgroup(), gridDim.x, 1);
+}
+template <int D, int KIND>
+__global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER_SIMD)) void ck_wide_kernel(ck_args a) {
+  typedef ck_wide<D, KIND> P;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  auto& L = ck_lengths_at<P>(lds, P::L0);
+  ck_load_lengths(a, L);
+  const int per_head = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
+  ck_wide_work<D, KIND>(a, lds, L, per_head, ck_workgroup(), gridDim.x, 0);
+}
+// Both at once: the workgroups are divided by what each has to do.  (One kernel after the other the few rows of a mixed batch take as long as
+// a workgroup needs to begin and to end: 12 sequences of 1 to 90 tokens over 3 bits, 152 us.)
+template <int D, int KIND> struct ck_both {
+  typedef ck_narrow<D, KIND> N;
+  typedef ck_wide<D, KIND> W;
+  static constexpr bool FITS = N::THREADS == W::THREADS && N::PER_CU == W::PER_CU;
+  static constexpr int L0 = N::L0 > W::L0 ? N::L0 : W::L0, LDS = L0 + (int)sizeof(ck_lengths<W::THREADS>);
+};
+template <int D, int KIND>
+__global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER_SIMD)) void ck_both_kernel(ck_args few, ck_args many) {
+  typedef ck_narrow<D, KIND> N;
+  typedef ck_wide<D, KIND> W;
+  extern __shared__ __align__(1024) unsigned char lds[];
+  auto& L = ck_lengths_at<W>(lds, ck_both<D, KIND>::L0);
+  ck_load_lengths(many, L);
+  const int few_total = ck_total<N::THREADS, N::N, N::START>(few, L, N::ROWS / few.GC), many_total = ck_total<W::THREADS, W::N, W::START>(many, L, W::ROWS / many.GC);
+  const int G = gridDim.x, g = ck_workgroup(), few_heads = few.KVH * few.HS;
+  const float few_cost = (float)N::COST * (float)few_heads * (float)few_total, many_cost = (float)W::COST * (float)(many.KVH * many.HS) * (float)many_total;
+  int ranges = 0;
+  if (few_total > 0) {
+    ranges = (int)((float)G * few_cost / ((few_cost + many_cost) * (float)few_heads) + 0.5f);
+    ranges = max(1, min(ranges, (many_total > 0 ? G - 1 : G) / few_heads));
+  }
+  const int taken = ranges * few_heads;
+  if (g < taken) ck_narrow_work<D, KIND>(few, lds, L, few_total, g, taken, W::WAVES);
+  else ck_wide_work<D, KIND>(many, lds, L, many_total, g - taken, G - taken, taken);
+}
+
 // ---- the pieces of a tile that several ranges share --------------------------------------------------------------------------
 // Workgroup (g, w): the 32 rows w of the tile that begins in workgroup g's range and does not end there; its other pieces are the first ones
-// of the ranges behind, which are `stride` workgroups apart.  Their maxima are looked through first, so that the sums of up to four pieces are on their way together.
+// of the ranges behind, which are a workgroup apart (many rows) or as many as there are heads (few).  Their maxima are looked through first, so that the sums of up to four pieces are on their way together.
+struct ck_cut { int HS, GC; };        // of the few rows' kernel
 template <int D, int KIND, int WAVES>
-__global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_kernel(ck_args a, int G, int stride) {
+__global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_kernel(ck_args a, ck_cut few) {
   constexpr int QUADS = D / 8, MINE = QUADS / 4;
   __shared__ __align__(16) float rows[ck_math<KIND>::packed ? 32 * (D + 4) : 1];
-  const int g = blockIdx.x, part = blockIdx.y;
-  const ck_record rec = a.rec[g];
-  if (!rec.valid || 32 * part >= rec.tokens * a.GC) return;      // (rows behind the tile's last: nothing was left of them)
+  const int part = blockIdx.y;
+  const ck_record rec = a.rec[blockIdx.x];
+  if (rec.valid == 0) return;
+  const bool narrow = WAVES == 1 || rec.valid == CK_LEFT_NARROW;
+  const int HS = narrow ? few.HS : a.HS, GC = narrow ? few.GC : a.GC;
+  if (32 * part >= rec.tokens * GC) return;      // (rows behind the tile's last: nothing was left of them)
+  const int stride = narrow ? a.KVH * HS : 1, g = (int)blockIdx.x - rec.base, G = rec.count;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31;
   ck_turn_rows<D, ck_math<KIND>::packed && D < 256 && WAVES == 1> matrix(a.turn_out, wave);
   // ranges first + 1 .. last hold a piece each, unless they are empty
@@ -1116,7 +1174,7 @@ __global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_
       }
       const bool there = r < R;
       more = there;
-      const int64_t slot = (2 * (int64_t)((there ? r : first) * stride + g % stride) + (!there || r == first ? 1 : 0)) * WAVES + part;
+      const int64_t slot = (2 * (int64_t)(rec.base + (there ? r : first) * stride + g % stride) + (!there || r == first ? 1 : 0)) * WAVES + part;
       e[k] = a.part_ml[slot * 64 + lane];
 #pragma unroll
       for (int i = 0; i < MINE; ++i) y[k][i] = ((const float4*)a.part)[(slot * QUADS + MINE * wave + i) * 64 + lane];
@@ -1141,8 +1199,8 @@ __global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_
     }
     m = top;
   }
-  const int row = 32 * part + col, j = row / a.GC, gq = (rec.head % a.HS) * a.GC + row - j * a.GC;
-  ck_results<D, KIND, 4, MINE>(a, x, ck_finish(l), matrix, j < rec.tokens && gq < a.G, rec.token + j, (rec.head / a.HS) * a.G + gq, rows);
+  const int row = 32 * part + col, j = row / GC, gq = (rec.head % HS) * GC + row - j * GC;
+  ck_results<D, KIND, 4, MINE>(a, x, ck_finish(l), matrix, j < rec.tokens && gq < a.G, rec.token + j, (rec.head / HS) * a.G + gq, rows);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
@@ -1165,6 +1223,10 @@ static inline ck_scratch ck_scratch_layout(int D) {
 }
 static inline uint32_t ck_reciprocal(int d) { return (uint32_t)(0xffffffffull / (uint32_t)d); }
 
+static inline int ck_lds(const void* kernel, int bytes) {
+  AKV_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return AKV_OK;
+}
 template <int D, int KIND>
 static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream) {
   typedef ck_wide<D, KIND> W;
@@ -1176,42 +1238,46 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
   // each takes its own, by the lengths on the device.
   const int64_t most = most_new > 0 && most_new < a.T ? most_new : a.T;
   const bool few = most * a.G <= CK_NARROW_ROWS, one = !few && a.S == 1;
+  typedef ck_narrow<D, KIND> N;
+  typedef ck_both<D, KIND> B;
+  ck_args n = a, m = a;
+  n.kind = few ? 0 : 1;
+  n.HS = (a.G + 31) / 32;
+  n.GC = (a.G + n.HS - 1) / n.HS;
+  m.kind = one ? 0 : 2;
+  m.HS = (a.G + W::ROWS - 1) / W::ROWS;
+  m.GC = (a.G + m.HS - 1) / m.HS;
+  const ck_cut cut = {n.HS, n.GC};
+  const int heads = n.KVH * n.HS, most_groups = ck_groups(W::PER_CU);
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
-  if (!one) {
-    ck_args n = a;
-    n.kind = few ? 0 : 1;
-    n.HS = (a.G + 31) / 32;
-    n.GC = (a.G + n.HS - 1) / n.HS;
-    typedef ck_narrow<D, KIND> P;
-    static akv_device_once once;
-    const int rc = once(dev, [&]() -> int {
-      AKV_HIP(hipFuncSetAttribute((const void*)ck_narrow_kernel<D, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS));
+  if constexpr (B::FITS) {
+    if (!few && !one && 2 * heads <= most_groups) {
+      static akv_device_once once;
+      if (const int rc = once(dev, [&]() -> int { return ck_lds((const void*)ck_both_kernel<D, KIND>, B::LDS); })) return rc;
+      ck_both_kernel<D, KIND><<<most_groups, W::THREADS, B::LDS, stream>>>(n, m);
+      AKV_LAUNCH_CHECK("ck_both_kernel");
+      ck_merge_kernel<D, KIND, W::WAVES><<<dim3(most_groups, W::WAVES), 256, 0, stream>>>(m, cut);
+      AKV_LAUNCH_CHECK("ck_merge_kernel");
       return AKV_OK;
-    });
-    if (rc) return rc;
-    const int heads = n.KVH * n.HS, ranges = ck_groups(P::PER_CU) / heads, G = heads * (ranges > 1 ? ranges : 1);
+    }
+  }
+  if (!one) {
+    static akv_device_once once;
+    if (const int rc = once(dev, [&]() -> int { return ck_lds((const void*)ck_narrow_kernel<D, KIND>, N::LDS); })) return rc;
+    const int ranges = ck_groups(N::PER_CU) / heads, G = heads * (ranges > 1 ? ranges : 1);
     if (G > CK_GROUPS) return akv_fail(AKV_ERR_UNSUPPORTED, "more than %d kv heads", CK_GROUPS);
-    ck_narrow_kernel<D, KIND><<<G, P::THREADS, P::LDS, stream>>>(n);
+    ck_narrow_kernel<D, KIND><<<G, N::THREADS, N::LDS, stream>>>(n);
     AKV_LAUNCH_CHECK("ck_narrow_kernel");
-    ck_merge_kernel<D, KIND, 1><<<dim3(G, 1), 256, 0, stream>>>(n, G, heads);
+    ck_merge_kernel<D, KIND, 1><<<dim3(G, 1), 256, 0, stream>>>(n, cut);
     AKV_LAUNCH_CHECK("ck_merge_kernel");
   }
   if (!few) {
-    ck_args n = a;
-    n.kind = one ? 0 : 2;
-    n.HS = (a.G + W::ROWS - 1) / W::ROWS;
-    n.GC = (a.G + n.HS - 1) / n.HS;
     static akv_device_once once;
-    const int rc = once(dev, [&]() -> int {
-      AKV_HIP(hipFuncSetAttribute((const void*)ck_wide_kernel<D, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, W::LDS));
-      return AKV_OK;
-    });
-    if (rc) return rc;
-    const int G = ck_groups(W::PER_CU);
-    ck_wide_kernel<D, KIND><<<G, W::THREADS, W::LDS, stream>>>(n);
+    if (const int rc = once(dev, [&]() -> int { return ck_lds((const void*)ck_wide_kernel<D, KIND>, W::LDS); })) return rc;
+    ck_wide_kernel<D, KIND><<<most_groups, W::THREADS, W::LDS, stream>>>(m);
     AKV_LAUNCH_CHECK("ck_wide_kernel");
-    ck_merge_kernel<D, KIND, W::WAVES><<<dim3(G, W::WAVES), 256, 0, stream>>>(n, G, 1);
+    ck_merge_kernel<D, KIND, W::WAVES><<<dim3(most_groups, W::WAVES), 256, 0, stream>>>(m, cut);
     AKV_LAUNCH_CHECK("ck_merge_kernel");
   }
   return AKV_OK;

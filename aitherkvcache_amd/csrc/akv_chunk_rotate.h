@@ -14,21 +14,24 @@
 // k of element j of a lane of half h in a step of sixteen: queries 8 h + j; results in the order in which the second product of attention
 // leaves them, 4 h + j and 8 + 4 h + j - 4
 __host__ __device__ constexpr int ck_result_k(int h, int j) { return 4 * h + (j & 3) + 8 * (j >> 2); }
-// (a pointer the compiler knows nothing of: it would keep the whole table in registers from one tile for the next)
-__device__ __forceinline__ const uint4* ck_turn_table(const uint4* table) {
-  asm volatile("" : "+s"(table));
-  return table;
+// (a pointer the compiler knows nothing of: it would keep the whole table in registers from one tile for the next; but one to device memory: reads
+// of LDS would wait for a generic one)
+typedef const __attribute__((address_space(1))) ck_u4* ck_table;
+__device__ __forceinline__ ck_table ck_turn_table(const uint4* table) {
+  ck_table t = (ck_table)(uintptr_t)table;
+  asm volatile("" : "+s"(t));
+  return t;
 }
-__device__ __forceinline__ const uint4* ck_turn_at(const uint4* table, int D, int term, int dt, int ks) {
-  return table + (((size_t)term * (D / 32) + dt) * (D / 16) + ks) * 64 + (threadIdx.x & 63);
+__device__ __forceinline__ ck_u4 ck_turn_at(ck_table table, int D, int term, int dt, int ks) {
+  return table[(((size_t)term * (D / 32) + dt) * (D / 16) + ks) * 64 + (threadIdx.x & 63)];
 }
 // Rows dt of M times rows held as operands: one term (queries) ...
 template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restrict__ all, int dt, const ck_u4 (&x)[D / 16]) {
-  const uint4* table = ck_turn_table(all);
+  const ck_table table = ck_turn_table(all);
   ck_f16v y = (ck_f16v)(0.f);
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) {
-    const ck_u4 lo = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 1, dt, ks)), hi = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 0, dt, ks));
+    const ck_u4 lo = ck_turn_at(table, D, 1, dt, ks), hi = ck_turn_at(table, D, 0, dt, ks);
     y = ck_math<CK_F16>::mfma(lo, x[ks], y);
     y = ck_math<CK_F16>::mfma(hi, x[ks], y);
     if ((ks & 3) == 3) __builtin_amdgcn_sched_barrier(0);      // (no more of the table than this in registers)
@@ -37,11 +40,11 @@ template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restr
 }
 // ... or two (results)
 template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restrict__ all, int dt, const ck_u4 (&x)[D / 16], const ck_u4 (&xl)[D / 16]) {
-  const uint4* table = ck_turn_table(all);
+  const ck_table table = ck_turn_table(all);
   ck_f16v y = (ck_f16v)(0.f);
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) {
-    const ck_u4 lo = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 1, dt, ks)), hi = __builtin_bit_cast(ck_u4, *ck_turn_at(table, D, 0, dt, ks));
+    const ck_u4 lo = ck_turn_at(table, D, 1, dt, ks), hi = ck_turn_at(table, D, 0, dt, ks);
     y = ck_math<CK_F16>::mfma(lo, x[ks], y);
     y = ck_math<CK_F16>::mfma(hi, xl[ks], y);
     y = ck_math<CK_F16>::mfma(hi, x[ks], y);
@@ -53,12 +56,12 @@ template <int D> __device__ __forceinline__ ck_f16v ck_turn(const uint4* __restr
 // requested before the results are there.
 template <int D, bool HELD> struct ck_turn_rows {
   const uint4* all;
-  uint4 x[HELD ? 2 * (D / 16) : 1];
+  ck_u4 x[HELD ? 2 * (D / 16) : 1];
   __device__ __forceinline__ ck_turn_rows(const uint4* table, int dt) : all(table) {
     if constexpr (HELD) {
       if (dt < D / 32) {
 #pragma unroll
-        for (int i = 0; i < 2 * (D / 16); ++i) x[i] = *ck_turn_at(table, D, i & 1, dt, i >> 1);
+        for (int i = 0; i < 2 * (D / 16); ++i) x[i] = ck_turn_at((ck_table)(uintptr_t)table, D, i & 1, dt, i >> 1);
       }
     }
   }
@@ -67,7 +70,7 @@ template <int D, bool HELD> struct ck_turn_rows {
     ck_f16v y = (ck_f16v)(0.f);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      const ck_u4 m_hi = __builtin_bit_cast(ck_u4, x[HELD ? 2 * ks : 0]), m_lo = __builtin_bit_cast(ck_u4, x[HELD ? 2 * ks + 1 : 0]);
+      const ck_u4 m_hi = x[HELD ? 2 * ks : 0], m_lo = x[HELD ? 2 * ks + 1 : 0];
       y = ck_math<CK_F16>::mfma(m_lo, hi[ks], y);
       y = ck_math<CK_F16>::mfma(m_hi, lo[ks], y);
       y = ck_math<CK_F16>::mfma(m_hi, hi[ks], y);

@@ -295,3 +295,26 @@ def test_rope_append_of_many_tokens(dev, dtype, cache_dtype, sections):
     check_rope(got, *rope_reference(x[:, :heads], pos, table, sections, False))
     check_rope(kc.flatten(0, 1)[slots], *rope_reference(x[:, heads:heads + kv], pos, table, sections, False))
     assert torch.equal(vc.flatten(0, 1)[slots], x[:, heads + kv:].to(cache_dtype))
+
+
+@pytest.mark.parametrize("d,heads,kv", [(256, 130, 130), (64, 300, 300), (128, 129, 129)])
+def test_mixed_batch_of_many_heads(dev, d, heads, kv):
+    """More kv heads than half the workgroups: few and many rows are not divided over one launch."""
+    b = Batch([(66, 100), (1, 70), (3, 40)], 16, dev, 11)
+    q, kc, vc = (vectors(140 + i, dev, BF, *s) for i, s in enumerate(((b.tokens, heads, d), (b.blocks, 16, kv, d), (b.blocks, 16, kv, d))))
+    check(akv.paged_chunk_attention(q, kc, vc, b.tables, b.ctx, b.starts), *dense_reference(b, q, kc, vc, 1 / math.sqrt(d), 0))
+    if d > 64:
+        p = Packed(b, d, 4, heads, kv, BF, dev, 141)
+        check(p.run(), *p.reference())
+
+
+@pytest.mark.parametrize("few,many", [(1, 40), (40, 1), (12, 12)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_shares_of_a_mixed_batch(dev, few, many, d):
+    """Workgroups divided between few and many rows, whichever has more to do."""
+    b = Batch([(1 + i % 3, 100 + 177 * i) for i in range(few)] + [(70 + 9 * i, 200 + 50 * i) for i in range(many)], 16, dev, 12)
+    q, kc, vc = (vectors(150 + i, dev, FP, *s) for i, s in enumerate(((b.tokens, 8, d), (b.blocks, 16, 2, d), (b.blocks, 16, 2, d))))
+    check(akv.paged_chunk_attention(q, kc, vc, b.tables, b.ctx, b.starts), *dense_reference(b, q, kc, vc, 1 / math.sqrt(d), 0))
+    for bits in (4, 3, 2):
+        p = Packed(b, d, bits, 8, 2, FP, dev, 151)
+        check(p.run(), *p.reference())
