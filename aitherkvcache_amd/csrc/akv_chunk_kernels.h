@@ -27,31 +27,45 @@
 
 // ---- packed codes -> float16 levels -----------------------------------------------------------------------------
 // Value of the levels' last place, so to say: a level is a float16 number times this.  Any unit would do (scores take it with the key's norm,
-// outputs in the end); of 64 between two powers of two every wavefront picks the one whose float16 levels are nearest to the
-// codebook, the same everywhere: 16 levels are then off by a third of what a power of two leaves, 2^-13.6 of themselves instead of 2^-12.
-template <int BITS> __device__ __forceinline__ float ck_unit(const float* __restrict__ centroids) {
-  const int lane = threadIdx.x & 63;
-  float c[1 << BITS], m = 0.f;
+// outputs in the end); of 64 N between two powers of two the one is picked whose float16 levels are nearest to the codebook.  With 64 the
+// sixteen levels of four bits are off by a third of what a power of two leaves, 2^-13.6 of themselves instead of 2^-12; with 1024 by a quarter.
+// `own`: level lane % 2^BITS.  ck_unit_key: the best of the units from..from + N - 1 of every lane of a wavefront, as a number that is less
+// for a better one; ck_unit_of: the unit.
+template <int BITS> __device__ __forceinline__ float ck_largest_level(float own, float (&c)[1 << BITS]) {
+  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < (1 << BITS); ++i) {
-    c[i] = centroids[i];
+    c[i] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), i));
     m = fmaxf(m, fabsf(c[i]));
   }
+  return m;
+}
+template <int BITS, int N, int TOTAL> __device__ __forceinline__ uint32_t ck_unit_key(float own, int from) {
+  float c[1 << BITS];
   // the largest to [16, 32) x (1 .. 2): levels down to 2^-18 of it are normal numbers
-  const float down = akv_row_scale(akv_row_exponent(m)) * (16.f + 0.25f * lane);
-  float off = 0.f;
+  const float up = akv_row_scale(akv_row_exponent(ck_largest_level<BITS>(own, c)));
+  uint32_t best = 0xffffffffu;
+#pragma unroll 1
+  for (int n = from; n < from + N; ++n) {
+    const float s = 16.f + (16.f / TOTAL) * (float)n;
+    float off = 0.f;
 #pragma unroll
-  for (int i = 0; i < (1 << BITS); ++i) {
-    const float x = c[i] * down, e = (float)(_Float16)x - x;
-    off = fmaf(e, e, off);
+    for (int i = 0; i < (1 << BITS); ++i) {
+      const float x = c[i] * (up * s), e = (float)(_Float16)x - x;
+      off = fmaf(e, e, off);
+    }
+    off *= __builtin_amdgcn_rcpf(s * s);
+    // the least, of equal ones the first; a codebook that is not finite leaves the first
+    best = min(best, (off < INFINITY ? __float_as_uint(off) & ~(uint32_t)(TOTAL - 1) : 0x7f800000u) | (uint32_t)n);
   }
-  off *= __builtin_amdgcn_rcpf((16.f + 0.25f * lane) * (16.f + 0.25f * lane));
-  // the least, of equal ones the first; a codebook that is not finite leaves the first
-  uint32_t key = off < INFINITY ? (__float_as_uint(off) & ~63u) | (uint32_t)lane : 0x7f800000u | (uint32_t)lane;
-  key = min(key, akv_lane_xor_u32<32>(key)); key = min(key, akv_lane_xor_u32<16>(key)); key = min(key, akv_lane_xor_u32<8>(key));
-  key = min(key, akv_lane_xor_u32<4>(key)); key = min(key, akv_lane_xor_u32<2>(key)); key = min(key, akv_lane_xor_u32<1>(key));
-  const float best = 16.f + 0.25f * (float)(__builtin_amdgcn_readfirstlane((int)(key & 63u)));
-  return akv_row_unscale(akv_row_exponent(m)) / best;
+  best = min(best, akv_lane_xor_u32<32>(best)); best = min(best, akv_lane_xor_u32<16>(best)); best = min(best, akv_lane_xor_u32<8>(best));
+  best = min(best, akv_lane_xor_u32<4>(best)); best = min(best, akv_lane_xor_u32<2>(best)); best = min(best, akv_lane_xor_u32<1>(best));
+  return best;
+}
+template <int BITS, int TOTAL> __device__ __forceinline__ float ck_unit_of(float own, uint32_t key) {
+  float c[1 << BITS];
+  const float s = 16.f + (16.f / TOTAL) * (float)(__builtin_amdgcn_readfirstlane((int)key) & (TOTAL - 1));
+  return akv_row_unscale(akv_row_exponent(ck_largest_level<BITS>(own, c))) / s;
 }
 // Levels from a table in LDS, of two codes at a time (four where a byte holds them).  COPIES of 64: every lane has its own, so that no two
 // meet a bank (a shared table of 256 entries cost 9 clocks a look-up: lanes meet banks, codes in the middle are frequent).
@@ -365,7 +379,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
   ck_find<T, P::N, P::START>(a, L, TM, (int)at, seq, tile, first);
   int64_t tile_at = first;             // the tile's place on the axis
 
-  float unit = 1.f, turned = 0.f;      // of the levels; what undoes the matrix's scale, times the scale of the scores
+  float unit = 1.f, level = 0.f, turned = 0.f;      // of the levels; the lane's level; what undoes the matrix's scale, times the scale of the scores
   bool filled = false;
 
   for (;;) {
@@ -429,7 +443,8 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
           un = ck_query_operand<D>(x, a.dtype);
         }
         if (!filled) {
-          unit = ck_unit<BITS>(a.centroids);
+          level = a.centroids[lane & ((1 << BITS) - 1)];
+          ((uint32_t*)ml)[wave] = ck_unit_key<BITS, 16 / W, 1024>(level, 16 / W * (64 * wave + lane));
           turned = a.turn_scale->up * (1.f / CK_TURN) * a.scale2;
         }
         __syncthreads();           // (the area has been read)
@@ -443,6 +458,10 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
           }
         }
         if (!filled) {
+          uint32_t key = ((uint32_t*)ml)[0];
+#pragma unroll
+          for (int w = 1; w < W; ++w) key = min(key, ((uint32_t*)ml)[w]);
+          unit = ck_unit_of<BITS, 1024>(level, key);
           ((lut_type*)lds)->fill(a.centroids, tid, T, unit);
           filled = true;
         }
@@ -733,7 +752,8 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
 
   float unit = 1.f;                // of the levels
   if constexpr (PACKED) {
-    unit = ck_unit<BITS>(a.centroids);
+    const float level = a.centroids[lane & ((1 << BITS) - 1)];
+    unit = ck_unit_of<BITS, 64>(level, ck_unit_key<BITS, 1, 64>(level, lane));
     lut.fill(a.centroids, tid, T, unit);
   }
   // where the lane reads its operands: a piece of a key, four coordinates of a value
@@ -1237,7 +1257,10 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
   // Few rows a sequence as far as the host can tell: the narrow kernel takes all of them.  One sequence of more: the wide one.  Otherwise
   // each takes its own, by the lengths on the device.
   const int64_t most = most_new > 0 && most_new < a.T ? most_new : a.T;
-  const bool few = most * a.G <= CK_NARROW_ROWS, one = !few && a.S == 1;
+  // Packed rows and float16: all of them as well.  The wide kernel has no registers for the queries' second term, without which float16
+  // outputs are off by 4e-4 to 5e-4 of their size instead of 2.1e-4 (their own rounding)
+  // to 2.8e-4.  Four bits, 32 heads of 128: 126 us over 12 turns of 1 to 90 tokens (wide kernel 144), 891 over two prompts of 1000 (493).
+  const bool few = most * a.G <= CK_NARROW_ROWS || (KIND >= 2 && a.dtype == AKV_F16), one = !few && a.S == 1;
   typedef ck_narrow<D, KIND> N;
   typedef ck_both<D, KIND> B;
   ck_args n = a, m = a;
