@@ -74,7 +74,7 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     scale           of the scores (1 / sqrt(head_dim));  window > 0: a token sees the newest `window` keys, its own among them
     out             where the result goes (same shape and type as query; rows behind the last sequence are left as they were);
                     without it a new tensor, zero in such rows
-    max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result does not
+    max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
     Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256."""
     result = _lib.calls().dense_chunk(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, scale, window, out,

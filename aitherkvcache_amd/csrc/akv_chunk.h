@@ -7,10 +7,9 @@
 //
 // The tiles of a sequence, of all sequences, once for every kv head, lie end to end on one axis, each as long as its units (runs of
 // keys) and START more, what a tile costs besides: rows, first keys, results.  Workgroup g of G takes what lies in [g F / G, (g + 1) F / G)
-// of that axis.  So every workgroup has as much to do, however the lengths are spread and whatever the causal edge leaves of a
-// tile, and few rows over many keys are split by themselves.  A
-// tile that lies in one range is finished there; the pieces of one that does not go to memory and are joined by ck_merge_kernel
-// in the order of the axis.  All of it is derived on the device: no call waits for a length.
+// of that axis.  So every workgroup has as much to do, however the lengths are spread and whatever the causal edge leaves of a tile, and
+// few rows over many keys are split by themselves.  A tile that lies in one range is finished there; the pieces of one that does not go
+// to memory and are joined by ck_merge_kernel in the order of the axis.  All of it is derived on the device: no call waits for a length.
 #pragma once
 #include "akv_attn_common.h"
 

@@ -10,11 +10,13 @@
 // axis takes the keys in the order in which a lane holds them, 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3 of sixteen.  V^T comes out of
 // LDS by transposing reads (ds_read_b64_tr_b16: four keys of a coordinate a lane).
 //
-// Packed rows are attended in the rotated domain: queries are rotated before (ck_rotate_q_kernel), outputs after
-// (ck_rotate_out_kernel), and in between a key is its norm times levels of the codebook.  Levels are float16 in units of a power of
-// two (relative precision 2^-11 whatever the codebook's size); a key's norm multiplies its score in float32; a value's norm v goes into the
-// exponent, w = 2^(s + log2 v - M), with M the running maximum of s + log2 v, so weights stay in [0, 1] for norms of any size,
-// and the sum of the softmax takes w / v.
+// Packed rows are attended in the rotated domain: queries are rotated on the way in, results on the way out (akv_chunk_rotate.h), and in
+// between a key is its norm times levels of the codebook.  Levels are float16 in a unit that loses little of them (ck_unit_key); a key's
+// norm multiplies its score in float32; a value's norm v goes into the exponent, w = 2^(s + log2 v - M), with M the running maximum of
+// s + log2 v, so weights stay in [0, 2^CK_FRAME] for norms of any size, and the sum of the softmax takes w / v.
+//
+// What is rounded to sixteen bits: the weights, once, as operand of the second product (relative 2^-11 or 2^-8, as of the values beside them);
+// packed: the levels (2^-14) and the queries (many rows: one float16 term; few rows: two, 2^-22).  Scores, maxima, sums and results are float32.
 #pragma once
 #include "akv_chunk_rotate.h"
 #include "akv_device_once.h"
@@ -326,13 +328,15 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 // ---- few rows a sequence ---------------------------------------------------------------------------------------------------
 // A tile is 32 rows, a unit 32 keys a wavefront: each takes its own, keys straight from memory into the operand, values through its
 // part of LDS (sixteen bytes c of value t lie at c ^ f(t), which 16 rows written and 4 read at a time meet all banks with); what the
-// wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Reading the cache bounds it, and for packed rows the
-// vector unit: some 300 instructions for 32 keys.
+// wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Packed codes of two units are on their way at a
+// time.  32 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
+// look-ups and operands in LDS (48%) and waits in turn bound it, some 22 us before the first unit and 10 after the last.  Heads of 256,
+// bfloat16, a window of 1024 keys, 38 MB: 39 us, which is latency: lengths, table, keys, the second unit's keys, pieces, their join.
 template <int D, int KIND> struct ck_narrow {
   static constexpr bool PACKED = KIND >= 2;
   static constexpr int WAVES = PACKED && D < 256 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32, N = 32 * WAVES, START = 3;
   static constexpr int PER_CU = PACKED || D == 256 ? 1 : 2, PER_SIMD = D == 256 ? 1 : 2;
-  static constexpr int COST = PACKED ? 3 : D == 256 ? 5 : 2;         // of a unit, beside ck_wide's (2.7 us and 3.6 us of packed rows of 128)
+  static constexpr int COST = PACKED ? 3 : D == 256 ? 5 : 2;         // of a unit, beside ck_wide's (packed rows of 128: 2.7 us and 3.6 us)
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8, QW = QUADS / WAVES;
   static constexpr int V_BYTES = 32 * 2 * D, ROW = D + 4;            // (of a value; floats of a row that is turned)
   // sums of the wavefronts: the upper half's are added to the lower's first where not all fit
@@ -688,6 +692,11 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
 // products and 16 weights 1417 clocks, in turns 1071).  Keys of unit u + 2 and values of u + 1 are on their way during unit u; packed ones
 // are put to LDS then, beside the value products, from codes that were requested a unit before (all at the end of a unit: 2000 rows over
 // 8000 keys, 32 heads, 445 us instead of 422).
+//
+// The matrix cores bound it as far as the chip's power allows: 2048 rows over 31000 keys, 32 heads of 128 in bfloat16 take 1060 to 1120 us by the
+// machine, 1000 TFLOP/s, where a large product of the library reaches 1280 (products 47% of the clocks; written out in turns by hand it is no
+// faster).  Heads of 64 are bound by the vector unit, 60% of the clocks.  Packed rows of 128: 630 TFLOP/s; codes are looked up by every
+// workgroup for its 256 rows, LDS is busy 46% and the vector unit 55% of the clocks, and registers leave no room for more in flight.
 //
 // Rows lie in LDS without padding, their pieces of sixteen bytes in an order that depends on the row, piece c at place c ^ f(row): sixteen
 // lanes that read one piece of sixteen keys, and 32 that read four coordinates each of four values, meet all 64 banks once
@@ -1129,7 +1138,8 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   ck_wide_work<D, KIND>(a, lds, L, per_head, ck_workgroup(), gridDim.x, 0);
 }
 // Both at once: the workgroups are divided by what each has to do.  (One kernel after the other the few rows of a mixed batch take as long as
-// a workgroup needs to begin and to end: 12 sequences of 1 to 90 tokens over 3 bits, 152 us.)
+// a workgroup needs to begin and to end: 12 sequences of 1 to 90 tokens over 3 bits 152 us, together 122; 24 of 1 to 300 over plain heads of
+// 64 119.5 and 118.)
 template <int D, int KIND> struct ck_both {
   typedef ck_narrow<D, KIND> N;
   typedef ck_wide<D, KIND> W;
@@ -1158,7 +1168,9 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
 
 // ---- the pieces of a tile that several ranges share --------------------------------------------------------------------------
 // Workgroup (g, w): the 32 rows w of the tile that begins in workgroup g's range and does not end there; its other pieces are the first ones
-// of the ranges behind, which are a workgroup apart (many rows) or as many as there are heads (few).  Their maxima are looked through first, so that the sums of up to four pieces are on their way together.
+// of the ranges behind, which are a workgroup apart (many rows) or as many as there are heads (few).  Up to four pieces are on their way
+// together, under a running maximum.  Reading the pieces bounds it (512 bytes a row of 128 and piece): 15 us after the first chunk of 2048
+// tokens, of which 67 MB are pieces; after few rows it is one trip to memory, 6 us.
 struct ck_cut { int HS, GC; };        // of the few rows' kernel
 template <int D, int KIND, int WAVES>
 __global__ __launch_bounds__(256, WAVES == 1 || D == 256 ? 2 : 4) void ck_merge_kernel(ck_args a, ck_cut few) {
@@ -1230,7 +1242,7 @@ static inline int ck_groups(int per_cu) {
   const int cus = akv_cached_cu_count();
   return (cus > 0 ? cus : 256) * per_cu;
 }
-#define CK_GROUPS 4096            // workgroups of a launch at most
+#define CK_GROUPS 2048            // workgroups of a launch at most
 struct ck_scratch { size_t rec, ml, part, bytes; };
 static inline ck_scratch ck_scratch_layout(int D) {
   const size_t wide = 2 * (size_t)ck_groups(1) * 8, slots = wide > 2 * CK_GROUPS ? wide : 2 * CK_GROUPS;      // (either kernel's)

@@ -164,7 +164,7 @@ class TQPagedAttention:
                         keys up to there (none: zeros)
         out             where the result goes (shape and type of query; rows behind the last sequence are left as they were);
                         without it a new tensor, zero in such rows
-        max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result does not
+        max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
         Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector."""
         from .chunk_attention import _check_out, _longest, check_chunk, check_query

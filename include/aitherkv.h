@@ -263,8 +263,8 @@ int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* str
  *   block_tables, context_lens, num_blocks as in akv_paged_attn: entries at or beyond ceil(ctx / block_size) are never
  *                read, entries inside are clamped into the cache
  *   max_query_len the longest chunk, as far as the caller knows it (0: not): which kernels are launched goes by it,
- *                results do not
- * d is 64, 128 or 256; any number of query heads a kv head, any block size.  The values of a chunk's own tokens are expected to
+ *                results do not (but for their last rounding)
+ * d is 64, 128 or 256; any number of query heads a kv head (32 of them a group), up to 2048 groups; any block size.  The values of a chunk's own tokens are expected to
  * be finite (a weight of zero is multiplied with them); rows of the cache past a context may hold anything.
  *
  * akv_dense_chunk_attn: over a cache [num_blocks][block_size][num_kv_heads][d] of the query's type (element
