@@ -329,7 +329,8 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 // A tile is 32 rows, a unit 32 keys a wavefront: each takes its own, keys straight from memory into the operand, values through its
 // part of LDS (sixteen bytes c of value t lie at c ^ f(t), which 16 rows written and 4 read at a time meet all banks with); what the
 // wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Packed codes of two units are on their way at a
-// time.  32 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
+// time, of one for heads of 256, whose sums leave no registers (9 sequences of 162 tokens over 39562 keys, 4 bits: 5373 us with two, 2005).
+//  32 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
 // look-ups and operands in LDS (48%) and waits in turn bound it, some 22 us before the first unit and 10 after the last.  Heads of 256,
 // bfloat16, a window of 1024 keys, 38 MB: 39 us, which is latency: lengths, table, keys, the second unit's keys, pieces, their join.
 template <int D, int KIND> struct ck_narrow {
@@ -344,7 +345,8 @@ template <int D, int KIND> struct ck_narrow {
   static constexpr int MERGE = LEFT * QUADS * 1024, TURN = 32 * ROW * 4;
   static constexpr int V0 = PACKED ? (int)sizeof(ck_lut<PACKED ? KIND : 4, 64>) : 0;
   static constexpr int AREA = MERGE > WAVES * V_BYTES ? MERGE : WAVES * V_BYTES, Q0 = V0 + (AREA > TURN ? AREA : TURN);
-  static constexpr bool Q_LDS = PACKED && D < 256;                   // rows as operands in LDS: registers hold the keys on their way
+  static constexpr int ON = PACKED && D < 256 ? 2 : 1;               // units ahead of which keys are requested
+  static constexpr bool Q_LDS = PACKED && (D < 256 || KIND < 4);                   // rows as operands in LDS: registers hold the keys on their way
   static constexpr int ML0 = Q0 + (Q_LDS ? 2 * KS * 1024 : 0), NRM0 = ML0 + WAVES * 512, UNDO0 = NRM0 + (PACKED ? WAVES * 3 * 128 : 0), L0 = UNDO0 + 128;
   static constexpr int LDS = L0 + (int)sizeof(ck_lengths<THREADS>);      // (nothing is static: the table of levels begins at 0)
   static __device__ __forceinline__ int f(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3); }
@@ -428,7 +430,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
     if (steps > 0) {
       ahead = ck_look(a, seq, key_of(0));
       request(0, even);
-      if constexpr (PACKED) request(1, odd);
+      if constexpr (P::ON == 2) request(1, odd);
     }
 
     // ---- the rows: columns of the operand
@@ -492,12 +494,11 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
           }
         };
         if constexpr (P::Q_LDS) {
-          if (wave < KS) {         // (a piece a wavefront; all read all of them)
-            static_assert(KS <= W, "a piece a wavefront");
+          for (int ks = wave; ks < KS; ks += W) {      // (divided over the wavefronts; all read all of them)
             ck_u4 hi, lo;
-            piece(wave, hi, lo);
-            q_lds[64 * wave] = hi;
-            q_lds[64 * (KS + wave)] = lo;
+            piece(ks, hi, lo);
+            q_lds[64 * ks] = hi;
+            q_lds[64 * (KS + ks)] = lo;
           }
         } else {
 #pragma unroll
@@ -566,8 +567,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
         }
       }
       // ---- the next keys (packed: those two units on) fly from here on, and the entries of those behind them
-      constexpr int ON = PACKED ? 2 : 1;
-      if (u + ON < steps) request(u + ON, w);
+      if (u + P::ON < steps) request(u + P::ON, w);
       akv_wave_sync();
       // keys 16 kb + 8 e + 4 h .. + 3, coordinate 32 dt + lane % 32 (eight rows on, f differs in its bit 1)
       auto value = [&](int kb, int dt, int e) {
@@ -605,7 +605,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
       }
       akv_wave_sync();             // (the next values go where these are)
     };
-    if constexpr (PACKED) {
+    if constexpr (P::ON == 2) {
       for (int u = 0; u < steps; u += 2) {
         unit_of(u, even);
         if (u + 1 < steps) unit_of(u + 1, odd);
