@@ -330,7 +330,7 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 // part of LDS (sixteen bytes c of value t lie at c ^ f(t), which 16 rows written and 4 read at a time meet all banks with); what the
 // wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Packed codes of two units are on their way at a
 // time, of one for heads of 256, whose sums leave no registers (9 sequences of 162 tokens over 39562 keys, 4 bits: 5373 us with two, 2005).
-//  32 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
+// 16 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
 // look-ups and operands in LDS (48%) and waits in turn bound it, some 22 us before the first unit and 10 after the last.  Heads of 256,
 // bfloat16, a window of 1024 keys, 38 MB: 39 us, which is latency: lengths, table, keys, the second unit's keys, pieces, their join.
 template <int D, int KIND> struct ck_narrow {
