@@ -89,10 +89,10 @@ struct ck_args {
 struct ck_seq { int q0, n, ctx; };               // first query row, query tokens, tokens
 
 template <int THREADS> struct ck_lengths {       // starts and lengths of the batch
-  int start[CK_SEQS + 1];
+  alignas(8) int start[CK_SEQS + 1];
   int ctx[CK_SEQS];
-  int sum[THREADS / 64];
-  int total;
+  int64_t sum[THREADS / 64];
+  int64_t total;
   int found[2];
 };
 
@@ -163,17 +163,26 @@ __device__ __forceinline__ int ck_units_of(const ck_args& a, const ck_lengths<TH
   return ck_keys<N>(a, s, tile, TM).units + START;
 }
 
-__device__ __forceinline__ int ck_wave_scan(int v) { return akv_wave_inclusive_scan(v); }
+// The axis may pass 2^31 (a chunk of a million tokens, few of them a tile, is a million tiles over up to a million tokens): places on it
+// have 64 bits.  A tile is at most (2^31 - 2^16) / 32 units long, so that those of a wavefront fit 32 bits together.
+__device__ __forceinline__ uint32_t ck_wave_scan(int v) { return (uint32_t)akv_wave_inclusive_scan(v); }
+__device__ __forceinline__ int64_t ck_readfirst(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
 
 // length of one kv head's part of the axis, in every thread
-template <int THREADS, int N, int START> __device__ __forceinline__ int ck_total(const ck_args& a, ck_lengths<THREADS>& L, int TM) {
-  int sum = 0, seq, tile;
+template <int THREADS, int N, int START> __device__ __forceinline__ int64_t ck_total(const ck_args& a, ck_lengths<THREADS>& L, int TM) {
+  static_assert(N >= 32 && 64ll * (0x7fff0000ll / N + 1 + START) <= 0xffffffffll, "the tiles of a wavefront fit 32 bits");
+  int64_t sum = 0;
+  int seq, tile;
   const int numbers = ck_tile_numbers(a, TM);
-  for (int x = threadIdx.x; x < numbers; x += THREADS) sum += ck_units_of<THREADS, N, START>(a, L, x, TM, seq, tile);
-  sum = akv_wave_sum(sum);
+  for (int x0 = 0; x0 < numbers; x0 += THREADS) {
+    const int x = x0 + (int)threadIdx.x, u = x < numbers ? ck_units_of<THREADS, N, START>(a, L, x, TM, seq, tile) : 0;
+    sum += (uint32_t)akv_wave_sum(u);
+  }
   if ((threadIdx.x & 63) == 0) L.sum[threadIdx.x >> 6] = sum;
   __syncthreads();
-  int all = 0;
+  int64_t all = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / 64; ++w) all += L.sum[w];
   __syncthreads();
@@ -182,24 +191,24 @@ template <int THREADS, int N, int START> __device__ __forceinline__ int ck_total
 
 // the tile that holds `at` (< total): its sequence, number and place on the axis
 template <int THREADS, int N, int START>
-__device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L, int TM, int at, int& seq, int& tile, int& first) {
+__device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L, int TM, int64_t at, int& seq, int& tile, int64_t& first) {
   const int numbers = ck_tile_numbers(a, TM);
-  int base = 0;
+  int64_t base = 0;
   for (int x0 = 0;; x0 += THREADS) {
     const int x = x0 + (int)threadIdx.x;
     int sq = 0, tl = 0;
     const int u = x < numbers ? ck_units_of<THREADS, N, START>(a, L, x, TM, sq, tl) : 0;
-    const int inc = ck_wave_scan(u);
+    const uint32_t inc = ck_wave_scan(u);
     if ((threadIdx.x & 63) == 63) L.sum[threadIdx.x >> 6] = inc;
     __syncthreads();
-    int before = base, all = 0;
+    int64_t before = base, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) {
-      const int s = L.sum[w];
+      const int64_t s = L.sum[w];
       if (w < (int)(threadIdx.x >> 6)) before += s;
       all += s;
     }
-    const int b = before + inc - u;
+    const int64_t b = before + inc - u;
     if (u > 0 && at >= b && at < b + u) {
       L.found[0] = sq;
       L.found[1] = tl;
@@ -211,7 +220,7 @@ __device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L
   }
   seq = __builtin_amdgcn_readfirstlane(L.found[0]);
   tile = __builtin_amdgcn_readfirstlane(L.found[1]);
-  first = __builtin_amdgcn_readfirstlane(L.total);
+  first = ck_readfirst(L.total);
 }
 
 // where workgroup g's range begins: floor(total g / G), G at most 2^15

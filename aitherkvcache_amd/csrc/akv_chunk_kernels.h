@@ -349,6 +349,7 @@ template <int D, int KIND> struct ck_narrow {
   static constexpr bool Q_LDS = PACKED && (D < 256 || KIND < 4);                   // rows as operands in LDS: registers hold the keys on their way
   static constexpr int ML0 = Q0 + (Q_LDS ? 2 * KS * 1024 : 0), NRM0 = ML0 + WAVES * 512, UNDO0 = NRM0 + (PACKED ? WAVES * 3 * 128 : 0), L0 = UNDO0 + 128;
   static constexpr int LDS = L0 + (int)sizeof(ck_lengths<THREADS>);      // (nothing is static: the table of levels begins at 0)
+  static_assert(L0 % 8 == 0 && LDS * PER_CU <= 160 * 1024, "fits");
   static __device__ __forceinline__ int f(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 2) & 3) : 4 * (r & 3) + ((r >> 2) & 3); }
 };
 
@@ -381,9 +382,9 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
   const int64_t end = ck_begin(share, g / heads + 1, R);
   if (tid == 0) a.rec[g].valid = 0;
   if (at >= end) return;
-  int seq, tile, first;
-  ck_find<T, P::N, P::START>(a, L, TM, (int)at, seq, tile, first);
-  int64_t tile_at = first;             // the tile's place on the axis
+  int seq, tile;
+  int64_t tile_at;                     // the tile's place on the axis
+  ck_find<T, P::N, P::START>(a, L, TM, at, seq, tile, tile_at);
 
   float unit = 1.f, level = 0.f, turned = 0.f;      // of the levels; the lane's level; what undoes the matrix's scale, times the scale of the scores
   bool filled = false;
@@ -719,6 +720,7 @@ template <int D, int KIND> struct ck_wide {
   static constexpr int K0 = 0, V0 = KRING * TILE, PLACE0 = V0 + 2 * TILE, NORM0 = PLACE0 + RING * N * 16;
   static constexpr int LUT0 = NORM0 + (KIND >= 2 ? RING * N * 16 : 0), L0 = LUT0 + (KIND >= 2 ? (int)sizeof(ck_lut<KIND >= 2 ? KIND : 4, 1>) : 0);
   static constexpr int LDS = L0 + (int)sizeof(ck_lengths<THREADS>);
+  static_assert(L0 % 8 == 0 && LDS * PER_CU <= 160 * 1024, "fits");
   static __device__ __forceinline__ int fk(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
   static __device__ __forceinline__ int fv(int r) { return D == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : 5 * (r & 3); }
 };
@@ -731,7 +733,7 @@ __device__ __forceinline__ void ck_landed() { asm volatile("s_waitcnt vmcnt(0)" 
 
 // What workgroup g of G does, number base + g of the launch; `per_head`: length of one kv head's part of the axis.
 template <int D, int KIND>
-__device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* const lds, ck_lengths<ck_wide<D, KIND>::THREADS>& L, const int per_head, const int g, const int G, const int base) {
+__device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* const lds, ck_lengths<ck_wide<D, KIND>::THREADS>& L, const int64_t per_head, const int g, const int G, const int base) {
   typedef ck_wide<D, KIND> P;
   typedef ck_math<KIND> M;
   constexpr bool PACKED = M::packed;
@@ -749,15 +751,16 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   const int heads = a.KVH * a.HS;
-  const int64_t total = (int64_t)per_head * heads;
+  const int64_t total = per_head * heads;
   const ck_share share = ck_share_of(total, G);
   int64_t at = ck_begin(share, g, G);
   const int64_t end = ck_begin(share, g + 1, G);
   if (tid == 0) a.rec[base + g].valid = 0;
   if (at >= end) return;
-  int head = (int)(at / per_head), seq, tile, first;
-  ck_find<T, N, P::START>(a, L, TM, (int)(at - (int64_t)head * per_head), seq, tile, first);
-  int64_t tile_at = (int64_t)head * per_head + first;
+  int head = total <= 0xffffffffll ? (int)((uint32_t)at / (uint32_t)per_head) : (int)(at / per_head), seq, tile;
+  int64_t tile_at;
+  ck_find<T, N, P::START>(a, L, TM, at - head * per_head, seq, tile, tile_at);
+  tile_at += head * per_head;
 
   float unit = 1.f;                // of the levels
   if constexpr (PACKED) {
@@ -1134,7 +1137,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   extern __shared__ __align__(1024) unsigned char lds[];
   auto& L = ck_lengths_at<P>(lds, P::L0);
   ck_load_lengths(a, L);
-  const int per_head = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
+  const int64_t per_head = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
   ck_wide_work<D, KIND>(a, lds, L, per_head, ck_workgroup(), gridDim.x, 0);
 }
 // Both at once: the workgroups are divided by what each has to do.  (One kernel after the other the few rows of a mixed batch take as long as
@@ -1153,7 +1156,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   extern __shared__ __align__(1024) unsigned char lds[];
   auto& L = ck_lengths_at<W>(lds, ck_both<D, KIND>::L0);
   ck_load_lengths(many, L);
-  const int few_total = ck_total<N::THREADS, N::N, N::START>(few, L, N::ROWS / few.GC), many_total = ck_total<W::THREADS, W::N, W::START>(many, L, W::ROWS / many.GC);
+  const int64_t few_total = ck_total<N::THREADS, N::N, N::START>(few, L, N::ROWS / few.GC), many_total = ck_total<W::THREADS, W::N, W::START>(many, L, W::ROWS / many.GC);
   const int G = gridDim.x, g = ck_workgroup(), few_heads = few.KVH * few.HS;
   const float few_cost = (float)N::COST * (float)few_heads * (float)few_total, many_cost = (float)W::COST * (float)(many.KVH * many.HS) * (float)many_total;
   int ranges = 0;

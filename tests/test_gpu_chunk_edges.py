@@ -1,0 +1,36 @@
+"""Attention of a chunk where its batch or its cache is out of the ordinary.  Tolerances as in test_gpu_chunk.py."""
+import math
+
+import pytest
+import torch
+
+import aitherkvcache_amd as akv
+from tests.test_gpu_chunk import BF, HALF, check, vectors
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- more work than 32 bits count ---------------------------------------------------------------------------------------------
+
+def repeated(dev, seqs, n, ctx, seed):
+    """A call whose sequences all hold the same 8192 keys over and over, and its result with bound: what they attend to is those keys
+    once (`ctx` a multiple of 8192; up to n - 1 of its keys at the end are hidden from a row, 2^-20 of them at most here)."""
+    d, heads, keys = 64, 8, 8192
+    q, kc, vc = (vectors(seed + i, dev, BF, *s) for i, s in enumerate(((seqs * n, heads, d), (2, keys // 2, 1, d), (2, keys // 2, 1, d))))
+    q *= 3
+    tables = torch.tensor([0, 1], dtype=torch.int32, device=dev).repeat(ctx // keys).expand(seqs, -1)
+    got = akv.paged_chunk_attention(q, kc, vc, tables, torch.full((seqs,), ctx, device=dev), torch.arange(seqs + 1, device=dev) * n, max_query_len=n)
+    k, v = kc.view(keys, d).double().T.contiguous(), vc.view(keys, d).double()
+    out, size = (torch.empty(seqs * n * heads, d, dtype=torch.float64, device=dev) for _ in range(2))
+    for i in range(0, len(out), 8192):
+        w = torch.softmax(q.view(-1, d)[i:i + 8192].double() @ k / math.sqrt(d), 1)
+        out[i:i + 8192], size[i:i + 8192] = w @ v, w @ v.abs()
+    # (sums of ctx / 64 steps or fewer, each rounded: 2^-24 of the sum so far)
+    return got, out.view(got.shape), ((2 * HALF[BF] + 2.0 ** -14 + ctx / 64 * 2.0 ** -24) * size).view(got.shape)
+
+
+@pytest.mark.parametrize("n,ctx", [(1, 1 << 25), (9, 1 << 24)], ids=["few", "many"])
+def test_axis_past_32_bits(dev, n, ctx):
+    """8192 sequences of 2^18 units each: the axis that is cut among the workgroups is longer than 2^31.  Takes seconds: so much
+    work is what it takes to get there."""
+    check(*repeated(dev, 8192, n, ctx, 300))
