@@ -146,7 +146,9 @@ template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, c
   return r;
 }
 
-// Tiles are numbered with gaps: tile j of sequence i is floor(start_i / TM) + i + j, which no two tiles share.
+// Tiles are numbered with gaps: tile j of sequence i is floor(start_i / TM) + i + j, which no two tiles share.  (Where starts go back some do,
+// and the axis has a part of the tiles: whatever a workgroup finds there is a tile of a sequence, and its way from one to the next ends
+// with the last sequence.)
 __device__ __forceinline__ int ck_tile_numbers(const ck_args& a, int TM) { return a.T / TM + a.S + 1; }
 template <int THREADS, int N, int START>
 __device__ __forceinline__ int ck_units_of(const ck_args& a, const ck_lengths<THREADS>& L, int x, int TM, int& seq, int& tile) {

@@ -680,7 +680,8 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
     int n = s.n;
     while ((int64_t)tile * TM >= n) {
       tile = 0;
-      n = ck_sequence(a, L, ++seq).n;
+      if (++seq > a.S) return;         // (starts that go back: the axis has fewer tiles than the sequences)
+      n = ck_sequence(a, L, seq).n;
     }
   }
 }
@@ -1108,7 +1109,10 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
     int n = s.n;
     while ((int64_t)tile * TM >= n) {
       tile = 0;
-      if (++seq > a.S) { seq = 0; ++head; }
+      if (++seq > a.S) {
+        seq = 0;
+        if (++head >= heads) return;   // (starts that go back)
+      }
       n = ck_sequence(a, L, seq).n;
     }
   }

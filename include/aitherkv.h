@@ -257,7 +257,8 @@ int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* str
  * context_lens[i] tokens (which the cache holds already): its token j stands at position context_lens[i] - n_i + j and
  * attends to the keys at its own position and before.  A row without a key (its position is negative) is zero.
  *   query        [num_tokens][num_q_heads][d] float16 or bfloat16, strides qs_tok / qs_head (last dim contiguous)
- *   query_starts [num_seqs + 1], non-decreasing, in [0, num_tokens] (clamped there)
+ *   query_starts [num_seqs + 1], non-decreasing, in [0, num_tokens] (clamped there; where one is less than the one before it rows
+ *                of the call are undefined, but nothing else is read or written than otherwise)
  *   out          like query, its type; rows at or behind query_starts[num_seqs] are zeroed where zero_tail is not 0
  *                and left as they were otherwise
  *   block_tables, context_lens, num_blocks as in akv_paged_attn: entries at or beyond ceil(ctx / block_size) are never

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import aitherkvcache_amd as akv
-from tests.test_gpu_chunk import BF, HALF, check, vectors
+from tests.test_gpu_chunk import BF, HALF, Batch, Packed, check, dense_reference, vectors
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,32 @@ def test_axis_past_32_bits(dev, n, ctx):
     """8192 sequences of 2^18 units each: the axis that is cut among the workgroups is longer than 2^31.  Takes seconds: so much
     work is what it takes to get there."""
     check(*repeated(dev, 8192, n, ctx, 300))
+
+
+# ---- starts that go back -----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("seqs", [7, 300])
+@pytest.mark.parametrize("longest", [None, 3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_starts_out_of_order(dev, seqs, longest, d):
+    """Starts that decrease, or lie outside of the call: every workgroup ends, rows that are not the call's stay as they were, and the
+    next call is right."""
+    b = Batch([(9, 60 + 40 * (i % 9)) for i in range(seqs)], 16, dev, 17)
+    p = Packed(b, d, 4, 8, 2, BF, dev, 310)
+    kc, vc = (vectors(311 + i, dev, BF, b.blocks, 16, 2, d) for i in range(2))
+    want = [p.reference(), dense_reference(b, p.q, kc, vc, 1 / math.sqrt(d), 0)]
+    good, n = b.starts.clone(), b.tokens
+    room = torch.full((n + 64, 8, d), 7.0, dtype=BF, device=dev)
+    calls = (lambda **more: p.run(max_query_len=longest, **more),
+             lambda **more: akv.paged_chunk_attention(p.q, kc, vc, b.tables, b.ctx, b.starts, max_query_len=longest, **more))
+    g = torch.Generator(device=dev).manual_seed(seqs)
+    for bad in (good.flip(0), good[torch.randperm(seqs + 1, device=dev, generator=g)], torch.randint(-50, n + 50, good.shape, device=dev, generator=g),
+                torch.where(torch.arange(seqs + 1, device=dev) % 2 == 0, n, 0), torch.full_like(good, n + 1000)):
+        b.starts = bad.to(torch.int32)
+        for call in calls:
+            call(out=room[32:-32])
+            call()
+    assert bool((room[:32] == 7).all()) and bool((room[-32:] == 7).all())
+    b.starts = good
+    for call, w in zip(calls, want):
+        check(call(), *w)
