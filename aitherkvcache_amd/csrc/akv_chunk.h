@@ -137,8 +137,8 @@ template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, c
   if (r.hi < 0) r.hi = 0;
   int lo = 0;
   if (a.window > 0) {
-    lo = s.ctx - s.n + t0 - a.window + 1;
-    if (lo < 0) lo = 0;
+    const int64_t oldest = (int64_t)(s.ctx - s.n + t0) - a.window + 1;      // (a row of negative position with a window near 2^31)
+    lo = oldest > 0 ? (int)oldest : 0;
   }
   r.first = lo / N;
   r.units = (r.hi + N - 1) / N - r.first;

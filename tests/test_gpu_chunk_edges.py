@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import aitherkvcache_amd as akv
-from tests.test_gpu_chunk import BF, HALF, Batch, Packed, check, dense_reference, vectors
+from tests.test_gpu_chunk import BF, HALF, Batch, Packed, check, dense_reference, run_dense, vectors
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,12 @@ def test_starts_out_of_order(dev, seqs, longest, d):
     b.starts = good
     for call, w in zip(calls, want):
         check(call(), *w)
+
+
+# ---- windows ---------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens", [[(3, 2), (9, 1), (5, 30)], [(100, 10), (300, 290), (90, 33)], [(100, 10), (3, 2)]], ids=["few", "many", "both"])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 40, 1 << 40, 7])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_windows_of_any_length_and_rows_before_the_first_key(dev, lens, window, d):
+    run_dense(Batch(lens, 16, dev, 18), d, 8, 2, BF, dev, 320, window=window)
