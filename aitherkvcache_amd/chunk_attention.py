@@ -76,7 +76,9 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
                     without it a new tensor, zero in such rows
     max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
-    Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256."""
+    Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256.
+    Values that some token of a sequence's chunk sees must be finite; past a context, or before every token's window, the caches and
+    tables may hold anything."""
     result = _lib.calls().dense_chunk(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, scale, window, out,
                                       max_query_len)
     if result is not None:

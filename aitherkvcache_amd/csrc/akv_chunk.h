@@ -128,19 +128,19 @@ template <int THREADS> __device__ __forceinline__ ck_seq ck_sequence(const ck_ar
   return s;
 }
 
-// keys [lo, hi) of tile j, TM tokens a tile; a tile has at least one unit of N keys
-struct ck_range { int first, units, hi; };
+// keys [lo, hi) that rows of tile j see, TM tokens a tile; a tile has at least one unit of N keys
+struct ck_range { int first, units, lo, hi; };
 template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, const ck_seq& s, int j, int TM) {
   const int t0 = j * TM, t1 = t0 + TM < s.n ? t0 + TM : s.n;
   ck_range r;
   r.hi = s.ctx - s.n + t1;
   if (r.hi < 0) r.hi = 0;
-  int lo = 0;
+  r.lo = 0;
   if (a.window > 0) {
     const int64_t oldest = (int64_t)(s.ctx - s.n + t0) - a.window + 1;      // (a row of negative position with a window near 2^31)
-    lo = oldest > 0 ? (int)oldest : 0;
+    r.lo = oldest > 0 ? (int)oldest : 0;
   }
-  r.first = lo / N;
+  r.first = r.lo / N;
   r.units = (r.hi + N - 1) / N - r.first;
   if (r.units < 1) r.units = 1;
   return r;

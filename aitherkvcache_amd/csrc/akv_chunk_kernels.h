@@ -20,6 +20,7 @@
 #pragma once
 #include "akv_chunk_rotate.h"
 #include "akv_device_once.h"
+#include <climits>
 #include <type_traits>
 
 // Smallest value norm that counts (its inverse, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
@@ -400,18 +401,23 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
     const int kvh = head / a.HS;
     const int pos_first = s.ctx - s.n + t0, pos_last = max(-1, s.ctx - s.n + t1 - 1);
 
-    // ---- 32 keys of the wavefront, a lane its half of one (behind the last key: the last one, masked)
+    // ---- 32 keys of the wavefront, a lane its half of one (outside of what the tile sees: its first or last key, masked.  What else lies
+    // there may be anything, and a weight of zero does not undo an infinity)
     const int base0 = (keys.first + u0) * P::N + 32 * wave;
     const int steps = keys.hi > base0 ? min(u1 - u0, (keys.hi - base0 + P::N - 1) / P::N) : 0;
-    auto key_of = [&](int u) { return min(base0 + u * P::N + col, keys.hi - 1); };
+    // (only the tile's first unit begins before its first key; packed rows have no windows)
+    auto key_of = [&](int u, int oldest = INT_MIN) {
+      const int key = min(base0 + u * P::N + col, keys.hi - 1);
+      return PACKED ? key : max(key, oldest);
+    };
     ck_u4 kd[PACKED ? 1 : KS], vd[PACKED ? 1 : KS];
     struct codes { uint32_t k[PACKED ? HW : 1], v[PACKED ? HW : 1]; float kn, vn; };
     codes even, odd;               // packed: those of two units (in turns, so that nothing in flight is ever moved)
     const uint8_t *const k_base = a.k + kvh * a.k_head + (PACKED ? 4 * HW : 16) * h, *const v_base = a.v + kvh * a.v_head + (PACKED ? 4 * HW : 16) * h;
     // (the entry after this unit's is requested first: what waits for it must not wait for the keys as well)
     ck_entry ahead = {0u, 0u};
-    auto request = [&](int u, codes& w) {
-      const ck_place p = ck_place_of(a, key_of(u), ahead);
+    auto request = [&](int u, codes& w, int oldest = INT_MIN) {
+      const ck_place p = ck_place_of(a, key_of(u, oldest), ahead);
       ahead = ck_look(a, seq, key_of(u + 1));
       const int64_t ko = ck_offset(p, a.k_blk, a.k_pos), vo = a.kv_alike ? ko : ck_offset(p, a.v_blk, a.v_pos);
       if constexpr (PACKED) {
@@ -429,8 +435,8 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
       }
     };
     if (steps > 0) {
-      ahead = ck_look(a, seq, key_of(0));
-      request(0, even);
+      ahead = ck_look(a, seq, key_of(0, keys.lo));
+      request(0, even, keys.lo);
       if constexpr (P::ON == 2) request(1, odd);
     }
 
@@ -800,13 +806,17 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
     const int base0 = (keys.first + u0) * N;
     // Places of a unit's keys, by one wavefront, a lane a key: the table's entry is requested, and what the rows of keys and
     // values lie at is written a unit later.  Every wavefront does so for one unit of the next WAVES, all at the same time: one that did
-    // it for the others would be what they wait for.  A key behind the last one has the last one's place: what is read for it is masked,
-    // and its value is as finite as that one's.
-    auto key_of = [&](int u) { return min(base0 + u * N + (lane & (N - 1)), keys.hi - 1); };
-    auto look = [&](int u) { return ck_look(a, seq, key_of(u)); };
+    // it for the others would be what they wait for.  A key behind the last one that the tile sees has the last one's place, one before the
+    // first the first one's: what is read for it is masked, and its value is as finite as that one's.
+    // (Only the tile's first unit begins before its first key; packed rows have no windows.)
+    auto key_of = [&](int u, int oldest = INT_MIN) {
+      const int key = min(base0 + u * N + (lane & (N - 1)), keys.hi - 1);
+      return PACKED ? key : max(key, oldest);
+    };
+    auto look = [&](int u, int oldest = INT_MIN) { return ck_look(a, seq, key_of(u, oldest)); };
     float kn = 0.f, vn = 1.f;      // packed: norms of the unit noted last
-    auto note = [&](int u, const ck_entry& e) {
-      const ck_place p = ck_place_of(a, key_of(u), e);
+    auto note = [&](int u, const ck_entry& e, int oldest = INT_MIN) {
+      const ck_place p = ck_place_of(a, key_of(u, oldest), e);
       int64_t* place = (int64_t*)(lds + P::PLACE0) + (u & (P::RING - 1)) * 2 * N;
       const int64_t k_at = ck_offset(p, a.k_blk, a.k_pos) + kvh * a.k_head;
       place[lane & (N - 1)] = k_at;
@@ -925,7 +935,7 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
     ck_entry ahead = {0u, 0u};
     __syncthreads();               // (LDS of the tile before has been read)
     if (units > 0) {
-      note(wave, look(wave));
+      note(wave, look(wave, keys.lo), keys.lo);
       note_norms(wave);
       __syncthreads();
       ahead = look(P::WAVES + wave);

@@ -166,7 +166,8 @@ class TQPagedAttention:
                         without it a new tensor, zero in such rows
         max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
-        Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector."""
+        Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector.
+        Norms of the sequences' tokens must be finite; past a context the caches and tables may hold anything."""
         from .chunk_attention import _check_out, _longest, check_chunk, check_query
         if self._block_selector is not None:
             raise ValueError("forward_chunk does not run the block selector")

@@ -265,8 +265,9 @@ int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* str
  *                read, entries inside are clamped into the cache
  *   max_query_len the longest chunk, as far as the caller knows it (0: not): which kernels are launched goes by it,
  *                results do not (but for their last rounding)
- * d is 64, 128 or 256; any number of query heads a kv head (32 of them a group), up to 2048 groups; any block size.  The values of a chunk's own tokens are expected to
- * be finite (a weight of zero is multiplied with them); rows of the cache past a context may hold anything.
+ * d is 64, 128 or 256; any number of query heads a kv head (32 of them a group), up to 2048 groups; any block size.  Values that some token of a sequence's
+ * chunk sees are expected to be finite (they are multiplied with weights of zero for the tokens that do not); rows of the cache
+ * past a context, or older than every token's window, may hold anything, and table entries of such blocks are not read.
  *
  * akv_dense_chunk_attn: over a cache [num_blocks][block_size][num_kv_heads][d] of the query's type (element
  * strides, rows at multiples of 16 bytes); window > 0: a token sees the newest `window` keys only (its own included).

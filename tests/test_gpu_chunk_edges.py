@@ -5,9 +5,13 @@ import pytest
 import torch
 
 import aitherkvcache_amd as akv
-from tests.test_gpu_chunk import BF, HALF, Batch, Packed, check, dense_reference, run_dense, vectors
+from tests.test_gpu_chunk import BF, FP, HALF, Batch, Packed, check, dense_reference, run_dense, vectors
 
 pytestmark = pytest.mark.gpu
+
+
+def dense_inputs(b, heads, kv, d, dtype, dev, seed):
+    return [vectors(seed + i, dev, dtype, *s) for i, s in enumerate(((b.tokens, heads, d), (b.blocks, b.block, kv, d), (b.blocks, b.block, kv, d)))]
 
 
 # ---- more work than 32 bits count ---------------------------------------------------------------------------------------------
@@ -72,3 +76,26 @@ def test_starts_out_of_order(dev, seqs, longest, d):
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_windows_of_any_length_and_rows_before_the_first_key(dev, lens, window, d):
     run_dense(Batch(lens, 16, dev, 18), d, 8, 2, BF, dev, 320, window=window)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+@pytest.mark.parametrize("lens", [[(3, 700), (1, 450), (7, 1201)], [(150, 700), (90, 333), (3, 900)]], ids=["few", "many"])
+def test_what_lies_before_every_window_is_not_read(dev, d, dtype, fill, lens):
+    """Blocks behind a sliding window have been given back: another request's numbers, or none, and entries of the table to match."""
+    for window in (1, 5, 63, 64, 100, 200):
+        b = Batch(lens, 16, dev, window, spare=3)
+        q, kc, vc = dense_inputs(b, 8, 2, d, dtype, dev, 200)
+        b.unused(fill, kc, vc)
+        want = dense_reference(b, q, kc, vc, 1 / math.sqrt(d), window)
+        spare = (set(range(b.blocks)) - {int(b.host[i, j]) for i, (_, c) in enumerate(lens) for j in range(-(-c // 16))}).pop()
+        for i, (n, c) in enumerate(lens):
+            old = max(0, c - n - window + 1)          # the first key that any of the sequence's tokens sees
+            for x in (kc, vc):
+                x[b.host[i, old // 16], :old % 16] = fill
+            for j in range(old // 16):
+                kc[b.host[i, j]] = vc[b.host[i, j]] = fill
+                b.host[i, j] = (spare, -1, int(b.host[i, j]))[j % 3]
+        tables = torch.from_numpy(b.host).to(dev, torch.int32)
+        check(akv.paged_chunk_attention(q, kc, vc, tables, b.ctx, b.starts, window=window), *want)
