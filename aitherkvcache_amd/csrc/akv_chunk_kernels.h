@@ -12,8 +12,8 @@
 //
 // Packed rows are attended in the rotated domain: queries are rotated on the way in, results on the way out (akv_chunk_rotate.h), and in
 // between a key is its norm times levels of the codebook.  Levels are float16 in a unit that loses little of them (ck_unit_key); a key's
-// norm multiplies its score in float32; a value's norm v goes into the exponent, w = 2^(s + log2 v - M), with M the running maximum of
-// s + log2 v, so weights stay in [0, 2^CK_FRAME] for norms of any size, and the sum of the softmax takes w / v.
+// norm multiplies its score in float32; a value's norm v goes into the exponent, w = 2^(s + log2 v - M), with M from the running maximum of
+// s + log2 v, so weights stay in [0, 2^(CK_LIFT + CK_FRAME)] for norms of any size, and the sum of the softmax takes w / v.
 //
 // What is rounded to sixteen bits: the weights, once, as operand of the second product (relative 2^-11 or 2^-8, as of the values beside them);
 // packed: the levels (2^-14) and the queries (many rows: one float16 term; few rows: two, 2^-22).  Scores, maxima, sums and results are float32.
@@ -23,10 +23,10 @@
 #include <climits>
 #include <type_traits>
 
-// Smallest value norm that counts (its inverse, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
+// Smallest value norm that counts (its inverse times weights of 2^13, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
 // frame of the exponents, as if its logarithm were 0, and its value is zero.  Norms of one sequence may
-// lie 2^120 apart: weights are float32 until the sum of the softmax has taken them.
-#define CK_TINY 0x1p-90f
+// lie 2^110 apart: weights are float32 until the sum of the softmax has taken them.
+#define CK_TINY 0x1p-80f
 
 // ---- packed codes -> float16 levels -----------------------------------------------------------------------------
 // Value of the levels' last place, so to say: a level is a float16 number times this.  Any unit would do (scores take it with the key's norm,
@@ -145,9 +145,13 @@ template <int BITS, int COPIES> struct ck_lut {
 
 // ---- one step of the softmax ----------------------------------------------------------------------------------------
 // A row's running state: weights are 2^(exponent - m), and l is their sum over the lane's own keys (the halves are added at the end).  m is
-// not the maximum so far but lies at most CK_FRAME below it: the sums are rescaled only when a row's maximum has outgrown that, and weights of
-// up to 2^CK_FRAME lose nothing, as their rounding is relative.
+// not the maximum so far but lies CK_LIFT to CK_LIFT + CK_FRAME below it: the sums are rescaled only when a row's maximum has outgrown that, and
+// weights of up to 2^13 lose nothing, as their rounding is relative and float16 reaches 2^16 (the other 2^3: scores of 2^26 are rounded to
+// steps of 8, of which a maximum may be off by half).  What lies far below the largest keeps the more: float16 weights are in steps of 2^-24
+// at least, 2^-29 of the largest (with the largest at 1 keys 2^-26 below it were lost however many or large they were).  A frame of 4 under
+// a lift of 7 rescales more often: a first chunk of 2048 tokens 75.2 us, this one 72.7.
 #define CK_FRAME 8.f
+#define CK_LIFT 5.f
 struct ck_row { float m, l; };
 // largest of NT tiles of 32 products, over both halves
 template <int NT> __device__ __forceinline__ float ck_max(const ck_f16v (&s)[NT]) {
@@ -164,9 +168,9 @@ template <int NT> __device__ __forceinline__ float ck_max(const ck_f16v (&s)[NT]
 }
 // Whether some row's largest exponent has outgrown its frame; `alpha` is then what the row's sums are multiplied with.
 __device__ __forceinline__ bool ck_outgrown(ck_row& r, float mx, float& alpha) {
-  const bool grown = mx > r.m + CK_FRAME;
+  const bool grown = mx - r.m > CK_LIFT + CK_FRAME;      // (the difference of two numbers so near is exact)
   if (!__ballot(grown)) return false;
-  const float m = grown ? mx : r.m;
+  const float m = grown ? mx - CK_LIFT : r.m;
   alpha = grown ? ck_exp2(r.m - m) : 1.f;
   r.m = m;
   r.l *= alpha;

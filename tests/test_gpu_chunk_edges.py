@@ -1,11 +1,13 @@
-"""Attention of a chunk where its batch or its cache is out of the ordinary.  Tolerances as in test_gpu_chunk.py."""
+"""Attention of a chunk where its batch or its cache is out of the ordinary.  Tolerances as in test_gpu_chunk.py, but that a
+16-bit weight is off by at most 2^-30 of its row's largest beside its own rounding (float16 has steps of 2^-24 at its lower end, half of one
+may be lost, and the largest weight is at least 2^5)."""
 import math
 
 import pytest
 import torch
 
 import aitherkvcache_amd as akv
-from tests.test_gpu_chunk import BF, FP, HALF, Batch, Packed, check, dense_reference, run_dense, vectors
+from tests.test_gpu_chunk import BF, FP, HALF, Batch, Packed, check, dense_reference, hidden_of, run_dense, softmax_rows, vectors
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +101,27 @@ def test_what_lies_before_every_window_is_not_read(dev, d, dtype, fill, lens):
                 b.host[i, j] = (spare, -1, int(b.host[i, j]))[j % 3]
         tables = torch.from_numpy(b.host).to(dev, torch.int32)
         check(akv.paged_chunk_attention(q, kc, vc, tables, b.ctx, b.starts, window=window), *want)
+
+
+# ---- weights far below the largest ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n", [2, 70], ids=["few", "many"])
+@pytest.mark.parametrize("gap", [18.4, 20.0])
+def test_small_weights_of_large_values(dev, d, dtype, n, gap):
+    """One key of 32 outweighs the others by a factor of exp(gap); their values make up for it."""
+    b = Batch([(n, 2600)], 16, dev, 13)
+    q, kc, vc = dense_inputs(b, 4, 2, d, dtype, dev, 210)
+    q.zero_(), kc.zero_()
+    q[..., 3] = 8.0
+    heavy = torch.from_numpy(b.host[0, 0:2600 // 16:2]).to(dev)
+    kc[heavy, 7, :, 3] = gap / 8 * math.sqrt(d)
+    vc.fill_(60000.0)
+    vc[heavy, 7] = 1.0
+    got = akv.paged_chunk_attention(q, kc, vc, b.tables, b.ctx, b.starts)
+    u, c = HALF[dtype], b.lens[0][1]
+    k, v = b.rows(kc, 0).double()[:, 0], b.rows(vc, 0).double()[:, 0]
+    w = softmax_rows(q[:, 0].double() @ k.T.contiguous() / math.sqrt(d), hidden_of(n, c, 0, dev))
+    out = (w @ v)[:, None].expand(n, 4, d)
+    check(got, out, (2 * u + 2.0 ** -14) * out + 2.0 ** -30 * w.amax(1)[:, None, None] * float(v.sum(0)[0]))
