@@ -23,10 +23,12 @@
 #include <climits>
 #include <type_traits>
 
-// Smallest value norm that counts (its inverse times weights of 2^13, summed over a cache, is finite).  A smaller one, such as 0, has weight 1 in the
-// frame of the exponents, as if its logarithm were 0, and its value is zero.  Norms of one sequence may
-// lie 2^110 apart: weights are float32 until the sum of the softmax has taken them.
+// Smallest value norm that counts (its inverse times weights of 2^13, summed over a cache, is finite).  A value of a smaller one,
+// such as 0, is zero, and in the exponents its norm is CK_NONE: far below those that come with it, or its score would lift the frame of the row
+// past what the others have to give (as 1 it made float16 zeros of values 2^-26 in size); no further below than that weight times inverse,
+// which the sum of the softmax still takes, are float32 numbers beside norms of up to 2^80.
 #define CK_TINY 0x1p-80f
+#define CK_NONE 0x1p-40f
 
 // ---- packed codes -> float16 levels -----------------------------------------------------------------------------
 // Value of the levels' last place, so to say: a level is a float16 number times this.  Any unit would do (scores take it with the key's norm,
@@ -565,7 +567,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
           for (int i = 0; i < KS / 2; ++i) *(ck_u4*)(vl + col * 2 * D + 16 * ((KS * h + p * (KS / 2) + i) ^ P::f(col))) = v[i] & keep;
         }
         if (h == 0) {
-          const float v = w.vn < CK_TINY ? 1.f : w.vn;
+          const float v = w.vn < CK_TINY ? CK_NONE : w.vn;
           nrm[wave][0][col] = w.kn * unit;
           nrm[wave][1][col] = __log2f(v);
           nrm[wave][2][col] = 1.f / v;
@@ -834,7 +836,7 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
     auto note_norms = [&](int u) {
       if constexpr (PACKED) {
         float* nr = (float*)(lds + P::NORM0) + (u & (P::RING - 1)) * 4 * N;
-        const float v = vn < CK_TINY ? 1.f : vn;
+        const float v = vn < CK_TINY ? CK_NONE : vn;
         const int key = lane & (N - 1);
         nr[key] = kn * unit;
         nr[N + key] = __log2f(v);

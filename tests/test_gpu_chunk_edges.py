@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import aitherkvcache_amd as akv
-from tests.test_gpu_chunk import BF, FP, HALF, Batch, Packed, check, dense_reference, hidden_of, run_dense, softmax_rows, vectors
+from tests.test_gpu_chunk import BF, FP, HALF, Batch, Packed, check, dense_reference, hidden_of, run_dense, softmax_rows, unpack, vectors
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,64 @@ def test_small_weights_of_large_values(dev, d, dtype, n, gap):
     w = softmax_rows(q[:, 0].double() @ k.T.contiguous() / math.sqrt(d), hidden_of(n, c, 0, dev))
     out = (w @ v)[:, None].expand(n, 4, d)
     check(got, out, (2 * u + 2.0 ** -14) * out + 2.0 ** -30 * w.amax(1)[:, None, None] * float(v.sum(0)[0]))
+
+
+# ---- norms of zero -------------------------------------------------------------------------------------------------------------------
+
+def packed_reference(p):
+    """(out, bound): as Packed.reference, the loss of small weights by what weight times norm is at most."""
+    b, q, d = p.b, p.q, p.d
+    pi, cen, scale = p.tq.rotation.double(), p.tq.centroids.double(), p.attn.scale
+    out, bound = (torch.zeros(q.shape, dtype=torch.float64, device=q.device) for _ in range(2))
+    group, at = q.shape[1] // p.k.shape[2], 0
+    for i, (n, c) in enumerate(b.lens):
+        ck, cv = (cen[unpack(b.rows(x, i), p.bits, d)] for x in (p.k, p.v))
+        kn, vn = b.rows(p.kn, i).double(), b.rows(p.vn, i).double()
+        hidden = hidden_of(n, c, 0, q.device)
+        for h in range(q.shape[1]):
+            j = h // group
+            turned = q[at:at + n, h].double() @ pi.T.contiguous()
+            k = ck[:, j] * kn[:, j, None]
+            a = softmax_rows(turned @ k.T.contiguous() * scale, hidden) * vn[:, j]          # weight times norm
+            out[at:at + n, h] = a @ cv[:, j] @ pi
+            e = ((turned.abs() @ k.abs().T.contiguous()) * scale).masked_fill(hidden, 0.0).amax(1, keepdim=True) * 2.0 ** -10
+            grown = torch.expm1(2 * e)
+            lost = 2.0 ** -30 * a.amax(1, keepdim=True) * cv[:, j].abs().sum(0)
+            bound[at:at + n, h] = ((grown + 2.0 ** -10 + 2.0 ** -13) * (1 + grown) * (a @ cv[:, j].abs()) + lost) @ pi.abs() + HALF[q.dtype] * out[at:at + n, h].abs() + 1e-38
+        at += n
+    return out, bound
+
+
+@pytest.mark.parametrize("d,bits", [(64, 3), (128, 4), (256, 2)])
+@pytest.mark.parametrize("lens", [[(3, 200), (1, 64)], [(90, 200), (70, 71)]], ids=["few", "many"])
+@pytest.mark.parametrize("size", [2.0 ** -50, 2.0 ** -26, 1.0, 2.0 ** 40])
+def test_zero_norms_beside_norms_of_any_size(dev, d, bits, lens, size):
+    """A value of zero has weight and no size: how large the others are does not change by it."""
+    b = Batch(lens, 16, dev, 14)
+    p = Packed(b, d, bits, 8, 2, BF, dev, 220)
+    p.kn.mul_(0.02)
+    p.vn.mul_(size)
+    for i, (_, c) in enumerate(lens):
+        p.vn[b.host[i, 0], 5] = 0.0
+        p.vn[b.host[i, c // 32], 2, 1] = 0.0
+    check(p.run(), *packed_reference(p))
+
+
+@pytest.mark.parametrize("d,bits", [(64, 3), (128, 4), (256, 2)])
+@pytest.mark.parametrize("lens", [[(3, 200)], [(90, 200)]], ids=["few", "many"])
+@pytest.mark.parametrize("score", [10.0, 24.0])
+def test_a_zero_value_may_outweigh_all_others(dev, d, bits, lens, score):
+    """Attention rests on keys whose values are zero, one of 32 (by exp(score)): what the others leave is small, and right."""
+    b = Batch(lens, 16, dev, 15)
+    p = Packed(b, d, bits, 8, 2, BF, dev, 221)
+    p.kn.mul_(0.02)
+    at = (int(b.host[0, 0]), 9)
+    heavy = torch.from_numpy(b.host[0, 0:lens[0][1] // 16:2]).to(dev)
+    p.k[heavy, 9] = p.k[at]
+    p.v.copy_(p.v[at].clone())                 # (values alike: nothing of the result cancels)
+    p.vn[heavy, 9] = 0.0
+    p.kn[heavy, 9] = score
+    code = p.tq.centroids.double()[unpack(p.k[at], bits, d)]                                # [kv heads, d]
+    row = code @ p.tq.rotation.double() * math.sqrt(d)
+    p.q = (row / (code * code).sum(-1, keepdim=True)).repeat_interleave(4, 0).expand(b.tokens, 8, d).to(BF).contiguous()
+    check(p.run(), *packed_reference(p))
