@@ -72,8 +72,8 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     block_tables    [num_seqs, blocks] int32 / int64;  context_lens [num_seqs] tokens of a sequence, its chunk included
     query_start_loc [num_seqs + 1]: sequence i owns query rows query_start_loc[i] .. query_start_loc[i + 1] - 1
     scale           of the scores (1 / sqrt(head_dim));  window > 0: a token sees the newest `window` keys, its own among them
-    out             where the result goes (same shape and type as query; rows behind the last sequence are left as they were);
-                    without it a new tensor, zero in such rows
+    out             where the result goes (same shape and type as query; rows before the first sequence or behind the last are left as
+                    they were); without it a new tensor, zero in such rows
     max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
     Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256.

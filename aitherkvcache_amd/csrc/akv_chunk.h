@@ -82,7 +82,7 @@ struct ck_args {
   int64_t max_blocks, num_blocks;
   int window;                                    // 0: none
   int kind;                                      // sequences of this launch: 0 all, 1 those of few rows, 2 the others
-  int tail;                                      // rows behind the last sequence are zeroed
+  int tail;                                      // rows of no sequence, behind the last or before the first, are zeroed
   float scale2;                                  // score scale x log2 e
 };
 
@@ -223,6 +223,19 @@ __device__ __forceinline__ void ck_find(const ck_args& a, ck_lengths<THREADS>& L
   seq = __builtin_amdgcn_readfirstlane(L.found[0]);
   tile = __builtin_amdgcn_readfirstlane(L.found[1]);
   first = ck_readfirst(L.total);
+}
+
+// Rows before the first sequence, by all workgroups: zeros.  (Those behind the last one are a sequence of no keys; these are as many as a caller
+// who takes a part of a batch leaves.)
+template <int THREADS> __device__ __forceinline__ void ck_clear_front(const ck_args& a, const ck_lengths<THREADS>& L, int D) {
+  const int rows = !a.tail ? 0 : a.S <= CK_SEQS ? L.start[0] : ck_start_of(a, 0);
+  if (rows == 0) return;
+  const int per = a.QH * (D / 4);
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (int64_t)rows * per; i += (int64_t)gridDim.x * THREADS) {
+    const int64_t token = i / per;
+    const int rest = (int)(i - token * per), head = rest / (D / 4);
+    *(ck_u2*)((uint16_t*)a.out + token * a.os_tok + (int64_t)head * a.os_head + 4 * (rest - head * (D / 4))) = (ck_u2){0u, 0u};
+  }
 }
 
 // where workgroup g's range begins: floor(total g / G), G at most 2^15

@@ -1148,6 +1148,7 @@ __global__ __launch_bounds__((ck_narrow<D, KIND>::THREADS), (ck_narrow<D, KIND>:
   extern __shared__ __align__(1024) unsigned char lds[];
   auto& L = ck_lengths_at<P>(lds, P::L0);
   ck_load_lengths(a, L);
+  ck_clear_front(a, L, D);
   const int64_t total = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
   ck_narrow_work<D, KIND>(a, lds, L, total, ck_workgroup(), gridDim.x, 1);
 }
@@ -1157,6 +1158,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   extern __shared__ __align__(1024) unsigned char lds[];
   auto& L = ck_lengths_at<P>(lds, P::L0);
   ck_load_lengths(a, L);
+  if (a.kind == 0) ck_clear_front(a, L, D);      // (the narrow kernel did otherwise)
   const int64_t per_head = ck_total<P::THREADS, P::N, P::START>(a, L, P::ROWS / a.GC);
   ck_wide_work<D, KIND>(a, lds, L, per_head, ck_workgroup(), gridDim.x, 0);
 }
@@ -1176,6 +1178,7 @@ __global__ __launch_bounds__((ck_wide<D, KIND>::THREADS), (ck_wide<D, KIND>::PER
   extern __shared__ __align__(1024) unsigned char lds[];
   auto& L = ck_lengths_at<W>(lds, ck_both<D, KIND>::L0);
   ck_load_lengths(many, L);
+  ck_clear_front(many, L, D);
   const int64_t few_total = ck_total<N::THREADS, N::N, N::START>(few, L, N::ROWS / few.GC), many_total = ck_total<W::THREADS, W::N, W::START>(many, L, W::ROWS / many.GC);
   const int G = gridDim.x, g = ck_workgroup(), few_heads = few.KVH * few.HS;
   const float few_cost = (float)N::COST * (float)few_heads * (float)few_total, many_cost = (float)W::COST * (float)(many.KVH * many.HS) * (float)many_total;

@@ -162,8 +162,8 @@ class TQPagedAttention:
         query_start_loc [num_seqs + 1]: sequence i owns query rows query_start_loc[i] .. query_start_loc[i + 1] - 1, the newest of
                         its context_lens[i] tokens; token j of n stands at position context_len - n + j and sees the
                         keys up to there (none: zeros)
-        out             where the result goes (shape and type of query; rows behind the last sequence are left as they were);
-                        without it a new tensor, zero in such rows
+        out             where the result goes (shape and type of query; rows before the first sequence or behind the last are left
+                        as they were); without it a new tensor, zero in such rows
         max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
         Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector.

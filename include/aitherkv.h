@@ -259,8 +259,8 @@ int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* str
  *   query        [num_tokens][num_q_heads][d] float16 or bfloat16, strides qs_tok / qs_head (last dim contiguous)
  *   query_starts [num_seqs + 1], non-decreasing, in [0, num_tokens] (clamped there; where one is less than the one before it rows
  *                of the call are undefined, but nothing else is read or written than otherwise)
- *   out          like query, its type; rows at or behind query_starts[num_seqs] are zeroed where zero_tail is not 0
- *                and left as they were otherwise
+ *   out          like query, its type; rows at or behind query_starts[num_seqs], and before query_starts[0], are zeroed where
+ *                zero_tail is not 0 and left as they were otherwise
  *   block_tables, context_lens, num_blocks as in akv_paged_attn: entries at or beyond ceil(ctx / block_size) are never
  *                read, entries inside are clamped into the cache
  *   max_query_len the longest chunk, as far as the caller knows it (0: not): which kernels are launched goes by it,

@@ -186,3 +186,37 @@ def test_a_zero_value_may_outweigh_all_others(dev, d, bits, lens, score):
     row = code @ p.tq.rotation.double() * math.sqrt(d)
     p.q = (row / (code * code).sum(-1, keepdim=True)).repeat_interleave(4, 0).expand(b.tokens, 8, d).to(BF).contiguous()
     check(p.run(), *packed_reference(p))
+
+
+# ---- rows of no sequence ------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lens", [[(3, 50)], [(90, 90)], [(3, 50), (90, 90)]], ids=["few", "many", "both"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_before_the_first_sequence(dev, lens, d):
+    """Starts that begin past row 0 (a part of a batch): rows of nobody are zero in a new tensor and left alone in a given one."""
+    b = Batch(lens, 16, dev, 16)
+    p = Packed(b, d, 4, 8, 2, BF, dev, 230)
+    _, kc, vc = dense_inputs(b, 8, 2, d, BF, dev, 231)
+    want = [p.reference(), dense_reference(b, p.q, kc, vc, 1 / math.sqrt(d), 0)]
+    p.q = torch.cat([torch.ones(37, 8, d, dtype=BF, device=dev), p.q, torch.ones(5, 8, d, dtype=BF, device=dev)])
+    b.starts = b.starts + 37
+    for call, w in zip((p.run, lambda **more: akv.paged_chunk_attention(p.q, kc, vc, b.tables, b.ctx, b.starts, **more)), want):
+        for _ in range(2):
+            torch.full_like(p.q, 7.0)                       # (what the next tensor of this size finds in memory)
+            got = call()
+            check(got[37:-5], *w)
+            assert not bool(got[:37].any()) and not bool(got[-5:].any())
+        mine = torch.full_like(p.q, 7.0)
+        call(out=mine)
+        check(mine[37:-5], *w)
+        assert bool((mine[:37] == 7).all()) and bool((mine[-5:] == 7).all())
+
+
+def test_rows_of_no_sequence_at_all(dev):
+    """No sequences: every row is nobody's, wherever the one start stands."""
+    kc = torch.ones(2, 16, 2, 64, dtype=FP, device=dev)
+    none = torch.zeros(0, 1, dtype=torch.int32, device=dev)
+    q = torch.ones(37, 8, 64, dtype=FP, device=dev)
+    for start in (0, 20, 37):
+        torch.full_like(q, 7.0)
+        assert not bool(akv.paged_chunk_attention(q, kc, kc, none, none[:, 0], torch.tensor([start], device=dev)).any())
