@@ -85,7 +85,8 @@ class _StandaloneImplBase:
     """Keeps what vLLM's attention impl constructor receives."""
 
     def __init__(self, num_heads, head_size, scale, num_kv_heads=None, alibi_slopes=None,
-                 sliding_window=None, kv_cache_dtype="auto", logits_soft_cap=None, **kwargs):
+                 sliding_window=None, kv_cache_dtype="auto", logits_soft_cap=None, attn_type="decoder",
+                 kv_sharing_target_layer_name=None, sinks=None, **kwargs):
         self.num_heads = num_heads
         self.head_size = head_size
         self.scale = float(scale)
@@ -94,6 +95,10 @@ class _StandaloneImplBase:
         self.sliding_window = (-1, -1) if sliding_window is None else (sliding_window - 1, 0)
         self.kv_cache_dtype = kv_cache_dtype
         self.logits_soft_cap = 0 if logits_soft_cap is None else logits_soft_cap
+        self.attn_type = getattr(attn_type, "value", attn_type)
+        self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
+        self.sinks = sinks
+        self.other_options = {k: v for k, v in kwargs.items() if v is not None and v is not False}
 
     def forward(self, *args, **kwargs):
         raise RuntimeError("attention over an uncompressed cache is vLLM's TritonAttentionImpl; "
@@ -115,19 +120,33 @@ def _vllm_unified_attention(impl, q, k_buf, v_buf, out, attn_metadata):
 
 
 def _dense_attention(impl, q, k_buf, v_buf, out, attn_metadata):
-    """vLLM's attention over the block buffer where vLLM is importable, paged_chunk_attention otherwise."""
-    try:
-        return _vllm_unified_attention(impl, q, k_buf, v_buf, out, attn_metadata)
-    except ImportError:
-        pass
+    """This package's attention over the block buffer: plain causal attention of a decoder layer, with or without a window.  What
+    else the impl was made with is refused, not left out."""
     from ..chunk_attention import paged_chunk_attention
     if impl.alibi_slopes is not None or impl.logits_soft_cap:
         raise NotImplementedError("ALiBi slopes and a soft cap of the scores need vLLM's attention; vLLM is not importable")
     left, right = impl.sliding_window
-    if right > 0:
-        raise NotImplementedError(f"a window of {impl.sliding_window} is not causal")
+    if right > 0 or not getattr(attn_metadata, "causal", True):
+        raise NotImplementedError(f"attention that is not causal (window {impl.sliding_window}) needs vLLM's; vLLM is not importable")
+    if getattr(impl, "attn_type", None) not in (None, "decoder"):
+        raise NotImplementedError(f"attention of type {impl.attn_type!r} needs vLLM's; vLLM is not importable")
+    others = {name: value for name, value in (("sinks", getattr(impl, "sinks", None)),
+                                              ("kv_sharing_target_layer_name", getattr(impl, "kv_sharing_target_layer_name", None)),
+                                              *getattr(impl, "other_options", {}).items()) if value is not None}
+    if others:
+        raise NotImplementedError(f"attention with {', '.join(sorted(others))} needs vLLM's; vLLM is not importable")
     paged_chunk_attention(q, k_buf, v_buf, attn_metadata.block_table, attn_metadata.seq_lens, attn_metadata.query_start_loc,
                           scale=impl.scale, window=left + 1 if left >= 0 else 0, out=out, max_query_len=attn_metadata.max_query_len)
+
+
+def _vllm_is_missing() -> bool:
+    try:
+        import vllm  # noqa: F401
+    except ModuleNotFoundError as e:
+        return e.name == "vllm"
+    except ImportError:
+        pass
+    return False
 
 
 # --------------------------------------------------------------------------------------------
@@ -203,6 +222,8 @@ def _make_impl_class():
         from vllm.v1.attention.backends.triton_attn import TritonAttentionImpl as base
     except ImportError:
         base = _StandaloneImplBase
+    # decided here, once: without vLLM this package's attention; with it vLLM's, and an import that fails inside it is an error
+    dense_attention = _dense_attention if base is _StandaloneImplBase and _vllm_is_missing() else _vllm_unified_attention
 
     from ..chunk_attention import rope_append
     from ..fused_attention import TQPagedAttention
@@ -231,7 +252,7 @@ def _make_impl_class():
         _INIT_AFTER_FORWARDS: ClassVar[int] = 2
         _MIN_BLOCKS_FOR_INIT: ClassVar[int] = 16
         # attention over an uncompressed block buffer: vLLM's kernel or this package's; replaceable (tests, other engines)
-        _dense_paged_attention = staticmethod(_dense_attention)
+        _dense_paged_attention = staticmethod(dense_attention)
 
         @classmethod
         def reset_class_state(cls) -> None:
