@@ -183,7 +183,10 @@ class TQPagedAttention:
         check_query(query)
         if k_packed.dim() != 4 or v_packed.dim() != 4 or k_norms.dim() != 3 or v_norms.dim() != 3:
             raise ValueError("expected caches [blocks, block_size, heads, bytes] and norms [blocks, block_size, heads]")
-        dev = _lib.require_gpu(query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc, out)
+        dev = _lib.require_gpu(query, k_packed, k_norms, v_packed, v_norms, block_tables, context_lens, query_start_loc, out, self.centroids, tq.rotation)
+        if self.centroids.numel() != 1 << self.bits:
+            raise ValueError(f"a codebook of {self.bits} bits has {1 << self.bits} levels, got shape {tuple(self.centroids.shape)}")
+        centroids = self.centroids.float().contiguous()
         num_tokens, num_q_heads, d = query.shape
         if d != self.head_dim or num_q_heads != self.num_query_heads:
             raise ValueError(f"query shape {tuple(query.shape)} does not match heads={self.num_query_heads}, head_dim={self.head_dim}")
@@ -210,7 +213,7 @@ class TQPagedAttention:
                 v_packed.data_ptr(), v_packed.stride(0), v_packed.stride(1), v_packed.stride(2),
                 v_norms.data_ptr(), v_norms.stride(0), v_norms.stride(1), v_norms.stride(2),
                 bt.data_ptr(), _lib.itype_code(bt), bt.stride(0), lens.data_ptr(), _lib.itype_code(lens),
-                starts.data_ptr(), _lib.itype_code(starts), tq.prepared_rotation().ptr, self.centroids.data_ptr(), self.bits,
+                starts.data_ptr(), _lib.itype_code(starts), tq.prepared_rotation().ptr, centroids.data_ptr(), self.bits,
                 result.data_ptr(), result.stride(0), result.stride(1), int(out is None),
                 num_seqs, num_tokens, num_q_heads, num_kv_heads, d, block_size, blocks, bt.shape[1],
                 _longest(max_query_len), self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))

@@ -188,6 +188,21 @@ def test_a_zero_value_may_outweigh_all_others(dev, d, bits, lens, score):
     check(p.run(), *packed_reference(p))
 
 
+# ---- codebooks ---------------------------------------------------------------------------------------------------------------------
+
+def test_codebooks_in_other_forms(dev):
+    """Levels as float64 or a strided view are what they are as float32; on the host, or too few, they are refused."""
+    p = Packed(Batch([(3, 90), (40, 77)], 16, dev, 19), 128, 4, 8, 2, BF, dev, 330)
+    want, levels = p.run(), p.tq.centroids
+    for same in (levels.double(), torch.stack([levels, -levels], 1)[:, 0]):
+        p.attn.centroids = same
+        assert torch.equal(p.run(), want)
+    for error, other in ((RuntimeError, levels.cpu()), (ValueError, levels[:8])):
+        p.attn.centroids = other
+        with pytest.raises(error):
+            p.run()
+
+
 # ---- rows of no sequence ------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("lens", [[(3, 50)], [(90, 90)], [(3, 50), (90, 90)]], ids=["few", "many", "both"])
