@@ -80,7 +80,7 @@ struct ck_args {
   int S, T, QH, KVH, G, HS, GC;                  // G query heads a kv head, in HS groups of GC
   int block_size; uint32_t bs_recip;
   int64_t max_blocks, num_blocks;
-  int window;                                    // 0: none
+  int window;                                    // 0: none; at most 2^30, as far as a position may lie below 0: their difference has 32 bits
   int kind;                                      // sequences of this launch: 0 all, 1 those of few rows, 2 the others
   int tail;                                      // rows of no sequence, behind the last or before the first, are zeroed
   float scale2;                                  // score scale x log2 e
@@ -137,8 +137,8 @@ template <int N> __device__ __forceinline__ ck_range ck_keys(const ck_args& a, c
   if (r.hi < 0) r.hi = 0;
   r.lo = 0;
   if (a.window > 0) {
-    const int64_t oldest = (int64_t)(s.ctx - s.n + t0) - a.window + 1;      // (a row of negative position with a window near 2^31)
-    r.lo = oldest > 0 ? (int)oldest : 0;
+    r.lo = s.ctx - s.n + t0 - a.window + 1;
+    if (r.lo < 0) r.lo = 0;
   }
   r.first = r.lo / N;
   r.units = (r.hi + N - 1) / N - r.first;

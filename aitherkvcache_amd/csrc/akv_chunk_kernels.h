@@ -234,7 +234,7 @@ template <int NT> __device__ __forceinline__ void ck_mask(ck_f16v (&s)[NT], int 
 
 // ---- rows and outputs of a tile -----------------------------------------------------------------------------------------
 struct ck_lane {                 // the row of a lane
-  int token, head, pos;          // query token of the call, query head, position (-1: no row, or one before the first key, sees nothing)
+  int token, head, pos;          // query token of the call, query head, position (below 0: no row, or one before the first key, sees nothing)
   bool valid;
 };
 __device__ __forceinline__ ck_lane ck_row_of(const ck_args& a, const ck_seq& s, int t0, int t1, int head, int row) {
@@ -244,7 +244,7 @@ __device__ __forceinline__ ck_lane ck_row_of(const ck_args& a, const ck_seq& s, 
   r.valid = t0 + j < t1 && g < a.G;
   r.token = r.valid ? s.q0 + t0 + j : 0;
   r.head = r.valid ? (head / a.HS) * a.G + g : 0;
-  r.pos = r.valid ? max(-1, s.ctx - s.n + t0 + j) : -1;      // (windows up to 2^31 - 1 are taken off)
+  r.pos = r.valid ? s.ctx - s.n + t0 + j : -1;
   return r;
 }
 // quad c of a row's outputs: coordinates 8 c + 4 h .. + 3, finished
@@ -405,7 +405,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
     if (u1 <= 0) return;           // (nothing but the start of the tile: it begins in the next range)
     const ck_lane row = ck_row_of(a, s, t0, t1, head, col);
     const int kvh = head / a.HS;
-    const int pos_first = s.ctx - s.n + t0, pos_last = max(-1, s.ctx - s.n + t1 - 1);
+    const int pos_first = s.ctx - s.n + t0, pos_last = s.ctx - s.n + t1 - 1;
 
     // ---- 32 keys of the wavefront, a lane its half of one (outside of what the tile sees: its first or last key, masked.  What else lies
     // there may be anything, and a weight of zero does not undo an infinity)
@@ -803,7 +803,7 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
     const int kvh = head / a.HS;
     // positions of the wavefront's rows
     const int w0 = t0 + 32 * wave / a.GC, w1 = min(t1, t0 + (32 * wave + 31) / a.GC + 1);
-    const int pos_first = s.ctx - s.n + w0, pos_last = w0 < t1 ? max(-1, s.ctx - s.n + w1 - 1) : -1;
+    const int pos_first = s.ctx - s.n + w0, pos_last = w0 < t1 ? s.ctx - s.n + w1 - 1 : -1;
     ck_f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = (ck_f16v)(0.f);

@@ -270,7 +270,8 @@ int akv_debug_read_probe(const void* src, size_t bytes, void* sink256, void* str
  * past a context, or older than every token's window, may hold anything, and table entries of such blocks are not read.
  *
  * akv_dense_chunk_attn: over a cache [num_blocks][block_size][num_kv_heads][d] of the query's type (element
- * strides, rows at multiples of 16 bytes); window > 0: a token sees the newest `window` keys only (its own included).
+ * strides, rows at multiples of 16 bytes); window > 0: a token sees the newest `window` keys only (its own included; of more than
+ * 2^30 only where the tables hold no more than that).
  * akv_paged_chunk_attn: over the packed cache of akv_paged_attn (rows at multiples of 4 bytes), scores and values of all
  * tokens, the chunk's own included, as decoded from it.
  * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must
