@@ -78,7 +78,8 @@ def paged_chunk_attention(query: torch.Tensor, key_cache: torch.Tensor, value_ca
 
     Token j of n stands at position context_len - n + j; one without a key gets zeros.  head_dim is 64, 128 or 256.
     Values that some token of a sequence's chunk sees must be finite; past a context, or before every token's window, the caches and
-    tables may hold anything."""
+    tables may hold anything.  Scores and sums are float32; a key's weight is rounded to the query's type before it meets its value
+    (in float16 also by 2^-30 of the row's largest), and so is the result."""
     result = _lib.calls().dense_chunk(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, scale, window, out,
                                       max_query_len)
     if result is not None:

@@ -48,8 +48,16 @@ template <int KIND> struct ck_math {
   }
 };
 
-#define CK_SEQS 256               // sequences whose starts and lengths are held in LDS (more are read from memory)
-#define CK_NARROW_ROWS 64         // a sequence of at most so many rows a kv head goes to the narrow kernel
+// Sequences whose starts and lengths are held in LDS.  More are read from memory, by every workgroup's search (256 of 1 to 3 tokens after 500
+// packed keys 177 us, 257 201, 1024 699).
+#define CK_SEQS 256
+// A sequence of at most so many rows a kv head goes to the narrow kernel.  Measured with all on it | all on the wide one, 4 rows a token, us.
+// 4 bits, 32 sequences after 4000 keys: heads of 128, 24 rows 82 | 194, 64 rows 145 | 197, 68 rows 203 | 196, 128 rows 275 | 201; of 256
+// 205 | 663, 384 | 681, 555 | 714, 739 | 758; of 64 49 | 94, 85 | 106, 118 | 112, 155 | 125.  One sequence after 20000: narrow at any of these.
+// Plain rows, one sequence of 24 to 64 rows after 20000 keys: heads of 64 39 | 44 to 61, of 128 50 | 38 and 54 | 43, of 256 87 | 70 and
+// 115 | 84; 32 sequences after 4000, where memory counts: 64 91 | 70 and 113 | 75, 128 139 | 119 and 171 | 122, 256 323 | 251 and 628 | 271:
+// plain rows would gain by a lower number.
+#define CK_NARROW_ROWS 64
 
 struct ck_record {                // what a workgroup leaves of the tile that begins in its range and ends in another
   int64_t end;                    // one past the tile on the axis

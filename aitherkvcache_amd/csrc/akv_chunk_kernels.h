@@ -15,8 +15,9 @@
 // norm multiplies its score in float32; a value's norm v goes into the exponent, w = 2^(s + log2 v - M), with M from the running maximum of
 // s + log2 v, so weights stay in [0, 2^(CK_LIFT + CK_FRAME)] for norms of any size, and the sum of the softmax takes w / v.
 //
-// What is rounded to sixteen bits: the weights, once, as operand of the second product (relative 2^-11 or 2^-8, as of the values beside them);
-// packed: the levels (2^-14) and the queries (many rows: one float16 term; few rows: two, 2^-22).  Scores, maxima, sums and results are float32.
+// What is rounded to sixteen bits: the weights, once, as operand of the second product (relative 2^-11 or 2^-8, as of the values beside them;
+// float16 ones, those over packed rows in either type, besides by 2^-30 of the row's largest); packed: the levels (2^-14) and the queries (many
+// rows: one float16 term; few rows: two, 2^-22).  Scores, maxima, sums and results are float32.
 #pragma once
 #include "akv_chunk_rotate.h"
 #include "akv_device_once.h"
@@ -337,14 +338,18 @@ template <int W> __device__ __forceinline__ void ck_load_words(uint32_t (&w)[W],
 // part of LDS (sixteen bytes c of value t lie at c ^ f(t), which 16 rows written and 4 read at a time meet all banks with); what the
 // wavefronts hold of the tile is added at the end of the tile or range.  No barrier inside.  Packed codes of two units are on their way at a
 // time, of one for heads of 256, whose sums leave no registers (9 sequences of 162 tokens over 39562 keys, 4 bits: 5373 us with two, 2005).
-// 16 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 158 us, 2.2 TB/s; the vector unit (45% of the time), the
-// look-ups and operands in LDS (48%) and waits in turn bound it, some 22 us before the first unit and 10 after the last.  Heads of 256,
-// bfloat16, a window of 1024 keys, 38 MB: 39 us, which is latency: lengths, table, keys, the second unit's keys, pieces, their join.
+// 16 users' drafts of four tokens over 1000 to 40000 keys of 4 bits, 350 MB: 151 us, 2.3 TB/s; the vector unit (46% of the time), the
+// look-ups and operands in LDS (47%) and waits in turn bound it, besides what lies before the first unit and behind the last.  Heads of 256,
+// bfloat16, a window of 1024 keys, 38 MB: 40 us, which is latency: lengths, table, keys, the second unit's keys, pieces, their join; and 19
+// reloads of spilled registers and 176 moves of sums a unit.
 template <int D, int KIND> struct ck_narrow {
   static constexpr bool PACKED = KIND >= 2;
   static constexpr int WAVES = PACKED && D < 256 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32, N = 32 * WAVES, START = 3;
   static constexpr int PER_CU = PACKED || D == 256 ? 1 : 2, PER_SIMD = D == 256 ? 1 : 2;
-  static constexpr int COST = PACKED ? 3 : D == 256 ? 5 : 2;         // of a unit, beside ck_wide's (packed rows of 128: 2.7 us and 3.6 us)
+  // Of a unit, beside ck_wide's, where both share a launch.  Measured over 32 sequences of one full tile after 8000 to 25000 keys, us: plain heads
+  // of 64 4.4 and 1.9, of 256 9.7 and 2.1; 4 bits, heads of 128 3.1 and 3.1, of 256 4.6 and 3.6; with keys of a few thousand, which
+  // caches hold, packed rows of 128 took 2.7 and 3.6.
+  static constexpr int COST = PACKED ? 3 : D == 256 ? 5 : 2;
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8, QW = QUADS / WAVES;
   static constexpr int V_BYTES = 32 * 2 * D, ROW = D + 4;            // (of a value; floats of a row that is turned)
   // sums of the wavefronts: the upper half's are added to the lower's first where not all fit
@@ -709,8 +714,10 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
 //
 // The matrix cores bound it as far as the chip's power allows: 2048 rows over 31000 keys, 32 heads of 128 in bfloat16 take 1060 to 1120 us by the
 // machine, 1000 TFLOP/s, where a large product of the library reaches 1280 (products 47% of the clocks; written out in turns by hand it is no
-// faster).  Heads of 64 are bound by the vector unit, 60% of the clocks.  Packed rows of 128: 630 TFLOP/s; codes are looked up by every
-// workgroup for its 256 rows, LDS is busy 46% and the vector unit 55% of the clocks, and registers leave no room for more in flight.
+// faster).  Heads of 64 are bound by the vector unit, 60% of the clocks.  Packed rows of 128: 640 TFLOP/s; codes are looked up by every
+// workgroup for its 256 rows, LDS is busy 47% and the vector unit 56% of the clocks, and registers leave no room for more in flight.  Heads of
+// 256: the sums do not stay where the products leave them, a step of 32 products has some 630 moves between the two register files (one
+// prompt of 2048 after 6000 keys 943 us, 480 TFLOP/s).
 //
 // Rows lie in LDS without padding, their pieces of sixteen bytes in an order that depends on the row, piece c at place c ^ f(row): sixteen
 // lanes that read one piece of sixteen keys, and 32 that read four coordinates each of four values, meet all 64 banks once
@@ -719,7 +726,10 @@ template <int D, int KIND> struct ck_wide {
   static constexpr bool AHEAD = D == 64 || (D == 128 && KIND < 2);    // registers for the keys of the step after the next
   static constexpr int EARLY = AHEAD ? D / 16 : KIND >= 2 && D < 256 ? D / 32 : 0;     // pieces of a step's keys that are read during the step before
   static constexpr int WAVES = D == 128 ? 8 : 4, THREADS = 64 * WAVES, ROWS = 32 * WAVES, N = D == 256 ? 32 : 64, STEPS = N / 32;
-  static constexpr int START = 192 / N;                               // (what a tile costs besides its units, in units)
+  // What a tile costs besides its units, in units; both kernels', as it is | none | twice as much: 2048 tokens after nothing 78.7 | 102 | 80.4 us, 40
+  // prompts of 30 to 200 67.7 | 74.4 | 67.9, 16 drafts over up to 40000 packed keys 175 | 182 | 175, 64 of 5 tokens after 20 to 400 30.1 | 32.7 | 29.6,
+  // a window of 1024 at heads of 256 39.0 | 43.3 | 41.1.
+  static constexpr int START = 192 / N;
   static constexpr int PER_CU = D == 256 || WAVES == 8 ? 1 : 2;       // workgroups a CU
   static constexpr int PER_SIMD = D == 256 ? 1 : 2;                   // wavefronts a SIMD
   static constexpr int KS = D / 16, DT = D / 32, QUADS = D / 8;
@@ -1296,8 +1306,9 @@ static int ck_launch(ck_args a, int most_new, void* scratch, hipStream_t stream)
   // each takes its own, by the lengths on the device.
   const int64_t most = most_new > 0 && most_new < a.T ? most_new : a.T;
   // Packed rows and float16: all of them as well.  The wide kernel has no registers for the queries' second term, without which float16
-  // outputs are off by 4e-4 to 5e-4 of their size instead of 2.1e-4 (their own rounding)
-  // to 2.8e-4.  Four bits, 32 heads of 128: 126 us over 12 turns of 1 to 90 tokens (wide kernel 144), 891 over two prompts of 1000 (493).
+  // outputs are off by 4.2e-4 to 5.4e-4 of their size instead of 2.2e-4 (their own rounding is 2.1e-4) to 2.9e-4.  Time with this rule | without,
+  // us, 4 bits, 32 heads: 12 turns of 1 to 90 tokens at heads of 64 75 | 94, of 128 126 | 117, of 256 312 | 444; two prompts of 1000 after 7000
+  // 482 | 349, 768 | 459, 2117 | 1762.
   const bool few = most * a.G <= CK_NARROW_ROWS || (KIND >= 2 && a.dtype == AKV_F16), one = !few && a.S == 1;
   typedef ck_narrow<D, KIND> N;
   typedef ck_both<D, KIND> B;

@@ -7,7 +7,8 @@
 // in, so memory bounds it: a thread takes a unit of sixteen coordinates of a row, eight pairs or sixteen that do not turn, in
 // pieces of eight (16 bytes); units of the token's other rows find the table's row in the first-level cache.  Where the axes take whole units a
 // unit has one position and reads the table in wide loads (with a position looked up for every pair 4097 tokens of three axes took 40 us).
-// 8192 tokens of 48 rows of 128 in bfloat16, 206 MB: 43.0 us, 4.8 TB/s (a large copy reaches 5.2); one token 4.7 us, the host's time.
+// 8192 tokens of 48 rows of 128 in bfloat16, 206 MB: 43.0 us, 4.8 TB/s, where the inputs come from memory (a large copy reaches 5.2), 33.8 where
+// the last-level cache holds them from the call before; one token 4.7 us, the host's time.
 #include "akv_common.h"
 
 #define RP_AXES 4

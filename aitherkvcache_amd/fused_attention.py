@@ -167,7 +167,9 @@ class TQPagedAttention:
         max_query_len   the longest chunk, if known on the host: what is launched goes by it, the result but for its last rounding does not
 
         Caches, norms and tables as in forward(); head_dim 64, 128 or 256, rows at multiples of 4 bytes.  No block selector.
-        Norms of the sequences' tokens must be finite; past a context the caches and tables may hold anything."""
+        Norms of the sequences' tokens must be finite; past a context the caches and tables may hold anything.
+        Rounded on the way, whatever the query's type: levels and weights to float16 (weights also by 2^-30 of the row's largest),
+        rotated queries to one float16 term, or to two where the query is float16 or chunks are short; sums are float32."""
         from .chunk_attention import _check_out, _longest, check_chunk, check_query
         if self._block_selector is not None:
             raise ValueError("forward_chunk does not run the block selector")
