@@ -152,9 +152,10 @@ template <int BITS, int COPIES> struct ck_lut {
 // weights of up to 2^13 lose nothing, as their rounding is relative and float16 reaches 2^16 (the other 2^3: scores of 2^26 are rounded to
 // steps of 8, of which a maximum may be off by half).  What lies far below the largest keeps the more: float16 weights are in steps of 2^-24
 // at least, 2^-29 of the largest (with the largest at 1 keys 2^-26 below it were lost however many or large they were).  A frame of 4 under
-// a lift of 7 rescales more often: a first chunk of 2048 tokens 75.2 us, this one 72.7.
+// a lift of 7 rescales more often: a first chunk of 2048 tokens 75.2 us, this one 72.7.  bfloat16 weights have the range as they are, and
+// values that may be of any size beside them: no lift.
 #define CK_FRAME 8.f
-#define CK_LIFT 5.f
+template <int KIND> constexpr float CK_LIFT = KIND == CK_BF16 ? 0.f : 5.f;
 struct ck_row { float m, l; };
 // largest of NT tiles of 32 products, over both halves
 template <int NT> __device__ __forceinline__ float ck_max(const ck_f16v (&s)[NT]) {
@@ -170,10 +171,10 @@ template <int NT> __device__ __forceinline__ float ck_max(const ck_f16v (&s)[NT]
   return fmaxf(a, akv_lane_xor<32>(a));
 }
 // Whether some row's largest exponent has outgrown its frame; `alpha` is then what the row's sums are multiplied with.
-__device__ __forceinline__ bool ck_outgrown(ck_row& r, float mx, float& alpha) {
-  const bool grown = mx - r.m > CK_LIFT + CK_FRAME;      // (the difference of two numbers so near is exact)
+template <int KIND> __device__ __forceinline__ bool ck_outgrown(ck_row& r, float mx, float& alpha) {
+  const bool grown = mx - r.m > CK_LIFT<KIND> + CK_FRAME;      // (the difference of two numbers so near is exact)
   if (!__ballot(grown)) return false;
-  const float m = grown ? mx - CK_LIFT : r.m;
+  const float m = grown ? mx - CK_LIFT<KIND> : r.m;
   alpha = grown ? ck_exp2(r.m - m) : 1.f;
   r.m = m;
   r.l *= alpha;
@@ -605,7 +606,7 @@ __device__ __forceinline__ void ck_narrow_work(const ck_args& a, unsigned char* 
       if constexpr (PACKED) ck_norms(sc, nrm[wave][0], nrm[wave][1]);
       if (base + 31 > pos_first || (a.window > 0 && base <= pos_last - a.window)) ck_mask(sc, base, row.pos, a.window);
       float alpha;
-      if (ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
+      if (ck_outgrown<KIND>(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha)) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= alpha;
       }
@@ -997,7 +998,7 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
       if constexpr (PACKED) ck_norms(sc, nr, nr + N);
       if (base0 + 31 > pos_first || (a.window > 0 && base0 <= pos_last - a.window)) ck_mask(sc, base0, row.pos, a.window);
       float alpha;
-      ck_outgrown(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha);      // (nothing to rescale yet)
+      ck_outgrown<KIND>(st, ck_max(sc) * (PACKED ? 1.f : a.scale2), alpha);      // (nothing to rescale yet)
     }
     const bool busy = 32 * wave < (t1 - t0) * a.GC;      // (a wavefront behind the tile's last row only brings keys and values)
     int k_slot = 0;                // of unit u
@@ -1081,7 +1082,7 @@ __device__ __forceinline__ void ck_wide_work(const ck_args& a, unsigned char* co
           mx = ck_max(sc);
         }
         float alpha;
-        if ((t + 1 < P::STEPS || u + 1 < units) && ck_outgrown(st, mx, alpha)) {
+        if ((t + 1 < P::STEPS || u + 1 < units) && ck_outgrown<KIND>(st, mx, alpha)) {
 #pragma unroll
           for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }

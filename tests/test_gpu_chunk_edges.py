@@ -127,6 +127,18 @@ def test_small_weights_of_large_values(dev, d, dtype, n, gap):
     check(got, out, (2 * u + 2.0 ** -14) * out + 2.0 ** -30 * w.amax(1)[:, None, None] * float(v.sum(0)[0]))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [2, 70], ids=["few", "many"])
+def test_large_bfloat16_values(dev, d, n):
+    """Values of up to 2^119 under equal scores: with weights of 1 their sum over 100 keys is a float32 number."""
+    b = Batch([(n, 100)], 16, dev, 25)
+    q, kc, vc = dense_inputs(b, 4, 2, d, BF, dev, 215)
+    q.zero_()
+    vc = (vc.float().abs().clamp(0.5, 2.0) * 2.0 ** 118).bfloat16()
+    got = akv.paged_chunk_attention(q, kc, vc, b.tables, b.ctx, b.starts)
+    check(got, *dense_reference(b, q, kc, vc, 1 / math.sqrt(d), 0))
+
+
 # ---- norms of zero -------------------------------------------------------------------------------------------------------------------
 
 def packed_reference(p):
