@@ -31,8 +31,9 @@ extern "C" int akv_dense_chunk_attn(const void* query, int dtype, int64_t qs_tok
   a.block_size = block_size; a.bs_recip = ck_reciprocal(block_size);
   a.max_blocks = num_blocks > 0 ? max_blocks_per_seq : 0; a.num_blocks = num_blocks;
   a.kv_alike = ks_blk == vs_blk && ks_pos == vs_pos && ks_head == vs_head;
-  // a window that reaches as far as the tables is none
-  a.window = window < a.max_blocks * block_size ? window : 0;
+  // a window that reaches as far as the tables (and lengths, ck_ctx_of) is none
+  const int64_t longest = a.max_blocks * block_size;
+  a.window = window < (longest < 0x7fff0000 ? longest : 0x7fff0000) ? window : 0;
   if (a.window > 1 << 30) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: windows of more than 2^30 tokens over longer tables", name);
   a.tail = zero_tail; a.scale2 = scale * 1.44269504088896341f;
   const hipStream_t s = (hipStream_t)stream;
