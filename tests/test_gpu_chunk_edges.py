@@ -247,3 +247,38 @@ def test_rows_of_no_sequence_at_all(dev):
     for start in (0, 20, 37):
         torch.full_like(q, 7.0)
         assert not bool(akv.paged_chunk_attention(q, kc, kc, none, none[:, 0], torch.tensor([start], device=dev)).any())
+
+
+# ---- caches laid out otherwise -----------------------------------------------------------------------------------------------------
+
+def relaid(x, order):
+    """The same cache with its dimensions in `order` in memory, rows 16 bytes apart and more."""
+    room = torch.zeros(*[x.shape[i] for i in order], x.shape[3] + (16 if x.dtype == torch.uint8 else 8), dtype=x.dtype, device=x.device)
+    back = [order.index(i) for i in range(3)]
+    y = room[..., :x.shape[3]].permute(*back, 3)
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("lens", [[(3, 150), (1, 40)], [(90, 200), (70, 70)], [(3, 150), (90, 200)]], ids=["few", "many", "both"])
+@pytest.mark.parametrize("orders", [((0, 2, 1), (0, 1, 2)), ((2, 0, 1), (1, 0, 2)), ((0, 2, 1), (0, 2, 1))])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_keys_and_values_laid_out_otherwise(dev, lens, orders, d):
+    """Heads before places, heads before blocks, places before blocks; keys and values each their own."""
+    b = Batch(lens, 16, dev, 26)
+    q, kc, vc = dense_inputs(b, 8, 2, d, BF, dev, 340)
+    b.unused(math.nan, kc, vc)
+    want = akv.paged_chunk_attention(q, kc, vc, b.tables, b.ctx, b.starts)
+    check(want, *dense_reference(b, q, kc, vc, 1 / math.sqrt(d), 0))
+    assert torch.equal(akv.paged_chunk_attention(q, relaid(kc, orders[0]), relaid(vc, orders[1]), b.tables, b.ctx, b.starts), want)
+    p = Packed(b, d, 3, 8, 2, BF, dev, 341)
+    want = p.run()
+    check(want, *p.reference())
+    p.k, p.v = relaid(p.k, orders[0]), relaid(p.v, orders[1])
+    assert torch.equal(p.run(), want)
+    p.kn, p.vn = (relaid(x[..., None], o)[..., 0] for x, o in ((p.kn, orders[1]), (p.vn, orders[0])))
+    assert torch.equal(p.run(), want)
+    slots = torch.randperm(b.blocks * 16, device=dev)[:b.tokens]
+    plain, other = [torch.zeros_like(kc) for _ in range(2)], [relaid(torch.zeros_like(kc), o) for o in orders]
+    for caches in (plain, other):
+        akv.rope_append(None, q[:, :2], q[:, 2:4], None, None, slots, *caches)
+    assert torch.equal(other[0], plain[0]) and torch.equal(other[1], plain[1])
