@@ -28,6 +28,14 @@ _ITYPE = {torch.int32: AKV_I32, torch.int64: AKV_I64}
 
 _p, _i, _i64, _sz, _f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 
+EVICT_CACHES = 8
+
+
+class EvictCache(C.Structure):
+    """akv_evict_cache"""
+    _fields_ = [("data", _p), ("s_blk", _i64), ("s_pos", _i64), ("s_head", _i64), ("row_bytes", _i64)]
+
+
 # name -> (restype, argtypes); must list every symbol include/aitherkv.h declares
 SIGNATURES = {
     "akv_version": (C.c_char_p, []),
@@ -114,6 +122,21 @@ SIGNATURES = {
     "akv_block_rep_finalize": (_i, [_p, _i, _i64, _p, _p, _p, _p, _p, _i64, _i, _i, _p]),
     "akv_block_scores": (_i, [_p, _p, _p, _p, _p, _i, _i64, _p, _i, _i, _i, _i, _i, _i64, _i, _i64, _p, _p]),
     "akv_block_select": (_i, [_p, _p, _i, _i64, _p, _i, _i, _i64, _i, _i, _i, _i, _p, _p, _p]),
+    "akv_block_index_update": (_i, [_p, _i, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i, _p, _p, _i, _i64, _i, _i, _i, _i64, _i64, _p]),
+    "akv_block_index_select_workspace_bytes": (_sz, [_i64, _i, _i64]),
+    "akv_block_index_select": (_i, [_p, _i, _i64, _i64, _p, _p, _p, _i, _i64, _p, _i, _p, _i, _p,
+                                    _i, _i64, _i, _i, _i, _i, _i64, _i64, _i, _i, _i, _p, _sz, _p]),
+    "akv_sparse_attn": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                             _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i, _p, _i64, _i64, _i,
+                             _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p]),
+    "akv_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i64]),
+    "akv_key_weights": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i64, _i,
+                             _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
+    "akv_packed_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i64]),
+    "akv_packed_key_weights": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i,
+                                    _p, _p, _i, _p, _i64, _i64, _i64, _i, _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
+    "akv_evict_select": (_i, [_p, _i64, _i64, _i64, _p, _i, _i, _i, _i, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p]),
+    "akv_evict_move": (_i, [_p, _i64, _i64, _p, _i, _i, _p, _i, _i64, _i64, _p, _i, _i64, _i64, C.POINTER(EvictCache), _i, _i, _i, _i, _i64, _p]),
     "akv_tri_encode": (_i, [_p, _i, _i64, _i, _i64, _i, _i, _p, _p, _p, _p]),
     "akv_tri_encode_paged": (_i, [_p, _i, _i64, _i, _i, _i64, _i64, _i, _p, _i, _i64, _p, _p, _p, _p]),
     "akv_tri_encode_paged_kv": (_i, [_p, _p, _i, _i64, _i, _i, _i64, _i64, _i, _p, _i, _i64, _p, _p, _p, _p, _p, _p, _p]),

@@ -221,6 +221,53 @@ class TQPagedAttention:
                 _longest(max_query_len), self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
         return result
 
+    def key_weights(self, query, k_packed, k_norms, block_tables, context_lens, query_start_loc, block_size: int = 16,
+                    num_kv_heads: Optional[int] = None, accumulated: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The softmax weight that every key of the packed cache gets from its sequence's newest tokens (causal, as forward_chunk weighs
+        them; a chunk of one token as forward), summed over these tokens and over the query heads of a kv head:
+        [num_seqs, num_kv_heads, length] float32, a key at its position.
+
+        query, k_packed, k_norms, block_tables, context_lens, query_start_loc as in forward_chunk
+        accumulated  as in paged_key_weights: float32, added to and returned; without it a new tensor as long as the tables
+
+        head_dim 64, 128 or 256, rows at multiples of 4 bytes; norms of the sequences' tokens must be finite.  Scores, weights and sums
+        are float32, levels and rotated queries two float16 terms each (2^-22)."""
+        from .chunk_attention import check_chunk, check_query
+        from .eviction import weights_for
+        tq = self._tq
+        if tq.rotation is not self.rotation:
+            self.rotation = tq.rotation
+        check_query(query)
+        if k_packed.dim() != 4 or k_norms.dim() != 3:
+            raise ValueError("expected a cache [blocks, block_size, heads, bytes] and norms [blocks, block_size, heads]")
+        num_tokens, num_q_heads, d = query.shape
+        if d != self.head_dim or num_q_heads != self.num_query_heads:
+            raise ValueError(f"query shape {tuple(query.shape)} does not match heads={self.num_query_heads}, head_dim={self.head_dim}")
+        if self.centroids.numel() != 1 << self.bits:
+            raise ValueError(f"a codebook of {self.bits} bits has {1 << self.bits} levels, got shape {tuple(self.centroids.shape)}")
+        if k_packed.dtype != torch.uint8 or k_packed.stride(-1) != 1 or k_packed.shape[-1] < self.packed_dim:
+            raise ValueError(f"k_packed must be uint8 with contiguous rows of >= {self.packed_dim} bytes")
+        if num_kv_heads is None:
+            num_kv_heads = k_packed.shape[2]
+        if block_size < 1:
+            raise ValueError(f"block_size {block_size}")
+        _lib.check_caches(block_size, num_kv_heads, k_packed, k_norms)
+        num_seqs, q, bt, lens, starts = check_chunk(query, num_kv_heads, block_tables, context_lens, query_start_loc)
+        dev = _lib.require_gpu(query, k_packed, k_norms, block_tables, context_lens, query_start_loc, accumulated, self.centroids, tq.rotation)
+        centroids = self.centroids.float().contiguous()
+        k_norms = k_norms if k_norms.dtype == torch.float32 else k_norms.float()
+        w = weights_for(accumulated, num_seqs, num_kv_heads, bt.shape[1] * block_size, dev)
+        L = _lib.lib()
+        ws = torch.empty(L.akv_packed_key_weights_workspace_bytes(num_tokens, num_q_heads, d, w.shape[2]), dtype=torch.uint8, device=dev)
+        with _lib.on_device(dev):
+            _lib.check(L.akv_packed_key_weights(
+                q.data_ptr(), _lib.dtype_code(q), q.stride(0), q.stride(1), k_packed.data_ptr(), k_packed.stride(0), k_packed.stride(1), k_packed.stride(2),
+                k_norms.data_ptr(), k_norms.stride(0), k_norms.stride(1), k_norms.stride(2), bt.data_ptr(), _lib.itype_code(bt), bt.stride(0),
+                lens.data_ptr(), _lib.itype_code(lens), starts.data_ptr(), _lib.itype_code(starts), tq.prepared_rotation().ptr, centroids.data_ptr(), self.bits,
+                w.data_ptr(), w.stride(0), w.stride(1), w.shape[2], int(accumulated is not None), num_seqs, num_tokens, num_q_heads, num_kv_heads, d, block_size,
+                min(k_packed.shape[0], k_norms.shape[0]), bt.shape[1], self.scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
+        return w
+
     def last_call_status(self) -> int:
         """0 when the most recent forward() / forward_no_alloc() ran clean; bit 0 set when it failed on the device (its
         outputs are NaN).  Synchronises the stream."""

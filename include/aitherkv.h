@@ -558,6 +558,93 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
                      int block_size, int max_selected, int num_sink_blocks, int num_recent_blocks,
                      void* filtered_block_tables, void* filtered_context_lens, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A part of a long context (no counterpart in the reference but for the idea of scoring blocks,
+ * aither_kvcache/block_selector.py): what a block's keys look like, the blocks that a token reads, attention over
+ * them, the weight every key gets, and tokens given up.  Sequences, starts, lengths and tables are those of a chunk
+ * of new tokens (above): starts are clamped into [0, num_tokens], lengths to what the tables hold, table entries into the cache,
+ * and entries at or beyond ceil(ctx / block_size) are never read.  Plain caches [num_blocks][block_size][num_kv_heads][d] of
+ * float16 or bfloat16, element strides, rows at multiples of 16 bytes; d is 64, 128 or 256.
+ *
+ * akv_block_index_update: of every block that the sequences' new tokens came to (query_starts NULL: of every
+ *   block of theirs), per kv head the mean of the keys it holds, in 8 bits: codes [num_blocks][num_kv_heads][d] int8, scales
+ *   [num_blocks][num_kv_heads] float32, contiguous.  scale = max |mean| (1 / 127), code = rint(mean (1 / max |mean| 127)), every operation
+ *   on the mean rounded to float32; zeros where the mean is not finite.
+ * akv_block_index_select: selected [num_tokens][num_kv_heads][num_selected] int32, table columns in ascending order, -1 behind the
+ *   last: of the blocks up to the token's own the first num_sink_blocks, the last num_recent_blocks (at least 1) and the best others
+ *   by (c_q . code) scale, c_q the sum of the group's queries in 8 bits like a mean; equal scores: the lower column.  Tokens
+ *   of no sequence, or before the first key, have -1.
+ * akv_sparse_attn: attention of every new token over the keys at its position and before in the blocks its kv head has
+ *   selected (a set: order and repetition do not matter; entries below 0 or past the token's own block are skipped); a row without a key
+ *   is zero.  selected has strides ss_tok / ss_head, at most 4096 entries a list.  zero_tail as above.  Values at the
+ *   positions up to the chunk's last in a selected block must be finite.  Blocks of at most 4096 tokens.
+ * akv_key_weights: weights [num_seqs][num_kv_heads][length] float32 (strides ws_seq / ws_head, length >= max_blocks_per_seq x block_size): the
+ *   softmax weight of every key summed over the sequence's new tokens and the group's heads; accumulate: added to what is there (only
+ *   keys of the context are touched), otherwise written, zeros elsewhere.
+ * akv_packed_key_weights: the same over packed rows and norms as in akv_paged_attn.
+ * akv_evict_select: per sequence and kv head min(ctx, keep) positions in ascending order (kept [num_seqs][num_kv_heads][keep] int32, -1 behind
+ *   the last): the first num_sink, the last num_recent and the heaviest others; equal weights: the lower position; a NaN counts
+ *   as -infinity.  kept_weights (like weights, another tensor): their weights, then zeros.  kept_lens [num_seqs] in the
+ *   type of context_lens (another tensor).  Lengths are clamped to `length`.
+ * akv_evict_move: rows of up to AKV_EVICT_CACHES caches [num_blocks][block_size][num_kv_heads][row_bytes] (byte strides): position kept[j] to position
+ *   j, in the blocks of out_tables, which no sequence of the call may read, or in place (out_tables NULL; no two sequences may
+ *   share a block then).  caches is a host pointer.
+ * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must not overlap in time.
+ * ------------------------------------------------------------------------------- */
+int akv_block_index_update(const void* key_cache, int dtype, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
+                           const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
+                           const void* query_starts, int qs_itype, int8_t* codes, float* scales,
+                           int num_seqs, int64_t num_tokens, int num_kv_heads, int d, int block_size,
+                           int64_t num_blocks, int64_t max_blocks_per_seq, void* stream);
+size_t akv_block_index_select_workspace_bytes(int64_t num_tokens, int num_kv_heads, int64_t max_blocks_per_seq);
+int akv_block_index_select(const void* query, int dtype, int64_t qs_tok, int64_t qs_head, const int8_t* codes, const float* scales,
+                           const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
+                           const void* query_starts, int qs_itype, int32_t* selected,
+                           int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
+                           int64_t num_blocks, int64_t max_blocks_per_seq,
+                           int num_selected, int num_sink_blocks, int num_recent_blocks,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
+                    const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
+                    const void* value_cache, int64_t vs_blk, int64_t vs_pos, int64_t vs_head,
+                    const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
+                    const void* query_starts, int qs_itype, const int32_t* selected, int64_t ss_tok, int64_t ss_head, int num_selected,
+                    void* out, int64_t os_tok, int64_t os_head, int zero_tail,
+                    int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
+                    int64_t num_blocks, int64_t max_blocks_per_seq, float scale, void* stream);
+size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length);
+int akv_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
+                    const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
+                    const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
+                    const void* query_starts, int qs_itype, float* weights, int64_t ws_seq, int64_t ws_head, int64_t length, int accumulate,
+                    int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
+                    int64_t num_blocks, int64_t max_blocks_per_seq, float scale,
+                    void* workspace, size_t workspace_bytes, void* stream);
+size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length);
+int akv_packed_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
+                           const uint8_t* k_packed, int64_t kps_blk, int64_t kps_pos, int64_t kps_head,
+                           const float* k_norms, int64_t kns_blk, int64_t kns_pos, int64_t kns_head,
+                           const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
+                           const void* query_starts, int qs_itype, const void* rot_prep, const float* centroids, int bits,
+                           float* weights, int64_t ws_seq, int64_t ws_head, int64_t length, int accumulate,
+                           int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
+                           int64_t num_blocks, int64_t max_blocks_per_seq, float scale,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int akv_evict_select(const float* weights, int64_t ws_seq, int64_t ws_head, int64_t length,
+                     const void* context_lens, int cl_itype, int num_seqs, int num_kv_heads, int keep, int num_sink, int num_recent,
+                     int32_t* kept, int64_t ks_seq, int64_t ks_head, float* kept_weights, int64_t os_seq, int64_t os_head,
+                     void* kept_lens, void* stream);
+#define AKV_EVICT_CACHES 8
+typedef struct {
+  void* data;                              /* device memory */
+  int64_t s_blk, s_pos, s_head, row_bytes; /* bytes */
+} akv_evict_cache;
+int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_head, const void* kept_lens, int kl_itype, int keep,
+                   const void* block_tables, int bt_itype, int64_t bt_stride, int64_t max_blocks_per_seq,
+                   const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq,
+                   const akv_evict_cache* caches, int num_caches,
+                   int num_seqs, int num_kv_heads, int block_size, int64_t num_blocks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
