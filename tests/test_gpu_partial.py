@@ -409,3 +409,33 @@ def test_evict_long(dev):
             ref = kept_reference(w[0, h].numpy(), n, n // 3, 4, 32)
             assert np.array_equal(kept[0, h].cpu().numpy(), ref)
             assert torch.equal(b.rows(cache, 0)[:n // 3, h], before[torch.from_numpy(ref).to(dev), h])
+
+
+@pytest.mark.parametrize("kind", ["alike", "two values", "outlier", "near", "rising"])
+def test_select_scores_of_all_kinds(dev, kind):
+    """Scores that fall into one part of the histogram, by the hundred or all of them, on tables of every width class."""
+    gen = torch.Generator().manual_seed(len(kind))
+    for context, pad in ((1500, 0), (3000, 2), (7000, 4000), (9000, 20000)):
+        b = Batch([(20, context), (3, context // 2)], 1, dev, seed=14, pad_cols=pad)
+        index = akv.BlockIndex(b.blocks, 2, 64, dev)
+        codes = torch.zeros(b.blocks, 2, 64, dtype=torch.int8)
+        codes[:, :, 0] = 100
+        scales = torch.ones(b.blocks, 2)
+        if kind == "two values":
+            scales[torch.rand(b.blocks, generator=gen) < 0.5] = 0.75
+        elif kind == "outlier":
+            scales = 1 + torch.rand(b.blocks, 2, generator=gen)
+            scales[3], codes[7, :, 0] = 1e30, -100
+            scales[7] = 1e30
+        elif kind == "near":
+            scales = 1 + torch.randint(40, (b.blocks, 2), generator=gen) * 2.0 ** -23
+        elif kind == "rising":
+            scales = 1.02 ** (torch.arange(b.blocks * 2).view(-1, 2) % 3001) * 1e-20
+        index.codes.copy_(codes)
+        index.scales.copy_(scales)
+        query = torch.zeros(b.tokens, 4, 64, dtype=BF, device=dev)
+        query[:, :, 0] = 1.0
+        query[1::2] *= -1
+        for k in (5, 400):
+            got = index.select(query, b.tables, b.ctx, b.starts, 1, k, num_sink_blocks=2, num_recent_blocks=2)
+            assert torch.equal(got.cpu(), selection(b, index, query, 2, k, 2, 2)), (context, k)

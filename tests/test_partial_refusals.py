@@ -248,8 +248,8 @@ def library_update(d=64, dtype=0, kc=P, tables=P, it=0, S=2, kvh=2, block=16, bl
     return status("akv_block_index_update", kc, dtype, 2048, 128, stride, tables, it, 2, P, 0, P, 0, codes, P, S, 5, kvh, d, block, blocks, cols, None)
 
 
-def library_select(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sinks=1, recent=2, ws=P, size=1 << 30, block=16, T=5):
-    return status("akv_block_index_select", q, dtype, 512, 64, P, P, P, 0, 2, P, 0, P, 0, P, 2, T, qh, kvh, d, block, 3, 2, k, sinks, recent, ws, size, None)
+def library_select(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sinks=1, recent=2, ws=P, size=1 << 30, block=16, T=5, cols=2):
+    return status("akv_block_index_select", q, dtype, 512, 64, P, P, P, 0, 2, P, 0, P, 0, P, 2, T, qh, kvh, d, block, 3, cols, k, sinks, recent, ws, size, None)
 
 
 def library_sparse(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sel=P, block=16, scale=0.1, cols=2, out=P, T=5):
@@ -287,7 +287,7 @@ INVALID, UNSUPPORTED, WORKSPACE = _lib.AKV_ERR_INVALID, _lib.AKV_ERR_UNSUPPORTED
     (library_select, INVALID, dict(dtype=7)), (library_select, INVALID, dict(q=None)), (library_select, INVALID, dict(qh=7)), (library_select, INVALID, dict(k=2)),
     (library_select, INVALID, dict(sinks=-1)), (library_select, INVALID, dict(recent=0)), (library_select, INVALID, dict(block=0)), (library_select, INVALID, dict(T=-1)),
     (library_select, UNSUPPORTED, dict(d=96)), (library_select, UNSUPPORTED, dict(dtype=2)), (library_select, UNSUPPORTED, dict(q=P + 4)),
-    (library_select, WORKSPACE, dict(ws=None)), (library_select, WORKSPACE, dict(size=8)), (library_select, WORKSPACE, dict(ws=P + 16)), (library_select, 0, dict(T=0)),
+    (library_select, WORKSPACE, dict(ws=None, cols=40000)), (library_select, WORKSPACE, dict(size=8, cols=40000)), (library_select, WORKSPACE, dict(ws=P + 16, cols=40000)), (library_select, 0, dict(T=0)),
     (library_sparse, INVALID, dict(dtype=7)), (library_sparse, INVALID, dict(q=None)), (library_sparse, INVALID, dict(out=None)), (library_sparse, INVALID, dict(sel=None)),
     (library_sparse, INVALID, dict(k=-1)), (library_sparse, INVALID, dict(qh=7)), (library_sparse, INVALID, dict(scale=0.0)), (library_sparse, INVALID, dict(scale=float("inf"))),
     (library_sparse, INVALID, dict(scale=float("nan"))), (library_sparse, UNSUPPORTED, dict(d=96)), (library_sparse, UNSUPPORTED, dict(dtype=2)),
@@ -316,6 +316,6 @@ def test_workspace_sizes():
     assert L.akv_block_index_select_workspace_bytes(0, 8, 100) == 0 and L.akv_block_index_select_workspace_bytes(4, 8, 0) == 0
     assert L.akv_key_weights_workspace_bytes(0, 8, 64, 100) == 0 and L.akv_key_weights_workspace_bytes(4, 8, 96, 100) == 0
     # scratch of long calls is held to slabs
-    assert L.akv_block_index_select_workspace_bytes(1 << 20, 8, 8192) <= 1 << 28
+    assert 0 < L.akv_block_index_select_workspace_bytes(1 << 20, 8, 40000) <= 1 << 28 and L.akv_block_index_select_workspace_bytes(1 << 20, 8, 8192) == 0
     assert L.akv_key_weights_workspace_bytes(1 << 20, 32, 128, 1 << 17) <= 1 << 29
     assert L.akv_packed_key_weights_workspace_bytes(1 << 20, 32, 128, 1 << 17) <= 1 << 29
