@@ -30,10 +30,20 @@ __device__ __forceinline__ int ab_ctx(const ab_batch& b, int i) {
   const int64_t cap = b.max_blocks * b.block_size;
   return ab_clamp(akv_load_index(b.lens, b.lens_it, i), cap < AB_MOST_TOKENS ? cap : AB_MOST_TOKENS);
 }
-// cache block of table column `col` (below max_blocks) of sequence `seq`
-__device__ __forceinline__ int64_t ab_block(const ab_batch& b, int seq, int64_t col) {
-  return akv_clamp_block(akv_load_index(b.tables, b.tables_it, (int64_t)seq * b.bt_stride + col), b.num_blocks);
+// A table entry as it is requested (both words of a 64-bit one), and the cache block from it.  (Taken apart, and without a branch, so that
+// several are on their way together.)
+struct ab_entry { uint32_t lo, hi; };
+__device__ __forceinline__ ab_entry ab_look(const ab_batch& b, int seq, int64_t col) {
+  const int wide = b.tables_it == AKV_I64;
+  const uint32_t* p = (const uint32_t*)b.tables + (((int64_t)seq * b.bt_stride + col) << wide);
+  return {p[0], p[wide]};
 }
+__device__ __forceinline__ int64_t ab_block(const ab_batch& b, ab_entry e) {
+  const int64_t id = b.tables_it == AKV_I64 ? (int64_t)((uint64_t)e.hi << 32 | e.lo) : (int64_t)(int32_t)e.lo;
+  return akv_clamp_block(id, b.num_blocks);
+}
+// cache block of table column `col` (below max_blocks) of sequence `seq`
+__device__ __forceinline__ int64_t ab_block(const ab_batch& b, int seq, int64_t col) { return ab_block(b, ab_look(b, seq, col)); }
 // the last i in [0, S) with number(i) <= x, for numbers that do not decrease; the same in all lanes (-1: none)
 template <class Number> __device__ __forceinline__ int ab_last(int S, int64_t x, Number number) {
   const int lane = threadIdx.x & 63;

@@ -141,11 +141,26 @@ __device__ __forceinline__ bool bi_token(const ab_batch& b, int token, int& seq,
 template <int D, int DT> __device__ __forceinline__ void bi_quantize(const bi_rank_args& a, int token, int head, int8_t (&c)[D / 64]) {
   constexpr int N = D / 64;
   const int lane = threadIdx.x & 63;
+  typedef uint16_t raw __attribute__((ext_vector_type(N < 2 ? 2 : N)));
   const uint16_t* q = (const uint16_t*)a.q + (int64_t)token * a.qs_tok + (int64_t)head * a.G * a.qs_head + N * lane;
   double sum[N] = {};
-  for (int g = 0; g < a.G; ++g)
+  for (int g0 = 0; g0 < a.G; g0 += 4) {          // four heads are requested together
+    uint16_t v[4][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] += (double)ab_math<DT>::low(q[(int64_t)g * a.qs_head + i]);
+    for (int g = 0; g < 4; ++g) {
+      const uint16_t* p = q + (int64_t)min(g0 + g, a.G - 1) * a.qs_head;
+      if constexpr (N == 1) v[g][0] = *p;
+      else {
+        const raw r = *(const raw*)p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[g][i] = r[i];
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] += g0 + g < a.G ? (double)ab_math<DT>::low(v[g][i]) : 0.0;
+  }
   float x[N], top = 0.f;
   bool fine = true;
 #pragma unroll
@@ -253,27 +268,35 @@ __global__ __launch_bounds__(256) void bi_select_kernel(bi_rank_args a) {
 
 // Sixteen tokens of a sequence and a kv head by one workgroup, scores and all: nothing goes to memory but the lists.
 //
-// A lane holds the scores of its token (lane % 16) and four columns of every sixteen, in registers as long as W x HELD tiles do, otherwise made
-// anew for each of the passes.  The k-th largest score is found by a histogram over equal parts of the range of a row's scores (a
-// part's number does not fall as the score rises, so whatever is rounded on the way the parts are in order), then among the scores of the one part in
-// which the count passes k; where these are more than a wavefront can sort out (scores that are alike), by halving the range of all scores bit
-// by bit.  Columns above it, and those that equal it, are marked in two bitmaps a token, from which the lists are written in order.
+// A lane holds the scores of one column of every sixteen and four of the tokens, in registers where tables have no more than W x HELD tiles;
+// HELD = 0: made anew for each of the passes.  The k-th largest score of a token is found by a histogram over equal parts of the range of its scores (a part's
+// number does not fall as the score rises, so whatever is rounded on the way the parts are in order), then among the scores of the one part in
+// which the count passes k; where these are more than fit (scores that are alike), by halving the range of all scores bit by
+// bit.  Columns above it, and those that equal it, are marked in two bitmaps a token, from which the lists are written in order.
+//
+// The vector unit bounds it: a wavefront's instruction takes four clocks, and with the scores of a lane for one token and four columns, their
+// scales from other lanes, a hundred of them a score cost 98 us for 2048 tokens over 1920 blocks.
 #define BI_PARTS 256
-#define BI_CANDIDATES 128
+#define BI_CANDIDATES 64
 struct bi_row {                         // of a token
-  float lo, scale;                      // of the histogram: part = (score - lo) scale
+  float scale, shift;                   // of the histogram: part = score x scale + shift
+  int part, taken, candidates, tied;    // the part in which the count passes k, how many of it are taken; scores in it; taken ones of those marked as equal
+  uint32_t order;                       // of the threshold, as far as it is known, where the count goes bit by bit
   float threshold;
-  int part, equal, candidates, found;       // the part in which the count passes k, how many of it are taken; how many scores at the threshold
 };
 template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) void bi_pick_kernel(bi_rank_args a) {
-  constexpr int KS = D / 64, ROW = D + 16, T = 64 * W, BATCH = 2;
+  constexpr int KS = D / 64, ROW = D + 16, T = 64 * W, HIST = BI_PARTS + 1;
+  constexpr int LANES = D / 16, AT_ONCE = 64 / LANES, LOADS = 16 / AT_ONCE;      // of a tile's codes: lanes a row, rows a load, loads
+  constexpr int BATCH = 4, STAGED = D == 256 ? 1 : 2;                            // tiles looked up together; tiles in LDS together
+  static_assert(HELD % 2 == 0 && W == 16, "whole batches; a wavefront a token");
   __shared__ __align__(16) int8_t qc[16 * ROW];
-  __shared__ int hist[16 * (BI_PARTS + 1)];
-  __shared__ float cand[16 * BI_CANDIDATES];
+  __shared__ int hist[16 * HIST];
+  __shared__ float2 cand[16 * BI_CANDIDATES];      // score, column
   __shared__ float range[2][W][16];
   __shared__ bi_row rows[16];
   __shared__ int again;
-  extern __shared__ uint32_t marks[];   // [16][words][2]: above, equal
+  __shared__ __align__(16) uint8_t stage[W][STAGED * 16 * D];
+  extern __shared__ uint16_t marks[];   // [16][2 words][2]: columns above, and those at, the threshold
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), head = blockIdx.x % a.KVH, col = lane & 15, hq = lane >> 4;
   const int64_t x = blockIdx.x / a.KVH;
   const int bs = a.b.block_size;
@@ -288,151 +311,166 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
   const int64_t first64 = s0 + 16 * (x - (s0 / 16 + (int64_t)seq));
   if (first64 >= s1) return;
   const int first = (int)first64, tokens = min(16, s1 - first);
-  const int pos0 = seq < a.b.S ? ab_ctx(a.b, seq) - (s1 - first) : -tokens, last = pos0 + tokens - 1;
-  const int columns = last < 0 ? 0 : last / bs + 1;       // up to the last token's own
-  auto columns_of = [&](int t) { return pos0 + t < 0 ? 0 : (pos0 + t) / bs + 1; };
-  // lists that take all there is
-  const bool all = columns <= a.k;
-  for (int t = wave; t < tokens; t += W) {
-    const int n = columns_of(t);
-    if (n > a.k) continue;
-    int32_t* out = a.out + ((int64_t)(first + t) * a.KVH + head) * a.k;
-    for (int i = lane; i < a.k; i += 64) out[i] = i < n ? i : -1;
-  }
-  if (all) return;
+  const int pos0 = seq < a.b.S ? ab_ctx(a.b, seq) - (s1 - first) : -tokens;
+  auto columns_of = [&](int t) { return t >= tokens || pos0 + t < 0 ? 0 : (pos0 + t) / bs + 1; };
+  const int columns = columns_of(tokens - 1), need = a.k - a.sinks - a.recent;      // up to the last token's own; those that are chosen
 
-  for (int t = wave; t < 16; t += W) {
+  // ---- a wavefront a token: lists that take all there is, queries in 8 bits
+  const int n = __builtin_amdgcn_readfirstlane(columns_of(wave));
+  int32_t* const out = a.out + ((int64_t)(first + wave) * a.KVH + head) * a.k;
+  const bool listed = wave < tokens && n > a.k;
+  if (wave < tokens && n <= a.k)
+    for (int i = lane; i < a.k; i += 64) out[i] = i < n ? i : -1;
+  if (columns <= a.k) return;
+  if (wave < 16) {
     int8_t c[KS] = {};
-    if (t < tokens) bi_quantize<D, DT>(a, first + t, head, c);
+    if (listed) bi_quantize<D, DT>(a, first + wave, head, c);
 #pragma unroll
-    for (int i = 0; i < KS; ++i) qc[t * ROW + KS * lane + i] = c[i];
+    for (int i = 0; i < KS; ++i) qc[wave * ROW + KS * lane + i] = c[i];
   }
-  const int words = (columns + 31) / 32;
-  for (int i = tid; i < 16 * (BI_PARTS + 1); i += T) hist[i] = 0;
-  for (int i = tid; i < tokens * words * 2; i += T) marks[i] = 0u;
+  for (int i = tid; i < 16 * HIST; i += T) hist[i] = 0;
   if (tid == 0) again = 0;
   __syncthreads();
+
+  // ---- scores
   ab_i4 q[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) q[ks] = *(const ab_i4*)(qc + col * ROW + 64 * ks + 16 * hq);
-  // columns of the lane's token: from .. to - 1 are free to be chosen, the others of its n are listed anyway
-  const int n = col < tokens ? columns_of(col) : 0;
-  const int from = a.sinks, to = n > a.k ? n - a.recent : 0, need = a.k - a.sinks - a.recent;
-  // scores of BATCH tiles of the wavefront, which takes tiles wave, wave + W, ...; -infinity where a column is not free
-  const int tiles = (columns + 15) / 16;
-  auto scores = [&](int tile0, ab_f4 (&s)[BATCH]) {
-    int64_t at[BATCH];
+  const int tiles = (columns + 15) / 16, half_words = 2 * ((columns + 31) / 32);
+  // columns sinks .. to - 1 of a token are free to be chosen; whole tiles that are free for every token need no mask
+  int shortest = 0;                     // of the tokens that choose, the first
+  while (columns_of(shortest) <= a.k) ++shortest;
+  const int free_tiles = (columns_of(shortest) - a.recent) / 16;
+  float lo[4], hi[4];
+  int free_to[4];                       // of the lane's tokens; 0: one that does not choose
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) at[i] = ab_block(a.b, seq, min(16 * (tile0 + W * i) + col, columns - 1)) * a.KVH + head;
-    ab_i4 c[BATCH][KS];
-    float scale[BATCH];
+  for (int e = 0; e < 4; ++e) {
+    lo[e] = INFINITY, hi[e] = -INFINITY;
+    const int m = columns_of(4 * hq + e);
+    free_to[e] = m > a.k ? m - a.recent : 0;
+  }
+  // Codes go from memory to LDS row by row, sixteen bytes a lane side by side, and from there to the operand: memory serves four lanes a
+  // clock where they read one line, and in the operand's order, a row a lane, one (120 tiles 25000 clocks).
+  const int8_t* const codes = a.codes + (int64_t)head * D + 16 * (lane % LANES);
+  uint8_t* const st = stage[wave];
+  const int my_row = lane / LANES;
+  // entries of the tiles tile0, tile0 + W, ... + (BATCH - 1) W: of tile lane / 16, column lane % 16
+  auto look = [&](int tile0) { return ab_look(a.b, seq, min(16 * (tile0 + W * hq) + col, columns - 1)); };
+  auto scores = [&](int tile0, ab_entry entry, ab_f4 (&s)[BATCH]) {
+    const int blk = (int)ab_block(a.b, entry);
+    const float scale = a.scales[(int64_t)blk * a.KVH + head];
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
+    for (int i0 = 0; i0 < BATCH; i0 += STAGED) {
+      ab_u4 v[STAGED][LOADS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) c[i][ks] = *(const ab_i4*)(a.codes + at[i] * D + 64 * ks + 16 * hq);
-      scale[i] = a.scales[at[i]];
-    }
+      for (int i = 0; i < STAGED; ++i)
 #pragma unroll
-    for (int i = 0; i < BATCH; ++i) {
-      ab_i4 acc = {0, 0, 0, 0};
+        for (int j = 0; j < LOADS; ++j) {
+          const int from = __shfl(blk, 16 * (i0 + i) + AT_ONCE * j + my_row, 64);
+          v[i][j] = *(const ab_u4*)(codes + (int64_t)from * a.KVH * D);
+        }
+      akv_wave_sync();                  // (what was there has been read)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(c[i][ks], q[ks], acc, 0, 0, 0);
+      for (int i = 0; i < STAGED; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int cc = 16 * (tile0 + W * i) + 4 * hq + e;
-        const float v = akv_mul_rn((float)acc[e], __shfl(scale[i], 4 * hq + e, 64));
-        s[i][e] = cc >= from && cc < to ? v : -INFINITY;
+        for (int j = 0; j < LOADS; ++j) {
+          const int r = AT_ONCE * j + my_row;
+          *(ab_u4*)(st + (16 * i + r) * D + 16 * ((lane % LANES) ^ (r & (LANES < 8 ? LANES - 1 : 7)))) = v[i][j];
+        }
+      akv_wave_sync();
+#pragma unroll
+      for (int i = 0; i < STAGED; ++i) {
+        const int tile = tile0 + W * (i0 + i);
+        ab_i4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[ks], *(const ab_i4*)(st + (16 * i + col) * D + 16 * ((4 * ks + hq) ^ (col & (LANES < 8 ? LANES - 1 : 7)))), acc, 0, 0, 0);
+        const float f = __shfl(scale, 16 * (i0 + i) + col, 64);
+        ab_f4& x = s[i0 + i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = akv_mul_rn((float)acc[e], f);
+        if (16 * tile < a.sinks || tile >= free_tiles) {
+          const int cc = 16 * tile + col;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool free = cc >= a.sinks && cc < free_to[e];
+            lo[e] = fminf(lo[e], free ? x[e] : INFINITY);
+            x[e] = free ? x[e] : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) lo[e] = fminf(lo[e], x[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hi[e] = fmaxf(hi[e], x[e]);
       }
     }
   };
-  const bool fits = tiles <= W * HELD;
-  ab_f4 held[HELD];
-  if (fits) {
+  constexpr bool fits = HELD > 0;       // (the tables' width says so)
+  ab_f4 held[HELD > 0 ? HELD : 1];
+  if constexpr (fits) {
+    constexpr int BATCHES = (HELD + BATCH - 1) / BATCH;
+    ab_entry entry[BATCHES];            // all requested before the first is needed
 #pragma unroll
-    for (int i = 0; i < HELD; i += BATCH) {
+    for (int i = 0; i < BATCHES; ++i) entry[i] = look(wave + W * BATCH * i);
+#pragma unroll
+    for (int i = 0; i < BATCHES; ++i) {
       ab_f4 s[BATCH];
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) s[j] = (ab_f4)(-INFINITY);
-      if (wave + W * i < tiles) scores(wave + W * i, s);
-      __builtin_amdgcn_sched_barrier(0);
+      if (wave + W * BATCH * i < tiles) scores(wave + W * BATCH * i, entry[i], s);
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) held[i + j] = s[j];
+      for (int j = 0; j < BATCH && BATCH * i + j < HELD; ++j) held[BATCH * i + j] = s[j];
     }
   }
+
   // ---- passes over the scores.  (One loop with the pass as a variable: there is one copy of the code that makes scores anew.)
   enum { RANGE, PARTS, CANDIDATES, BITS, MARKS };
-  float lo = INFINITY, hi = -INFINITY, my_lo = 0.f, my_scale = 0.f, threshold = INFINITY;
-  int part = 0, count = 0, bit = 31, more = 0;
-  int cq = 4 * hq;
-  uint32_t order = 0u;                  // BITS: the threshold's, as far as it is known
-  auto part_of = [&](float s) { return min(BI_PARTS - 1, (int)((s - my_lo) * my_scale)); };
+  float scale[4], shift[4];
+  int part[4], bit = 31;
+  auto part_of = [&](float s, int e) { return min((uint32_t)(BI_PARTS - 1), (uint32_t)max(0.f, fmaf(s, scale[e], shift[e]))); };
+  int row0 = 4 * hq, my_col = col;      // the lane's first token, its column of a tile
+  // sixteen columns of token 4 hq + e: a lane of the token writes their marks
+  auto mark = [&](int tile, int e, uint64_t lanes, int which) {
+    if (my_col == 0) marks[(2 * (row0 + e) + which) * half_words + tile] = (uint16_t)(lanes >> (16 * hq));
+  };
   auto take = [&](int pass, int tile, const ab_f4& s) {
-    if (pass == RANGE) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        lo = fminf(lo, s[e] == -INFINITY ? INFINITY : s[e]);
-        hi = fmaxf(hi, s[e]);
-      }
-    } else if (pass == PARTS) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s[e] != -INFINITY) atomicAdd(hist + col * (BI_PARTS + 1) + part_of(s[e]), 1);
-    } else if (pass == CANDIDATES) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (s[e] != -INFINITY && part_of(s[e]) == part) {
-          const int at = atomicAdd(&rows[col].candidates, 1);
-          if (at < BI_CANDIDATES) cand[col * BI_CANDIDATES + at] = s[e];
+    for (int e = 0; e < 4; ++e) {
+      if (pass == PARTS) {
+        // (what is not free counts in the lowest part, above which no count starts)
+        if (free_to[e] > 0) atomicAdd(hist + (row0 + e) * HIST + part_of(s[e], e), 1);
+      } else if (pass == CANDIDATES) {
+        const int p = (int)part_of(s[e], e);
+        mark(tile, e, __ballot(p > part[e]), 0);
+        if (p == part[e] && s[e] != -INFINITY) {
+          const int at = atomicAdd(&rows[row0 + e].candidates, 1);
+          if (at < BI_CANDIDATES) cand[(row0 + e) * BI_CANDIDATES + at] = make_float2(s[e], __int_as_float(16 * tile + my_col));
         }
-    } else if (pass == BITS) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) count += s[e] != -INFINITY && bi_order(s[e]) >= (order | 1u << bit);
-    } else {
-      uint32_t above = 0u, equal = 0u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = 16 * tile + cq + e;
-        above |= (uint32_t)(s[e] > threshold || (c < n && (c < from || c >= to))) << e;
-        equal |= (uint32_t)(s[e] == threshold) << e;
+      } else if (pass == BITS) {
+        if (s[e] != -INFINITY && bi_order(s[e]) >= (rows[row0 + e].order | 1u << bit)) atomicAdd(hist + row0 + e, 1);
+      } else if (pass == MARKS) {
+        const float threshold = rows[row0 + e].threshold;
+        const uint64_t above = __ballot(s[e] > threshold), equal = __ballot(s[e] == threshold);
+        if (rows[row0 + e].candidates > BI_CANDIDATES) {
+          mark(tile, e, above, 0);
+          mark(tile, e, equal, 1);
+        }
       }
-      const int shift = 16 * (tile & 1) + cq;
-      uint32_t* m = marks + (col * words + (tile >> 1)) * 2;
-      if (above) atomicOr(m, above << shift);
-      if (equal) atomicOr(m + 1, equal << shift);
     }
   };
-  int pass = need > 0 ? RANGE : MARKS;
+  int pass = fits ? PARTS : RANGE;      // (the range of scores that are held is known)
 #pragma unroll 1
   for (;;) {
-    // (what a pass makes of a score is not made before the loop and kept: registers hold the scores)
-    asm volatile("" : "+v"(cq));
+    if (pass == PARTS) {
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) asm volatile("" : "+v"(held[i]));
-    if (fits) {
-#define BI_PASS(P)                              \
-  case P:                                       \
-    _Pragma("unroll") for (int i = 0; i < HELD; ++i) \
-        if (wave + W * i < tiles) take(P, wave + W * i, held[i]); \
-    break;
-      switch (pass) { BI_PASS(RANGE) BI_PASS(PARTS) BI_PASS(CANDIDATES) BI_PASS(BITS) BI_PASS(MARKS) }
-#undef BI_PASS
-    } else {
-#pragma unroll 1
-      for (int tile = wave; tile < tiles; tile += W * BATCH) {
-        ab_f4 s[BATCH];
-        scores(tile, s);
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-          if (tile + W * i < tiles) take(pass, tile + W * i, s[i]);
-      }
-    }
-    if (pass == MARKS) break;
-    if (pass == RANGE) {
-      lo = -akv_rows_max(-lo);
-      hi = akv_rows_max(hi);
-      if (hq == 0) {
-        range[0][wave][col] = lo;
-        range[1][wave][col] = hi;
+      for (int e = 0; e < 4; ++e) {
+        float l = lo[e], h = hi[e];
+        l = fminf(l, akv_lane_xor<1>(l)); l = fminf(l, akv_lane_xor<2>(l)); l = fminf(l, akv_lane_xor<4>(l)); l = fminf(l, akv_lane_xor<8>(l));
+        h = fmaxf(h, akv_lane_xor<1>(h)); h = fmaxf(h, akv_lane_xor<2>(h)); h = fmaxf(h, akv_lane_xor<4>(h)); h = fmaxf(h, akv_lane_xor<8>(h));
+        if (col == 0) {
+          range[0][wave][4 * hq + e] = l;
+          range[1][wave][4 * hq + e] = h;
+        }
       }
       __syncthreads();
       if (tid < 16) {
@@ -441,20 +479,50 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
           l = fminf(l, range[0][w][tid]);
           h = fmaxf(h, range[1][w][tid]);
         }
-        const float scale = BI_PARTS / (h - l);
-        rows[tid].lo = l;
-        rows[tid].scale = scale < INFINITY ? scale : 0.f;      // (scores that are all alike, or nearly: one part; and none where h < l)
-        rows[tid].candidates = 0;
+        const float f = BI_PARTS / (h - l);
+        const bool fine = f < INFINITY && fabsf(l * f) < INFINITY;      // (scores that are all alike, or nearly: one part; and none where h < l)
+        rows[tid].scale = fine ? f : 0.f;
+        rows[tid].shift = fine ? -l * f : 0.f;
+        rows[tid].candidates = rows[tid].tied = 0;
+        rows[tid].part = BI_PARTS;
       }
       __syncthreads();
-      my_lo = rows[col].lo;
-      my_scale = rows[col].scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        scale[e] = rows[4 * hq + e].scale;
+        shift[e] = rows[4 * hq + e].shift;
+      }
+    }
+    // (what a pass makes of a score is not made before the loop and kept: registers hold the scores)
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) asm volatile("" : "+v"(held[i]));
+    asm volatile("" : "+v"(row0), "+v"(my_col));
+    if constexpr (fits) {
+#define BI_PASS(P)                                   \
+  case P:                                            \
+    _Pragma("unroll") for (int i = 0; i < HELD; ++i) \
+        if (wave + W * i < tiles) take(P, wave + W * i, held[i]); \
+    break;
+      switch (pass) { BI_PASS(PARTS) BI_PASS(CANDIDATES) BI_PASS(BITS) BI_PASS(MARKS) }
+#undef BI_PASS
+    } else {
+#pragma unroll 1
+      for (int tile = wave; tile < tiles; tile += W * BATCH) {
+        ab_f4 s[BATCH];
+        scores(tile, look(tile), s);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+          if (tile + W * i < tiles) take(pass, tile + W * i, s[i]);
+      }
+    }
+    __syncthreads();
+    if (pass == MARKS) break;
+    if (pass == RANGE) {
       pass = PARTS;
     } else if (pass == PARTS) {
-      __syncthreads();
-      for (int t = wave; t < tokens; t += W) {
+      if (listed && need > 0) {
         // a lane four parts, the first lane the uppermost
-        const int* h = hist + t * (BI_PARTS + 1) + BI_PARTS - 4 - 4 * lane;
+        const int* h = hist + wave * HIST + BI_PARTS - 4 - 4 * lane;
         const int c[4] = {h[3], h[2], h[1], h[0]}, sum = c[0] + c[1] + c[2] + c[3], inc = akv_wave_inclusive_scan(sum);
         int before = inc - sum;
         if (before < need && need <= inc) {
@@ -462,101 +530,102 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
 #pragma unroll
           for (int j = 0; j < 3; ++j)
             if (i == j && before + c[j] < need) before += c[j], ++i;
-          rows[t].part = BI_PARTS - 1 - 4 * lane - i;
-          rows[t].equal = need - before;          // of that part
+          rows[wave].part = BI_PARTS - 1 - 4 * lane - i;
+          rows[wave].taken = need - before;
         }
       }
       __syncthreads();
-      part = rows[col].part;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] = rows[4 * hq + e].part;
       pass = CANDIDATES;
     } else if (pass == CANDIDATES) {
-      __syncthreads();
-      for (int t = wave; t < tokens; t += W) {
-        const int have = rows[t].candidates, want = rows[t].equal;
-        if (columns_of(t) <= a.k) continue;
+      if (listed && need > 0) {
+        const int have = rows[wave].candidates, want = rows[wave].taken;
         if (have > BI_CANDIDATES) {
           if (lane == 0) again = 1;
-          continue;
-        }
-        const float* c = cand + t * BI_CANDIDATES;
-        for (int i0 = 0; i0 < have; i0 += 64) {
-          const float mine = c[min(i0 + lane, have - 1)];
-          int above = 0, same = 0;
-          for (int i = 0; i < have; ++i) {
-            above += c[i] > mine;
-            same += c[i] == mine;
-          }
-          if (above < want && want <= above + same) {       // (lanes of one value write the same)
-            rows[t].threshold = mine;
-            rows[t].found = want - above;
+        } else {
+          // rank among them, of equal ones the lower column first
+          const float2* c = cand + wave * BI_CANDIDATES;
+          for (int i0 = 0; i0 < have; i0 += 64) {
+            const float2 mine = c[min(i0 + lane, have - 1)];
+            const int mine_col = __float_as_int(mine.y);
+            int above = 0;
+            for (int i = 0; i < have; ++i) above += c[i].x > mine.x || (c[i].x == mine.x && __float_as_int(c[i].y) < mine_col);
+            if (above < want && i0 + lane < have) atomicOr((uint32_t*)marks + wave * half_words + (mine_col >> 5), 1u << (mine_col & 31));
           }
         }
       }
       __syncthreads();
-      pass = again ? BITS : MARKS;
+      if (!again) break;
+      if (tid < 16) {
+        rows[tid].order = 0u;
+        hist[tid] = 0;
+      }
+      __syncthreads();
+      pass = BITS;
     } else {
-      count += akv_lane_xor<16>(count);
-      count += akv_lane_xor<32>(count);
-      int* sums = hist + (bit & 1) * W * 16;
-      __syncthreads();
-      if (hq == 0) sums[wave * 16 + col] = count;
-      __syncthreads();
-      int total = 0;
-      for (int w = 0; w < W; ++w) total += sums[w * 16 + col];
-      if (total >= need) order |= 1u << bit;
-      else more = total;                // above the threshold, in the end
-      count = 0;
-      if (--bit < 0) {
-        if (n > a.k && rows[col].candidates > BI_CANDIDATES && wave == 0 && hq == 0) {
-          rows[col].threshold = __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xffffffffu));
-          rows[col].found = need - more;
-        }
-        __syncthreads();
-        pass = MARKS;
+      // (the counts of all tokens; those that have their marks let them pass)
+      if (tid < 16) {
+        bi_row& r = rows[tid];
+        const int c = hist[tid];
+        if (c >= need) r.order |= 1u << bit;
+        else r.tied = need - c;         // not above the threshold, in the end
+        if (bit == 0) r.threshold = __uint_as_float(r.order ^ ((r.order >> 31) ? 0x80000000u : 0xffffffffu));
+        if (bit == 0 && r.candidates <= BI_CANDIDATES) r.tied = 0;
+        hist[tid] = 0;
       }
+      __syncthreads();
+      if (--bit < 0) pass = MARKS;
     }
-    if (pass == MARKS && n > a.k) threshold = rows[col].threshold;
   }
-  __syncthreads();
-  for (int t = wave; t < tokens; t += W) {
-    if (columns_of(t) <= a.k) continue;
-    int32_t* out = a.out + ((int64_t)(first + t) * a.KVH + head) * a.k;
-    int tied = need > 0 ? rows[t].found : 0, at = 0;
-    for (int w0 = 0; w0 < words; w0 += 64) {
-      const int w = w0 + lane;
-      uint32_t take = w < words ? marks[(t * words + w) * 2] : 0u, same = w < words ? marks[(t * words + w) * 2 + 1] : 0u;
-      const int s = __popc(same), s_inc = akv_wave_inclusive_scan(s);
-      for (int left = min(s, tied - (s_inc - s)); left > 0; --left) {
+  // ---- lists: what is listed anyway, what is marked, and the first of those that equal the threshold
+  if (!listed) return;
+  const uint32_t* above = (const uint32_t*)marks + wave * half_words;      // (half_words words a token: two bitmaps)
+  const uint32_t* equal = above + half_words / 2;
+  int tied = rows[wave].tied, at = 0;
+  for (int w0 = 0; 32 * w0 < n; w0 += 64) {
+    const int w = w0 + lane, c0 = 32 * w;
+    // bits below column c of the word
+    auto below = [&](int c) { return c <= c0 ? 0u : c - c0 >= 32 ? ~0u : (1u << (c - c0)) - 1; };
+    const uint32_t free = below(n - a.recent) & ~below(a.sinks);
+    uint32_t take = below(n) & ~free, same = 0u;
+    if (need > 0 && free) {
+      take |= above[w] & free;
+      if (tied > 0) same = equal[w] & free;
+    }
+    if (tied > 0) {
+      const int s = __popc(same), inc = akv_wave_inclusive_scan(s);
+      for (int left = min(s, tied - (inc - s)); left > 0; --left) {
         take |= same & -same;
         same &= same - 1;
       }
-      const int c = __popc(take), c_inc = akv_wave_inclusive_scan(c);
-      int to_at = at + c_inc - c;
-      for (; take; take &= take - 1) out[to_at++] = 32 * w + __ffs(take) - 1;
-      tied -= __builtin_amdgcn_readlane(s_inc, 63);
-      at += __builtin_amdgcn_readlane(c_inc, 63);
+      tied -= __builtin_amdgcn_readlane(inc, 63);
     }
+    const int c = __popc(take), inc = akv_wave_inclusive_scan(c);
+    int to = at + inc - c;
+    for (; take; take &= take - 1) out[to++] = c0 + __ffs(take) - 1;
+    at += __builtin_amdgcn_readlane(inc, 63);
   }
 }
 
 // Wider tables go the long way over scores in memory.
 #define BI_WIDE 16384
-template <int D, int DT> static int bi_pick(const bi_rank_args& a, int64_t max_blocks, hipStream_t stream) {
-  const int64_t units = ((int64_t)a.b.T / 16 + a.b.S + 1) * a.KVH;
-  const int bytes = (int)(16 * ((max_blocks + 31) / 32) * 8);
-  if (units > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "akv_block_index_select: more than 2^31 rows");
+template <int D, int DT, int HELD> static int bi_pick(const bi_rank_args& a, int64_t units, int bytes, hipStream_t stream) {
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
   static akv_device_once once;
-  if (const int rc = once(dev, [&]() -> int {
-        const int rc8 = ab_lds((const void*)bi_pick_kernel<D, DT, 16, 8>, 16 * BI_WIDE / 4);
-        return rc8 ? rc8 : ab_lds((const void*)bi_pick_kernel<D, DT, 16, 14>, 16 * BI_WIDE / 4);
-      }))
-    return rc;
-  if (max_blocks <= 16 * 16 * 8) bi_pick_kernel<D, DT, 16, 8><<<(uint32_t)units, 1024, bytes, stream>>>(a);
-  else bi_pick_kernel<D, DT, 16, 14><<<(uint32_t)units, 1024, bytes, stream>>>(a);
+  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)bi_pick_kernel<D, DT, 16, HELD>, 16 * BI_WIDE / 4); })) return rc;
+  bi_pick_kernel<D, DT, 16, HELD><<<(uint32_t)units, 1024, bytes, stream>>>(a);
   AKV_LAUNCH_CHECK("bi_pick_kernel");
   return AKV_OK;
+}
+template <int D, int DT> static int bi_pick(const bi_rank_args& a, int64_t max_blocks, hipStream_t stream) {
+  const int64_t units = ((int64_t)a.b.T / 16 + a.b.S + 1) * a.KVH, tiles = (max_blocks + 15) / 16;
+  const int bytes = (int)(16 * ((max_blocks + 31) / 32) * 8);
+  if (units > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "akv_block_index_select: more than 2^31 rows");
+  if (tiles <= 16 * 8) return bi_pick<D, DT, 8>(a, units, bytes, stream);
+  if (tiles <= 16 * 14) return bi_pick<D, DT, 14>(a, units, bytes, stream);
+  return bi_pick<D, DT, 0>(a, units, bytes, stream);
 }
 
 // scores of so many bytes at most are held at a time
