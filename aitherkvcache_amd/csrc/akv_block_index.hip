@@ -288,7 +288,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
   constexpr int KS = D / 64, ROW = D + 16, T = 64 * W, HIST = BI_PARTS + 1;
   constexpr int LANES = D / 16, AT_ONCE = 64 / LANES, LOADS = 16 / AT_ONCE;      // of a tile's codes: lanes a row, rows a load, loads
   constexpr int BATCH = 4, STAGED = D == 256 ? 1 : 2;                            // tiles looked up together; tiles in LDS together
-  static_assert(HELD % 2 == 0 && W == 16, "whole batches; a wavefront a token");
+  static_assert(HELD % 2 == 0 && (W == 16 || W == 8), "whole batches; a wavefront a token");
   __shared__ __align__(16) int8_t qc[16 * ROW];
   __shared__ int hist[16 * HIST];
   __shared__ float2 cand[16 * BI_CANDIDATES];      // score, column
@@ -315,18 +315,22 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
   auto columns_of = [&](int t) { return t >= tokens || pos0 + t < 0 ? 0 : (pos0 + t) / bs + 1; };
   const int columns = columns_of(tokens - 1), need = a.k - a.sinks - a.recent;      // up to the last token's own; those that are chosen
 
-  // ---- a wavefront a token: lists that take all there is, queries in 8 bits
-  const int n = __builtin_amdgcn_readfirstlane(columns_of(wave));
-  int32_t* const out = a.out + ((int64_t)(first + wave) * a.KVH + head) * a.k;
-  const bool listed = wave < tokens && n > a.k;
-  if (wave < tokens && n <= a.k)
+  // ---- lists that take all there is; queries in 8 bits
+  auto listed = [&](int t) { return columns_of(t) > a.k; };      // (the others' lists are written here)
+  auto list_of = [&](int t) { return a.out + ((int64_t)(first + t) * a.KVH + head) * a.k; };
+  for (int t = wave; t < tokens; t += W) {
+    const int n = columns_of(t);
+    if (n > a.k) continue;
+    int32_t* out = list_of(t);
     for (int i = lane; i < a.k; i += 64) out[i] = i < n ? i : -1;
+  }
   if (columns <= a.k) return;
-  if (wave < 16) {
-    int8_t c[KS] = {};
-    if (listed) bi_quantize<D, DT>(a, first + wave, head, c);
 #pragma unroll
-    for (int i = 0; i < KS; ++i) qc[wave * ROW + KS * lane + i] = c[i];
+  for (int t = wave; t < 16; t += W) {
+    int8_t c[KS] = {};
+    if (listed(t)) bi_quantize<D, DT>(a, first + t, head, c);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qc[t * ROW + KS * lane + i] = c[i];
   }
   for (int i = tid; i < 16 * HIST; i += T) hist[i] = 0;
   if (tid == 0) again = 0;
@@ -356,70 +360,76 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
   const int my_row = lane / LANES;
   // entries of the tiles tile0, tile0 + W, ... + (BATCH - 1) W: of tile lane / 16, column lane % 16
   auto look = [&](int tile0) { return ab_look(a.b, seq, min(16 * (tile0 + W * hq) + col, columns - 1)); };
-  auto scores = [&](int tile0, ab_entry entry, ab_f4 (&s)[BATCH]) {
-    const int blk = (int)ab_block(a.b, entry);
-    const float scale = a.scales[(int64_t)blk * a.KVH + head];
+  struct rows_of_codes { ab_u4 v[STAGED][LOADS]; };
+  auto request = [&](int blk, int i0, rows_of_codes& r) {      // tiles i0 .. i0 + STAGED - 1 of a batch
 #pragma unroll
-    for (int i0 = 0; i0 < BATCH; i0 += STAGED) {
-      ab_u4 v[STAGED][LOADS];
+    for (int i = 0; i < STAGED; ++i)
 #pragma unroll
-      for (int i = 0; i < STAGED; ++i)
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int from = __shfl(blk, 16 * (i0 + i) + AT_ONCE * j + my_row, 64);
-          v[i][j] = *(const ab_u4*)(codes + (int64_t)from * a.KVH * D);
-        }
-      akv_wave_sync();                  // (what was there has been read)
-#pragma unroll
-      for (int i = 0; i < STAGED; ++i)
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int r = AT_ONCE * j + my_row;
-          *(ab_u4*)(st + (16 * i + r) * D + 16 * ((lane % LANES) ^ (r & (LANES < 8 ? LANES - 1 : 7)))) = v[i][j];
-        }
-      akv_wave_sync();
-#pragma unroll
-      for (int i = 0; i < STAGED; ++i) {
-        const int tile = tile0 + W * (i0 + i);
-        ab_i4 acc = {0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[ks], *(const ab_i4*)(st + (16 * i + col) * D + 16 * ((4 * ks + hq) ^ (col & (LANES < 8 ? LANES - 1 : 7)))), acc, 0, 0, 0);
-        const float f = __shfl(scale, 16 * (i0 + i) + col, 64);
-        ab_f4& x = s[i0 + i];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = akv_mul_rn((float)acc[e], f);
-        if (16 * tile < a.sinks || tile >= free_tiles) {
-          const int cc = 16 * tile + col;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool free = cc >= a.sinks && cc < free_to[e];
-            lo[e] = fminf(lo[e], free ? x[e] : INFINITY);
-            x[e] = free ? x[e] : -INFINITY;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) lo[e] = fminf(lo[e], x[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) hi[e] = fmaxf(hi[e], x[e]);
+      for (int j = 0; j < LOADS; ++j) {
+        const int from = __shfl(blk, 16 * (i0 + i) + AT_ONCE * j + my_row, 64);
+        r.v[i][j] = *(const ab_u4*)(codes + (int64_t)from * a.KVH * D);
       }
+  };
+  auto to_stage = [&](const rows_of_codes& c) {
+    akv_wave_sync();                    // (what was there has been read)
+#pragma unroll
+    for (int i = 0; i < STAGED; ++i)
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int r = AT_ONCE * j + my_row;
+        *(ab_u4*)(st + (16 * i + r) * D + 16 * ((lane % LANES) ^ (r & (LANES < 8 ? LANES - 1 : 7)))) = c.v[i][j];
+      }
+    akv_wave_sync();
+  };
+  auto score = [&](int tile, int i0, int i, float scale, ab_f4& x) {
+    ab_i4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[ks], *(const ab_i4*)(st + (16 * i + col) * D + 16 * ((4 * ks + hq) ^ (col & (LANES < 8 ? LANES - 1 : 7)))), acc, 0, 0, 0);
+    const float f = __shfl(scale, 16 * (i0 + i) + col, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = akv_mul_rn((float)acc[e], f);
+    if (16 * tile < a.sinks || tile >= free_tiles) {
+      const int cc = 16 * tile + col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool free = cc >= a.sinks && cc < free_to[e];
+        lo[e] = fminf(lo[e], free ? x[e] : INFINITY);
+        x[e] = free ? x[e] : -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lo[e] = fminf(lo[e], x[e]);
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) hi[e] = fmaxf(hi[e], x[e]);
   };
   constexpr bool fits = HELD > 0;       // (the tables' width says so)
   ab_f4 held[HELD > 0 ? HELD : 1];
   if constexpr (fits) {
     constexpr int BATCHES = (HELD + BATCH - 1) / BATCH;
-    ab_entry entry[BATCHES];            // all requested before the first is needed
+    // entries are all requested before the first is needed, then scales; codes a step ahead
+    ab_entry entry[BATCHES];
+    int blk[BATCHES];
+    float scale[BATCHES];
 #pragma unroll
     for (int i = 0; i < BATCHES; ++i) entry[i] = look(wave + W * BATCH * i);
 #pragma unroll
     for (int i = 0; i < BATCHES; ++i) {
-      ab_f4 s[BATCH];
+      blk[i] = (int)ab_block(a.b, entry[i]);
+      scale[i] = a.scales[(int64_t)blk[i] * a.KVH + head];
+    }
+    rows_of_codes c[2];
+    request(blk[0], 0, c[0]);
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) s[j] = (ab_f4)(-INFINITY);
-      if (wave + W * BATCH * i < tiles) scores(wave + W * BATCH * i, entry[i], s);
+    for (int i = 0; i < HELD; i += STAGED) {
+      held[i] = (ab_f4)(-INFINITY);
+      if (STAGED == 2) held[i + 1] = (ab_f4)(-INFINITY);
+      if (wave + W * i >= tiles) continue;
+      const int next = i + STAGED < HELD ? i + STAGED : i;
+      if (next > i) request(blk[next / BATCH], next % BATCH, c[next / STAGED & 1]);
+      to_stage(c[i / STAGED & 1]);
 #pragma unroll
-      for (int j = 0; j < BATCH && BATCH * i + j < HELD; ++j) held[BATCH * i + j] = s[j];
+      for (int j = 0; j < STAGED; ++j) score(wave + W * (i + j), i % BATCH, j, scale[i / BATCH], held[i + j]);
     }
   }
 
@@ -508,11 +518,21 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
     } else {
 #pragma unroll 1
       for (int tile = wave; tile < tiles; tile += W * BATCH) {
-        ab_f4 s[BATCH];
-        scores(tile, look(tile), s);
+        const int blk = (int)ab_block(a.b, look(tile));
+        const float scale = a.scales[(int64_t)blk * a.KVH + head];
+        rows_of_codes c[2];
+        request(blk, 0, c[0]);
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-          if (tile + W * i < tiles) take(pass, tile + W * i, s[i]);
+        for (int i = 0; i < BATCH; i += STAGED) {
+          if (i + STAGED < BATCH) request(blk, i + STAGED, c[(i / STAGED + 1) & 1]);
+          to_stage(c[i / STAGED & 1]);
+#pragma unroll
+          for (int j = 0; j < STAGED; ++j) {
+            ab_f4 s;
+            score(tile + W * (i + j), i, j, scale, s);
+            if (tile + W * (i + j) < tiles) take(pass, tile + W * (i + j), s);
+          }
+        }
       }
     }
     __syncthreads();
@@ -520,9 +540,10 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
     if (pass == RANGE) {
       pass = PARTS;
     } else if (pass == PARTS) {
-      if (listed && need > 0) {
+      for (int t = wave; t < 16; t += W) {
+        if (!listed(t) || need == 0) continue;
         // a lane four parts, the first lane the uppermost
-        const int* h = hist + wave * HIST + BI_PARTS - 4 - 4 * lane;
+        const int* h = hist + t * HIST + BI_PARTS - 4 - 4 * lane;
         const int c[4] = {h[3], h[2], h[1], h[0]}, sum = c[0] + c[1] + c[2] + c[3], inc = akv_wave_inclusive_scan(sum);
         int before = inc - sum;
         if (before < need && need <= inc) {
@@ -530,8 +551,8 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
 #pragma unroll
           for (int j = 0; j < 3; ++j)
             if (i == j && before + c[j] < need) before += c[j], ++i;
-          rows[wave].part = BI_PARTS - 1 - 4 * lane - i;
-          rows[wave].taken = need - before;
+          rows[t].part = BI_PARTS - 1 - 4 * lane - i;
+          rows[t].taken = need - before;
         }
       }
       __syncthreads();
@@ -539,19 +560,20 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
       for (int e = 0; e < 4; ++e) part[e] = rows[4 * hq + e].part;
       pass = CANDIDATES;
     } else if (pass == CANDIDATES) {
-      if (listed && need > 0) {
-        const int have = rows[wave].candidates, want = rows[wave].taken;
+      for (int t = wave; t < 16; t += W) {
+        if (!listed(t) || need == 0) continue;
+        const int have = rows[t].candidates, want = rows[t].taken;
         if (have > BI_CANDIDATES) {
           if (lane == 0) again = 1;
         } else {
           // rank among them, of equal ones the lower column first
-          const float2* c = cand + wave * BI_CANDIDATES;
+          const float2* c = cand + t * BI_CANDIDATES;
           for (int i0 = 0; i0 < have; i0 += 64) {
             const float2 mine = c[min(i0 + lane, have - 1)];
             const int mine_col = __float_as_int(mine.y);
             int above = 0;
             for (int i = 0; i < have; ++i) above += c[i].x > mine.x || (c[i].x == mine.x && __float_as_int(c[i].y) < mine_col);
-            if (above < want && i0 + lane < have) atomicOr((uint32_t*)marks + wave * half_words + (mine_col >> 5), 1u << (mine_col & 31));
+            if (above < want && i0 + lane < have) atomicOr((uint32_t*)marks + t * half_words + (mine_col >> 5), 1u << (mine_col & 31));
           }
         }
       }
@@ -579,43 +601,47 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
     }
   }
   // ---- lists: what is listed anyway, what is marked, and the first of those that equal the threshold
-  if (!listed) return;
-  const uint32_t* above = (const uint32_t*)marks + wave * half_words;      // (half_words words a token: two bitmaps)
-  const uint32_t* equal = above + half_words / 2;
-  int tied = rows[wave].tied, at = 0;
-  for (int w0 = 0; 32 * w0 < n; w0 += 64) {
-    const int w = w0 + lane, c0 = 32 * w;
-    // bits below column c of the word
-    auto below = [&](int c) { return c <= c0 ? 0u : c - c0 >= 32 ? ~0u : (1u << (c - c0)) - 1; };
-    const uint32_t free = below(n - a.recent) & ~below(a.sinks);
-    uint32_t take = below(n) & ~free, same = 0u;
-    if (need > 0 && free) {
-      take |= above[w] & free;
-      if (tied > 0) same = equal[w] & free;
-    }
-    if (tied > 0) {
-      const int s = __popc(same), inc = akv_wave_inclusive_scan(s);
-      for (int left = min(s, tied - (inc - s)); left > 0; --left) {
-        take |= same & -same;
-        same &= same - 1;
+  for (int t = wave; t < tokens; t += W) {
+    if (!listed(t)) continue;
+    const int n = columns_of(t);
+    int32_t* out = list_of(t);
+    const uint32_t* above = (const uint32_t*)marks + t * half_words;      // (half_words words a token: two bitmaps)
+    const uint32_t* equal = above + half_words / 2;
+    int tied = rows[t].tied, at = 0;
+    for (int w0 = 0; 32 * w0 < n; w0 += 64) {
+      const int w = w0 + lane, c0 = 32 * w;
+      // bits below column c of the word
+      auto below = [&](int c) { return c <= c0 ? 0u : c - c0 >= 32 ? ~0u : (1u << (c - c0)) - 1; };
+      const uint32_t free = below(n - a.recent) & ~below(a.sinks);
+      uint32_t take = below(n) & ~free, same = 0u;
+      if (need > 0 && free) {
+        take |= above[w] & free;
+        if (tied > 0) same = equal[w] & free;
       }
-      tied -= __builtin_amdgcn_readlane(inc, 63);
+      if (tied > 0) {
+        const int s = __popc(same), inc = akv_wave_inclusive_scan(s);
+        for (int left = min(s, tied - (inc - s)); left > 0; --left) {
+          take |= same & -same;
+          same &= same - 1;
+        }
+        tied -= __builtin_amdgcn_readlane(inc, 63);
+      }
+      const int c = __popc(take), inc = akv_wave_inclusive_scan(c);
+      int to = at + inc - c;
+      for (; take; take &= take - 1) out[to++] = c0 + __ffs(take) - 1;
+      at += __builtin_amdgcn_readlane(inc, 63);
     }
-    const int c = __popc(take), inc = akv_wave_inclusive_scan(c);
-    int to = at + inc - c;
-    for (; take; take &= take - 1) out[to++] = c0 + __ffs(take) - 1;
-    at += __builtin_amdgcn_readlane(inc, 63);
   }
 }
 
 // Wider tables go the long way over scores in memory.
 #define BI_WIDE 16384
-template <int D, int DT, int HELD> static int bi_pick(const bi_rank_args& a, int64_t units, int bytes, hipStream_t stream) {
+template <int D, int DT, int W, int HELD> static int bi_pick(const bi_rank_args& a, int64_t units, int bytes, hipStream_t stream) {
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
   static akv_device_once once;
-  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)bi_pick_kernel<D, DT, 16, HELD>, 16 * BI_WIDE / 4); })) return rc;
-  bi_pick_kernel<D, DT, 16, HELD><<<(uint32_t)units, 1024, bytes, stream>>>(a);
+  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)bi_pick_kernel<D, DT, W, HELD>, 16 * BI_WIDE / 4); })) return rc;
+  bi_pick_kernel<D, DT, W, HELD><<<(uint32_t)units, 64 * W, bytes, stream>>>(a);
   AKV_LAUNCH_CHECK("bi_pick_kernel");
   return AKV_OK;
 }
@@ -623,9 +649,10 @@ template <int D, int DT> static int bi_pick(const bi_rank_args& a, int64_t max_b
   const int64_t units = ((int64_t)a.b.T / 16 + a.b.S + 1) * a.KVH, tiles = (max_blocks + 15) / 16;
   const int bytes = (int)(16 * ((max_blocks + 31) / 32) * 8);
   if (units > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "akv_block_index_select: more than 2^31 rows");
-  if (tiles <= 16 * 8) return bi_pick<D, DT, 8>(a, units, bytes, stream);
-  if (tiles <= 16 * 14) return bi_pick<D, DT, 14>(a, units, bytes, stream);
-  return bi_pick<D, DT, 0>(a, units, bytes, stream);
+  if (tiles <= 8 * 16 && units > ab_cus()) return bi_pick<D, DT, 8, 16>(a, units, bytes, stream);
+  if (tiles <= 16 * 8) return bi_pick<D, DT, 16, 8>(a, units, bytes, stream);
+  if (tiles <= 16 * 14) return bi_pick<D, DT, 16, 14>(a, units, bytes, stream);
+  return bi_pick<D, DT, 16, 0>(a, units, bytes, stream);
 }
 
 // scores of so many bytes at most are held at a time
