@@ -284,7 +284,7 @@ struct bi_row {                         // of a token
   uint32_t order;                       // of the threshold, as far as it is known, where the count goes bit by bit
   float threshold;
 };
-template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) void bi_pick_kernel(bi_rank_args a) {
+template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4) void bi_pick_kernel(bi_rank_args a) {
   constexpr int KS = D / 64, ROW = D + 16, T = 64 * W, HIST = BI_PARTS + 1;
   constexpr int LANES = D / 16, AT_ONCE = 64 / LANES, LOADS = 16 / AT_ONCE;      // of a tile's codes: lanes a row, rows a load, loads
   constexpr int BATCH = 4, STAGED = D == 256 ? 1 : 2;                            // tiles looked up together; tiles in LDS together
@@ -437,31 +437,45 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W) v
   enum { RANGE, PARTS, CANDIDATES, BITS, MARKS };
   float scale[4], shift[4];
   int part[4], bit = 31;
-  auto part_of = [&](float s, int e) { return min((uint32_t)(BI_PARTS - 1), (uint32_t)max(0.f, fmaf(s, scale[e], shift[e]))); };
+  auto part_of = [&](float s, int e) { return (int)__builtin_amdgcn_fmed3f(fmaf(s, scale[e], shift[e]), 0.f, BI_PARTS - 1.f); };
   int row0 = 4 * hq, my_col = col;      // the lane's first token, its column of a tile
   // sixteen columns of token 4 hq + e: a lane of the token writes their marks
   auto mark = [&](int tile, int e, uint64_t lanes, int which) {
-    if (my_col == 0) marks[(2 * (row0 + e) + which) * half_words + tile] = (uint16_t)(lanes >> (16 * hq));
+    const uint32_t mine = hq < 2 ? (uint32_t)lanes : (uint32_t)(lanes >> 32);
+    marks[(2 * (row0 + e) + which) * half_words + tile] = (uint16_t)(mine >> (16 * (hq & 1)));
   };
   auto take = [&](int pass, int tile, const ab_f4& s) {
+    if (pass == PARTS) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (pass == PARTS) {
+      for (int e = 0; e < 4; ++e)
         // (what is not free counts in the lowest part, above which no count starts)
         if (free_to[e] > 0) atomicAdd(hist + (row0 + e) * HIST + part_of(s[e], e), 1);
-      } else if (pass == CANDIDATES) {
-        const int p = (int)part_of(s[e], e);
-        mark(tile, e, __ballot(p > part[e]), 0);
+    } else if (pass == CANDIDATES) {
+      uint64_t above[4] = {};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int p = part_of(s[e], e);
+        above[e] = __ballot(p > part[e]);
         if (p == part[e] && s[e] != -INFINITY) {
           const int at = atomicAdd(&rows[row0 + e].candidates, 1);
           if (at < BI_CANDIDATES) cand[(row0 + e) * BI_CANDIDATES + at] = make_float2(s[e], __int_as_float(16 * tile + my_col));
         }
-      } else if (pass == BITS) {
+      }
+      if (my_col == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mark(tile, e, above[e], 0);
+      }
+    } else if (pass == BITS) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
         if (s[e] != -INFINITY && bi_order(s[e]) >= (rows[row0 + e].order | 1u << bit)) atomicAdd(hist + row0 + e, 1);
-      } else if (pass == MARKS) {
+    } else if (pass == MARKS) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
         const float threshold = rows[row0 + e].threshold;
         const uint64_t above = __ballot(s[e] > threshold), equal = __ballot(s[e] == threshold);
-        if (rows[row0 + e].candidates > BI_CANDIDATES) {
+        if (my_col == 0 && rows[row0 + e].candidates > BI_CANDIDATES) {
           mark(tile, e, above, 0);
           mark(tile, e, equal, 1);
         }
