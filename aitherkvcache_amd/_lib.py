@@ -129,10 +129,10 @@ SIGNATURES = {
     "akv_sparse_attn": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                              _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i, _p, _i64, _i64, _i,
                              _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p]),
-    "akv_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i64]),
+    "akv_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i64]),
     "akv_key_weights": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i64, _i,
                              _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
-    "akv_packed_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i64]),
+    "akv_packed_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i64]),
     "akv_packed_key_weights": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i,
                                     _p, _p, _i, _p, _i64, _i64, _i64, _i, _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
     "akv_evict_select": (_i, [_p, _i64, _i64, _i64, _p, _i, _i, _i, _i, _i, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _p]),

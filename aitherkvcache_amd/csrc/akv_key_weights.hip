@@ -12,6 +12,7 @@
 // float16 terms each (three products, 2^-22).
 #include "akv_batch.h"
 #include "akv_device_once.h"
+#include <type_traits>
 
 #define KW_F16 0
 #define KW_BF16 1                       // 2, 3, 4: packed codes of so many bits
@@ -23,13 +24,18 @@ struct kw_args {
   const float* kn; int64_t kn_blk, kn_pos, kn_head;   // packed: norms, elements
   const float* centroids;
   const float* turn;                    // Pi^T, row-major
-  uint16_t* turned; float* turned_by;   // packed: queries of the slab [token - t0][QH][2][D], and what undoes their scale (times that of the scores)
+  uint16_t* turned; float* turned_by;   // packed: queries of the slab [KVH][rows][2][D], and what undoes their scale (times that of the scores)
   float2* part;                         // [parts][KVH][rows] maximum and sum
   float2* stat;                         // [KVH][rows] maximum and inverse sum
   float* out; int64_t os_seq, os_head;
   int64_t length;                       // floats of a row of the result
   int KVH, QH, G, t0, t1, add;
-  int parts;
+  uint32_t g_recip;
+  int parts, splits;
+  float* sums;                          // [splits][S][KVH][length], where there are several
+  float* scores; int64_t stride;        // few rows: [token - t0][QH][stride]
+  float2* few_part; int few_parts;      // [token - t0][QH][few_parts]
+  int runs;
   float scale2;
 };
 
@@ -38,6 +44,8 @@ template <int D, int KIND> struct kw_plan {
   static constexpr int DT = KIND == KW_BF16 ? AKV_BF16 : AKV_F16, KS = D / 16, TERMS = PACKED ? 2 : 1;
   static constexpr int KT = D * TERMS <= 128 ? 2 : 1, N = 4 * 32 * KT;      // tiles of 32 keys a wavefront; keys of a part
   static constexpr int CHUNKS = TERMS * D / 8, ROW = 16 * CHUNKS;           // of a row of queries in LDS
+  static constexpr int RT = PACKED && D == 256 ? 1 : 2, ROWS = 32 * RT;     // many rows: tiles and rows of a step
+  static constexpr int LDS = 2 * ROWS * ROW;
   static __device__ __forceinline__ int f(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
 };
 
@@ -53,20 +61,67 @@ __device__ __forceinline__ kw_rows kw_rows_of(const kw_args& a, int seq, int ctx
   r.pos0 = ctx - (s1 - r.first);
   return r;
 }
-// 32 rows from r0 on into LDS: sixteen bytes c of row r lie at c ^ f(r); rows past the last are zero
-template <int D, int KIND> __device__ __forceinline__ void kw_stage(const kw_args& a, const kw_rows& R, int r0, int kvh, unsigned char* lds) {
-  typedef kw_plan<D, KIND> P;
-  for (int i = threadIdx.x; i < 32 * P::CHUNKS; i += 256) {
-    const int r = i / P::CHUNKS, c = i % P::CHUNKS, row = r0 + r;
-    ab_u4 v = {0u, 0u, 0u, 0u};
-    if (row < R.rows) {
-      const int t = row / a.G, token = R.first + t, head = kvh * a.G + row - t * a.G;
-      if constexpr (P::PACKED) v = *(const ab_u4*)(a.turned + ((int64_t)(token - a.t0) * a.QH + head) * (2 * D) + 8 * c);
-      else v = *(const ab_u4*)((const uint16_t*)a.q + (int64_t)token * a.qs_tok + (int64_t)head * a.qs_head + 8 * c);
-    }
-    *(ab_u4*)(lds + r * P::ROW + 16 * (c ^ P::f(r))) = v;
-  }
+__device__ __forceinline__ uint32_t kw_div(const kw_args& a, uint32_t row) {      // row / G
+  uint32_t rest;
+  return akv_div32(row, (uint32_t)a.G, a.g_recip, rest);
 }
+// token and head of row r
+__device__ __forceinline__ void kw_row(const kw_args& a, const kw_rows& R, int kvh, int row, int& token, int& head) {
+  uint32_t g;
+  token = R.first + (int)akv_div32((uint32_t)row, (uint32_t)a.G, a.g_recip, g);
+  head = kvh * a.G + (int)g;
+}
+// position of row r (the same in all lanes)
+__device__ __forceinline__ int kw_pos(const kw_args& a, const kw_rows& R, int row) { return R.pos0 + (int)kw_div(a, (uint32_t)row); }
+// where row `row` of a kv head lies in the arrays of the slab
+__device__ __forceinline__ int64_t kw_slab_row(const kw_args& a, const kw_rows& R, int kvh, int row) {
+  return (int64_t)kvh * ((int64_t)(a.t1 - a.t0) * a.G) + (int64_t)(R.first - a.t0) * a.G + row;
+}
+// ROWS rows from r0 on into registers and from there to LDS: sixteen bytes c of row r lie at c ^ f(r); rows past the last are zero.
+template <int D, int KIND, int ROWS> struct kw_stage {
+  typedef kw_plan<D, KIND> P;
+  static constexpr int LOADS = ROWS * P::CHUNKS / 256, AT_ONCE = 256 / P::CHUNKS;      // rows of a load
+  ab_u4 v[LOADS];
+  __device__ __forceinline__ void request(const kw_args& a, const kw_rows& R, int r0, int kvh) {
+    const int mine = (int)threadIdx.x / P::CHUNKS, c = (int)threadIdx.x % P::CHUNKS;
+    const uint8_t* p = nullptr;
+    int64_t step = 0;                   // bytes from load to load, where whole tokens make up a load
+    if constexpr (P::PACKED) {
+      p = (const uint8_t*)a.turned + kw_slab_row(a, R, kvh, r0 + mine) * P::ROW + 16 * c;
+      step = AT_ONCE * P::ROW;
+    } else if (AT_ONCE % a.G == 0) {
+      int token, head;
+      kw_row(a, R, kvh, r0 + mine, token, head);
+      p = (const uint8_t*)a.q + 2 * ((int64_t)token * a.qs_tok + (int64_t)head * a.qs_head) + 16 * c;
+      step = 2 * (int64_t)(AT_ONCE / a.G) * a.qs_tok;
+    }
+    if (r0 + ROWS <= R.rows && (P::PACKED || step != 0)) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) v[i] = *(const ab_u4*)(p + i * step);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = r0 + AT_ONCE * i + mine;
+      v[i] = (ab_u4){0u, 0u, 0u, 0u};
+      if (row < R.rows) {
+        if constexpr (P::PACKED) v[i] = *(const ab_u4*)(p + i * step);
+        else {
+          int token, head;
+          kw_row(a, R, kvh, row, token, head);
+          v[i] = *(const ab_u4*)((const uint8_t*)a.q + 2 * ((int64_t)token * a.qs_tok + (int64_t)head * a.qs_head) + 16 * c);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(unsigned char* lds) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = AT_ONCE * i + (int)threadIdx.x / P::CHUNKS;
+      *(ab_u4*)(lds + r * P::ROW + 16 * (((int)threadIdx.x % P::CHUNKS) ^ P::f(r))) = v[i];
+    }
+  }
+};
 
 // ---- keys of a wavefront as operands
 template <int BITS> struct kw_levels {                // level of a code: float16 terms, the first in the lower half
@@ -127,30 +182,46 @@ template <int D, int KIND> struct kw_keys {
       }
     }
   }
-  // products of tile t with the 32 rows in LDS; KEYS_FIRST: a key's are in the registers, a row's in a lane
-  template <bool KEYS_FIRST> __device__ __forceinline__ ab_f16 product(int t, const unsigned char* rows) const {
+  // products of the tiles with the 32 rows in LDS; KEYS_FIRST: a key's are in the registers, a row's in a lane.  Rows come out of LDS in runs, one of
+  // them on its way while the one before is multiplied (left to itself the compiler asks for one operand at a time and waits for it).
+  template <bool KEYS_FIRST> __device__ __forceinline__ void products(const unsigned char* rows, ab_f16 (&s)[P::KT]) const {
     typedef ab_math<P::DT> M;
+    constexpr int STEPS = 4 / P::TERMS, RUNS = P::KS / STEPS;
     const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
     const unsigned char* r = rows + col * P::ROW;
-    ab_f16 y = (ab_f16)(0.f);
+    ab_u4 q[2][STEPS][P::TERMS];
+    auto read = [&](int run) {
 #pragma unroll
-    for (int ks = 0; ks < P::KS; ++ks) {
-      // (packed: a lane has the half row h, plain: half of every sixteen coordinates)
-      const int c = P::PACKED ? P::KS * h + ks : 2 * ks + h;
-      const ab_u4 q = *(const ab_u4*)(r + 16 * (c ^ P::f(col)));
-      if constexpr (P::PACKED) {
-        const ab_u4 q_lo = *(const ab_u4*)(r + 16 * ((D / 8 + c) ^ P::f(col)));
-        if constexpr (KEYS_FIRST) {
-          y = M::mfma32(lo[t][ks], q, y);
-          y = M::mfma32(hi[t][ks], q_lo, y);
-        } else {
-          y = M::mfma32(q, lo[t][ks], y);
-          y = M::mfma32(q_lo, hi[t][ks], y);
+      for (int i = 0; i < STEPS; ++i) {
+        // (packed: a lane has the half row h, plain: half of every sixteen coordinates)
+        const int ks = run * STEPS + i, c = P::PACKED ? P::KS * h + ks : 2 * ks + h;
+#pragma unroll
+        for (int e = 0; e < P::TERMS; ++e) q[run & 1][i][e] = *(const ab_u4*)(r + 16 * ((e * (D / 8) + c) ^ P::f(col)));
+      }
+    };
+#pragma unroll
+    for (int t = 0; t < P::KT; ++t) s[t] = (ab_f16)(0.f);
+    read(0);
+#pragma unroll
+    for (int run = 0; run < RUNS; ++run) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (run + 1 < RUNS) read(run + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int ks = run * STEPS + i;
+#pragma unroll
+        for (int t = 0; t < P::KT; ++t) {
+          const ab_u4(&x)[P::TERMS] = q[run & 1][i];
+          if constexpr (P::PACKED) {
+            s[t] = KEYS_FIRST ? M::mfma32(lo[t][ks], x[0], s[t]) : M::mfma32(x[0], lo[t][ks], s[t]);
+            s[t] = KEYS_FIRST ? M::mfma32(hi[t][ks], x[1], s[t]) : M::mfma32(x[1], hi[t][ks], s[t]);
+          }
+          s[t] = KEYS_FIRST ? M::mfma32(hi[t][ks], x[0], s[t]) : M::mfma32(x[0], hi[t][ks], s[t]);
         }
       }
-      y = KEYS_FIRST ? M::mfma32(hi[t][ks], q, y) : M::mfma32(q, hi[t][ks], y);
     }
-    return y;
+    __builtin_amdgcn_sched_barrier(0);
   }
 };
 
@@ -196,26 +267,59 @@ template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a
     const uint32_t e = akv_row_exponent(t);
     const float v = (y[i][0] + y[i][1]) * akv_row_scale(e) * 8192.f;      // the largest to [2^13, 2^14)
     const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
-    a.turned[r * (2 * D) + d] = __builtin_bit_cast(uint16_t, hi);
-    a.turned[r * (2 * D) + D + d] = __builtin_bit_cast(uint16_t, lo);
-    if (d == 0) a.turned_by[r] = akv_row_unscale(e) * (1.f / 8192.f) * a.scale2;
+    const int64_t token = r / a.QH, head = r - token * a.QH, to = head / a.G * ((int64_t)(a.t1 - a.t0) * a.G) + token * a.G + head % a.G;
+    a.turned[to * (2 * D) + d] = __builtin_bit_cast(uint16_t, hi);
+    a.turned[to * (2 * D) + D + d] = __builtin_bit_cast(uint16_t, lo);
+    if (d == 0) a.turned_by[to] = akv_row_unscale(e) * (1.f / 8192.f) * a.scale2;
   }
 }
 
-// ---- maxima and sums of the rows over a part of the keys
+// maximum and sum of a lane's row over the wavefront's keys; c: what makes scores of the products
+template <int KT> __device__ __forceinline__ void kw_row_stats(const ab_f16 (&s)[KT], float c, float& m, float& l) {
+  float a = s[0][0], b = s[0][1];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int i = t == 0 ? 2 : 0; i < 16; i += 2) {
+      a = fmaxf(a, s[t][i]);
+      b = fmaxf(b, s[t][i + 1]);
+    }
+  a = fmaxf(a, b);
+  m = fmaxf(a, akv_lane_xor<32>(a)) * c;
+  const float ref = m == -INFINITY || m != m ? 0.f : m;
+  float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      l0 += __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -ref));
+      l1 += __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], c, -ref));
+    }
+  l = l0 + l1;
+  l += akv_lane_xor<32>(l);
+  if (m != m || m == -INFINITY) m = -INFINITY, l = 0.f;      // (-inf times 0: a row that is none)
+}
+
+// ---- many rows: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
+// has one barrier.  Workgroups of `splits` take steps in turn.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
-  __shared__ __align__(16) unsigned char rows[32 * P::ROW];
-  __shared__ float2 ml[4][32];
+  constexpr int ROWS = P::ROWS, RT = P::RT;
+  extern __shared__ __align__(16) unsigned char rows[];          // [2][ROWS][ROW]
+  __shared__ float2 ml[2][4][ROWS];
   __shared__ __align__(16) float norms[P::PACKED ? P::N : 4];
   __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq), from = part * P::N;
   if (from >= ctx) return;
   const kw_rows R = kw_rows_of(a, seq, ctx);
   if (R.rows == 0 || R.pos0 + (R.rows - 1) / a.G < from) return;
+  const int first = (max(0, from - R.pos0) * a.G / ROWS + split) * ROWS, step = ROWS * a.splits;      // rows before see nothing of the part
+  if (first >= R.rows) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
   const int base = from + 32 * P::KT * wave;
+  kw_stage<D, KIND, ROWS> next;
+  next.request(a, R, first, kvh);
   kw_keys<D, KIND> K;
   float unit = 1.f;
   if constexpr (P::PACKED) {
@@ -229,57 +333,62 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
 #pragma unroll
       for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t] * unit;
   }
-  const int64_t all = (int64_t)(a.t1 - a.t0) * a.G, at = (int64_t)(R.first - a.t0) * a.G;
-  float2* to = a.part + ((int64_t)part * a.KVH + kvh) * all + at;
-  const int skip = max(0, from - R.pos0) * a.G / 32 * 32;      // rows before see nothing of the part
-  for (int r0 = skip; r0 < R.rows; r0 += 32) {
-    __syncthreads();
-    kw_stage<D, KIND>(a, R, r0, kvh, rows);
-    __syncthreads();
-    const int row = r0 + col, pos = row < R.rows ? R.pos0 + row / a.G : -1;
-    float m = -INFINITY, l = 0.f;
-    if (any) {
-      float c = a.scale2;
-      if constexpr (P::PACKED) c = row < R.rows ? a.turned_by[(int64_t)(R.first - a.t0 + row / a.G) * a.QH + kvh * a.G + row % a.G] : 0.f;
-      ab_f16 s[P::KT];
-      const bool edge = base + 32 * P::KT - 1 > R.pos0 + r0 / a.G;
-#pragma unroll
-      for (int t = 0; t < P::KT; ++t) {
-        s[t] = K.template product<true>(t, rows);
-        if constexpr (P::PACKED) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const float4 n = *(const float4*)(norms + 32 * (P::KT * wave + t) + 8 * b + 4 * h);
-            s[t][4 * b] *= n.x; s[t][4 * b + 1] *= n.y; s[t][4 * b + 2] *= n.z; s[t][4 * b + 3] *= n.w;
-          }
-        }
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i] = base + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) <= pos ? s[t][i] : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[t][i]);
-      }
-      m = fmaxf(m, akv_lane_xor<32>(m)) * c;
-      const float ref = m == -INFINITY || m != m ? 0.f : m;
-#pragma unroll
-      for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -ref));
-      l += akv_lane_xor<32>(l);
-      if (m != m) m = -INFINITY, l = 0.f;      // (-inf times 0: a row that is none)
-    }
-    if (h == 0) ml[wave][col] = make_float2(m, l);
-    __syncthreads();
-    if (tid < 32 && row < R.rows) {
+  const int64_t slab = kw_slab_row(a, R, kvh, 0);
+  float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
+  // what the wavefronts have of a step's rows, together
+  auto join = [&](int r0, int buf) {
+    if (tid < ROWS && r0 + tid < R.rows) {
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][tid].x);
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[buf][w][tid].x);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) sum += ml[w][tid].x == -INFINITY ? 0.f : ml[w][tid].y * __builtin_amdgcn_exp2f(ml[w][tid].x - top);
-      to[row] = make_float2(top, sum);
+      for (int w = 0; w < 4; ++w) sum += ml[buf][w][tid].x == -INFINITY ? 0.f : ml[buf][w][tid].y * __builtin_amdgcn_exp2f(ml[buf][w][tid].x - top);
+      to[r0 + tid] = make_float2(top, sum);
     }
+  };
+  next.put(rows);
+  int buf = 0, r0 = first;
+  for (;; r0 += step, buf ^= 1) {
+    __syncthreads();
+    const bool more = r0 + step < R.rows;
+    if (more) next.request(a, R, r0 + step, kvh);
+    if (any) {
+#pragma unroll 1
+      for (int i = 0; i < RT; ++i) {
+        const int row = r0 + 32 * i + col;
+        float c = a.scale2, m, l;
+        if constexpr (P::PACKED) c = a.turned_by[slab + min(row, R.rows - 1)];
+        ab_f16 s[P::KT];
+        K.template products<true>(rows + (ROWS * buf + 32 * i) * P::ROW, s);
+        if constexpr (P::PACKED) {
+#pragma unroll
+          for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const float4 n = *(const float4*)(norms + 32 * (P::KT * wave + t) + 8 * b + 4 * h);
+              s[t][4 * b] *= n.x; s[t][4 * b + 1] *= n.y; s[t][4 * b + 2] *= n.z; s[t][4 * b + 3] *= n.w;
+            }
+        }
+        if (base + 32 * P::KT - 1 > kw_pos(a, R, min(r0 + 32 * i, R.rows - 1))) {
+          const int pos = row < R.rows ? kw_pos(a, R, row) : -1;
+#pragma unroll
+          for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[t][e] = base + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= pos ? s[t][e] : -INFINITY;
+        }
+        kw_row_stats<P::KT>(s, c, m, l);
+        if (h == 0) ml[buf][wave][32 * i + col] = make_float2(m, l);
+      }
+    } else if (h == 0) {
+#pragma unroll
+      for (int i = 0; i < RT; ++i) ml[buf][wave][32 * i + col] = make_float2(-INFINITY, 0.f);
+    }
+    if (r0 > first) join(r0 - step, buf ^ 1);
+    if (!more) break;
+    next.put(rows + ROWS * (buf ^ 1) * P::ROW);
   }
+  __syncthreads();
+  join(r0, buf);
 }
 
 // ---- the parts of a row together, a wavefront a row
@@ -306,24 +415,48 @@ template <int N> __global__ __launch_bounds__(256) void kw_join_kernel(kw_args a
   if (lane == 0) a.stat[kvh * all + row] = l > 0.f ? make_float2(top, 1.f / l) : make_float2(0.f, 0.f);
 }
 
-// ---- weights of a part's keys, summed over the rows
+// ---- weights of a part's keys, summed over the rows; steps as above.  Workgroups that share a part leave their sums to kw_add_kernel.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
-  __shared__ __align__(16) unsigned char rows[32 * P::ROW];
-  __shared__ __align__(16) float ref[32], inv[32], by[32];
+  constexpr int ROWS = P::ROWS, RT = P::RT;
+  extern __shared__ __align__(16) unsigned char rows[];          // [2][ROWS][ROW]
+  __shared__ __align__(16) float ref[2][ROWS], inv[2][ROWS], by[2][ROWS];
   __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t from = (int64_t)part * P::N;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
-  float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head;
+  const bool add = a.add && a.splits == 1;
+  float* to = a.splits == 1 ? a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head : a.sums + (((int64_t)split * a.b.S + seq) * a.KVH + kvh) * a.length;
   const kw_rows R = kw_rows_of(a, seq, ctx);
-  if (from >= ctx || R.rows == 0 || R.pos0 + (R.rows - 1) / a.G < from) {
-    if (!a.add)
+  const int first = from < ctx ? (max(0, (int)from - R.pos0) * a.G / ROWS + split) * ROWS : R.rows, step = ROWS * a.splits;
+  if (first >= R.rows || R.pos0 + (R.rows - 1) / a.G < from) {
+    if (!add)
       for (int64_t i = from + tid; i < from + P::N && i < a.length; i += 256) to[i] = 0.f;
     return;
   }
   const int base = (int)from + 32 * P::KT * wave;
+  const int64_t slab = kw_slab_row(a, R, kvh, 0);
+  kw_stage<D, KIND, ROWS> next;
+  float2 e = make_float2(0.f, 0.f);
+  float c = 0.f;
+  auto request = [&](int r0) {
+    next.request(a, R, r0, kvh);
+    if (tid < ROWS) {
+      const bool there = r0 + tid < R.rows;
+      e = there ? a.stat[slab + r0 + tid] : make_float2(0.f, 0.f);
+      if constexpr (P::PACKED) c = there ? a.turned_by[slab + r0 + tid] : 0.f;
+    }
+  };
+  auto put = [&](int buf) {
+    next.put(rows + ROWS * buf * P::ROW);
+    if (tid < ROWS) {
+      ref[buf][tid] = e.x;
+      inv[buf][tid] = e.y;
+      if constexpr (P::PACKED) by[buf][tid] = c;
+    }
+  };
+  request(first);
   kw_keys<D, KIND> K;
   float unit = 1.f;
   if constexpr (P::PACKED) {
@@ -332,98 +465,285 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kern
   }
   const bool any = base < ctx;
   if (any) K.load(a, seq, kvh, base, ctx, levels.level);
+  if constexpr (P::PACKED) {
+#pragma unroll
+    for (int t = 0; t < P::KT; ++t) K.norm[t] *= unit;
+  }
   float w[P::KT] = {};
-  const int64_t all = (int64_t)(a.t1 - a.t0) * a.G;
-  const float2* stat = a.stat + (int64_t)kvh * all + (int64_t)(R.first - a.t0) * a.G;
-  const int skip = max(0, (int)from - R.pos0) * a.G / 32 * 32;
-  for (int r0 = skip; r0 < R.rows; r0 += 32) {
+  put(0);
+  int buf = 0;
+  for (int r0 = first;; r0 += step, buf ^= 1) {
     __syncthreads();
-    kw_stage<D, KIND>(a, R, r0, kvh, rows);
-    if (tid < 32) {
-      const int row = r0 + tid;
-      float2 e = make_float2(0.f, 0.f);
-      float c = 0.f;
-      if (row < R.rows) {
-        e = stat[row];
-        c = a.scale2;
-        if constexpr (P::PACKED) c = a.turned_by[(int64_t)(R.first - a.t0 + row / a.G) * a.QH + kvh * a.G + row % a.G];
+    const bool more = r0 + step < R.rows;
+    if (more) request(r0 + step);
+    if (any) {
+#pragma unroll 1
+      for (int i = 0; i < RT; ++i) {
+        const int row0 = r0 + 32 * i;
+        const bool edge = base + 32 * P::KT - 1 > kw_pos(a, R, min(row0, R.rows - 1));
+        ab_f16 s[P::KT];
+        K.template products<false>(rows + (ROWS * buf + 32 * i) * P::ROW, s);
+        // what makes a score of a product: by row, packed by key and row
+        auto weights = [&](auto masked) {
+          float sum[P::KT][4] = {};
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int at = 32 * i + 8 * b + 4 * h;
+            const float4 m4 = *(const float4*)(ref[buf] + at), i4 = *(const float4*)(inv[buf] + at);
+            float c[4] = {a.scale2, a.scale2, a.scale2, a.scale2};
+            if constexpr (P::PACKED) {
+              const float4 x = *(const float4*)(by[buf] + at);
+              c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
+            }
+            const float m[4] = {m4.x, m4.y, m4.z, m4.w}, iv[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              int pos = 0;
+              if constexpr (masked.value) pos = kw_pos(a, R, row0 + 8 * b + 4 * h + j);
+#pragma unroll
+              for (int t = 0; t < P::KT; ++t) {
+                float x = __builtin_amdgcn_exp2f(fmaf(P::PACKED ? s[t][4 * b + j] * K.norm[t] : s[t][4 * b + j], c[j], -m[j]));
+                if constexpr (masked.value) x = base + 32 * t + col <= pos ? x : 0.f;
+                sum[t][j] = fmaf(x, iv[j], sum[t][j]);
+              }
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < P::KT; ++t) w[t] += (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]);
+        };
+        if (edge) weights(std::true_type{});
+        else weights(std::false_type{});
       }
-      ref[tid] = e.x;
-      inv[tid] = e.y;
-      by[tid] = c;
     }
-    __syncthreads();
-    if (!any) continue;
-    const bool edge = base + 32 * P::KT - 1 > R.pos0 + r0 / a.G;
-#pragma unroll
-    for (int t = 0; t < P::KT; ++t) {
-      const ab_f16 s = K.template product<false>(t, rows);
-      float n = 1.f;
-      if constexpr (P::PACKED) n = K.norm[t] * unit;
-      const int key = base + 32 * t + col;
-      float sum = 0.f;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float4 m4 = *(const float4*)(ref + 8 * b + 4 * h), i4 = *(const float4*)(inv + 8 * b + 4 * h), c4 = *(const float4*)(by + 8 * b + 4 * h);
-        const float m[4] = {m4.x, m4.y, m4.z, m4.w}, iv[4] = {i4.x, i4.y, i4.z, i4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float e = __builtin_amdgcn_exp2f(fmaf(P::PACKED ? s[4 * b + i] * n : s[4 * b + i], c[i], -m[i]));
-          if (edge) e = key <= R.pos0 + (r0 + 8 * b + 4 * h + i) / a.G ? e : 0.f;
-          sum = fmaf(e, iv[i], sum);
-        }
-      }
-      w[t] += sum;
-    }
+    if (!more) break;
+    put(buf ^ 1);
   }
 #pragma unroll
   for (int t = 0; t < P::KT; ++t) {
     const float sum = w[t] + akv_lane_xor<32>(w[t]);
     const int64_t key = (int64_t)base + 32 * t + col;
     if (h == 0 && key < a.length) {
-      if (key < ctx) to[key] = a.add ? to[key] + sum : sum;
-      else if (!a.add) to[key] = 0.f;
+      if (key < ctx) to[key] = add ? to[key] + sum : sum;
+      else if (!add) to[key] = 0.f;
     }
+  }
+}
+// the sums of the workgroups that share a part, in their order
+__global__ __launch_bounds__(256) void kw_add_kernel(kw_args a) {
+  const int64_t key = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int kvh = blockIdx.y, seq = blockIdx.z;
+  if (key >= a.length) return;
+  float sum = 0.f;
+  for (int s = 0; s < a.splits; ++s) sum += a.sums[(((int64_t)s * a.b.S + seq) * a.KVH + kvh) * a.length + key];
+  float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head + key;
+  if (!a.add) *to = sum;
+  else if (key < ab_ctx(a.b, seq)) *to += sum;
+}
+
+// ---- few rows a sequence: keys are read once, as long as a sequence and kv head has no more rows than a tile; scores are kept, four bytes a row and
+// key, and read back by kw_few_sum with the statistics of the rows.  A workgroup of four wavefronts takes `runs` x N keys, the next ones on
+// their way while the ones before are multiplied.
+#define KW_FEW 32
+template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kernel(kw_args a) {
+  typedef kw_plan<D, KIND> P;
+  __shared__ __align__(16) unsigned char rows[32 * P::ROW];
+  __shared__ float2 ml[4][32];
+  __shared__ __align__(16) float norms[P::PACKED ? P::N : 4];
+  __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int ctx = ab_ctx(a.b, seq);
+  const int64_t from64 = (int64_t)part * P::N * a.runs;
+  if (from64 >= ctx) return;
+  const int from = (int)from64;
+  const kw_rows R = kw_rows_of(a, seq, ctx);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
+  float unit = 1.f;
+  if constexpr (P::PACKED) unit = kw_fill(levels, a.centroids);
+  for (int r0 = 0; r0 < R.rows; r0 += 32) {
+    const int last = R.pos0 + (min(r0 + 32, R.rows) - 1) / a.G;  // position of the tile's last row
+    if (last < from) continue;
+    kw_stage<D, KIND, 32> q;
+    q.request(a, R, r0, kvh);
+    __syncthreads();                   // (the tile before has been read)
+    q.put(rows);
+    __syncthreads();
+    const bool valid = r0 + col < R.rows;
+    int token, head;
+    kw_row(a, R, kvh, min(r0 + col, R.rows - 1), token, head);
+    const int pos = valid ? R.pos0 + token - R.first : -1;
+    float c = a.scale2;
+    if constexpr (P::PACKED) c = a.turned_by[kw_slab_row(a, R, kvh, min(r0 + col, R.rows - 1))];
+    float* scores = a.scores + ((int64_t)(token - a.t0) * a.QH + head) * a.stride;
+    float m = -INFINITY, l = 0.f;
+    kw_keys<D, KIND> K;
+    const int end = min(from + P::N * a.runs, last + 1);         // keys that some row sees
+    int base = from + 32 * P::KT * wave;
+    if (base < end) K.load(a, seq, kvh, base, ctx, levels.level);
+    for (; base < end; base += P::N) {
+      if constexpr (P::PACKED) {
+        akv_wave_sync();
+        if (h == 0)
+#pragma unroll
+          for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t] * unit;
+        akv_wave_sync();
+      }
+      ab_f16 s[P::KT];
+      K.template products<true>(rows, s);
+      if (base + P::N < end) K.load(a, seq, kvh, base + P::N, ctx, levels.level);
+      const bool edge = __ballot(base + 32 * P::KT - 1 > pos && valid) != 0;
+#pragma unroll
+      for (int t = 0; t < P::KT; ++t) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          float4 n = make_float4(1.f, 1.f, 1.f, 1.f);
+          if constexpr (P::PACKED) n = *(const float4*)(norms + 32 * (P::KT * wave + t) + 8 * b + 4 * h);
+          s[t][4 * b] *= n.x * c; s[t][4 * b + 1] *= n.y * c; s[t][4 * b + 2] *= n.z * c; s[t][4 * b + 3] *= n.w * c;
+        }
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t][i] = base + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) <= pos ? s[t][i] : -INFINITY;
+        }
+        if (valid) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) *(float4*)(scores + base + 32 * t + 8 * b + 4 * h) = make_float4(s[t][4 * b], s[t][4 * b + 1], s[t][4 * b + 2], s[t][4 * b + 3]);
+        }
+      }
+      float top, sum;
+      kw_row_stats<P::KT>(s, 1.f, top, sum);
+      const float to = fmaxf(m, top);
+      if (to > -INFINITY) {
+        l = l * __builtin_amdgcn_exp2f(m - to) + sum * __builtin_amdgcn_exp2f(top - to);
+        m = to;
+      }
+    }
+    if (h == 0) ml[wave][col] = make_float2(m, l);
+    __syncthreads();
+    if (tid < 32 && valid) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][tid].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += ml[w][tid].x == -INFINITY ? 0.f : ml[w][tid].y * __builtin_amdgcn_exp2f(ml[w][tid].x - top);
+      a.few_part[((int64_t)(token - a.t0) * a.QH + head) * a.few_parts + part] = make_float2(top, sum);
+    }
+  }
+}
+// Weights of KW_FEW_KEYS keys from the scores that were kept; `keys` of a part of kw_few_kernel.
+#define KW_FEW_KEYS 1024
+__global__ __launch_bounds__(256) void kw_few_sum_kernel(kw_args a, int keys) {
+  __shared__ float2 stat[KW_FEW];
+  const int kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int ctx = ab_ctx(a.b, seq);
+  const int64_t key0 = (int64_t)blockIdx.x * KW_FEW_KEYS, key = key0 + 4 * tid;
+  const kw_rows R = kw_rows_of(a, seq, ctx);
+  float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head;
+  float w[4] = {};
+  for (int r0 = 0; r0 < R.rows; r0 += KW_FEW) {
+    const int count = min(KW_FEW, R.rows - r0), last = R.pos0 + (r0 + count - 1) / a.G;
+    if (key0 > last) continue;
+    __syncthreads();                   // (the statistics before have been read)
+    for (int r = wave; r < count; r += 4) {
+      int token, head;
+      kw_row(a, R, kvh, r0 + r, token, head);
+      const float2* e = a.few_part + ((int64_t)(token - a.t0) * a.QH + head) * a.few_parts;
+      float m = -INFINITY, l = 0.f;
+      for (int p = lane; p <= last / keys; p += 64) {
+        const float2 x = e[p];
+        const float top = fmaxf(m, x.x);
+        if (top == -INFINITY) continue;
+        l = l * __builtin_amdgcn_exp2f(m - top) + x.y * __builtin_amdgcn_exp2f(x.x - top);
+        m = top;
+      }
+      const float top = akv_wave_max(m);
+      l = akv_wave_sum(m == -INFINITY ? 0.f : l * __builtin_amdgcn_exp2f(m - top));
+      if (lane == 0) stat[r] = l > 0.f ? make_float2(top, 1.f / l) : make_float2(0.f, 0.f);
+    }
+    __syncthreads();
+    if (key > last) continue;          // (scores are kept up to there, those behind a row's own position as -infinity)
+    for (int r = 0; r < count; ++r) {
+      int token, head;
+      kw_row(a, R, kvh, r0 + r, token, head);
+      const float4 s = *(const float4*)(a.scores + ((int64_t)(token - a.t0) * a.QH + head) * a.stride + key);
+      const float m = stat[r].x, iv = stat[r].y, x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key + i <= last) w[i] = fmaf(__builtin_amdgcn_exp2f(x[i] - m), iv, w[i]);
+    }
+  }
+  const int end = R.rows > 0 ? R.pos0 + (R.rows - 1) / a.G : -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (key + i >= a.length) continue;
+    if (!a.add) to[key + i] = w[i];
+    else if (key + i <= end) to[key + i] += w[i];
   }
 }
 
 // ---- launches
 #define KW_SCRATCH (256ll << 20)
-struct kw_scratch { int64_t tokens; size_t stat, part, turned, by, bytes; int parts; };
-// scratch of a call, its tokens in slabs of what KW_SCRATCH holds (a multiple of 32, or all)
-static inline kw_scratch kw_layout(int64_t T, int QH, int D, bool packed, int keys, int64_t length) {
+struct kw_scratch { int64_t tokens; size_t stat, part, turned, by, scores, few_part, sums, bytes; int parts, few_parts, runs, splits; int64_t stride; bool few; };
+// Scratch of a call, its tokens in slabs of what KW_SCRATCH holds (a multiple of 32, or all).  Scores are kept where the batch has no more than a
+// tile of rows a sequence and kv head on average: a key of 128 coordinates that is read again costs 256 bytes, the scores of 4 rows written and
+// read 32.
+static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, bool packed, int keys, int64_t length) {
   kw_scratch w = {};
-  w.parts = (int)((length + keys - 1) / keys);
-  const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0));
+  w.few = T * (QH / KVH) <= (int64_t)KW_FEW * S;
+  w.stride = (length + keys * 4 - 1) / (keys * 4) * (keys * 4);
+  // runs of keys a workgroup: as many as leave four workgroups a CU
+  w.runs = 4;
+  while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < 4 * ab_cus()) w.runs /= 2;
+  w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
+  w.parts = w.few ? 0 : (int)((length + keys - 1) / keys);
+  // workgroups that share the rows of a part: as many as give every CU two
+  w.splits = 1;
+  while (!w.few && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
+  const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
   w.tokens = KW_SCRATCH / per / 32 * 32;
   if (w.tokens < 32) w.tokens = 32;
   if (w.tokens > T) w.tokens = T;
-  const int64_t rows = w.tokens * QH;
+  const size_t rows = (size_t)(w.tokens * QH);
   w.stat = 0;
-  w.part = akv_align256((size_t)rows * 8);
-  w.turned = w.part + akv_align256((size_t)rows * 8 * w.parts);
-  w.by = w.turned + (packed ? akv_align256((size_t)rows * 4 * D) : 0);
-  w.bytes = w.by + (packed ? akv_align256((size_t)rows * 4) : 0);
+  w.part = akv_align256(rows * 8);
+  w.turned = w.part + akv_align256(rows * 8 * w.parts);
+  w.by = w.turned + (packed ? akv_align256(rows * 4 * D) : 0);
+  w.scores = w.by + (packed ? akv_align256(rows * 4) : 0);
+  w.few_part = w.scores + (w.few ? akv_align256(rows * 4 * w.stride) : 0);
+  w.sums = w.few_part + (w.few ? akv_align256(rows * 8 * w.few_parts) : 0);
+  w.bytes = w.sums + (w.splits > 1 ? akv_align256((size_t)w.splits * S * KVH * length * 4) : 0);
   return w;
 }
 static inline int kw_part(int D, bool packed) { return D * (packed ? 2 : 1) <= 128 ? 256 : 128; }
-static inline size_t kw_bytes(int64_t T, int QH, int D, bool packed, int64_t length) {
-  return T <= 0 || QH <= 0 || length <= 0 || !ab_head_size(D) ? 0 : kw_layout(T, QH, D, packed, kw_part(D, packed), length).bytes;
+static inline size_t kw_bytes(int64_t T, int S, int QH, int KVH, int D, bool packed, int64_t length) {
+  return T <= 0 || S <= 0 || QH <= 0 || KVH <= 0 || length <= 0 || !ab_head_size(D) ? 0 : kw_layout(T, S, QH, KVH, D, packed, kw_part(D, packed), length).bytes;
 }
-extern "C" size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_q_heads, d, false, length); }
-extern "C" size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_q_heads, d, true, length); }
+extern "C" size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, false, length); }
+extern "C" size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, true, length); }
 
 template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scratch, hipStream_t stream) {
   typedef kw_plan<D, KIND> P;
   static_assert(P::N == (D * P::TERMS <= 128 ? 256 : 128), "kw_part");
-  const kw_scratch w = kw_layout(T, a.QH, D, P::PACKED, P::N, a.length);
-  a.stat = (float2*)((char*)scratch + w.stat);
-  a.part = (float2*)((char*)scratch + w.part);
-  a.turned = (uint16_t*)((char*)scratch + w.turned);
-  a.turned_by = (float*)((char*)scratch + w.by);
-  a.parts = w.parts;
+  const kw_scratch w = kw_layout(T, a.b.S, a.QH, a.KVH, D, P::PACKED, P::N, a.length);
+  char* const at = (char*)scratch;
+  a.stat = (float2*)(at + w.stat);
+  a.part = (float2*)(at + w.part);
+  a.turned = (uint16_t*)(at + w.turned);
+  a.turned_by = (float*)(at + w.by);
+  a.scores = (float*)(at + w.scores);
+  a.few_part = (float2*)(at + w.few_part);
+  a.sums = (float*)(at + w.sums);
+  a.splits = w.splits;
+  a.parts = w.parts; a.few_parts = w.few_parts; a.stride = w.stride; a.runs = w.runs;
+  a.g_recip = (uint32_t)(0xffffffffull / (uint32_t)a.G);
+  int dev = 0;
+  AKV_HIP(hipGetDevice(&dev));
+  static akv_device_once once;
+  if (const int rc = once(dev, [&]() -> int {
+        const int rc1 = ab_lds((const void*)kw_stats_kernel<D, KIND>, P::LDS);
+        return rc1 ? rc1 : ab_lds((const void*)kw_sum_kernel<D, KIND>, P::LDS);
+      }))
+    return rc;
   const int add = a.add;
-  const dim3 grid((uint32_t)w.parts, (uint32_t)a.KVH, (uint32_t)a.b.S);
+  const dim3 grid((uint32_t)((a.length + P::N - 1) / P::N * w.splits), (uint32_t)a.KVH, (uint32_t)a.b.S);
   int64_t t = 0;
   do {                                  // (without a token: zeros)
     a.t0 = (int)t;
@@ -435,13 +755,27 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
         kw_turn_kernel<D><<<(uint32_t)((rows + 7) / 8), 256, 0, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_turn_kernel");
       }
-      kw_stats_kernel<D, KIND><<<grid, 256, 0, stream>>>(a);
-      AKV_LAUNCH_CHECK("kw_stats_kernel");
-      kw_join_kernel<P::N><<<(uint32_t)((rows + 3) / 4), 256, 0, stream>>>(a);
-      AKV_LAUNCH_CHECK("kw_join_kernel");
+      if (w.few) {
+        kw_few_kernel<D, KIND><<<dim3((uint32_t)w.few_parts, (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a);
+        AKV_LAUNCH_CHECK("kw_few_kernel");
+      } else {
+        kw_stats_kernel<D, KIND><<<grid, 256, P::LDS, stream>>>(a);
+        AKV_LAUNCH_CHECK("kw_stats_kernel");
+        kw_join_kernel<P::N><<<(uint32_t)((rows + 3) / 4), 256, 0, stream>>>(a);
+        AKV_LAUNCH_CHECK("kw_join_kernel");
+      }
     }
-    kw_sum_kernel<D, KIND><<<grid, 256, 0, stream>>>(a);
-    AKV_LAUNCH_CHECK("kw_sum_kernel");
+    if (w.few) {
+      kw_few_sum_kernel<<<dim3((uint32_t)((a.length + KW_FEW_KEYS - 1) / KW_FEW_KEYS), (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a, P::N * w.runs);
+      AKV_LAUNCH_CHECK("kw_few_sum_kernel");
+    } else {
+      kw_sum_kernel<D, KIND><<<grid, 256, P::LDS, stream>>>(a);
+      AKV_LAUNCH_CHECK("kw_sum_kernel");
+      if (w.splits > 1) {
+        kw_add_kernel<<<dim3((uint32_t)((a.length + 255) / 256), (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a);
+        AKV_LAUNCH_CHECK("kw_add_kernel");
+      }
+    }
     t += w.tokens;
   } while (t < T);
   return AKV_OK;
@@ -459,7 +793,7 @@ static inline int kw_check(const char* name, const kw_args& a, int dtype, int64_
   AKV_REQUIRE(a.out && (T == 0 || a.q) && a.b.starts, "%s: null pointer", name);
   if (T * (int64_t)a.QH > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^31 rows", name);
   if (!ab_aligned(a.q, 16) || ((a.qs_tok | a.qs_head) & 7)) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: queries must lie at multiples of 16 bytes", name);
-  const size_t need = kw_bytes(T, a.QH, d, packed, a.length);
+  const size_t need = kw_bytes(T, a.b.S, a.QH, a.KVH, d, packed, a.length);
   if (need && (!workspace || workspace_bytes < need || !ab_aligned(workspace, 256))) return akv_fail(AKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", name, need);
   return AKV_OK;
 }

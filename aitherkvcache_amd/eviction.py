@@ -53,7 +53,7 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, block_tables
     dev = _lib.require_gpu(query, key_cache, block_tables, context_lens, query_start_loc, accumulated)
     w = weights_for(accumulated, num_seqs, kv_heads, bt.shape[1] * block_size, dev)
     L = _lib.lib()
-    ws = torch.empty(L.akv_key_weights_workspace_bytes(num_tokens, num_q_heads, d, w.shape[2]), dtype=torch.uint8, device=dev)
+    ws = torch.empty(L.akv_key_weights_workspace_bytes(num_tokens, num_seqs, num_q_heads, kv_heads, d, w.shape[2]), dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         _lib.check(L.akv_key_weights(
             q.data_ptr(), _lib.dtype_code(q), q.stride(0), q.stride(1), key_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),

@@ -258,7 +258,7 @@ class TQPagedAttention:
         k_norms = k_norms if k_norms.dtype == torch.float32 else k_norms.float()
         w = weights_for(accumulated, num_seqs, num_kv_heads, bt.shape[1] * block_size, dev)
         L = _lib.lib()
-        ws = torch.empty(L.akv_packed_key_weights_workspace_bytes(num_tokens, num_q_heads, d, w.shape[2]), dtype=torch.uint8, device=dev)
+        ws = torch.empty(L.akv_packed_key_weights_workspace_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, w.shape[2]), dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
             _lib.check(L.akv_packed_key_weights(
                 q.data_ptr(), _lib.dtype_code(q), q.stride(0), q.stride(1), k_packed.data_ptr(), k_packed.stride(0), k_packed.stride(1), k_packed.stride(2),

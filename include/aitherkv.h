@@ -612,7 +612,7 @@ int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_hea
                     void* out, int64_t os_tok, int64_t os_head, int zero_tail,
                     int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
                     int64_t num_blocks, int64_t max_blocks_per_seq, float scale, void* stream);
-size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length);
+size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length);
 int akv_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
                     const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
                     const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
@@ -620,7 +620,7 @@ int akv_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_hea
                     int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
                     int64_t num_blocks, int64_t max_blocks_per_seq, float scale,
                     void* workspace, size_t workspace_bytes, void* stream);
-size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_q_heads, int d, int64_t length);
+size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length);
 int akv_packed_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
                            const uint8_t* k_packed, int64_t kps_blk, int64_t kps_pos, int64_t kps_head,
                            const float* k_norms, int64_t kns_blk, int64_t kns_pos, int64_t kns_head,

@@ -314,8 +314,9 @@ def test_library_refuses(call, want, change):
 def test_workspace_sizes():
     L = _lib.lib()
     assert L.akv_block_index_select_workspace_bytes(0, 8, 100) == 0 and L.akv_block_index_select_workspace_bytes(4, 8, 0) == 0
-    assert L.akv_key_weights_workspace_bytes(0, 8, 64, 100) == 0 and L.akv_key_weights_workspace_bytes(4, 8, 96, 100) == 0
     # scratch of long calls is held to slabs
     assert 0 < L.akv_block_index_select_workspace_bytes(1 << 20, 8, 40000) <= 1 << 28 and L.akv_block_index_select_workspace_bytes(1 << 20, 8, 8192) == 0
-    assert L.akv_key_weights_workspace_bytes(1 << 20, 32, 128, 1 << 17) <= 1 << 29
-    assert L.akv_packed_key_weights_workspace_bytes(1 << 20, 32, 128, 1 << 17) <= 1 << 29
+    for weights in (L.akv_key_weights_workspace_bytes, L.akv_packed_key_weights_workspace_bytes):
+        assert weights(0, 1, 8, 8, 64, 100) == 0 and weights(4, 1, 8, 8, 96, 100) == 0 and weights(4, 0, 8, 8, 64, 100) == 0
+        for seqs in (1, 256, 1 << 16):
+            assert 0 < weights(1 << 20, seqs, 32, 8, 128, 1 << 17) <= 5 << 27
