@@ -43,10 +43,10 @@ template <int D, int KIND> struct kw_plan {
   static constexpr bool PACKED = KIND >= 2;
   static constexpr int DT = KIND == KW_BF16 ? AKV_BF16 : AKV_F16, KS = D / 16, TERMS = PACKED ? 2 : 1;
   static constexpr int KT = D * TERMS <= 128 ? 2 : 1, N = 4 * 32 * KT;      // tiles of 32 keys a wavefront; keys of a part
-  static constexpr int CHUNKS = TERMS * D / 8, ROW = 16 * CHUNKS;           // of a row of queries in LDS
+  static constexpr int CHUNKS = TERMS * D / 8, BYTES = 16 * CHUNKS;         // of a row of queries
+  static constexpr int ROW = BYTES + 16;                                    // in LDS: sixteen rows begin four banks apart each, and places are constants
   static constexpr int RT = PACKED && D == 256 ? 1 : 2, ROWS = 32 * RT;     // many rows: tiles and rows of a step
   static constexpr int LDS = 2 * ROWS * ROW;
-  static __device__ __forceinline__ int f(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
 };
 
 // ---- rows of queries
@@ -77,49 +77,49 @@ __device__ __forceinline__ int kw_pos(const kw_args& a, const kw_rows& R, int ro
 __device__ __forceinline__ int64_t kw_slab_row(const kw_args& a, const kw_rows& R, int kvh, int row) {
   return (int64_t)kvh * ((int64_t)(a.t1 - a.t0) * a.G) + (int64_t)(R.first - a.t0) * a.G + row;
 }
-// ROWS rows from r0 on into registers and from there to LDS: sixteen bytes c of row r lie at c ^ f(r); rows past the last are zero.
+// ROWS rows into registers and from there to LDS; rows past the last are zero.
 template <int D, int KIND, int ROWS> struct kw_stage {
   typedef kw_plan<D, KIND> P;
   static constexpr int LOADS = ROWS * P::CHUNKS / 256, AT_ONCE = 256 / P::CHUNKS;      // rows of a load
   ab_u4 v[LOADS];
-  __device__ __forceinline__ void request(const kw_args& a, const kw_rows& R, int r0, int kvh) {
-    const int mine = (int)threadIdx.x / P::CHUNKS, c = (int)threadIdx.x % P::CHUNKS;
-    const uint8_t* p = nullptr;
-    int64_t step = 0;                   // bytes from load to load, where whole tokens make up a load
+  const uint8_t* p;                     // where the thread's first piece of row r0 lies
+  int64_t load, step;                   // bytes from load to load, and from step to step (0: rows of a load are not whole tokens)
+  __device__ __forceinline__ const uint8_t* at(const kw_args& a, const kw_rows& R, int kvh, int row) const {
+    const int c = 16 * ((int)threadIdx.x % P::CHUNKS);
+    if constexpr (P::PACKED) return (const uint8_t*)a.turned + kw_slab_row(a, R, kvh, row) * P::BYTES + c;
+    int token, head;
+    kw_row(a, R, kvh, row, token, head);
+    return (const uint8_t*)a.q + 2 * ((int64_t)token * a.qs_tok + (int64_t)head * a.qs_head) + c;
+  }
+  // rows r0 .., and after that every `rows` behind
+  __device__ __forceinline__ kw_stage(const kw_args& a, const kw_rows& R, int r0, int kvh, int rows) {
+    p = at(a, R, kvh, r0 + (int)threadIdx.x / P::CHUNKS);
     if constexpr (P::PACKED) {
-      p = (const uint8_t*)a.turned + kw_slab_row(a, R, kvh, r0 + mine) * P::ROW + 16 * c;
-      step = AT_ONCE * P::ROW;
-    } else if (AT_ONCE % a.G == 0) {
-      int token, head;
-      kw_row(a, R, kvh, r0 + mine, token, head);
-      p = (const uint8_t*)a.q + 2 * ((int64_t)token * a.qs_tok + (int64_t)head * a.qs_head) + 16 * c;
-      step = 2 * (int64_t)(AT_ONCE / a.G) * a.qs_tok;
+      load = AT_ONCE * P::BYTES;
+      step = (int64_t)rows * P::BYTES;
+    } else {
+      const bool whole = AT_ONCE % a.G == 0 && rows % a.G == 0;
+      load = whole ? 2 * (int64_t)(AT_ONCE / a.G) * a.qs_tok : 0;
+      step = whole ? 2 * (int64_t)(rows / a.G) * a.qs_tok : 0;
     }
-    if (r0 + ROWS <= R.rows && (P::PACKED || step != 0)) {
+  }
+  __device__ __forceinline__ void request(const kw_args& a, const kw_rows& R, int r0, int kvh) {
+    if (r0 + ROWS <= R.rows && step != 0) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) v[i] = *(const ab_u4*)(p + i * step);
-      return;
-    }
+      for (int i = 0; i < LOADS; ++i) v[i] = *(const ab_u4*)(p + i * load);
+    } else {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int row = r0 + AT_ONCE * i + mine;
-      v[i] = (ab_u4){0u, 0u, 0u, 0u};
-      if (row < R.rows) {
-        if constexpr (P::PACKED) v[i] = *(const ab_u4*)(p + i * step);
-        else {
-          int token, head;
-          kw_row(a, R, kvh, row, token, head);
-          v[i] = *(const ab_u4*)((const uint8_t*)a.q + 2 * ((int64_t)token * a.qs_tok + (int64_t)head * a.qs_head) + 16 * c);
-        }
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = r0 + AT_ONCE * i + (int)threadIdx.x / P::CHUNKS;
+        v[i] = (ab_u4){0u, 0u, 0u, 0u};
+        if (row < R.rows) v[i] = *(const ab_u4*)at(a, R, kvh, row);
       }
     }
+    p += step;
   }
   __device__ __forceinline__ void put(unsigned char* lds) const {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int r = AT_ONCE * i + (int)threadIdx.x / P::CHUNKS;
-      *(ab_u4*)(lds + r * P::ROW + 16 * (((int)threadIdx.x % P::CHUNKS) ^ P::f(r))) = v[i];
-    }
+    for (int i = 0; i < LOADS; ++i) *(ab_u4*)(lds + (AT_ONCE * i + (int)threadIdx.x / P::CHUNKS) * P::ROW + 16 * ((int)threadIdx.x % P::CHUNKS)) = v[i];
   }
 };
 
@@ -188,15 +188,15 @@ template <int D, int KIND> struct kw_keys {
     typedef ab_math<P::DT> M;
     constexpr int STEPS = 4 / P::TERMS, RUNS = P::KS / STEPS;
     const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-    const unsigned char* r = rows + col * P::ROW;
+    const unsigned char* r = rows + col * P::ROW + 16 * (P::PACKED ? P::KS * h : h);
     ab_u4 q[2][STEPS][P::TERMS];
     auto read = [&](int run) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         // (packed: a lane has the half row h, plain: half of every sixteen coordinates)
-        const int ks = run * STEPS + i, c = P::PACKED ? P::KS * h + ks : 2 * ks + h;
+        const int ks = run * STEPS + i;
 #pragma unroll
-        for (int e = 0; e < P::TERMS; ++e) q[run & 1][i][e] = *(const ab_u4*)(r + 16 * ((e * (D / 8) + c) ^ P::f(col)));
+        for (int e = 0; e < P::TERMS; ++e) q[run & 1][i][e] = *(const ab_u4*)(r + 16 * (e * (D / 8) + (P::PACKED ? ks : 2 * ks)));
       }
     };
 #pragma unroll
@@ -318,7 +318,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
   if (first >= R.rows) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
   const int base = from + 32 * P::KT * wave;
-  kw_stage<D, KIND, ROWS> next;
+  kw_stage<D, KIND, ROWS> next(a, R, first, kvh, step);
   next.request(a, R, first, kvh);
   kw_keys<D, KIND> K;
   float unit = 1.f;
@@ -335,15 +335,17 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
   }
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
   float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
-  // what the wavefronts have of a step's rows, together
+  // what the wavefronts have of a step's rows, together: four lanes a row, every wavefront a quarter
   auto join = [&](int r0, int buf) {
-    if (tid < ROWS && r0 + tid < R.rows) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[buf][w][tid].x);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum += ml[buf][w][tid].x == -INFINITY ? 0.f : ml[buf][w][tid].y * __builtin_amdgcn_exp2f(ml[buf][w][tid].x - top);
-      to[r0 + tid] = make_float2(top, sum);
+    const int r = ROWS / 4 * wave + (lane >> 2);
+    if (lane < ROWS) {
+      const float2 e = ml[buf][lane & 3][r];
+      float top = fmaxf(e.x, akv_lane_xor<1>(e.x));
+      top = fmaxf(top, akv_lane_xor<2>(top));
+      float sum = e.x == -INFINITY ? 0.f : e.y * __builtin_amdgcn_exp2f(e.x - top);
+      sum += akv_lane_xor<1>(sum);
+      sum += akv_lane_xor<2>(sum);
+      if ((lane & 3) == 0 && r0 + r < R.rows) to[r0 + r] = make_float2(top, sum);
     }
   };
   next.put(rows);
@@ -352,6 +354,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
     __syncthreads();
     const bool more = r0 + step < R.rows;
     if (more) next.request(a, R, r0 + step, kvh);
+    if (r0 > first) join(r0 - step, buf ^ 1);
     if (any) {
 #pragma unroll 1
       for (int i = 0; i < RT; ++i) {
@@ -383,7 +386,6 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
 #pragma unroll
       for (int i = 0; i < RT; ++i) ml[buf][wave][32 * i + col] = make_float2(-INFINITY, 0.f);
     }
-    if (r0 > first) join(r0 - step, buf ^ 1);
     if (!more) break;
     next.put(rows + ROWS * (buf ^ 1) * P::ROW);
   }
@@ -437,7 +439,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kern
   }
   const int base = (int)from + 32 * P::KT * wave;
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
-  kw_stage<D, KIND, ROWS> next;
+  kw_stage<D, KIND, ROWS> next(a, R, first, kvh, step);
   float2 e = make_float2(0.f, 0.f);
   float c = 0.f;
   auto request = [&](int r0) {
@@ -562,7 +564,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kern
   for (int r0 = 0; r0 < R.rows; r0 += 32) {
     const int last = R.pos0 + (min(r0 + 32, R.rows) - 1) / a.G;  // position of the tile's last row
     if (last < from) continue;
-    kw_stage<D, KIND, 32> q;
+    kw_stage<D, KIND, 32> q(a, R, r0, kvh, 32);
     q.request(a, R, r0, kvh);
     __syncthreads();                   // (the tile before has been read)
     q.put(rows);
