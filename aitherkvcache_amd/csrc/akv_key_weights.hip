@@ -12,7 +12,6 @@
 // float16 terms each (three products, 2^-22).
 #include "akv_batch.h"
 #include "akv_device_once.h"
-#include <type_traits>
 
 #define KW_F16 0
 #define KW_BF16 1                       // 2, 3, 4: packed codes of so many bits
@@ -42,10 +41,10 @@ struct kw_args {
 template <int D, int KIND> struct kw_plan {
   static constexpr bool PACKED = KIND >= 2;
   static constexpr int DT = KIND == KW_BF16 ? AKV_BF16 : AKV_F16, KS = D / 16, TERMS = PACKED ? 2 : 1;
-  static constexpr int KT = D * TERMS <= 128 ? 2 : 1, N = 4 * 32 * KT;      // tiles of 32 keys a wavefront; keys of a part
+  static constexpr int KT = !PACKED && D <= 128 ? 2 : 1, N = 4 * 32 * KT;      // tiles of 32 keys a wavefront; keys of a part
   static constexpr int CHUNKS = TERMS * D / 8, BYTES = 16 * CHUNKS;         // of a row of queries
   static constexpr int ROW = BYTES + 16;                                    // in LDS: sixteen rows begin four banks apart each, and places are constants
-  static constexpr int RT = PACKED && D == 256 ? 1 : 2, ROWS = 32 * RT;     // many rows: tiles and rows of a step
+  static constexpr int RT = 2, ROWS = 32 * RT;                              // many rows over plain keys: tiles and rows of a step
   static constexpr int LDS = 2 * ROWS * ROW;
 };
 
@@ -150,32 +149,47 @@ template <int BITS, int W> __device__ __forceinline__ uint32_t kw_code(const uin
 }
 template <int D, int KIND> struct kw_keys {
   typedef kw_plan<D, KIND> P;
+  static constexpr int W = P::PACKED ? D * (P::PACKED ? KIND : 4) / 64 : 1;      // packed: words of half a row
   ab_u4 hi[P::KT][P::KS], lo[P::PACKED ? P::KT : 1][P::PACKED ? P::KS : 1];
-  float norm[P::KT];                    // packed: of the lane's key
-  // keys base .. base + 32 KT - 1 of a sequence of ctx > base tokens (those past the last: the last)
-  __device__ __forceinline__ void load(const kw_args& a, int seq, int kvh, int base, int ctx, const uint32_t* levels) {
+  uint32_t raw[P::PACKED ? P::KT : 1][W];
+  float norm[P::KT], raw_norm[P::KT];   // packed: of the lane's key
+  // keys base .. base + 32 KT - 1 of a sequence of ctx > base tokens (those past the last: the last); packed: as they lie in memory
+  __device__ __forceinline__ void request(const kw_args& a, int seq, int kvh, int base, int ctx) {
     const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+    ab_entry e[P::KT];
+    uint32_t place[P::KT];
 #pragma unroll
     for (int t = 0; t < P::KT; ++t) {
       const int key = min(base + 32 * t + col, ctx - 1);
-      uint32_t place;
-      const uint32_t c = akv_div32((uint32_t)key, (uint32_t)a.b.block_size, a.b.bs_recip, place);
-      const int64_t blk = ab_block(a.b, seq, c);
-      const uint8_t* p = a.k + blk * a.k_blk + (int64_t)place * a.k_pos + (int64_t)kvh * a.k_head;
+      e[t] = ab_look(a.b, seq, akv_div32((uint32_t)key, (uint32_t)a.b.block_size, a.b.bs_recip, place[t]));
+    }
+#pragma unroll
+    for (int t = 0; t < P::KT; ++t) {
+      const int64_t blk = ab_block(a.b, e[t]);
+      const uint8_t* p = a.k + blk * a.k_blk + (int64_t)place[t] * a.k_pos + (int64_t)kvh * a.k_head;
       if constexpr (!P::PACKED) {
 #pragma unroll
         for (int ks = 0; ks < P::KS; ++ks) hi[t][ks] = *(const ab_u4*)(p + 32 * ks + 16 * h);
       } else {
-        constexpr int BITS = KIND, W = D * BITS / 64;      // words of half a row
-        uint32_t w[W];
+        struct __attribute__((packed, aligned(4))) words { uint32_t v[W]; };      // (rows lie at multiples of four bytes)
+        const words x = *(const words*)(p + 4 * W * h);
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = *(const uint32_t*)(p + 4 * (W * h + i));
-        norm[t] = a.kn[blk * a.kn_blk + (int64_t)place * a.kn_pos + (int64_t)kvh * a.kn_head];
+        for (int i = 0; i < W; ++i) raw[t][i] = x.v[i];
+        raw_norm[t] = a.kn[blk * a.kn_blk + (int64_t)place[t] * a.kn_pos + (int64_t)kvh * a.kn_head];
+      }
+    }
+  }
+  // packed: codes to levels
+  __device__ __forceinline__ void decode(const uint32_t* levels, float unit) {
+    if constexpr (P::PACKED) {
+#pragma unroll
+      for (int t = 0; t < P::KT; ++t) {
+        norm[t] = raw_norm[t] * unit;
 #pragma unroll
         for (int ks = 0; ks < P::KS; ++ks)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t x = levels[kw_code<BITS>(w, ks, 2 * i)], y = levels[kw_code<BITS>(w, ks, 2 * i + 1)];
+            const uint32_t x = levels[kw_code<KIND>(raw[t], ks, 2 * i)], y = levels[kw_code<KIND>(raw[t], ks, 2 * i + 1)];
             hi[t][ks][i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
             lo[t][ks][i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
           }
@@ -186,7 +200,7 @@ template <int D, int KIND> struct kw_keys {
   // them on its way while the one before is multiplied (left to itself the compiler asks for one operand at a time and waits for it).
   template <bool KEYS_FIRST> __device__ __forceinline__ void products(const unsigned char* rows, ab_f16 (&s)[P::KT]) const {
     typedef ab_math<P::DT> M;
-    constexpr int STEPS = 4 / P::TERMS, RUNS = P::KS / STEPS;
+    constexpr int STEPS = P::PACKED ? D == 256 ? 1 : 2 : 4, RUNS = P::KS / STEPS;
     const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
     const unsigned char* r = rows + col * P::ROW + 16 * (P::PACKED ? P::KS * h : h);
     ab_u4 q[2][STEPS][P::TERMS];
@@ -228,14 +242,14 @@ template <int D, int KIND> struct kw_keys {
 // ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows
 template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a) {
   constexpr int PER = 256 / D > 0 ? 256 / D : 1, LANES = D < 256 ? D : 256, R = 8 / PER;      // threads of a row; rows of a thread
-  __shared__ float x[8][D];
-  __shared__ float top[8][4];
-  const int64_t rows = (int64_t)(a.t1 - a.t0) * a.QH, r0 = (int64_t)blockIdx.x * 8;
+  __shared__ __align__(16) float x[8][D];
+  const uint32_t rows = (uint32_t)(a.t1 - a.t0) * (uint32_t)a.QH, r0 = blockIdx.x * 8u, QH = (uint32_t)a.QH, G = (uint32_t)a.G;
   for (int i = threadIdx.x; i < 8 * D; i += 256) {
-    const int64_t r = r0 + i / D;
+    const uint32_t r = r0 + i / D;
     float v = 0.f;
     if (r < rows) {
-      const int64_t at = (r / a.QH + a.t0) * a.qs_tok + (r % a.QH) * a.qs_head + i % D;
+      const uint32_t token = r / QH;
+      const int64_t at = (int64_t)(token + (uint32_t)a.t0) * a.qs_tok + (int64_t)(r - token * QH) * a.qs_head + i % D;
       v = a.dtype == AKV_F16 ? akv_elem<AKV_F16>::load(a.q, at) : akv_elem<AKV_BF16>::load(a.q, at);
     }
     x[i / D][i % D] = v;
@@ -243,34 +257,46 @@ template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a
   __syncthreads();
   const int d = threadIdx.x % LANES, who = threadIdx.x / LANES;
   float y[R][2] = {};
-  for (int j = 0; j < D; j += 2) {
-    const float p = a.turn[(size_t)j * D + d], p1 = a.turn[(size_t)(j + 1) * D + d];
+  // (short loops: the first workgroups wait for the code as well, and unrolled it was 11 KB and cost 19 us)
+#pragma unroll 1
+  for (int j = 0; j < D; j += 8) {
+    float p[8];                         // (on their way together)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = a.turn[(size_t)(j + e) * D + d];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      y[i][0] = fmaf(p, x[who * R + i][j], y[i][0]);
-      y[i][1] = fmaf(p1, x[who * R + i][j + 1], y[i][1]);
+      const float4 u = *(const float4*)&x[who * R + i][j], v = *(const float4*)&x[who * R + i][j + 4];
+      y[i][0] = fmaf(p[0], u.x, y[i][0]); y[i][1] = fmaf(p[1], u.y, y[i][1]);
+      y[i][0] = fmaf(p[2], u.z, y[i][0]); y[i][1] = fmaf(p[3], u.w, y[i][1]);
+      y[i][0] = fmaf(p[4], v.x, y[i][0]); y[i][1] = fmaf(p[5], v.y, y[i][1]);
+      y[i][0] = fmaf(p[6], v.z, y[i][0]); y[i][1] = fmaf(p[7], v.w, y[i][1]);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const float t = akv_wave_max(fabsf(y[i][0] + y[i][1]));
-    if ((threadIdx.x & 63) == 0) top[who * R + i][(threadIdx.x % LANES) / 64] = t;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int64_t r = r0 + who * R + i;
-    if (r >= rows) break;
-    float t = 0.f;
+  for (int i = 0; i < R; ++i) x[who * R + i][d] = y[i][0] + y[i][1];
+  __syncthreads();
+  // a wavefront a row: scaled so that the largest lies in [2^13, 2^14), and as two terms
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x >> 6; i < 8 && r0 + i < rows; i += 4) {
+    float v[D / 64], t = 0.f;
 #pragma unroll
-    for (int w = 0; w < LANES / 64; ++w) t = fmaxf(t, top[who * R + i][w]);
-    const uint32_t e = akv_row_exponent(t);
-    const float v = (y[i][0] + y[i][1]) * akv_row_scale(e) * 8192.f;      // the largest to [2^13, 2^14)
-    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
-    const int64_t token = r / a.QH, head = r - token * a.QH, to = head / a.G * ((int64_t)(a.t1 - a.t0) * a.G) + token * a.G + head % a.G;
-    a.turned[to * (2 * D) + d] = __builtin_bit_cast(uint16_t, hi);
-    a.turned[to * (2 * D) + D + d] = __builtin_bit_cast(uint16_t, lo);
-    if (d == 0) a.turned_by[to] = akv_row_unscale(e) * (1.f / 8192.f) * a.scale2;
+    for (int e = 0; e < D / 64; ++e) {
+      v[e] = x[i][64 * e + lane];
+      t = fmaxf(t, fabsf(v[e]));
+    }
+    const uint32_t exponent = akv_row_exponent(akv_wave_max(t)), token = (r0 + i) / QH, head = r0 + i - token * QH, kvh = head / G;
+    const int64_t to = (int64_t)kvh * (a.t1 - a.t0) * a.G + (int64_t)token * a.G + (head - kvh * G);
+    const float scale = akv_row_scale(exponent) * 8192.f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const float u = v[e] * scale;
+      const _Float16 hi = (_Float16)u, lo = (_Float16)(u - (float)hi);
+      a.turned[to * (2 * D) + 64 * e + lane] = __builtin_bit_cast(uint16_t, hi);
+      a.turned[to * (2 * D) + D + 64 * e + lane] = __builtin_bit_cast(uint16_t, lo);
+    }
+    if (lane == 0) a.turned_by[to] = akv_row_unscale(exponent) * (1.f / 8192.f) * a.scale2;
   }
 }
 
@@ -300,15 +326,13 @@ template <int KT> __device__ __forceinline__ void kw_row_stats(const ab_f16 (&s)
   if (m != m || m == -INFINITY) m = -INFINITY, l = 0.f;      // (-inf times 0: a row that is none)
 }
 
-// ---- many rows: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
+// ---- many rows over plain keys: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
 // has one barrier.  Workgroups of `splits` take steps in turn.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
   constexpr int ROWS = P::ROWS, RT = P::RT;
   extern __shared__ __align__(16) unsigned char rows[];          // [2][ROWS][ROW]
   __shared__ float2 ml[2][4][ROWS];
-  __shared__ __align__(16) float norms[P::PACKED ? P::N : 4];
-  __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
   const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq), from = part * P::N;
   if (from >= ctx) return;
@@ -321,18 +345,8 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
   kw_stage<D, KIND, ROWS> next(a, R, first, kvh, step);
   next.request(a, R, first, kvh);
   kw_keys<D, KIND> K;
-  float unit = 1.f;
-  if constexpr (P::PACKED) {
-    unit = kw_fill(levels, a.centroids);
-    __syncthreads();
-  }
   const bool any = base < ctx;
-  if (any) K.load(a, seq, kvh, base, ctx, levels.level);
-  if constexpr (P::PACKED) {
-    if (any && h == 0)
-#pragma unroll
-      for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t] * unit;
-  }
+  if (any) K.request(a, seq, kvh, base, ctx);
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
   float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
   // what the wavefronts have of a step's rows, together: four lanes a row, every wavefront a quarter
@@ -359,19 +373,9 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
 #pragma unroll 1
       for (int i = 0; i < RT; ++i) {
         const int row = r0 + 32 * i + col;
-        float c = a.scale2, m, l;
-        if constexpr (P::PACKED) c = a.turned_by[slab + min(row, R.rows - 1)];
+        float m, l;
         ab_f16 s[P::KT];
         K.template products<true>(rows + (ROWS * buf + 32 * i) * P::ROW, s);
-        if constexpr (P::PACKED) {
-#pragma unroll
-          for (int t = 0; t < P::KT; ++t)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const float4 n = *(const float4*)(norms + 32 * (P::KT * wave + t) + 8 * b + 4 * h);
-              s[t][4 * b] *= n.x; s[t][4 * b + 1] *= n.y; s[t][4 * b + 2] *= n.z; s[t][4 * b + 3] *= n.w;
-            }
-        }
         if (base + 32 * P::KT - 1 > kw_pos(a, R, min(r0 + 32 * i, R.rows - 1))) {
           const int pos = row < R.rows ? kw_pos(a, R, row) : -1;
 #pragma unroll
@@ -379,7 +383,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[t][e] = base + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= pos ? s[t][e] : -INFINITY;
         }
-        kw_row_stats<P::KT>(s, c, m, l);
+        kw_row_stats<P::KT>(s, a.scale2, m, l);
         if (h == 0) ml[buf][wave][32 * i + col] = make_float2(m, l);
       }
     } else if (h == 0) {
@@ -394,7 +398,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
 }
 
 // ---- the parts of a row together, a wavefront a row
-template <int N> __global__ __launch_bounds__(256) void kw_join_kernel(kw_args a) {
+__global__ __launch_bounds__(256) void kw_join_kernel(kw_args a, int keys) {
   const int lane = threadIdx.x & 63;
   const int64_t all = (int64_t)(a.t1 - a.t0) * a.G, x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (x >= all * a.KVH) return;
@@ -405,7 +409,7 @@ template <int N> __global__ __launch_bounds__(256) void kw_join_kernel(kw_args a
   const int s1 = ab_start(a.b, seq + 1), pos = ab_ctx(a.b, seq) - (s1 - token);
   if (token >= s1) return;
   float m = -INFINITY, l = 0.f;
-  for (int p = lane; pos >= 0 && p <= pos / N; p += 64) {
+  for (int p = lane; pos >= 0 && p <= pos / keys; p += 64) {
     const float2 e = a.part[((int64_t)p * a.KVH + kvh) * all + row];
     const float top = fmaxf(m, e.x);
     if (top == -INFINITY) continue;
@@ -417,13 +421,52 @@ template <int N> __global__ __launch_bounds__(256) void kw_join_kernel(kw_args a
   if (lane == 0) a.stat[kvh * all + row] = l > 0.f ? make_float2(top, 1.f / l) : make_float2(0.f, 0.f);
 }
 
+// Weights of 32 rows from row0 on, added up for the lane's keys base + 32 t + lane % 32: reference, inverse sum and (packed) scale of each row, from the
+// lane's first one; norms of the keys.
+template <int D, int KIND>
+__device__ __forceinline__ void kw_weights(const kw_args& a, const kw_rows& R, ab_f16 (&s)[kw_plan<D, KIND>::KT], const float* ref, const float* inv, const float* by,
+                                           const float* norm, int row0, int base, float (&w)[kw_plan<D, KIND>::KT]) {
+  typedef kw_plan<D, KIND> P;
+  const int h = (threadIdx.x & 63) >> 5, col = threadIdx.x & 31;
+  if constexpr (P::PACKED) {
+#pragma unroll
+    for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] *= norm[t];
+  }
+  if (base + 32 * P::KT - 1 > kw_pos(a, R, min(row0, R.rows - 1))) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = row0 + 8 * (i >> 2) + 4 * h + (i & 3), pos = row < R.rows ? kw_pos(a, R, row) : 0x7fffffff;      // (rows past the last weigh nothing, and have no scale)
+#pragma unroll
+      for (int t = 0; t < P::KT; ++t) s[t][i] = base + 32 * t + col <= pos ? s[t][i] : -INFINITY;
+    }
+  }
+  float sum[P::KT][4] = {};
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const float4 m4 = *(const float4*)(ref + 8 * b), i4 = *(const float4*)(inv + 8 * b);
+    float c[4] = {a.scale2, a.scale2, a.scale2, a.scale2};
+    if constexpr (P::PACKED) {
+      const float4 x = *(const float4*)(by + 8 * b);
+      c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
+    }
+    const float m[4] = {m4.x, m4.y, m4.z, m4.w}, iv[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < P::KT; ++t) sum[t][j] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][4 * b + j], c[j], -m[j])), iv[j], sum[t][j]);
+  }
+#pragma unroll
+  for (int t = 0; t < P::KT; ++t) w[t] += (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]);
+}
+
 // ---- weights of a part's keys, summed over the rows; steps as above.  Workgroups that share a part leave their sums to kw_add_kernel.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
   constexpr int ROWS = P::ROWS, RT = P::RT;
   extern __shared__ __align__(16) unsigned char rows[];          // [2][ROWS][ROW]
-  __shared__ __align__(16) float ref[2][ROWS], inv[2][ROWS], by[2][ROWS];
-  __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
+  __shared__ __align__(16) float ref[2][ROWS], inv[2][ROWS];
   const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t from = (int64_t)part * P::N;
@@ -441,13 +484,10 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kern
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
   kw_stage<D, KIND, ROWS> next(a, R, first, kvh, step);
   float2 e = make_float2(0.f, 0.f);
-  float c = 0.f;
   auto request = [&](int r0) {
     next.request(a, R, r0, kvh);
     if (tid < ROWS) {
-      const bool there = r0 + tid < R.rows;
-      e = there ? a.stat[slab + r0 + tid] : make_float2(0.f, 0.f);
-      if constexpr (P::PACKED) c = there ? a.turned_by[slab + r0 + tid] : 0.f;
+      e = r0 + tid < R.rows ? a.stat[slab + r0 + tid] : make_float2(0.f, 0.f);
     }
   };
   auto put = [&](int buf) {
@@ -455,22 +495,12 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kern
     if (tid < ROWS) {
       ref[buf][tid] = e.x;
       inv[buf][tid] = e.y;
-      if constexpr (P::PACKED) by[buf][tid] = c;
     }
   };
   request(first);
   kw_keys<D, KIND> K;
-  float unit = 1.f;
-  if constexpr (P::PACKED) {
-    unit = kw_fill(levels, a.centroids);
-    __syncthreads();
-  }
   const bool any = base < ctx;
-  if (any) K.load(a, seq, kvh, base, ctx, levels.level);
-  if constexpr (P::PACKED) {
-#pragma unroll
-    for (int t = 0; t < P::KT; ++t) K.norm[t] *= unit;
-  }
+  if (any) K.request(a, seq, kvh, base, ctx);
   float w[P::KT] = {};
   put(0);
   int buf = 0;
@@ -482,39 +512,11 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_sum_kern
 #pragma unroll 1
       for (int i = 0; i < RT; ++i) {
         const int row0 = r0 + 32 * i;
-        const bool edge = base + 32 * P::KT - 1 > kw_pos(a, R, min(row0, R.rows - 1));
         ab_f16 s[P::KT];
         K.template products<false>(rows + (ROWS * buf + 32 * i) * P::ROW, s);
-        // what makes a score of a product: by row, packed by key and row
-        auto weights = [&](auto masked) {
-          float sum[P::KT][4] = {};
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int at = 32 * i + 8 * b + 4 * h;
-            const float4 m4 = *(const float4*)(ref[buf] + at), i4 = *(const float4*)(inv[buf] + at);
-            float c[4] = {a.scale2, a.scale2, a.scale2, a.scale2};
-            if constexpr (P::PACKED) {
-              const float4 x = *(const float4*)(by[buf] + at);
-              c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
-            }
-            const float m[4] = {m4.x, m4.y, m4.z, m4.w}, iv[4] = {i4.x, i4.y, i4.z, i4.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              int pos = 0;
-              if constexpr (masked.value) pos = kw_pos(a, R, row0 + 8 * b + 4 * h + j);
-#pragma unroll
-              for (int t = 0; t < P::KT; ++t) {
-                float x = __builtin_amdgcn_exp2f(fmaf(P::PACKED ? s[t][4 * b + j] * K.norm[t] : s[t][4 * b + j], c[j], -m[j]));
-                if constexpr (masked.value) x = base + 32 * t + col <= pos ? x : 0.f;
-                sum[t][j] = fmaf(x, iv[j], sum[t][j]);
-              }
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < P::KT; ++t) w[t] += (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]);
-        };
-        if (edge) weights(std::true_type{});
-        else weights(std::false_type{});
+        const float* rf = ref[buf] + 32 * i + 4 * h;
+        const float* iv = inv[buf] + 32 * i + 4 * h;
+        kw_weights<D, KIND>(a, R, s, rf, iv, nullptr, nullptr, row0, base, w);
       }
     }
     if (!more) break;
@@ -540,6 +542,168 @@ __global__ __launch_bounds__(256) void kw_add_kernel(kw_args a) {
   float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head + key;
   if (!a.add) *to = sum;
   else if (key < ab_ctx(a.b, seq)) *to += sum;
+}
+
+// ---- many rows over packed keys: a block of rows stays in LDS while the wavefronts walk through `runs` x N keys, each by itself, the next codes on their
+// way: codes are a quarter of the keys' bytes and cost more to turn into levels than to read again for the next block of rows.
+template <int D> struct kw_block { static constexpr int ROWS = D == 256 ? 64 : 128; };
+// rows r0 .. into LDS, those past the last as zeros
+template <int D, int KIND> __device__ __forceinline__ void kw_put_block(const kw_args& a, const kw_rows& R, int r0, int kvh, unsigned char* rows) {
+  typedef kw_plan<D, KIND> P;
+  constexpr int ROWS = kw_block<D>::ROWS, LOADS = ROWS * P::CHUNKS / 256, AT_ONCE = 256 / P::CHUNKS;
+  const int r = (int)threadIdx.x / P::CHUNKS, c = 16 * ((int)threadIdx.x % P::CHUNKS);
+  const uint8_t* p = (const uint8_t*)a.turned + kw_slab_row(a, R, kvh, r0 + r) * P::BYTES + c;
+#pragma unroll
+  for (int i0 = 0; i0 < LOADS; i0 += 8) {
+    ab_u4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r0 + AT_ONCE * (i0 + i) + r < R.rows ? *(const ab_u4*)(p + (int64_t)(AT_ONCE * (i0 + i)) * P::BYTES) : (ab_u4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *(ab_u4*)(rows + (AT_ONCE * (i0 + i) + r) * P::ROW + c) = v[i];
+  }
+}
+template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_stats_kernel(kw_args a) {
+  typedef kw_plan<D, KIND> P;
+  constexpr int ROWS = kw_block<D>::ROWS;
+  constexpr bool AHEAD = D < 256;       // (the next codes have registers)
+  extern __shared__ __align__(16) unsigned char rows[];          // [ROWS][ROW]
+  __shared__ float2 ml[4][ROWS];
+  __shared__ float by[ROWS];
+  __shared__ __align__(16) float norms[P::N];
+  __shared__ kw_levels<KIND> levels;
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int ctx = ab_ctx(a.b, seq);
+  const int64_t from64 = (int64_t)part * P::N * a.runs;
+  if (from64 >= ctx) return;
+  const int from = (int)from64;
+  const kw_rows R = kw_rows_of(a, seq, ctx);
+  if (R.rows == 0 || kw_pos(a, R, R.rows - 1) < from) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
+  const float unit = kw_fill(levels, a.centroids);
+  const int64_t slab = kw_slab_row(a, R, kvh, 0);
+  float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
+  for (int r0 = 0; r0 < R.rows; r0 += ROWS) {
+    const int count = min(ROWS, R.rows - r0), last = kw_pos(a, R, r0 + count - 1), end = min(from + P::N * a.runs, last + 1);
+    if (last < from) continue;
+    kw_keys<D, KIND> K;
+    int base = from + 32 * P::KT * wave;
+    if (AHEAD && base < end) K.request(a, seq, kvh, base, ctx);
+    __syncthreads();                   // (the block before has been read)
+    kw_put_block<D, KIND>(a, R, r0, kvh, rows);
+    if (tid < ROWS) by[tid] = tid < count ? a.turned_by[slab + r0 + tid] : 0.f;
+    for (int i = lane; i < ROWS; i += 64) ml[wave][i] = make_float2(-INFINITY, 0.f);
+    __syncthreads();
+    for (; base < end; base += P::N) {
+      if (!AHEAD) K.request(a, seq, kvh, base, ctx);
+      K.decode(levels.level, unit);
+      akv_wave_sync();
+      if (h == 0)
+#pragma unroll
+        for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t];
+      akv_wave_sync();
+      if (AHEAD && base + P::N < end) K.request(a, seq, kvh, base + P::N, ctx);
+#pragma unroll 1
+      for (int i = 0; i < count; i += 32) {
+        if (kw_pos(a, R, min(r0 + i + 31, R.rows - 1)) < base) continue;
+        ab_f16 s[P::KT];
+        K.template products<true>(rows + i * P::ROW, s);
+#pragma unroll
+        for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float4 n = *(const float4*)(norms + 32 * (P::KT * wave + t) + 8 * b + 4 * h);
+            s[t][4 * b] *= n.x; s[t][4 * b + 1] *= n.y; s[t][4 * b + 2] *= n.z; s[t][4 * b + 3] *= n.w;
+          }
+        if (base + 32 * P::KT - 1 > kw_pos(a, R, r0 + i)) {
+          const int pos = i + col < count ? kw_pos(a, R, r0 + i + col) : -1;
+#pragma unroll
+          for (int t = 0; t < P::KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[t][e] = base + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) <= pos ? s[t][e] : -INFINITY;
+        }
+        float m, l;
+        kw_row_stats<P::KT>(s, by[i + col], m, l);
+        const float2 old = ml[wave][i + col];
+        const float top = fmaxf(old.x, m), ref = top == -INFINITY ? 0.f : top;
+        l = old.y * __builtin_amdgcn_exp2f(old.x - ref) + l * __builtin_amdgcn_exp2f(m - ref);
+        if (h == 0) ml[wave][i + col] = make_float2(top, l);
+      }
+    }
+    __syncthreads();
+    if (tid < count) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][tid].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += ml[w][tid].x == -INFINITY ? 0.f : ml[w][tid].y * __builtin_amdgcn_exp2f(ml[w][tid].x - top);
+      to[r0 + tid] = make_float2(top, sum);
+    }
+  }
+}
+template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_sum_kernel(kw_args a) {
+  typedef kw_plan<D, KIND> P;
+  constexpr int ROWS = kw_block<D>::ROWS;
+  constexpr bool AHEAD = D < 256;       // (the next codes have registers)
+  extern __shared__ __align__(16) unsigned char rows[];          // [ROWS][ROW]
+  __shared__ __align__(16) float ref[ROWS], inv[ROWS], by[ROWS];
+  __shared__ kw_levels<KIND> levels;
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int ctx = ab_ctx(a.b, seq);
+  const int64_t from = (int64_t)part * P::N * a.runs;
+  const kw_rows R = kw_rows_of(a, seq, ctx);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
+  float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head;
+  if (from >= ctx || R.rows == 0 || kw_pos(a, R, R.rows - 1) < from) {
+    if (!a.add)
+      for (int64_t i = from + tid; i < from + P::N * a.runs && i < a.length; i += 256) to[i] = 0.f;
+    return;
+  }
+  const float unit = kw_fill(levels, a.centroids);
+  const int64_t slab = kw_slab_row(a, R, kvh, 0);
+  bool add = a.add;                     // (the first block that sees something of the keys writes, the others add)
+  for (int r0 = 0; r0 < R.rows; r0 += ROWS) {
+    const int count = min(ROWS, R.rows - r0), last = kw_pos(a, R, r0 + count - 1);
+    if (last < from) continue;
+    kw_keys<D, KIND> K;
+    int base = (int)from + 32 * P::KT * wave;
+    const int64_t behind = min(from + P::N * a.runs, a.length);
+    if (AHEAD && base <= last) K.request(a, seq, kvh, base, ctx);
+    __syncthreads();                   // (the block before has been read)
+    kw_put_block<D, KIND>(a, R, r0, kvh, rows);
+    if (tid < ROWS) {
+      const float2 e = tid < count ? a.stat[slab + r0 + tid] : make_float2(0.f, 0.f);
+      ref[tid] = e.x;
+      inv[tid] = e.y;
+      by[tid] = tid < count ? a.turned_by[slab + r0 + tid] : 0.f;
+    }
+    __syncthreads();
+    for (; base < behind; base += P::N) {
+      float w[P::KT] = {};
+      if (base <= last) {
+        if (!AHEAD) K.request(a, seq, kvh, base, ctx);
+        K.decode(levels.level, unit);
+        if (AHEAD && base + P::N <= last && base + P::N < behind) K.request(a, seq, kvh, base + P::N, ctx);
+#pragma unroll 1
+        for (int i = 0; i < count; i += 32) {
+          if (kw_pos(a, R, min(r0 + i + 31, R.rows - 1)) < base) continue;
+          ab_f16 s[P::KT];
+          K.template products<false>(rows + i * P::ROW, s);
+          const int at = i + 4 * h;
+          kw_weights<D, KIND>(a, R, s, ref + at, inv + at, by + at, K.norm, r0 + i, base, w);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < P::KT; ++t) {
+        const float sum = w[t] + akv_lane_xor<32>(w[t]);
+        const int64_t key = (int64_t)base + 32 * t + col;
+        if (h == 0 && key < a.length) {
+          if (!add) to[key] = key < ctx ? sum : 0.f;
+          else if (key <= last) to[key] += sum;
+        }
+      }
+    }
+    add = true;
+  }
 }
 
 // ---- few rows a sequence: keys are read once, as long as a sequence and kv head has no more rows than a tile; scores are kept, four bytes a row and
@@ -580,18 +744,19 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kern
     kw_keys<D, KIND> K;
     const int end = min(from + P::N * a.runs, last + 1);         // keys that some row sees
     int base = from + 32 * P::KT * wave;
-    if (base < end) K.load(a, seq, kvh, base, ctx, levels.level);
+    if (base < end) K.request(a, seq, kvh, base, ctx);
     for (; base < end; base += P::N) {
       if constexpr (P::PACKED) {
+        K.decode(levels.level, unit);
         akv_wave_sync();
         if (h == 0)
 #pragma unroll
-          for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t] * unit;
+          for (int t = 0; t < P::KT; ++t) norms[32 * (P::KT * wave + t) + col] = K.norm[t];
         akv_wave_sync();
       }
       ab_f16 s[P::KT];
       K.template products<true>(rows, s);
-      if (base + P::N < end) K.load(a, seq, kvh, base + P::N, ctx, levels.level);
+      if (base + P::N < end) K.request(a, seq, kvh, base + P::N, ctx);
       const bool edge = __ballot(base + 32 * P::KT - 1 > pos && valid) != 0;
 #pragma unroll
       for (int t = 0; t < P::KT; ++t) {
@@ -691,14 +856,14 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   kw_scratch w = {};
   w.few = T * (QH / KVH) <= (int64_t)KW_FEW * S;
   w.stride = (length + keys * 4 - 1) / (keys * 4) * (keys * 4);
-  // runs of keys a workgroup: as many as leave four workgroups a CU
+  // runs of keys a workgroup: as many as leave forty workgroups a CU, over packed keys, whose rows have to come to LDS first, four
   w.runs = 4;
-  while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < 4 * ab_cus()) w.runs /= 2;
+  while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < (w.few ? 40 : 4) * ab_cus()) w.runs /= 2;
   w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
-  w.parts = w.few ? 0 : (int)((length + keys - 1) / keys);
+  w.parts = w.few ? 0 : packed ? (int)(w.stride / (keys * w.runs)) : (int)((length + keys - 1) / keys);
   // workgroups that share the rows of a part: as many as give every CU two
   w.splits = 1;
-  while (!w.few && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
+  while (!w.few && !packed && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
   const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
   w.tokens = KW_SCRATCH / per / 32 * 32;
   if (w.tokens < 32) w.tokens = 32;
@@ -714,7 +879,7 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   w.bytes = w.sums + (w.splits > 1 ? akv_align256((size_t)w.splits * S * KVH * length * 4) : 0);
   return w;
 }
-static inline int kw_part(int D, bool packed) { return D * (packed ? 2 : 1) <= 128 ? 256 : 128; }
+static inline int kw_part(int D, bool packed) { return !packed && D <= 128 ? 256 : 128; }
 static inline size_t kw_bytes(int64_t T, int S, int QH, int KVH, int D, bool packed, int64_t length) {
   return T <= 0 || S <= 0 || QH <= 0 || KVH <= 0 || length <= 0 || !ab_head_size(D) ? 0 : kw_layout(T, S, QH, KVH, D, packed, kw_part(D, packed), length).bytes;
 }
@@ -723,7 +888,7 @@ extern "C" size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int
 
 template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scratch, hipStream_t stream) {
   typedef kw_plan<D, KIND> P;
-  static_assert(P::N == (D * P::TERMS <= 128 ? 256 : 128), "kw_part");
+  static_assert(P::N == (!P::PACKED && D <= 128 ? 256 : 128), "kw_part");
   const kw_scratch w = kw_layout(T, a.b.S, a.QH, a.KVH, D, P::PACKED, P::N, a.length);
   char* const at = (char*)scratch;
   a.stat = (float2*)(at + w.stat);
@@ -739,13 +904,18 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
   static akv_device_once once;
+  constexpr int LDS = P::PACKED ? kw_block<D>::ROWS * P::ROW : P::LDS;
   if (const int rc = once(dev, [&]() -> int {
-        const int rc1 = ab_lds((const void*)kw_stats_kernel<D, KIND>, P::LDS);
-        return rc1 ? rc1 : ab_lds((const void*)kw_sum_kernel<D, KIND>, P::LDS);
+        const void *one, *two;
+        if constexpr (P::PACKED) one = (const void*)kw_packed_stats_kernel<D, KIND>, two = (const void*)kw_packed_sum_kernel<D, KIND>;
+        else one = (const void*)kw_stats_kernel<D, KIND>, two = (const void*)kw_sum_kernel<D, KIND>;
+        const int rc1 = ab_lds(one, LDS);
+        return rc1 ? rc1 : ab_lds(two, LDS);
       }))
     return rc;
   const int add = a.add;
-  const dim3 grid((uint32_t)((a.length + P::N - 1) / P::N * w.splits), (uint32_t)a.KVH, (uint32_t)a.b.S);
+  const int keys = P::PACKED ? P::N * w.runs : P::N;
+  const dim3 grid((uint32_t)((a.length + keys - 1) / keys * w.splits), (uint32_t)a.KVH, (uint32_t)a.b.S);
   int64_t t = 0;
   do {                                  // (without a token: zeros)
     a.t0 = (int)t;
@@ -761,9 +931,10 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
         kw_few_kernel<D, KIND><<<dim3((uint32_t)w.few_parts, (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_few_kernel");
       } else {
-        kw_stats_kernel<D, KIND><<<grid, 256, P::LDS, stream>>>(a);
+        if constexpr (P::PACKED) kw_packed_stats_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
+        else kw_stats_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_stats_kernel");
-        kw_join_kernel<P::N><<<(uint32_t)((rows + 3) / 4), 256, 0, stream>>>(a);
+        kw_join_kernel<<<(uint32_t)((rows + 3) / 4), 256, 0, stream>>>(a, keys);
         AKV_LAUNCH_CHECK("kw_join_kernel");
       }
     }
@@ -771,7 +942,8 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
       kw_few_sum_kernel<<<dim3((uint32_t)((a.length + KW_FEW_KEYS - 1) / KW_FEW_KEYS), (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a, P::N * w.runs);
       AKV_LAUNCH_CHECK("kw_few_sum_kernel");
     } else {
-      kw_sum_kernel<D, KIND><<<grid, 256, P::LDS, stream>>>(a);
+      if constexpr (P::PACKED) kw_packed_sum_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
+      else kw_sum_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
       AKV_LAUNCH_CHECK("kw_sum_kernel");
       if (w.splits > 1) {
         kw_add_kernel<<<dim3((uint32_t)((a.length + 255) / 256), (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a);
