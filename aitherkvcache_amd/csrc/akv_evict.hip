@@ -22,12 +22,22 @@ __device__ __forceinline__ uint32_t ev_order(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// One workgroup of 16 wavefronts a (kv head, sequence), each of which takes a run of the positions, NR of every lane in registers (NR = 0: read
-// again and again).  The keep-th largest order is found by halving its range, bit by bit; what is above it stays, and the first ones that equal it.
+// One workgroup of 16 wavefronts a (kv head, sequence), each of which takes a run of the positions.  Orders lie in LDS (where they fit, otherwise they are
+// made again from the weights).  The keep-th largest is found eight bits at a time, from the highest in which the orders differ: a histogram of
+// the next eight bits of those that share the bits known so far.  What is above it stays, and the first ones that equal it.
+//
+// Few workgroups have much to do here, so that each waits for its code too: the loops are short.  Weights are alike in their upper bits, so that counters have
+// copies; when few share the known bits they are listed, and later levels read the list alone.  8 heads of 32768 positions take 32 us: a bit at a time with
+// orders in registers 42, one copy of a counter and no list 36.  16 sequences of 8 heads of 8192 take 16 us, and took 57 with registers.
 #define EV_THREADS 1024
-template <int NR> __global__ __launch_bounds__(EV_THREADS) void ev_select_kernel(ev_args a) {
+#define EV_HELD 32768                   // orders in LDS
+#define EV_COPIES 16                    // of a counter: weights are alike, and lanes that add to one word wait for each other
+#define EV_LIST 2048                    // those that share the known bits, once they are few
+__global__ __launch_bounds__(EV_THREADS) void ev_select_kernel(ev_args a, int room) {
   constexpr int WAVES = EV_THREADS / 64;
-  __shared__ int sums[2][WAVES], ties[WAVES];
+  static_assert(256 * EV_COPIES == 4 * EV_THREADS && EV_COPIES == 16, "counters");
+  extern __shared__ uint32_t orders[];   // [room], then the list
+  __shared__ __attribute__((aligned(16))) int hist[256 * EV_COPIES], sums[WAVES], ties[WAVES], found[3], listed;
   const int kvh = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = ab_clamp(akv_load_index(a.lens, a.lens_it, seq), a.length);
   const float* w = a.w + (int64_t)seq * a.ws_seq + (int64_t)kvh * a.ws_head;
@@ -38,74 +48,199 @@ template <int NR> __global__ __launch_bounds__(EV_THREADS) void ev_select_kernel
     if (a.lens_it == AKV_I64) ((int64_t*)a.out_lens)[seq] = stay;
     else ((int32_t*)a.out_lens)[seq] = stay;
   }
-  for (int i = stay + tid; i < a.keep; i += EV_THREADS) kept[i] = -1;
-  for (int64_t i = stay + tid; i < a.length; i += EV_THREADS) out[i] = 0.f;
+  // zeros behind
+  const int64_t even = min(a.length, stay + (int64_t)(-((int64_t)((uintptr_t)(out + stay) >> 2)) & 3));      // from here on sixteen bytes at a time
+  if (tid < even - stay) out[stay + tid] = 0.f;
+  for (int64_t i = even + 4 * tid; i < a.length; i += 4 * EV_THREADS) {
+    if (i + 3 < a.length) *(ab_f4*)(out + i) = (ab_f4){0.f, 0.f, 0.f, 0.f};
+    else
+      for (int64_t k = i; k < a.length; ++k) out[k] = 0.f;
+  }
   if (n <= a.keep) {
-    for (int i = tid; i < n; i += EV_THREADS) {
-      kept[i] = i;
-      out[i] = w[i];
+    for (int i = tid; i < a.keep; i += EV_THREADS) {
+      kept[i] = i < n ? i : -1;
+      if (i < n) out[i] = w[i];
     }
     return;
   }
-  const int each = (n + EV_THREADS - 1) / EV_THREADS, first = wave * each * 64;      // positions of a lane; of the wavefront the first
-  auto order = [&](int i) { return i >= n ? 0u : i < a.sinks || i >= n - a.recent ? 0xffffffffu : ev_order(w[i]); };
-  uint32_t held[NR > 0 ? NR : 1];
+  const bool held = n <= room, wide = ((uintptr_t)w & 15) == 0;
+  // orders of four positions i .. i + 3 (0 past the last); what stays anyway is above all others
+  auto rank = [&](int i, float x) { return i >= n ? 0u : i < a.sinks || i >= n - a.recent ? 0xffffffffu : ev_order(x); };
+  auto weights = [&](int i) {
+    if (wide && i + 3 < n) return *(const ab_f4*)(w + i);
+    ab_f4 x;
 #pragma unroll
-  for (int c = 0; c < NR; ++c) held[c] = c < each ? order(first + 64 * c + lane) : 0u;
-  auto count = [&](auto test) {           // lanes of the wavefront's positions that pass
-    int k = 0;
-    if constexpr (NR > 0) {
-#pragma unroll
-      for (int c = 0; c < NR; ++c) k += __popcll(__ballot(test(held[c])));
-    } else {
-      for (int c = 0; c < each; ++c) k += __popcll(__ballot(test(order(first + 64 * c + lane))));
-    }
-    return k;
+    for (int k = 0; k < 4; ++k) x[k] = w[min(i + k, n - 1)];
+    return x;
   };
-  uint32_t t = 0u;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | 1u << bit;
-    const int mine = count([&](uint32_t o) { return o >= c; });
-    if (lane == 0) sums[bit & 1][wave] = mine;
-    __syncthreads();
-    int all = 0;
+  auto made = [&](int i) {
+    const ab_f4 x = weights(i);
+    ab_u4 o;
 #pragma unroll
-    for (int v = 0; v < WAVES; ++v) all += sums[bit & 1][v];
-    if (all >= a.keep) t = c;
-    if (all == a.keep) break;             // (the same in every thread)
+    for (int k = 0; k < 4; ++k) o[k] = rank(i + k, x[k]);
+    return o;
+  };
+  auto order = [&](int i) { return held ? *(const ab_u4*)(orders + i) : made(i); };
+  constexpr int ROUND = 4 * EV_THREADS;
+  const int rounds = (n + ROUND - 1) / ROUND;
+  // the bits that all others share: those above the highest in which some differ
+  uint32_t both = 0xffffffffu, any = 0u;
+  for (int r = 0; r < rounds; r += 4) {
+    ab_f4 x[4];                         // (on their way together)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = weights(min((r + q) * ROUND + 4 * tid, (n - 1) & ~3));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (r + q >= rounds) break;
+      const int i = (r + q) * ROUND + 4 * tid;
+      ab_u4 o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[k] = rank(i + k, x[q][k]);
+        both &= o[k] + 1u > 1u ? o[k] : 0xffffffffu;
+        any |= o[k] + 1u > 1u ? o[k] : 0u;
+      }
+      if (held) *(ab_u4*)(orders + i) = o;
+    }
   }
-  // (order 0 is no position's: t > 0)
-  const int above = count([&](uint32_t o) { return o > t; }), tied = count([&](uint32_t o) { return o == t; });
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) {
+    both &= __shfl_xor(both, m, 64);
+    any |= __shfl_xor(any, m, 64);
+  }
+  if (lane == 0) {
+    sums[wave] = (int)both;
+    ties[wave] = (int)any;
+  }
+  __syncthreads();
+  for (int v = 0; v < WAVES; ++v) {
+    both &= (uint32_t)sums[v];
+    any |= (uint32_t)ties[v];
+  }
+  int need = a.keep - a.sinks - a.recent;      // how many of those that share the known bits stay
+  int unknown = any > both ? 32 - __clz(any ^ both) : 0, sharing = n - a.sinks - a.recent;
+  // the threshold, as far as it is known
+  uint32_t t = need == 0 ? 0xffffffffu : unknown == 32 ? 0u : both >> unknown << unknown;
+  if (need == 0) sharing = unknown = 0;
+  uint32_t* const list = orders + room;
+  bool gathered = false;
+  int in_list = 0;
+  while (unknown > 0 && need != sharing) {     // (all that share the bits stay: the search is over)
+    const int width = min(8, unknown), shift = unknown - width;
+    __syncthreads();
+    *(ab_u4*)(hist + 4 * tid) = (ab_u4){0u, 0u, 0u, 0u};
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    const uint32_t range = unknown == 32 ? 0xffffffffu : (1u << unknown) - 1;
+    auto take = [&](uint32_t o) { atomicAdd(hist + (o >> shift & ((1u << width) - 1)) * EV_COPIES + (lane & (EV_COPIES - 1)), 1); };
+    auto shares = [&](uint32_t o) { return (o ^ t) <= range && o + 1u > 1u; };      // (neither what stays anyway nor what is past the last)
+    if (gathered) {
+      for (int i = tid; i < in_list; i += EV_THREADS)
+        if (shares(list[i])) take(list[i]);
+    } else {
+      const bool gather = unknown < 32 && sharing <= EV_LIST;
+#pragma unroll 2
+      for (int r = 0; r < rounds; ++r) {
+        const ab_u4 o = order(r * ROUND + 4 * tid);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (shares(o[k])) {
+            take(o[k]);
+            if (gather) list[min(atomicAdd(&listed, 1), EV_LIST - 1)] = o[k];
+          }
+      }
+      gathered = gather;
+      in_list = sharing;
+    }
+    __syncthreads();
+    {
+      // copies together: four of them a thread, a counter four threads
+      const ab_u4 x = *(const ab_u4*)(hist + 4 * tid);
+      int sum = (int)(x[0] + x[1] + x[2] + x[3]);
+      sum += __shfl_xor(sum, 1, 64);
+      sum += __shfl_xor(sum, 2, 64);
+      __syncthreads();
+      if ((tid & 3) == 0) hist[tid >> 2] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // a lane four values, the first lane the uppermost
+      const int* h = hist + 252 - 4 * lane;
+      const int c[4] = {h[3], h[2], h[1], h[0]}, sum = c[0] + c[1] + c[2] + c[3], inc = akv_wave_inclusive_scan(sum);
+      int before = inc - sum;
+      if (before < need && need <= inc) {
+        int i = 0;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (i == k && before + c[k] < need) before += c[k], ++i;
+        found[0] = 255 - 4 * lane - i;
+        found[1] = need - before;
+        found[2] = i == 0 ? c[0] : i == 1 ? c[1] : i == 2 ? c[2] : c[3];
+      }
+    }
+    __syncthreads();
+    t |= (uint32_t)found[0] << shift;
+    need = found[1];
+    sharing = found[2];
+    unknown = shift;
+  }
+  // (where the search ended early everything from t on stays, and nothing has to be counted as equal)
+  const bool exact = need != sharing;
+  const uint32_t from = exact ? t + 1 : t;     // what stays whatever is equal (with need > 0 t is below 0xffffffff)
+  const int each = (rounds * ROUND) / WAVES, first = wave * each;      // the wavefront's run of positions
+  int above = 0, tied = 0;
+  for (int i = first; i < first + each; i += 256) {
+    const ab_u4 o = order(i + 4 * lane);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      above += o[k] >= from;
+      tied += exact && o[k] == t;
+    }
+  }
+  above = akv_wave_sum(above);
+  tied = akv_wave_sum(tied);
   __syncthreads();
   if (lane == 0) {
-    sums[0][wave] = above;
+    sums[wave] = above;
     ties[wave] = tied;
   }
   __syncthreads();
-  int all = 0, before = 0, tied_before = 0;
-  for (int v = 0; v < WAVES; ++v) {
-    all += sums[0][v];
-    if (v < wave) before += sums[0][v], tied_before += ties[v];
+  int at = 0, equal = exact ? need : 0;
+  for (int v = 0; v < wave; ++v) {
+    at += sums[v] + min(equal, ties[v]);
+    equal -= min(equal, ties[v]);
   }
-  int equal = max(0, a.keep - all - tied_before), at = before + min(a.keep - all, tied_before);
-  const uint64_t below = (1ull << lane) - 1;
-  auto put = [&](int c, uint32_t o) {
-    const uint64_t same = __ballot(o == t);
-    const bool take = o > t || (o == t && __popcll(same & below) < equal);
-    const uint64_t taken = __ballot(take);
-    if (take) {
-      const int i = first + 64 * c + lane, to = at + __popcll(taken & below);
-      kept[to] = i;
-      out[to] = w[i];
-    }
-    at += __popcll(taken);
-    equal -= min(equal, (int)__popcll(same));
-  };
-  if constexpr (NR > 0) {
+  for (int i0 = first; i0 < first + each && i0 < n; i0 += 256) {
+    const int i = i0 + 4 * lane;
+    const ab_u4 o = order(i);
+    int left = 0;                       // equal ones that the lanes before leave
+    if (exact) {
+      int mine = 0;
 #pragma unroll
-    for (int c = 0; c < NR; ++c) put(c, held[c]);
-  } else {
-    for (int c = 0; c < each; ++c) put(c, order(first + 64 * c + lane));
+      for (int k = 0; k < 4; ++k) mine += o[k] == t;
+      const int inc = akv_wave_inclusive_scan(mine);
+      left = equal - (inc - mine);
+      equal -= min(equal, __builtin_amdgcn_readlane(inc, 63));
+    }
+    uint32_t take = 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool same = exact && o[k] == t;
+      take |= (uint32_t)(o[k] >= from || (same && left > 0)) << k;
+      left -= same;
+    }
+    const int mine = __popc(take), inc = akv_wave_inclusive_scan(mine);
+    int to = at + inc - mine;
+    at += __builtin_amdgcn_readlane(inc, 63);
+    // the weight from its order, but where that does not tell (a weight read again is waited for)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (!(take >> k & 1)) continue;
+      float x = __uint_as_float(o[k] ^ ((o[k] >> 31) ? 0x80000000u : 0xffffffffu));
+      if (o[k] == 0xffffffffu || o[k] == 0x80000000u || o[k] == 0x007fffffu) x = w[i + k];
+      kept[to] = i + k;
+      out[to++] = x;
+    }
   }
 }
 
@@ -124,11 +259,12 @@ extern "C" int akv_evict_select(const float* weights, int64_t ws_seq, int64_t ws
   a.w = weights; a.ws_seq = ws_seq; a.ws_head = ws_head; a.lens = context_lens; a.lens_it = cl_itype;
   a.kept = kept; a.ks_seq = ks_seq; a.ks_head = ks_head; a.out = kept_weights; a.os_seq = os_seq; a.os_head = os_head; a.out_lens = kept_lens;
   a.length = length; a.keep = keep; a.sinks = num_sink; a.recent = num_recent;
-  const dim3 grid((uint32_t)num_kv_heads, (uint32_t)num_seqs);
-  const hipStream_t s = (hipStream_t)stream;
-  if (length <= 8 * EV_THREADS) ev_select_kernel<8><<<grid, EV_THREADS, 0, s>>>(a);
-  else if (length <= 32 * EV_THREADS) ev_select_kernel<32><<<grid, EV_THREADS, 0, s>>>(a);
-  else ev_select_kernel<0><<<grid, EV_THREADS, 0, s>>>(a);
+  int dev = 0;
+  AKV_HIP(hipGetDevice(&dev));
+  static akv_device_once once;
+  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)ev_select_kernel, 4 * (EV_HELD + EV_LIST)); })) return rc;
+  const int room = (int)(length < EV_HELD ? (length + 4095) / 4096 * 4096 : EV_HELD);      // (whole rounds of the kernel)
+  ev_select_kernel<<<dim3((uint32_t)num_kv_heads, (uint32_t)num_seqs), EV_THREADS, 4 * (size_t)(room + EV_LIST), (hipStream_t)stream>>>(a, room);
   AKV_LAUNCH_CHECK("ev_select_kernel");
   return AKV_OK;
 }
@@ -137,15 +273,15 @@ extern "C" int akv_evict_select(const float* weights, int64_t ws_seq, int64_t ws
 #define EV_CACHES AKV_EVICT_CACHES
 struct ev_cache {
   uint8_t* p; int64_t blk, pos, head;   // bytes
-  int units, log;                       // of a row: pieces of 2^log bytes
-  int slice, first;                     // pieces of a slice; number of the cache's first slice or piece
+  int units, log, per;                  // of a row: units of 2^log bytes; units of a piece
+  int pieces, slice, first;             // of a row; pieces of a slice; number of the cache's first slice or piece
 };
 struct ev_move_args {
   ab_batch b;                           // lens: tokens that stay
   const void* to_tables; int to_it; int64_t to_stride, to_blocks;
   const int32_t* kept; int64_t ks_seq, ks_head;
   ev_cache c[EV_CACHES];
-  int caches, keep, pieces;
+  int caches, keep, pieces, heads;      // pieces: of a token and head
 };
 struct ev_row { int64_t blk; uint32_t pos; };
 __device__ __forceinline__ ev_row ev_row_of(const ev_move_args& a, int seq, int position, bool to) {
@@ -157,72 +293,87 @@ __device__ __forceinline__ ev_row ev_row_of(const ev_move_args& a, int seq, int 
 __device__ __forceinline__ uint8_t* ev_at(const ev_cache& c, ev_row r, int head, int unit) {
   return c.p + r.blk * c.blk + (int64_t)r.pos * c.pos + (int64_t)head * c.head + ((int64_t)unit << c.log);
 }
+// up to sixteen bytes, as units of 2^log bytes
 struct ev_piece { ab_u4 v; };
-__device__ __forceinline__ void ev_load(ev_piece& x, const uint8_t* p, int log) {
+struct __attribute__((packed, aligned(4))) ev_words { uint32_t v[4]; };
+__device__ __forceinline__ void ev_load(ev_piece& x, const uint8_t* p, int log, int units) {
   if (log == 4) x.v = *(const ab_u4*)p;
-  else if (log == 3) { const ab_u2 y = *(const ab_u2*)p; x.v[0] = y[0]; x.v[1] = y[1]; }
-  else if (log == 2) x.v[0] = *(const uint32_t*)p;
-  else if (log == 1) x.v[0] = *(const uint16_t*)p;
-  else x.v[0] = *p;
+  else if (log == 2 && units >= 4) x.v = __builtin_bit_cast(ab_u4, *(const ev_words*)p);
+  else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < units) x.v[k] = log == 2 ? ((const uint32_t*)p)[k] : log == 1 ? ((const uint16_t*)p)[k] : p[k];
+  }
 }
-__device__ __forceinline__ void ev_store(const ev_piece& x, uint8_t* p, int log) {
+__device__ __forceinline__ void ev_store(const ev_piece& x, uint8_t* p, int log, int units) {
   if (log == 4) *(ab_u4*)p = x.v;
-  else if (log == 3) *(ab_u2*)p = (ab_u2){x.v[0], x.v[1]};
-  else if (log == 2) *(uint32_t*)p = x.v[0];
-  else if (log == 1) *(uint16_t*)p = (uint16_t)x.v[0];
-  else *p = (uint8_t)x.v[0];
+  else if (log == 2 && units >= 4) *(ev_words*)p = __builtin_bit_cast(ev_words, x.v);
+  else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < units) {
+        if (log == 2) ((uint32_t*)p)[k] = x.v[k];
+        else if (log == 1) ((uint16_t*)p)[k] = (uint16_t)x.v[k];
+        else p[k] = (uint8_t)x.v[k];
+      }
+  }
 }
 
-// To blocks that nobody reads: a thread a piece.
+// To blocks that nobody reads: a thread a piece of a row, heads of a token side by side, as the rows lie where they go to.
+// (With four bytes a thread and a division of 64 bits for it, 16 sequences of 2048 tokens of 4 bits took 68 us.)
 __global__ __launch_bounds__(256) void ev_copy_kernel(ev_move_args a) {
-  const int head = blockIdx.y, seq = blockIdx.z;
+  const int seq = blockIdx.y;
   const int n = min(ab_clamp(akv_load_index(a.b.lens, a.b.lens_it, seq), AB_MOST_TOKENS), a.keep);
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int j = (int)(x / a.pieces);
-  if (j >= n) return;
-  int piece = (int)(x - (int64_t)j * a.pieces), i = 0;
+  const uint32_t x = blockIdx.x * 256 + threadIdx.x, per = (uint32_t)a.heads * (uint32_t)a.pieces;
+  const uint32_t j = x / per, rest = x - j * per, head = rest / (uint32_t)a.pieces;
+  if ((int64_t)j >= n) return;
+  const int piece = (int)(rest - head * (uint32_t)a.pieces);
+  int i = 0;
   while (i + 1 < a.caches && piece >= a.c[i + 1].first) ++i;
   const ev_cache& c = a.c[i];
   const int from = a.kept[(int64_t)seq * a.ks_seq + (int64_t)head * a.ks_head + j];
-  if (from < 0 || from >= a.b.max_blocks * a.b.block_size || j >= a.to_blocks * a.b.block_size) return;
+  if (from < 0 || from >= a.b.max_blocks * a.b.block_size || (int64_t)j >= a.to_blocks * a.b.block_size) return;
+  const int unit = c.per * (piece - c.first), units = min(c.per, c.units - unit);
   ev_piece v;
-  ev_load(v, ev_at(c, ev_row_of(a, seq, from, false), head, piece - c.first), c.log);
-  ev_store(v, ev_at(c, ev_row_of(a, seq, j, true), head, piece - c.first), c.log);
+  ev_load(v, ev_at(c, ev_row_of(a, seq, from, false), (int)head, unit), c.log, units);
+  ev_store(v, ev_at(c, ev_row_of(a, seq, (int)j, true), (int)head, unit), c.log, units);
 }
 
 // In place.  A token never moves back, so what a tile of tokens writes lies before everything that later tiles read, and a workgroup that walks
 // the tiles in order needs only to have read a tile before it writes it.  Slices of the rows are independent of each other, and
 // so are heads and sequences: a workgroup each.
-#define EV_HELD 8
+#define EV_PIECES 8
 __global__ __launch_bounds__(256) void ev_compact_kernel(ev_move_args a) {
   const int head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;
   int i = 0;
   while (i + 1 < a.caches && (int)blockIdx.x >= a.c[i + 1].first) ++i;
   const ev_cache& c = a.c[i];
-  const int u0 = ((int)blockIdx.x - c.first) * c.slice, units = min(c.slice, c.units - u0);
+  const int p0 = ((int)blockIdx.x - c.first) * c.slice, pieces = min(c.slice, c.pieces - p0);      // of a row
   const int64_t cap = min(a.b.max_blocks, a.to_blocks) * a.b.block_size;
   const int n = min(ab_clamp(akv_load_index(a.b.lens, a.b.lens_it, seq), cap < AB_MOST_TOKENS ? cap : AB_MOST_TOKENS), a.keep);
   const int32_t* kept = a.kept + (int64_t)seq * a.ks_seq + (int64_t)head * a.ks_head;
-  const int tile = 256 * EV_HELD / units;        // tokens
+  const int tile = 256 * EV_PIECES / pieces;      // tokens
   for (int j0 = 0; j0 < n; j0 += tile) {
-    ev_piece v[EV_HELD];
-    uint8_t* to[EV_HELD];
+    ev_piece v[EV_PIECES];
+    uint8_t* to[EV_PIECES];
+    int count[EV_PIECES];               // units
 #pragma unroll
-    for (int k = 0; k < EV_HELD; ++k) {
-      const int x = 256 * k + tid, t = x / units, j = j0 + t, unit = u0 + x - t * units;
+    for (int k = 0; k < EV_PIECES; ++k) {
+      const int x = 256 * k + tid, t = x / pieces, j = j0 + t, unit = c.per * (p0 + x - t * pieces);
+      count[k] = min(c.per, c.units - unit);
       to[k] = nullptr;
       if (t >= tile || j >= n) continue;
       const int from = kept[j];
       if (from <= j || from >= a.b.max_blocks * a.b.block_size) continue;      // (where it is already)
       to[k] = ev_at(c, ev_row_of(a, seq, j, true), head, unit);
-      ev_load(v[k], ev_at(c, ev_row_of(a, seq, from, false), head, unit), c.log);
+      ev_load(v[k], ev_at(c, ev_row_of(a, seq, from, false), head, unit), c.log, count[k]);
     }
     // every load of the workgroup has its value before the first store
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < EV_HELD; ++k)
-      if (to[k]) ev_store(v[k], to[k], c.log);
+    for (int k = 0; k < EV_PIECES; ++k)
+      if (to[k]) ev_store(v[k], to[k], c.log, count[k]);
   }
 }
 
@@ -250,22 +401,24 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
     if (x.row_bytes > 1 << 20) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: rows of more than 2^20 bytes", name);
     ev_cache& c = a.c[i];
     c.p = (uint8_t*)x.data; c.blk = x.s_blk; c.pos = x.s_pos; c.head = x.s_head;
-    // pieces as wide as rows, their places and their ends allow
+    // units as wide as rows, their places and their ends allow
     const uint64_t all = (uint64_t)(uintptr_t)x.data | (uint64_t)x.s_blk | (uint64_t)x.s_pos | (uint64_t)x.s_head | (uint64_t)x.row_bytes;
-    for (c.log = 4; all & ((1u << c.log) - 1); --c.log) {}
+    c.log = all & 1 ? 0 : all & 3 ? 1 : all & 15 ? 2 : 4;
     c.units = (int)(x.row_bytes >> c.log);
-    c.slice = c.units < 4 ? c.units : 4;
+    c.per = c.log == 4 ? 1 : 4;
+    c.pieces = (c.units + c.per - 1) / c.per;
+    c.slice = c.pieces < 4 ? c.pieces : 4;
     c.first = (int)(out_tables ? pieces : slices);
-    slices += (c.units + c.slice - 1) / c.slice;
-    pieces += c.units;
+    slices += (c.pieces + c.slice - 1) / c.slice;
+    pieces += c.pieces;
   }
-  a.pieces = (int)pieces;
+  a.pieces = (int)pieces; a.heads = num_kv_heads;
   const hipStream_t s = (hipStream_t)stream;
   if (out_tables) {
-    const int64_t most = out_blocks_per_seq * block_size < keep ? out_blocks_per_seq * block_size : keep, groups = (most * pieces + 255) / 256;
-    if (groups > 0x7fffffff) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^39 pieces", name);
-    if (groups == 0) return AKV_OK;
-    ev_copy_kernel<<<dim3((uint32_t)groups, (uint32_t)num_kv_heads, (uint32_t)num_seqs), 256, 0, s>>>(a);
+    const int64_t most = out_blocks_per_seq * block_size < keep ? out_blocks_per_seq * block_size : keep, all = most * pieces * num_kv_heads;
+    if (all > 0xffffff00ll) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^32 pieces a sequence", name);
+    if (all == 0) return AKV_OK;
+    ev_copy_kernel<<<dim3((uint32_t)((all + 255) / 256), (uint32_t)num_seqs), 256, 0, s>>>(a);
     AKV_LAUNCH_CHECK("ev_copy_kernel");
   } else {
     ev_compact_kernel<<<dim3((uint32_t)slices, (uint32_t)num_kv_heads, (uint32_t)num_seqs), 256, 0, s>>>(a);
