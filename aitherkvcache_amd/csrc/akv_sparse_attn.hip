@@ -1,13 +1,13 @@
 // akv_sparse_attn: causal attention of new tokens over the blocks of a paged cache of plain rows that each token and kv head has selected.
 //
-//   S^T[key, row] = K[key, :] . Q[row, :]          v_mfma_f32_16x16x32, A = 16 keys, B = 16 rows
-//   O^T[d, row] = sum_key V[key, d] P^T[key, row]  A = 16 coordinates, B = 16 rows
+//   S^T[key, row] = K[key, :] . Q[row, :]          v_mfma_f32_32x32x16, A = 32 keys, B = 32 rows
+//   O^T[d, row] = sum_key V[key, d] P^T[key, row]  A = 32 coordinates, B = 32 rows
 //
-// The rows of a tile are (token, query head) pairs of one kv head, as many tokens of a sequence as fit sixteen rows.  Neighbouring tokens
-// select much the same blocks, so the tile reads the union of what its tokens selected, each block once, and a bit a token says whose it is.
-// A lane holds one row and, of sixteen keys, four: the softmax is taken in the lane with an exchange between the four rows of lanes, and
-// the weights of two groups of sixteen keys are the operand of the second product, whose k axis takes keys in the order in which lanes hold
-// them.  V^T comes out of LDS by transposing reads (four keys of a coordinate a lane).
+// The rows of a tile are (token, query head) pairs of one kv head, as many tokens of a sequence as fit 32 rows.  Neighbouring tokens select much
+// the same blocks, so the tile reads the union of what its tokens selected, each block once, and a bit a token says whose it is.  A lane holds one
+// row and half of 32 keys: the softmax is taken in the lane with one exchange between the halves of the wavefront, and the weights are the operand of
+// the second product, whose k axis takes keys in the order in which lanes hold them.  V^T comes out of LDS by transposing reads (four keys of a
+// coordinate a lane).
 #include "akv_batch.h"
 #include "akv_device_once.h"
 
@@ -28,19 +28,21 @@ struct sa_args {
 #define SA_FRAME 8.f
 template <int DT> constexpr float SA_LIFT = DT == AKV_BF16 ? 0.f : 5.f;
 
-template <int D> struct sa_lds {        // behind bitmaps (or in their place) and lists
-  static constexpr int WAVES = 4, V_BYTES = 32 * 2 * D, STAGE = WAVES * V_BYTES;
-  static __device__ __forceinline__ int f(int r) { return D == 64 ? 2 * ((r >> 1) & 3) : 2 * (r & 7); }
+
+// Of a wavefront in LDS, behind bitmaps (or in their place) and before lists: 32 keys, then in their place 32 values, then 64 coordinates of its sums.
+// Rows lie apart so that the operands' reads meet no bank twice: sixteen bytes more for keys, 32 for transposing reads of values.
+template <int D, int W> struct sa_lds {
+  static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * D + 32, WAVE = 32 * V_ROW, AREA = W * (WAVE > 8192 ? WAVE : 8192);
 };
 
-template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_args a) {
-  typedef sa_lds<D> P;
+template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void sa_kernel(sa_args a) {
+  typedef sa_lds<D, W> P;
   typedef ab_math<DT> M;
-  constexpr int KS = D / 32, OT = D / 16, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, W = P::WAVES;
+  constexpr int KS = D / 16, OT = D / 32, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, THREADS = 64 * W;
   extern __shared__ __align__(1024) unsigned char lds[];
   __shared__ int wave_sum[W];
-  __shared__ float2 ml[W][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, hq = lane >> 4;
+  __shared__ float2 ml[W][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = lane & 31, half = lane >> 5;
   const int heads = a.KVH * a.HS, bs = a.b.block_size;
   const int head = blockIdx.x % heads;
   const int64_t x = blockIdx.x / heads;
@@ -50,7 +52,7 @@ template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_
   const int front = a.tail ? ab_start(a.b, 0) : 0;
   if (front > 0) {
     const int64_t per = (int64_t)a.QH * (D / 4);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + tid; i < front * per; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < front * per; i += (int64_t)gridDim.x * THREADS) {
       const int64_t token = i / per, rest = i - token * per, hd = rest / (D / 4);
       *(ab_u2*)((uint16_t*)a.out + token * a.os_tok + hd * a.os_head + 4 * (rest - hd * (D / 4))) = (ab_u2){0u, 0u};
     }
@@ -64,7 +66,7 @@ template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_
   const int first = (int)first64, tokens = min(a.TG, s1 - first);
   const int pos0 = seq < a.b.S ? ab_ctx(a.b, seq) - (s1 - first) : -tokens;      // position of the first token
   const int last = pos0 + tokens - 1;
-  const int t_row = col / a.GC, g_row = g0 + col - t_row * a.GC;
+  const int t_row = row / a.GC, g_row = g0 + row - t_row * a.GC;
   const bool valid = t_row < tokens && g_row < a.G;
   const int pos = valid ? pos0 + t_row : -1;
   const int64_t q_row = valid ? (int64_t)(first + t_row) * a.qs_tok + (int64_t)(kvh * a.G + g_row) * a.qs_head : 0;
@@ -73,22 +75,21 @@ template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     q[ks] = (ab_u4){0u, 0u, 0u, 0u};
-    if (valid) q[ks] = *(const ab_u4*)((const uint16_t*)a.q + q_row + 32 * ks + 8 * hq);
+    if (valid) q[ks] = *(const ab_u4*)((const uint16_t*)a.q + q_row + 16 * ks + 8 * half);
   }
 
   // ---- the union of what the tokens selected
-  unsigned char* const stage = lds;
   uint32_t* const bits = (uint32_t*)lds;             // [TG][words], before the values
   const int cap = min(a.TG * a.k_sel, a.words * 32);
-  const int area = max(P::STAGE, (a.TG * a.words * 4 + 15) & ~15);
+  const int area = max(P::AREA, (a.TG * a.words * 4 + 15) & ~15);
   int* const cols = (int*)(lds + area);
   int* const blks = cols + cap;
-  uint16_t* const masks = (uint16_t*)(blks + cap);
+  uint32_t* const masks = (uint32_t*)(blks + cap);
   const int words = last >= 0 ? last / bs / 32 + 1 : 0;
-  for (int i = tid; i < tokens * words; i += 256) bits[i] = 0u;
+  for (int i = tid; i < tokens * words; i += THREADS) bits[i] = 0u;
   __syncthreads();
   if (words > 0) {
-    for (int i = tid; i < tokens * a.k_sel; i += 256) {
+    for (int i = tid; i < tokens * a.k_sel; i += THREADS) {
       const int t = i / a.k_sel;
       const int c = a.selected[(int64_t)(first + t) * a.ss_tok + (int64_t)kvh * a.ss_head + (i - t * a.k_sel)];
       if (pos0 + t >= 0 && c >= 0 && c <= (pos0 + t) / bs) atomicOr(bits + t * words + (c >> 5), 1u << (c & 31));
@@ -96,7 +97,7 @@ template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_
   }
   __syncthreads();
   int count = 0;
-  for (int w0 = 0; w0 < words; w0 += 256) {
+  for (int w0 = 0; w0 < words; w0 += THREADS) {
     uint32_t u = 0u;
     if (w0 + tid < words)
       for (int t = 0; t < tokens; ++t) u |= bits[t * words + w0 + tid];
@@ -112,160 +113,201 @@ template <int D, int DT> __global__ __launch_bounds__(256, 2) void sa_kernel(sa_
     for (; u; u &= u - 1) cols[at++] = 32 * (w0 + tid) + __ffs(u) - 1;
     __syncthreads();
   }
-  for (int i = tid; i < count; i += 256) {
+  for (int i = tid; i < count; i += THREADS) {
     const int c = cols[i];
     uint32_t m = 0u;
     for (int t = 0; t < tokens; ++t) m |= ((bits[t * words + (c >> 5)] >> (c & 31)) & 1u) << t;
     blks[i] = (int)ab_block(a.b, seq, c);
-    masks[i] = (uint16_t)m;
+    masks[i] = m;
   }
   __syncthreads();           // (the bitmaps have been read)
 
-  // ---- the wavefront's groups of 2 x 16 keys
-  const int groups = count * a.parts;
-  unsigned char* const vl = stage + wave * P::V_BYTES;
-  uint32_t v_at[OT];
+  // ---- the wavefront's units of 2 x 16 keys: rows arrive in the order in which they lie, and go through LDS into that of the operands
+  const int sixteens = count * a.parts, units = (sixteens + 1) / 2;
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + wave * P::WAVE;
+  const uint32_t k_at = at + row * P::K_ROW + 16 * half, v_at = at + (4 * half + (lane & 15) / 4) * P::V_ROW + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+  typedef __attribute__((address_space(3))) ab_u4 lds_u4;
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s4 lds_s4;
+  const uint8_t* const kp = a.k + (int64_t)kvh * a.k_head;
+  const uint8_t* const vp = a.v + (int64_t)kvh * a.v_head;
+  const uint32_t k_pos = (uint32_t)a.k_pos, v_pos = (uint32_t)a.v_pos;
+  uint32_t k_off[VI / 2], v_off[VI / 2];             // a thread's pieces of a sixteen
 #pragma unroll
-  for (int dt = 0; dt < OT; ++dt) {
-    const int r = 4 * hq + (lane & 15) / 4, c = 2 * dt + ((lane & 3) >> 1);
-    v_at[dt] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)vl + r * 2 * D + 16 * (c ^ P::f(r)) + 8 * (lane & 1);
+  for (int i = 0; i < VI / 2; ++i) {
+    k_off[i] = (RPI * i + lane / LPR) * k_pos + 16 * (lane % LPR);
+    v_off[i] = (RPI * i + lane / LPR) * v_pos + 16 * (lane % LPR);
   }
-  struct keys {
-    ab_u4 k[2][KS], v[VI];
-    int base[2], end[2];               // of sixteen keys: position of the first, one past the last of the block (0: none)
-    uint32_t mask[2];
+  // An entry of the lists for each sixteen of a unit, in two lanes in turn (looked up a unit ahead, so that nothing waits for it), and what is made of it.
+  struct entry { int blk, col, mask, place; };
+  struct unit { const uint8_t *k[2], *v[2]; int left[2], base[2], mask[2]; };        // keys of the block from there on, position of the first, whose they are
+  auto look = [&](int p) {
+    const int st = 2 * p + (lane & 1);
+    uint32_t part;
+    const int e = (int)akv_div32((uint32_t)max(0, min(st, sixteens - 1)), (uint32_t)a.parts, a.parts_recip, part);
+    return entry{blks[e], cols[e], st < sixteens ? (int)masks[e] : 0, 16 * (int)part};
   };
-  auto request = [&](int p, keys& w) {
+  auto find = [&](const entry& x) {
+    unit u;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int st = __builtin_amdgcn_readfirstlane(min(2 * p + s, groups - 1));
-      uint32_t part;
-      const int e = (int)akv_div32((uint32_t)st, (uint32_t)a.parts, a.parts_recip, part);
-      const int64_t blk = __builtin_amdgcn_readfirstlane(blks[e]);
-      const int c = __builtin_amdgcn_readfirstlane(cols[e]), place = 16 * (int)part;
-      w.base[s] = c * bs + place;
-      w.end[s] = 2 * p + s < groups ? c * bs + bs : 0;
-      w.mask[s] = __builtin_amdgcn_readfirstlane(masks[e]);
-      const uint8_t* kp = a.k + blk * a.k_blk + (int64_t)kvh * a.k_head + (int64_t)min(place + col, bs - 1) * a.k_pos + 16 * hq;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) w.k[s][ks] = *(const ab_u4*)(kp + 64 * ks);
-      const uint8_t* vp = a.v + blk * a.v_blk + (int64_t)kvh * a.v_head + 16 * (lane % LPR);
-#pragma unroll
-      for (int i = 0; i < VI / 2; ++i) {
-        // (a value that no token of the tile may see is zero, whatever lies there)
-        const int r = RPI * i + lane / LPR, key = w.base[s] + r;
-        w.v[s * (VI / 2) + i] = *(const ab_u4*)(vp + (int64_t)min(place + r, bs - 1) * a.v_pos);
-        if (key > last || key >= w.end[s]) w.v[s * (VI / 2) + i] = (ab_u4){0u, 0u, 0u, 0u};
-      }
+      const int64_t blk = __builtin_amdgcn_readlane(x.blk, s);
+      const int place = __builtin_amdgcn_readlane(x.place, s);
+      u.k[s] = kp + blk * a.k_blk + place * a.k_pos;
+      u.v[s] = vp + blk * a.v_blk + place * a.v_pos;
+      u.left[s] = min(16, bs - place);
+      u.base[s] = __builtin_amdgcn_readlane(x.col, s) * bs + place;
+      u.mask[s] = __builtin_amdgcn_readlane(x.mask, s);
     }
+    return u;
   };
-  ab_f4 o[OT];
+  auto request = [&](ab_u4* to, const uint8_t* const* from, const int* left, const uint32_t* off, uint32_t pos) {
 #pragma unroll
-  for (int i = 0; i < OT; ++i) o[i] = (ab_f4){0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  for (int p = wave; 2 * p < groups; p += W) {
-    keys w;
-    request(p, w);
-    akv_wave_sync();                   // (the values before have been read)
+    for (int i = 0; i < VI; ++i) to[i] = *(const ab_u4*)(from[2 * i / VI] + min(off[i % (VI / 2)], (left[2 * i / VI] - 1) * pos + 16 * (lane % LPR)));
+  };
+  // (A weight of zero times a value that is not finite is no zero.  What no token of the tile may see is a zero in LDS, whatever lies in the cache; where a token
+  // would meet such a value of another, the tile is done again a token at a time.)
+  for (int only = -1;;) {
+    const int seen = only < 0 ? last : pos0 + only;  // position of the last key that is seen
+    const uint32_t mine = only < 0 ? 0xffffffffu : 1u << only;
+    ab_f16 o[OT];
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      const int r = RPI * i + lane / LPR;
-      *(ab_u4*)(vl + r * 2 * D + 16 * ((lane % LPR) ^ P::f(r))) = w.v[i];
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    ab_u4 k[VI], v[VI];
+    unit now = {};
+    entry ahead = {};
+    if (wave < units) {
+      now = find(look(wave));
+      ahead = look(wave + W);
+      request(k, now.k, now.left, k_off, k_pos);
+      request(v, now.v, now.left, v_off, v_pos);
     }
-    ab_f4 s[2];
+    for (int p = wave; p < units; p += W) {
+      const bool more = p + W < units;
+      const unit next = find(ahead);
+      ahead = look(p + 2 * W);
+      akv_wave_sync();                   // (the values before have been read)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = (ab_f4){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::K_ROW + 16 * (lane % LPR)) = k[i];
+      if (more) request(k, next.k, next.left, k_off, k_pos);
+      akv_wave_sync();
+      ab_f16 s;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[t] = M::mfma16(w.k[t][ks], q[ks], s[t]);
-    }
-    float top = -INFINITY;
+      for (int j = 0; j < 16; ++j) s[j] = 0.f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int limit = ((w.mask[t] >> t_row) & 1u) ? min(w.end[t] - 1, pos) : -1;
+      for (int ks = 0; ks < KS; ++ks) s = M::mfma32(*(const lds_u4*)(uintptr_t)(k_at + 32 * ks), q[ks], s);
+      akv_wave_sync();                   // (the keys have been read)
+      int held[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = w.base[t] + 4 * hq + i <= limit ? s[t][i] * a.scale2 : -INFINITY;
-        top = fmaxf(top, s[t][i]);
+      for (int t = 0; t < 2; ++t) held[t] = now.mask[t] & mine ? min(now.left[t], seen + 1 - now.base[t]) : 0;
+      if (min(held[0], held[1]) < 16) {
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+          if (RPI * (i % (VI / 2)) + lane / LPR >= held[2 * i / VI]) v[i] = (ab_u4){0u, 0u, 0u, 0u};
       }
-    }
-    top = akv_rows_max(top);
-    const bool grown = top - m > SA_LIFT<DT> + SA_FRAME;
-    if (__ballot(grown)) {
-      const float to = grown ? top - SA_LIFT<DT> : m, alpha = grown ? __builtin_amdgcn_exp2f(m - to) : 1.f;
-      m = to;
-      l *= alpha;
 #pragma unroll
-      for (int i = 0; i < OT; ++i) o[i] *= alpha;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
-    ab_u4 pw;
+      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::V_ROW + 16 * (lane % LPR)) = v[i];
+      if (more) request(v, next.v, next.left, v_off, v_pos);
+      float top = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
+        const int limit = ((now.mask[t] & mine) >> t_row & 1 ? min(now.left[t] - 1, pos - now.base[t]) : -1) - 4 * half;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
-        l += s[t][i];
+        for (int i = 0; i < 8; ++i) {
+          s[8 * t + i] = 8 * (i / 4) + i % 4 <= limit ? s[8 * t + i] : -INFINITY;
+          top = fmaxf(top, s[8 * t + i]);
+        }
       }
-      pw[2 * t] = M::pair(s[t][0], s[t][1]);
-      pw[2 * t + 1] = M::pair(s[t][2], s[t][3]);
-    }
-    akv_wave_sync();
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s4 lds_s4;
+      auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.scale2;
+      const bool grown = top - m > SA_LIFT<DT> + SA_FRAME;
+      if (__ballot(grown)) {
+        const float to = grown ? top - SA_LIFT<DT> : m, alpha = grown ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+        m = to;
+        l *= alpha;
 #pragma unroll
-    for (int dt = 0; dt < OT; ++dt) {
-      const ab_u2 lo = __builtin_bit_cast(ab_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)v_at[dt]));
-      const ab_u2 hi = __builtin_bit_cast(ab_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(v_at[dt] + 16 * 2 * D)));
-      o[dt] = M::mfma16((ab_u4){lo[0], lo[1], hi[0], hi[1]}, pw, o[dt]);
+        for (int i = 0; i < OT; ++i) o[i] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      ab_u4 pw[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -ref));
+        l += s[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pw[i / 4][i % 4] = M::pair(s[2 * i], s[2 * i + 1]);
+      akv_wave_sync();
+#pragma unroll
+      for (int dt = 0; dt < OT; ++dt)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const ab_u2 lo = __builtin_bit_cast(ab_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(v_at + 64 * dt + 16 * t * P::V_ROW)));
+          const ab_u2 hi = __builtin_bit_cast(ab_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(v_at + 64 * dt + (16 * t + 8) * P::V_ROW)));
+          o[dt] = M::mfma32((ab_u4){lo[0], lo[1], hi[0], hi[1]}, pw[t], o[dt]);
+        }
+      now = next;
     }
-  }
 
-  // ---- the wavefronts' sums together
-  l = akv_rows_sum(l);
-  if (hq == 0) ml[wave][col] = make_float2(m, l);
-  __syncthreads();           // (the values have been read)
-  float4* const part = (float4*)stage;
+    // ---- the wavefronts' sums together
+    auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+    if (half == 0) ml[wave][row] = make_float2(m, l);
+    __syncthreads();         // (the values have been read)
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int dt = 0; dt < OT; ++dt) part[(wave * OT + dt) * 64 + lane] = make_float4(o[dt][0], o[dt][1], o[dt][2], o[dt][3]);
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f, f[W];
+    for (int w = 0; w < W; ++w) top = fmaxf(top, ml[w][row].x);
 #pragma unroll
-  for (int w = 0; w < W; ++w) top = fmaxf(top, ml[w][col].x);
+    for (int w = 0; w < W; ++w) sum = fmaf(ml[w][row].y, top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][row].x - top), sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum, f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    uint32_t most = 0u;      // of the sums' bits without the sign: 0x7f800000 or more where one is not finite
+    uint16_t* const to = (uint16_t*)a.out + (int64_t)(first + t_row) * a.os_tok + (int64_t)(kvh * a.G + g_row) * a.os_head + 4 * half;
+    float4* const part = (float4*)lds;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    f[w] = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][col].x - top);
-    sum = fmaf(ml[w][col].y, f[w], sum);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (valid) {
-    uint16_t* to = (uint16_t*)a.out + (int64_t)(first + t_row) * a.os_tok + (int64_t)(kvh * a.G + g_row) * a.os_head + 4 * hq;
-    for (int dt = wave; dt < OT; dt += W) {
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int d0 = 0; d0 < OT; d0 += 2) {
+      // 64 coordinates at a time; of their eight groups of 4 + 4 (a lane of each half four) a wavefront adds 8 / W
+      if (d0 > 0) __syncthreads();
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float4 z = part[(w * OT + dt) * 64 + lane];
-        y.x = fmaf(z.x, f[w], y.x); y.y = fmaf(z.y, f[w], y.y); y.z = fmaf(z.z, f[w], y.z); y.w = fmaf(z.w, f[w], y.w);
+      for (int i = 0; i < 8; ++i) {
+        const ab_f16& x = o[d0 + i / 4];
+        part[(wave * 8 + i) * 64 + lane] = make_float4(x[4 * (i % 4)] * f, x[4 * (i % 4) + 1] * f, x[4 * (i % 4) + 2] * f, x[4 * (i % 4) + 3] * f);
       }
-      *(ab_u2*)(to + 16 * dt) = (ab_u2){M::pair(y.x * inv, y.y * inv), M::pair(y.z * inv, y.w * inv)};
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8 / W; ++j) {
+        const int i = wave * (8 / W) + j;
+        float4 y = part[i * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+          const float4 z = part[(w * 8 + i) * 64 + lane];
+          y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        }
+        if (valid) {
+          most = max(max(most, max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu)), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
+          if (only < 0 || t_row == only) *(ab_u2*)(to + 32 * d0 + 8 * i) = (ab_u2){M::pair(y.x * inv, y.y * inv), M::pair(y.z * inv, y.w * inv)};
+        }
+      }
     }
+    if (tokens == 1) break;
+    const bool again = __syncthreads_or(most >= 0x7f800000u);
+    if (only < 0 && !again) break;
+    if (++only == tokens) break;
   }
 }
 
 #define SA_LDS (150 << 10)
 #define SA_MOST_SELECTED 4096
-template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
-  a.HS = (a.G + 15) / 16;
-  a.GC = (a.G + a.HS - 1) / a.HS;
-  a.parts = (a.b.block_size + 15) / 16;
-  a.parts_recip = (uint32_t)(0xffffffffull / (uint32_t)a.parts);
-  a.words = (int)((a.b.max_blocks + 31) / 32);
-  if (a.words < 1) a.words = 1;
+#define SA_MOST_STRIDE ((1ll << 27) - 1)          // of a block's tokens: sixteen of them within 2^32 bytes
+template <int D, int DT, int W> static int sa_run(sa_args a, hipStream_t stream) {
+  typedef sa_lds<D, W> P;
   int64_t bytes = 0;
-  for (a.TG = 16 / a.GC;; a.TG = (a.TG + 1) / 2) {
+  for (a.TG = 32 / a.GC;; a.TG = (a.TG + 1) / 2) {
     const int64_t bits = ((int64_t)a.TG * a.words * 4 + 15) & ~15ll, all = (int64_t)a.words * 32;
     const int64_t cap = (int64_t)a.TG * a.k_sel < all ? (int64_t)a.TG * a.k_sel : all;
-    bytes = (bits > sa_lds<D>::STAGE ? bits : sa_lds<D>::STAGE) + 10 * cap;
+    bytes = (bits > P::AREA ? bits : P::AREA) + 12 * cap;
     if (bytes <= SA_LDS || a.TG == 1) break;
   }
   if (bytes > SA_LDS) return akv_fail(AKV_ERR_UNSUPPORTED, "akv_sparse_attn: block tables of %lld columns", (long long)a.b.max_blocks);
@@ -274,10 +316,19 @@ template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
   static akv_device_once once;
-  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)sa_kernel<D, DT>, SA_LDS); })) return rc;
-  sa_kernel<D, DT><<<(uint32_t)units, 256, bytes, stream>>>(a);
+  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)sa_kernel<D, DT, W>, SA_LDS); })) return rc;
+  sa_kernel<D, DT, W><<<(uint32_t)units, 64 * W, bytes, stream>>>(a);
   AKV_LAUNCH_CHECK("sa_kernel");
   return AKV_OK;
+}
+template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
+  a.HS = (a.G + 31) / 32;
+  a.GC = (a.G + a.HS - 1) / a.HS;
+  a.parts = (a.b.block_size + 15) / 16;
+  a.parts_recip = (uint32_t)(0xffffffffull / (uint32_t)a.parts);
+  a.words = (int)((a.b.max_blocks + 31) / 32);
+  if (a.words < 1) a.words = 1;
+  return sa_run<D, DT, 4>(a, stream);
 }
 
 extern "C" int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head, const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head, const void* value_cache,
@@ -301,6 +352,8 @@ extern "C" int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int
   if (num_selected > SA_MOST_SELECTED) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than %d selected blocks", name, SA_MOST_SELECTED);
   if (!ab_aligned(query, 16) || !ab_aligned(key_cache, 16) || !ab_aligned(value_cache, 16) || !ab_aligned(out, 8) || ((qs_tok | qs_head | ks_blk | ks_pos | ks_head | vs_blk | vs_pos | vs_head) & 7) || ((os_tok | os_head) & 3))
     return akv_fail(AKV_ERR_UNSUPPORTED, "%s: rows must lie at multiples of 16 bytes (outputs of 8)", name);
+  if (block_size == 1) ks_pos = vs_pos = 0;
+  if (ks_pos < 0 || vs_pos < 0 || ks_pos > SA_MOST_STRIDE || vs_pos > SA_MOST_STRIDE) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: tokens of a block 2^27 elements apart", name);
   sa_args a = {};
   a.b = ab_make(block_tables, bt_itype, bt_stride, context_lens, cl_itype, query_starts, qs_itype, num_seqs, num_tokens, block_size, num_blocks, max_blocks_per_seq);
   a.q = query; a.qs_tok = qs_tok; a.qs_head = qs_head;
