@@ -32,10 +32,10 @@ template <int DT> constexpr float SA_LIFT = DT == AKV_BF16 ? 0.f : 5.f;
 // Of a wavefront in LDS, behind bitmaps (or in their place) and before lists: 32 keys, then in their place 32 values, then 64 coordinates of its sums.
 // Rows lie apart so that the operands' reads meet no bank twice: sixteen bytes more for keys, 32 for transposing reads of values.
 template <int D, int W> struct sa_lds {
-  static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * D + 32, WAVE = 32 * V_ROW, AREA = W * (WAVE > 8192 ? WAVE : 8192);
+  static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * D + 32, WAVE = 32 * V_ROW, AREA = W * (WAVE > 8192 ? WAVE : 8192) + 32 * K_ROW;
 };
 
-template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void sa_kernel(sa_args a) {
+template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 128 ? 3 : 4) void sa_kernel(sa_args a) {
   typedef sa_lds<D, W> P;
   typedef ab_math<DT> M;
   constexpr int KS = D / 16, OT = D / 32, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, THREADS = 64 * W;
@@ -69,14 +69,6 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
   const int t_row = row / a.GC, g_row = g0 + row - t_row * a.GC;
   const bool valid = t_row < tokens && g_row < a.G;
   const int pos = valid ? pos0 + t_row : -1;
-  const int64_t q_row = valid ? (int64_t)(first + t_row) * a.qs_tok + (int64_t)(kvh * a.G + g_row) * a.qs_head : 0;
-
-  ab_u4 q[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    q[ks] = (ab_u4){0u, 0u, 0u, 0u};
-    if (valid) q[ks] = *(const ab_u4*)((const uint16_t*)a.q + q_row + 16 * ks + 8 * half);
-  }
 
   // ---- the union of what the tokens selected
   uint32_t* const bits = (uint32_t*)lds;             // [TG][words], before the values
@@ -121,6 +113,15 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
     masks[i] = m;
   }
   __syncthreads();           // (the bitmaps have been read)
+
+  // rows of queries for the operand's reads, the same for all wavefronts
+  const uint32_t q_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + P::AREA - 32 * P::K_ROW, q_at = q_lds + row * P::K_ROW + 16 * half;
+  for (int i = tid; i < 32 * LPR; i += THREADS) {
+    const int r = i / LPR, t = r / a.GC, g = g0 + r - t * a.GC;
+    ab_u4 x = {0u, 0u, 0u, 0u};
+    if (t < tokens && t < a.TG && g < a.G) x = *(const ab_u4*)((const uint16_t*)a.q + (int64_t)(first + t) * a.qs_tok + (int64_t)(kvh * a.G + g) * a.qs_head + 8 * (i % LPR));
+    *(__attribute__((address_space(3))) ab_u4*)(uintptr_t)(q_lds + r * P::K_ROW + 16 * (i % LPR)) = x;
+  }
 
   // ---- the wavefront's units of 2 x 16 keys: rows arrive in the order in which they lie, and go through LDS into that of the operands
   const int sixteens = count * a.parts, units = (sixteens + 1) / 2;
@@ -167,6 +168,7 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
   };
   // (A weight of zero times a value that is not finite is no zero.  What no token of the tile may see is a zero in LDS, whatever lies in the cache; where a token
   // would meet such a value of another, the tile is done again a token at a time.)
+  __syncthreads();
   for (int only = -1;;) {
     const int seen = only < 0 ? last : pos0 + only;  // position of the last key that is seen
     const uint32_t mine = only < 0 ? 0xffffffffu : 1u << only;
@@ -176,14 +178,13 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     float m = -INFINITY, l = 0.f;
-    ab_u4 k[VI], v[VI];
+    ab_u4 x[VI];             // keys or values on their way
     unit now = {};
     entry ahead = {};
     if (wave < units) {
       now = find(look(wave));
       ahead = look(wave + W);
-      request(k, now.k, now.left, k_off, k_pos);
-      request(v, now.v, now.left, v_off, v_pos);
+      request(x, now.k, now.left, k_off, k_pos);
     }
     for (int p = wave; p < units; p += W) {
       const bool more = p + W < units;
@@ -191,36 +192,32 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
       ahead = look(p + 2 * W);
       akv_wave_sync();                   // (the values before have been read)
 #pragma unroll
-      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::K_ROW + 16 * (lane % LPR)) = k[i];
-      if (more) request(k, next.k, next.left, k_off, k_pos);
+      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::K_ROW + 16 * (lane % LPR)) = x[i];
+      request(x, now.v, now.left, v_off, v_pos);
       akv_wave_sync();
       ab_f16 s;
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = M::mfma32(*(const lds_u4*)(uintptr_t)(k_at + 32 * ks), q[ks], s);
-      akv_wave_sync();                   // (the keys have been read)
-      int held[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) held[t] = now.mask[t] & mine ? min(now.left[t], seen + 1 - now.base[t]) : 0;
-      if (min(held[0], held[1]) < 16) {
-#pragma unroll
-        for (int i = 0; i < VI; ++i)
-          if (RPI * (i % (VI / 2)) + lane / LPR >= held[2 * i / VI]) v[i] = (ab_u4){0u, 0u, 0u, 0u};
-      }
-#pragma unroll
-      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::V_ROW + 16 * (lane % LPR)) = v[i];
-      if (more) request(v, next.v, next.left, v_off, v_pos);
-      float top = -INFINITY;
+      for (int ks = 0; ks < KS; ++ks) s = M::mfma32(*(const lds_u4*)(uintptr_t)(k_at + 32 * ks), *(const lds_u4*)(uintptr_t)(q_at + 32 * ks), s);
+      // Where every token stands behind all 32 keys, a row is selected or not: what is added to its scores says so.  (A score that is no finite number makes
+      // the sum none, and the tile is done again.)
+      const bool plain = only < 0 && min(now.left[0], now.left[1]) >= 16 && max(now.base[0], now.base[1]) + 15 <= pos0;
+      float off[2], most_of[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int limit = ((now.mask[t] & mine) >> t_row & 1 ? min(now.left[t] - 1, pos - now.base[t]) : -1) - 4 * half;
+        const bool his = (now.mask[t] & mine) >> t_row & 1;
+        if (!plain) {
+          const int limit = (his ? min(now.left[t] - 1, pos - now.base[t]) : -1) - 4 * half;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          s[8 * t + i] = 8 * (i / 4) + i % 4 <= limit ? s[8 * t + i] : -INFINITY;
-          top = fmaxf(top, s[8 * t + i]);
+          for (int i = 0; i < 8; ++i) s[8 * t + i] = 8 * (i / 4) + i % 4 <= limit ? s[8 * t + i] : -INFINITY;
         }
+        most_of[t] = s[8 * t];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) most_of[t] = fmaxf(most_of[t], s[8 * t + i]);
+        off[t] = his ? 0.f : -INFINITY;
       }
+      float top = fmaxf(off[0] < 0.f ? -INFINITY : most_of[0], off[1] < 0.f ? -INFINITY : most_of[1]);
       auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1])) * a.scale2;
       const bool grown = top - m > SA_LIFT<DT> + SA_FRAME;
@@ -232,14 +229,27 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 
         for (int i = 0; i < OT; ++i) o[i] *= alpha;
       }
       const float ref = m == -INFINITY ? 0.f : m;
+      off[0] = plain ? off[0] - ref : -ref;
+      off[1] = plain ? off[1] - ref : -ref;
       ab_u4 pw[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -ref));
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, off[i / 8]));
         l += s[i];
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) pw[i / 4][i % 4] = M::pair(s[2 * i], s[2 * i + 1]);
+      int held[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) held[t] = now.mask[t] & mine ? min(now.left[t], seen + 1 - now.base[t]) : 0;
+      if (min(held[0], held[1]) < 16) {
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+          if (RPI * (i % (VI / 2)) + lane / LPR >= held[2 * i / VI]) x[i] = (ab_u4){0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::V_ROW + 16 * (lane % LPR)) = x[i];
+      if (more) request(x, next.k, next.left, k_off, k_pos);
       akv_wave_sync();
 #pragma unroll
       for (int dt = 0; dt < OT; ++dt)
