@@ -35,7 +35,7 @@ template <int D, int W> struct sa_lds {
   static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * D + 32, WAVE = 32 * V_ROW, AREA = W * (WAVE > 8192 ? WAVE : 8192) + 32 * K_ROW;
 };
 
-template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, D == 256 ? 1 : D == 128 ? 3 : 4) void sa_kernel(sa_args a) {
+template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 : D == 256 ? 1 : D == 128 ? 3 : 4) void sa_kernel(sa_args a) {
   typedef sa_lds<D, W> P;
   typedef ab_math<DT> M;
   constexpr int KS = D / 16, OT = D / 32, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, THREADS = 64 * W;
@@ -338,6 +338,10 @@ template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
   a.parts_recip = (uint32_t)(0xffffffffull / (uint32_t)a.parts);
   a.words = (int)((a.b.max_blocks + 31) / 32);
   if (a.words < 1) a.words = 1;
+  // one token after another, and not a tile for every other CU: eight wavefronts share its keys
+  const int64_t tokens = a.b.T < a.b.S ? a.b.T : a.b.S;
+  if constexpr (D < 256)
+    if (a.b.T <= a.b.S && 2 * tokens * a.KVH * a.HS <= ab_cus()) return sa_run<D, DT, 8>(a, stream);
   return sa_run<D, DT, 4>(a, stream);
 }
 
