@@ -154,7 +154,8 @@ _BOUND = ("akv_paged_attn_workspace_bytes", "akv_paged_attn", "akv_encode_paged_
           "akv_hybrid_paged_attn", "akv_hybrid25_paged_attn", "akv_hybrid_encode_paged_kv", "akv_hybrid25_encode_paged_kv",
           "akv_decode_blocks_kv", "akv_tri_encode_paged_kv", "akv_tri_decode_workspace_bytes", "akv_tri_decode_paged",
           "akv_rope_append", "akv_dense_chunk_attn_workspace_bytes", "akv_dense_chunk_attn", "akv_paged_chunk_attn_workspace_bytes",
-          "akv_paged_chunk_attn")
+          "akv_paged_chunk_attn", "akv_block_index_update", "akv_block_index_select_workspace_bytes", "akv_block_index_select",
+          "akv_sparse_attn", "akv_key_weights_workspace_bytes", "akv_key_weights")
 
 
 def available() -> bool:

@@ -55,6 +55,10 @@ class BlockIndex:
                         blocks of every sequence (the cache was filled or rearranged by other means)
 
         A last block that is not full has the mean of the keys in it; a mean that is not finite is kept as zeros.  Sums are 64 bits."""
+        result = _lib.calls().index_update(key_cache, block_tables, context_lens, query_start_loc, self.codes, self.scales, self.num_blocks,
+                                           self.num_kv_heads, self.head_dim)
+        if result is not None:
+            return _lib.check(result)
         _check_rows("key_cache", key_cache, 4)
         if key_cache.dtype not in (torch.float16, torch.bfloat16):
             raise NotImplementedError(f"keys are float16 or bfloat16, got {key_cache.dtype}")
@@ -86,6 +90,10 @@ class BlockIndex:
         out              where the result goes (that shape, int32, contiguous)
 
         Products are of whole numbers: the result does not hang on the order of a sum."""
+        result = _lib.calls().index_select(query, block_tables, context_lens, query_start_loc, self.codes, self.scales, out, self.num_blocks,
+                                           self.num_kv_heads, self.head_dim, block_size, num_selected, num_sink_blocks, num_recent_blocks)
+        if result is not None:
+            return result if type(result) is not int else _lib.check(result)
         check_query(query)
         num_tokens, num_q_heads, d = query.shape
         if d != self.head_dim:
@@ -132,9 +140,12 @@ def paged_sparse_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
               order and repetition do not matter; entries below 0, or past the token's own block, are skipped.  At most 4096 entries
 
     A token sees the keys of its selected blocks up to its own position; one without a key gets zeros.  head_dim is 64, 128 or 256.
-    Values at positions up to the chunk's last in selected blocks must be finite; past a context, and in blocks that are not selected, the
-    caches may hold anything.  Scores and sums are float32; a key's weight is rounded to the query's type before it meets its value
+    Past a context, and in blocks that are not selected, the caches may hold anything; a value that is not finite reaches only tokens that
+    see it.  A block has at most 4096 tokens, less than 256 MB apart.  Scores and sums are float32; a key's weight is rounded to the query's type before it meets its value
     (in float16 also by 2^-30 of the row's largest), and so is the result."""
+    result = _lib.calls().sparse_attention(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, selected, scale, out)
+    if result is not None:
+        return result if type(result) is not int else _lib.check(result)
     check_query(query)
     _check_rows("key_cache", key_cache, 4)
     _check_rows("value_cache", value_cache, 4)

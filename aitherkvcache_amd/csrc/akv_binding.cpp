@@ -36,9 +36,15 @@ struct Library {
   decltype(&akv_dense_chunk_attn) dense_chunk;
   decltype(&akv_paged_chunk_attn_workspace_bytes) paged_chunk_bytes;
   decltype(&akv_paged_chunk_attn) paged_chunk;
+  decltype(&akv_block_index_update) index_update;
+  decltype(&akv_block_index_select_workspace_bytes) index_select_bytes;
+  decltype(&akv_block_index_select) index_select;
+  decltype(&akv_sparse_attn) sparse_attn;
+  decltype(&akv_key_weights_workspace_bytes) key_weights_bytes;
+  decltype(&akv_key_weights) key_weights;
 } g_lib;
 static_assert(std::is_same_v<decltype(&akv_hybrid_paged_attn), decltype(&akv_hybrid25_paged_attn)> && std::is_same_v<decltype(&akv_hybrid_encode_paged_kv), decltype(&akv_hybrid25_encode_paged_kv)>);
-constexpr int kFunctions = 17;
+constexpr int kFunctions = 23;
 PyObject* g_raw_stream = nullptr;      // torch's function: handle of the current stream of a device
 
 // the tensors of a call; ok() once all of them are plain device tensors of one device
@@ -327,7 +333,7 @@ PyObject* spectral_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return rc ? status(rc) : THPVariable_Wrap(std::move(out));
 }
 
-// ---- a chunk of new tokens: the three calls run on the current device only (on another one: the long way, which changes to it)
+// ---- a chunk of new tokens: the calls run on the current device only (on another one: the long way, which changes to it)
 bool here(const Tensors& ts) { return ts.ok() && c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index() == ts.device(); }
 bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 bool fits_int(int64_t v) { return v >= 0 && v <= INT_MAX; }
@@ -409,6 +415,121 @@ PyObject* packed_chunk(PyObject*, PyObject* const* a, Py_ssize_t n) {
                              out.stride(0), out.stride(1), (int)(a[18] == Py_None), (int)(qs.numel() - 1), q.size(0), (int)heads, (int)kv_heads, (int)d, (int)block, blocks, bt.size(1),
                              (int)v[7], (float)PyFloat_AS_DOUBLE(a[17]), ws.mutable_data_ptr(), (size_t)ws.numel(), stream);
   return result_of(rc, a[18], std::move(out));
+}
+
+// means of blocks as BlockIndex keeps them: codes [blocks, heads, d] and scales [blocks, heads]
+bool index_rows(const at::Tensor& codes, const at::Tensor& scales, int64_t blocks, int64_t heads, int64_t d) {
+  return codes.dim() == 3 && codes.scalar_type() == at::kChar && codes.is_contiguous() && codes.size(0) == blocks && codes.size(1) == heads && codes.size(2) == d && scales.dim() == 2 &&
+         scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.size(0) == blocks && scales.size(1) == heads;
+}
+bool plain_head(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+// (key cache, block_tables, context_lens, query_start_loc or None, codes, scales, blocks, kv heads, head size)
+PyObject* index_update(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t blocks, heads, d;
+  if (n != 9 || !integer(a[6], blocks) || !integer(a[7], heads) || !integer(a[8], d)) Py_RETURN_NONE;
+  static const at::Tensor none;
+  const bool some = a[3] != Py_None;
+  Tensors ts;
+  const at::Tensor &kc = ts.take(a[0]), &bt = ts.take(a[1]), &cl = ts.take(a[2]), &codes = ts.take(a[4]), &scales = ts.take(a[5]);
+  const at::Tensor& qs = some ? ts.take(a[3]) : none;
+  if (!ts.ok() || !here(ts) || !half_type(kc) || !dense_rows(kc, kc.scalar_type()) || kc.size(0) != blocks || kc.size(2) != heads || kc.size(3) != d || !plain_head(d) || kc.size(1) < 1 ||
+      !fits_int(kc.size(1)) || !fits_int(heads) || !index_rows(codes, scales, blocks, heads, d) || bt.dim() != 2 || bt.stride(1) != 1 || cl.dim() != 1 || !cl.is_contiguous() ||
+      index_code(bt) < 0 || index_code(cl) < 0)
+    Py_RETURN_NONE;
+  if (some && (qs.dim() != 1 || qs.numel() < 1 || !qs.is_contiguous() || index_code(qs) < 0)) Py_RETURN_NONE;
+  const int64_t seqs = some ? qs.numel() - 1 : cl.numel();
+  if (seqs < 1 || !fits_int(seqs) || bt.size(0) < seqs || cl.numel() < seqs) Py_RETURN_NONE;
+  // (a sequence has no more new tokens than its table has places)
+  const int64_t most = (1 << 30) - 1, places = std::min(bt.size(1), most) * std::min(kc.size(1), most);
+  const int64_t tokens = !some ? 0 : places > most / seqs ? most : seqs * places;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  return status(without_gil(g_lib.index_update, kc.const_data_ptr(), float_code(kc), kc.stride(0), kc.stride(1), kc.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0),
+                            cl.const_data_ptr(), index_code(cl), some ? qs.const_data_ptr() : nullptr, some ? index_code(qs) : 0, (int8_t*)codes.mutable_data_ptr(),
+                            (float*)scales.mutable_data_ptr(), (int)seqs, tokens, (int)heads, (int)d, (int)kc.size(1), blocks, bt.size(1), stream));
+}
+
+// (query, block_tables, context_lens, query_start_loc, codes, scales, out or None, blocks, kv heads, head size, block size, selected, sink and recent blocks)
+PyObject* index_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t v[7];
+  if (n != 14) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i)
+    if (!integer(a[7 + i], v[i]) || !fits_int(v[i])) Py_RETURN_NONE;
+  const int64_t blocks = v[0], heads = v[1], d = v[2], block = v[3], k = v[4], sinks = v[5], recent = v[6];
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &bt = ts.take(a[1]), &cl = ts.take(a[2]), &qs = ts.take(a[3]), &codes = ts.take(a[4]), &scales = ts.take(a[5]);
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs) || q.size(2) != d || !plain_head(d) || heads < 1 || q.size(1) % heads != 0 || block < 1 || recent < 1 || k - sinks < recent ||
+      !index_rows(codes, scales, blocks, heads, d))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  if (a[6] != Py_None) {
+    out = ts.take(a[6]);
+    if (!ts.ok() || out.dim() != 3 || out.size(0) != q.size(0) || out.size(1) != heads || out.size(2) != k || out.scalar_type() != at::kInt || !out.is_contiguous()) Py_RETURN_NONE;
+  }
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[6] == Py_None) out = at::empty({q.size(0), heads, k}, q.options().dtype(at::kInt));
+  const int64_t bytes = (int64_t)g_lib.index_select_bytes(q.size(0), (int)heads, bt.size(1));
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const int rc = without_gil(g_lib.index_select, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), (const int8_t*)codes.const_data_ptr(), (const float*)scales.const_data_ptr(),
+                             bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(), index_code(cl), qs.const_data_ptr(), index_code(qs), (int32_t*)out.mutable_data_ptr(),
+                             (int)(qs.numel() - 1), q.size(0), (int)q.size(1), (int)heads, (int)d, (int)block, blocks, bt.size(1), (int)k, (int)sinks, (int)recent,
+                             bytes > 0 ? ws.mutable_data_ptr() : nullptr, (size_t)bytes, stream);
+  return result_of(rc, a[6], std::move(out));
+}
+
+// (query, key cache, value cache, block_tables, context_lens, query_start_loc, selected, scale or None, out or None)
+PyObject* sparse_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 9 || (a[7] != Py_None && !PyFloat_CheckExact(a[7]))) Py_RETURN_NONE;
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &kc = ts.take(a[1]), &vc = ts.take(a[2]), &bt = ts.take(a[3]), &cl = ts.take(a[4]), &qs = ts.take(a[5]), &sel = ts.take(a[6]);
+  at::Tensor out;
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs) || !chunk_result(ts, a[8], q, out)) Py_RETURN_NONE;
+  const int64_t heads = q.size(1), d = q.size(2);
+  if (!dense_rows(kc, q.scalar_type()) || !dense_rows(vc, q.scalar_type()) || kc.sizes().slice(1) != vc.sizes().slice(1) || kc.size(3) != d || kc.size(2) == 0 || heads % kc.size(2) != 0 ||
+      !fits_int(kc.size(1)) || !plain_head(d) || sel.dim() != 3 || sel.size(0) != q.size(0) || sel.size(1) != kc.size(2) || sel.scalar_type() != at::kInt || sel.stride(2) != 1 ||
+      !fits_int(sel.size(2)))
+    Py_RETURN_NONE;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[8] == Py_None) out = at::empty(q.sizes(), q.options());
+  const float scale = a[7] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)PyFloat_AS_DOUBLE(a[7]);
+  const int rc = without_gil(g_lib.sparse_attn, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), kc.const_data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
+                             vc.const_data_ptr(), vc.stride(0), vc.stride(1), vc.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(), index_code(cl),
+                             qs.const_data_ptr(), index_code(qs), (const int32_t*)sel.const_data_ptr(), sel.stride(0), sel.stride(1), (int)sel.size(2), out.mutable_data_ptr(),
+                             out.stride(0), out.stride(1), (int)(a[8] == Py_None), (int)(qs.numel() - 1), q.size(0), (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1),
+                             std::min(kc.size(0), vc.size(0)), bt.size(1), scale, stream);
+  return result_of(rc, a[8], std::move(out));
+}
+
+// (query, key cache, block_tables, context_lens, query_start_loc, accumulated or None, scale or None)
+PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7 || (a[6] != Py_None && !PyFloat_CheckExact(a[6]))) Py_RETURN_NONE;
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &kc = ts.take(a[1]), &bt = ts.take(a[2]), &cl = ts.take(a[3]), &qs = ts.take(a[4]);
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs)) Py_RETURN_NONE;
+  const int64_t heads = q.size(1), d = q.size(2), seqs = qs.numel() - 1;
+  if (!dense_rows(kc, q.scalar_type()) || kc.size(3) != d || kc.size(2) == 0 || heads % kc.size(2) != 0 || !fits_int(kc.size(1)) || !plain_head(d) || !fits_int(bt.size(1))) Py_RETURN_NONE;
+  const int64_t places = bt.size(1) * kc.size(1);
+  at::Tensor w;
+  if (a[5] != Py_None) {
+    w = ts.take(a[5]);
+    if (!ts.ok() || w.dim() != 3 || w.scalar_type() != at::kFloat || w.size(0) < seqs || w.size(1) != kc.size(2) || w.size(2) < places || w.stride(2) != 1 || w.stride(1) == 0 || w.stride(0) == 0)
+      Py_RETURN_NONE;
+  }
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[5] == Py_None) w = at::empty({seqs, kc.size(2), places}, q.options().dtype(at::kFloat));
+  const int64_t bytes = (int64_t)g_lib.key_weights_bytes(q.size(0), (int)seqs, (int)heads, (int)kc.size(2), (int)d, w.size(2));
+  const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const float scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)PyFloat_AS_DOUBLE(a[6]);
+  const int rc = without_gil(g_lib.key_weights, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), kc.const_data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
+                             bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(), index_code(cl), qs.const_data_ptr(), index_code(qs), (float*)w.mutable_data_ptr(),
+                             w.stride(0), w.stride(1), w.size(2), (int)(a[5] != Py_None), (int)seqs, q.size(0), (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1), kc.size(0), bt.size(1),
+                             scale, bytes > 0 ? ws.mutable_data_ptr() : nullptr, (size_t)bytes, stream);
+  return result_of(rc, a[5], std::move(w));
 }
 
 // (query or None, key, value, positions, table or None, slot_mapping, key cache, value cache, sections (tuple or list) or None,
@@ -502,6 +623,10 @@ PyMethodDef kMethods[] = {
     {"rope_append", (PyCFunction)(void (*)(void))guarded<rope_append>, METH_FASTCALL, nullptr},
     {"dense_chunk", (PyCFunction)(void (*)(void))guarded<dense_chunk>, METH_FASTCALL, nullptr},
     {"packed_chunk", (PyCFunction)(void (*)(void))guarded<packed_chunk>, METH_FASTCALL, nullptr},
+    {"index_update", (PyCFunction)(void (*)(void))guarded<index_update>, METH_FASTCALL, nullptr},
+    {"index_select", (PyCFunction)(void (*)(void))guarded<index_select>, METH_FASTCALL, nullptr},
+    {"sparse_attention", (PyCFunction)(void (*)(void))guarded<sparse_attention>, METH_FASTCALL, nullptr},
+    {"key_weights", (PyCFunction)(void (*)(void))guarded<key_weights>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

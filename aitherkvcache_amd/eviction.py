@@ -43,6 +43,9 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, block_tables
 
     To weigh a prompt by its last tokens pass those tokens only.  head_dim is 64, 128 or 256.  Keys of a context must be finite; past it the
     cache may hold anything.  Scores, weights and sums are float32."""
+    result = _lib.calls().key_weights(query, key_cache, block_tables, context_lens, query_start_loc, accumulated, scale)
+    if result is not None:
+        return result if type(result) is not int else _lib.check(result)
     check_query(query)
     _check_rows("key_cache", key_cache, 4)
     num_tokens, num_q_heads, d = query.shape

@@ -576,8 +576,8 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  *   of no sequence, or before the first key, have -1.
  * akv_sparse_attn: attention of every new token over the keys at its position and before in the blocks its kv head has
  *   selected (a set: order and repetition do not matter; entries below 0 or past the token's own block are skipped); a row without a key
- *   is zero.  selected has strides ss_tok / ss_head, at most 4096 entries a list.  zero_tail as above.  Values at the
- *   positions up to the chunk's last in a selected block must be finite.  Blocks of at most 4096 tokens.
+ *   is zero.  selected has strides ss_tok / ss_head, at most 4096 entries a list.  zero_tail as above.  A value
+ *   that is not finite reaches only tokens that see it.  Blocks of at most 4096 tokens, less than 2^27 elements apart.
  * akv_key_weights: weights [num_seqs][num_kv_heads][length] float32 (strides ws_seq / ws_head, length >= max_blocks_per_seq x block_size): the
  *   softmax weight of every key summed over the sequence's new tokens and the group's heads; accumulate: added to what is there (only
  *   keys of the context are touched), otherwise written, zeros elsewhere.
