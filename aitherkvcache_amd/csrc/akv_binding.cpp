@@ -42,9 +42,12 @@ struct Library {
   decltype(&akv_sparse_attn) sparse_attn;
   decltype(&akv_key_weights_workspace_bytes) key_weights_bytes;
   decltype(&akv_key_weights) key_weights;
+  decltype(&akv_packed_key_weights_workspace_bytes) packed_weights_bytes;
+  decltype(&akv_packed_key_weights) packed_weights;
+  decltype(&akv_evict) evict;
 } g_lib;
 static_assert(std::is_same_v<decltype(&akv_hybrid_paged_attn), decltype(&akv_hybrid25_paged_attn)> && std::is_same_v<decltype(&akv_hybrid_encode_paged_kv), decltype(&akv_hybrid25_encode_paged_kv)>);
-constexpr int kFunctions = 23;
+constexpr int kFunctions = 26;
 PyObject* g_raw_stream = nullptr;      // torch's function: handle of the current stream of a device
 
 // the tensors of a call; ok() once all of them are plain device tensors of one device
@@ -504,6 +507,13 @@ PyObject* sparse_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return result_of(rc, a[8], std::move(out));
 }
 
+// where weights go: `given`, or a new tensor
+bool weights_result(Tensors& ts, PyObject* given, int64_t seqs, int64_t heads, int64_t places, at::Tensor& w) {
+  if (given == Py_None) return true;
+  w = ts.take(given);
+  return ts.ok() && w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) >= seqs && w.size(1) == heads && w.size(2) >= places && w.stride(2) == 1 && w.stride(1) != 0 && w.stride(0) != 0;
+}
+
 // (query, key cache, block_tables, context_lens, query_start_loc, accumulated or None, scale or None)
 PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 7 || (a[6] != Py_None && !PyFloat_CheckExact(a[6]))) Py_RETURN_NONE;
@@ -514,11 +524,7 @@ PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!dense_rows(kc, q.scalar_type()) || kc.size(3) != d || kc.size(2) == 0 || heads % kc.size(2) != 0 || !fits_int(kc.size(1)) || !plain_head(d) || !fits_int(bt.size(1))) Py_RETURN_NONE;
   const int64_t places = bt.size(1) * kc.size(1);
   at::Tensor w;
-  if (a[5] != Py_None) {
-    w = ts.take(a[5]);
-    if (!ts.ok() || w.dim() != 3 || w.scalar_type() != at::kFloat || w.size(0) < seqs || w.size(1) != kc.size(2) || w.size(2) < places || w.stride(2) != 1 || w.stride(1) == 0 || w.stride(0) == 0)
-      Py_RETURN_NONE;
-  }
+  if (!weights_result(ts, a[5], seqs, kc.size(2), places, w)) Py_RETURN_NONE;
   void* stream;
   if (!stream_of(ts.device(), stream)) return nullptr;
   if (a[5] == Py_None) w = at::empty({seqs, kc.size(2), places}, q.options().dtype(at::kFloat));
@@ -530,6 +536,96 @@ PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
                              w.stride(0), w.stride(1), w.size(2), (int)(a[5] != Py_None), (int)seqs, q.size(0), (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1), kc.size(0), bt.size(1),
                              scale, bytes > 0 ? ws.mutable_data_ptr() : nullptr, (size_t)bytes, stream);
   return result_of(rc, a[5], std::move(w));
+}
+
+// (query, k_packed, k_norms, block_tables, context_lens, query_start_loc, centroids, accumulated or None, prepared rotation, kv heads or
+//  None, query heads, head size, bytes of a row, bits, block size, scale)
+PyObject* packed_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t v[7];
+  if (n != 16 || !PyFloat_CheckExact(a[15])) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i)
+    if (!integer(a[8 + i], v[i], 0, i == 1)) Py_RETURN_NONE;
+  Tensors ts;
+  const at::Tensor &q = ts.take(a[0]), &kp = ts.take(a[1]), &kn = ts.take(a[2]), &bt = ts.take(a[3]), &cl = ts.take(a[4]), &qs = ts.take(a[5]), &cen = ts.take(a[6]);
+  const int64_t heads = v[2], d = v[3], row = v[4], bits = v[5], block = v[6];
+  if (!ts.ok() || !here(ts) || !chunk_inputs(q, bt, cl, qs) || q.size(1) != heads || q.size(2) != d || kp.dim() != 4 || bits < 2 || bits > 4 || cen.numel() != 1 << bits ||
+      !floats(cen, 1 << bits) || block < 1 || !fits_int(block) || !plain_head(d) || !fits_int(bt.size(1)))
+    Py_RETURN_NONE;
+  const int64_t kv_heads = a[9] == Py_None ? kp.size(2) : v[1], seqs = qs.numel() - 1, places = bt.size(1) * block;
+  if (kv_heads <= 0 || heads % kv_heads != 0 || !packed_rows(kp, row, block, kv_heads) || !norm_rows(kn, block, kv_heads)) Py_RETURN_NONE;
+  at::Tensor w;
+  if (!weights_result(ts, a[7], seqs, kv_heads, places, w)) Py_RETURN_NONE;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  if (a[7] == Py_None) w = at::empty({seqs, kv_heads, places}, q.options().dtype(at::kFloat));
+  const int64_t bytes = (int64_t)g_lib.packed_weights_bytes(q.size(0), (int)seqs, (int)heads, (int)kv_heads, (int)d, w.size(2));
+  const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const int rc = without_gil(g_lib.packed_weights, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), (const uint8_t*)kp.const_data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
+                             (const float*)kn.const_data_ptr(), kn.stride(0), kn.stride(1), kn.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(),
+                             index_code(cl), qs.const_data_ptr(), index_code(qs), (const void*)(uintptr_t)v[0], (const float*)cen.const_data_ptr(), (int)bits, (float*)w.mutable_data_ptr(),
+                             w.stride(0), w.stride(1), w.size(2), (int)(a[7] != Py_None), (int)seqs, q.size(0), (int)heads, (int)kv_heads, (int)d, (int)block,
+                             std::min(kp.size(0), kn.size(0)), bt.size(1), (float)PyFloat_AS_DOUBLE(a[15]), bytes > 0 ? ws.mutable_data_ptr() : nullptr, (size_t)bytes, stream);
+  return result_of(rc, a[7], std::move(w));
+}
+
+// (weights, block_tables, context_lens, caches (list or tuple), keep, first and last tokens that stay, out_tables or None)
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t v[3];
+  if (n != 8 || (!PyList_CheckExact(a[3]) && !PyTuple_CheckExact(a[3]))) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!integer(a[4 + i], v[i]) || v[i] < 0 || v[i] > 1 << 30) Py_RETURN_NONE;
+  const int64_t keep = v[0], sinks = v[1], recent = v[2];
+  const bool list = PyList_CheckExact(a[3]), moves_out = a[7] != Py_None;
+  const Py_ssize_t count = list ? PyList_GET_SIZE(a[3]) : PyTuple_GET_SIZE(a[3]);
+  if (count < 1 || count > AKV_EVICT_CACHES || keep < 1 || keep < sinks + recent) Py_RETURN_NONE;
+  static const at::Tensor none;
+  Tensors ts;
+  const at::Tensor &w = ts.take(a[0]), &bt = ts.take(a[1]), &cl = ts.take(a[2]);
+  const at::Tensor& ot = moves_out ? ts.take(a[7]) : none;
+  if (!ts.ok() || !here(ts) || w.dim() != 3 || w.scalar_type() != at::kFloat || w.stride(2) != 1 || w.stride(1) == 0 || w.stride(0) == 0 || w.size(1) < 1 || !fits_int(w.size(1)) ||
+      bt.dim() != 2 || bt.stride(1) != 1 || index_code(bt) < 0 || cl.dim() != 1 || !cl.is_contiguous() || index_code(cl) < 0)
+    Py_RETURN_NONE;
+  const int64_t seqs = cl.numel(), heads = w.size(1);
+  if (seqs < 1 || !fits_int(seqs) || bt.size(0) < seqs || w.size(0) < seqs) Py_RETURN_NONE;
+  akv_evict_cache held[AKV_EVICT_CACHES];
+  int64_t block = 0, blocks = 0;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const at::Tensor& t = ts.take(list ? PyList_GET_ITEM(a[3], i) : PyTuple_GET_ITEM(a[3], i));
+    if (!ts.ok() || t.dim() < 3 || t.numel() == 0 || t.size(2) != heads) Py_RETURN_NONE;
+    int64_t row = 1;
+    for (int64_t j = t.dim() - 1; j >= 3; --j) {
+      if (t.size(j) != 1 && t.stride(j) != row) Py_RETURN_NONE;
+      row *= t.size(j);
+    }
+    if (i == 0) block = t.size(1), blocks = t.size(0);
+    if (t.size(1) != block || !fits_int(block)) Py_RETURN_NONE;
+    blocks = std::min(blocks, t.size(0));
+    const int64_t size = t.element_size();
+    held[i] = {t.mutable_data_ptr(), t.stride(0) * size, t.stride(1) * size, t.stride(2) * size, row * size};
+  }
+  if (!fits_int(bt.size(1)) || w.size(2) != bt.size(1) * block || w.size(2) == 0) Py_RETURN_NONE;
+  if (moves_out && (ot.dim() != 2 || ot.size(0) < seqs || !fits_int(ot.size(1)) || ot.size(1) * block < std::min(keep, w.size(2)) || ot.stride(1) != 1 || index_code(ot) < 0)) Py_RETURN_NONE;
+  void* stream;
+  if (!stream_of(ts.device(), stream)) return nullptr;
+  at::Tensor kept = at::empty({seqs, heads, keep}, w.options().dtype(at::kInt)), left = at::empty({seqs, heads, w.size(2)}, w.options()), now = at::empty({seqs}, cl.options());
+  const int rc = without_gil(g_lib.evict, (const float*)w.const_data_ptr(), w.stride(0), w.stride(1), w.size(2), cl.const_data_ptr(), index_code(cl), (int)seqs, (int)heads, (int)keep,
+                             (int)sinks, (int)recent, (int32_t*)kept.mutable_data_ptr(), kept.stride(0), kept.stride(1), (float*)left.mutable_data_ptr(), left.stride(0), left.stride(1),
+                             now.mutable_data_ptr(), bt.const_data_ptr(), index_code(bt), bt.stride(0), bt.size(1), moves_out ? ot.const_data_ptr() : nullptr,
+                             moves_out ? index_code(ot) : 0, moves_out ? ot.stride(0) : 0, moves_out ? ot.size(1) : 0, (const akv_evict_cache*)held, (int)count, (int)block, blocks,
+                             stream);
+  if (rc) return status(rc);
+  PyObject* result = PyTuple_New(3);
+  if (!result) return nullptr;
+  at::Tensor* const three[] = {&kept, &now, &left};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* t = THPVariable_Wrap(std::move(*three[i]));
+    if (!t) {
+      Py_DECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, i, t);
+  }
+  return result;
 }
 
 // (query or None, key, value, positions, table or None, slot_mapping, key cache, value cache, sections (tuple or list) or None,
@@ -627,6 +723,8 @@ PyMethodDef kMethods[] = {
     {"index_select", (PyCFunction)(void (*)(void))guarded<index_select>, METH_FASTCALL, nullptr},
     {"sparse_attention", (PyCFunction)(void (*)(void))guarded<sparse_attention>, METH_FASTCALL, nullptr},
     {"key_weights", (PyCFunction)(void (*)(void))guarded<key_weights>, METH_FASTCALL, nullptr},
+    {"packed_weights", (PyCFunction)(void (*)(void))guarded<packed_weights>, METH_FASTCALL, nullptr},
+    {"evict", (PyCFunction)(void (*)(void))guarded<evict>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -426,3 +426,14 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
   }
   return AKV_OK;
 }
+
+extern "C" int akv_evict(const float* weights, int64_t ws_seq, int64_t ws_head, int64_t length, const void* context_lens, int cl_itype, int num_seqs, int num_kv_heads, int keep,
+                         int num_sink, int num_recent, int32_t* kept, int64_t ks_seq, int64_t ks_head, float* kept_weights, int64_t os_seq, int64_t os_head, void* kept_lens,
+                         const void* block_tables, int bt_itype, int64_t bt_stride, int64_t max_blocks_per_seq, const void* out_tables, int ot_itype, int64_t ot_stride,
+                         int64_t out_blocks_per_seq, const akv_evict_cache* caches, int num_caches, int block_size, int64_t num_blocks, void* stream) {
+  if (const int rc = akv_evict_select(weights, ws_seq, ws_head, length, context_lens, cl_itype, num_seqs, num_kv_heads, keep, num_sink, num_recent, kept, ks_seq, ks_head, kept_weights,
+                                      os_seq, os_head, kept_lens, stream))
+    return rc;
+  return akv_evict_move(kept, ks_seq, ks_head, kept_lens, cl_itype, keep, block_tables, bt_itype, bt_stride, max_blocks_per_seq, out_tables, ot_itype, ot_stride, out_blocks_per_seq, caches,
+                        num_caches, num_seqs, num_kv_heads, block_size, num_blocks, stream);
+}

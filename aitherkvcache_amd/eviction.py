@@ -94,6 +94,9 @@ def evict_tokens(weights: torch.Tensor, block_tables: torch.Tensor, context_lens
     Returns (kept [num_seqs, num_kv_heads, keep] int32: positions in ascending order, -1 behind the last; the sequences' lengths now, in
     the type of context_lens; weights of the tokens that stayed, at their new positions, zeros behind, in a new tensor).  Rows behind the
     tokens that stayed are left as they were.  Positions that are part of a key (rotary ones) stay in it."""
+    result = _lib.calls().evict(weights, block_tables, context_lens, caches, keep, num_sink, num_recent, out_tables)
+    if result is not None:
+        return result if type(result) is not int else _lib.check(result)
     check_weights("weights", weights, 0, None, 0)
     if block_tables.dim() != 2 or context_lens.dim() != 1:
         raise ValueError("expected block_tables [num_seqs, blocks] and context_lens [num_seqs]")

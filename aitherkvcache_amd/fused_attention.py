@@ -237,6 +237,12 @@ class TQPagedAttention:
         tq = self._tq
         if tq.rotation is not self.rotation:
             self.rotation = tq.rotation
+        if query.is_cuda:
+            result = _lib.calls().packed_weights(query, k_packed, k_norms, block_tables, context_lens, query_start_loc, self.centroids, accumulated,
+                                                 tq.prepared_rotation().ptr, num_kv_heads, self.num_query_heads, self.head_dim, self.packed_dim,
+                                                 self.bits, block_size, self.scale)
+            if result is not None:
+                return result if type(result) is not int else _lib.check(result)
         check_query(query)
         if k_packed.dim() != 4 or k_norms.dim() != 3:
             raise ValueError("expected a cache [blocks, block_size, heads, bytes] and norms [blocks, block_size, heads]")

@@ -589,6 +589,7 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  * akv_evict_move: rows of up to AKV_EVICT_CACHES caches [num_blocks][block_size][num_kv_heads][row_bytes] (byte strides): position kept[j] to position
  *   j, in the blocks of out_tables, which no sequence of the call may read, or in place (out_tables NULL; no two sequences may
  *   share a block then).  caches is a host pointer.
+ * akv_evict: akv_evict_select, then akv_evict_move by what it chose.
  * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must not overlap in time.
  * ------------------------------------------------------------------------------- */
 int akv_block_index_update(const void* key_cache, int dtype, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
@@ -644,6 +645,12 @@ int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_head, const v
                    const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq,
                    const akv_evict_cache* caches, int num_caches,
                    int num_seqs, int num_kv_heads, int block_size, int64_t num_blocks, void* stream);
+int akv_evict(const float* weights, int64_t ws_seq, int64_t ws_head, int64_t length,
+              const void* context_lens, int cl_itype, int num_seqs, int num_kv_heads, int keep, int num_sink, int num_recent,
+              int32_t* kept, int64_t ks_seq, int64_t ks_head, float* kept_weights, int64_t os_seq, int64_t os_head, void* kept_lens,
+              const void* block_tables, int bt_itype, int64_t bt_stride, int64_t max_blocks_per_seq,
+              const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq,
+              const akv_evict_cache* caches, int num_caches, int block_size, int64_t num_blocks, void* stream);
 
 #ifdef __cplusplus
 }

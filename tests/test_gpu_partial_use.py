@@ -37,9 +37,15 @@ def test_binding_and_long_way_give_the_same(dev, monkeypatch, dtype, index):
             assert akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, into, 0.2, out=out) is out
             acc = torch.full((3, 2, b.tables.shape[1] * 16 + 3), 2.0, device=dev)
             assert akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts, accumulated=acc, scale=0.3) is acc
-            got.append([part, ix.codes, ix.scales, sel, into, out, acc, akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel),
+            p = Packed(b, 128, 4, 8, 2, dtype, dev, 41, primary=True)
+            packed = p.attn.key_weights(p.q, p.k, p.kn, b.tables, b.ctx, b.starts)
+            more = packed.clone()
+            assert p.attn.key_weights(p.q, p.k, p.kn, b.tables, b.ctx, b.starts, num_kv_heads=2, accumulated=more) is more
+            k2, v2, k3, v3 = k.clone(), v.clone(), torch.cat([k, k]), torch.cat([v, v])
+            cuts = [*akv.evict_tokens(packed, b.tables, b.ctx, [k2, v2, p.k, p.kn], 60), *akv.evict_tokens(more, b.tables, b.ctx, (k3, v3), 60, 3, 4, b.tables[:, :4] + b.blocks)]
+            got.append([packed, more, k2, v2, k3, v3, *cuts, part, ix.codes, ix.scales, sel, into, out, acc, akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel),
                         akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts)])
-            assert c.taken == (8 if take else 0)
+            assert c.taken == (12 if take else 0)
     for x, y in zip(*got):
         assert torch.equal(x, y)
 
