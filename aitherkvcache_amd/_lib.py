@@ -126,9 +126,10 @@ SIGNATURES = {
     "akv_block_index_select_workspace_bytes": (_sz, [_i64, _i, _i64]),
     "akv_block_index_select": (_i, [_p, _i, _i64, _i64, _p, _p, _p, _i, _i64, _p, _i, _p, _i, _p,
                                     _i, _i64, _i, _i, _i, _i, _i64, _i64, _i, _i, _i, _p, _sz, _p]),
+    "akv_sparse_attn_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i]),
     "akv_sparse_attn": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                              _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i, _p, _i64, _i64, _i,
-                             _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p]),
+                             _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
     "akv_key_weights_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i64]),
     "akv_key_weights": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i, _i64, _p, _i, _p, _i, _p, _i64, _i64, _i64, _i,
                              _i, _i64, _i, _i, _i, _i, _i64, _i64, _f, _p, _sz, _p]),
@@ -157,7 +158,7 @@ _BOUND = ("akv_paged_attn_workspace_bytes", "akv_paged_attn", "akv_encode_paged_
           "akv_decode_blocks_kv", "akv_tri_encode_paged_kv", "akv_tri_decode_workspace_bytes", "akv_tri_decode_paged",
           "akv_rope_append", "akv_dense_chunk_attn_workspace_bytes", "akv_dense_chunk_attn", "akv_paged_chunk_attn_workspace_bytes",
           "akv_paged_chunk_attn", "akv_block_index_update", "akv_block_index_select_workspace_bytes", "akv_block_index_select",
-          "akv_sparse_attn", "akv_key_weights_workspace_bytes", "akv_key_weights",
+          "akv_sparse_attn_workspace_bytes", "akv_sparse_attn", "akv_key_weights_workspace_bytes", "akv_key_weights",
           "akv_packed_key_weights_workspace_bytes", "akv_packed_key_weights", "akv_evict")
 
 

@@ -163,13 +163,15 @@ def paged_sparse_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
         _check_out("out", out, query)
     dev = _lib.require_gpu(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, selected, out)
     result = out if out is not None else torch.empty((num_tokens, num_q_heads, d), dtype=query.dtype, device=dev)
+    L = _lib.lib()
+    ws = torch.empty(L.akv_sparse_attn_workspace_bytes(num_tokens, num_seqs, num_q_heads, kv_heads, d, block_size, sel.shape[2]), dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
-        _lib.check(_lib.lib().akv_sparse_attn(
+        _lib.check(L.akv_sparse_attn(
             q.data_ptr(), _lib.dtype_code(q), q.stride(0), q.stride(1),
             key_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),
             value_cache.data_ptr(), value_cache.stride(0), value_cache.stride(1), value_cache.stride(2),
             bt.data_ptr(), _lib.itype_code(bt), bt.stride(0), lens.data_ptr(), _lib.itype_code(lens), starts.data_ptr(), _lib.itype_code(starts),
             sel.data_ptr(), sel.stride(0), sel.stride(1), sel.shape[2], result.data_ptr(), result.stride(0), result.stride(1), int(out is None),
             num_seqs, num_tokens, num_q_heads, kv_heads, d, block_size, min(blocks, value_cache.shape[0]), bt.shape[1],
-            1.0 / math.sqrt(d) if scale is None else scale, _lib.stream_ptr(dev)))
+            1.0 / math.sqrt(d) if scale is None else scale, ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
     return result

@@ -39,6 +39,7 @@ struct Library {
   decltype(&akv_block_index_update) index_update;
   decltype(&akv_block_index_select_workspace_bytes) index_select_bytes;
   decltype(&akv_block_index_select) index_select;
+  decltype(&akv_sparse_attn_workspace_bytes) sparse_bytes;
   decltype(&akv_sparse_attn) sparse_attn;
   decltype(&akv_key_weights_workspace_bytes) key_weights_bytes;
   decltype(&akv_key_weights) key_weights;
@@ -47,7 +48,7 @@ struct Library {
   decltype(&akv_evict) evict;
 } g_lib;
 static_assert(std::is_same_v<decltype(&akv_hybrid_paged_attn), decltype(&akv_hybrid25_paged_attn)> && std::is_same_v<decltype(&akv_hybrid_encode_paged_kv), decltype(&akv_hybrid25_encode_paged_kv)>);
-constexpr int kFunctions = 26;
+constexpr int kFunctions = 27;
 PyObject* g_raw_stream = nullptr;      // torch's function: handle of the current stream of a device
 
 // the tensors of a call; ok() once all of them are plain device tensors of one device
@@ -498,12 +499,15 @@ PyObject* sparse_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream;
   if (!stream_of(ts.device(), stream)) return nullptr;
   if (a[8] == Py_None) out = at::empty(q.sizes(), q.options());
+  const int64_t bytes = (int64_t)g_lib.sparse_bytes(q.size(0), (int)(qs.numel() - 1), (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1), (int)sel.size(2));
+  at::Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
   const float scale = a[7] == Py_None ? (float)(1.0 / std::sqrt((double)d)) : (float)PyFloat_AS_DOUBLE(a[7]);
   const int rc = without_gil(g_lib.sparse_attn, q.const_data_ptr(), float_code(q), q.stride(0), q.stride(1), kc.const_data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
                              vc.const_data_ptr(), vc.stride(0), vc.stride(1), vc.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0), cl.const_data_ptr(), index_code(cl),
                              qs.const_data_ptr(), index_code(qs), (const int32_t*)sel.const_data_ptr(), sel.stride(0), sel.stride(1), (int)sel.size(2), out.mutable_data_ptr(),
                              out.stride(0), out.stride(1), (int)(a[8] == Py_None), (int)(qs.numel() - 1), q.size(0), (int)heads, (int)kc.size(2), (int)d, (int)kc.size(1),
-                             std::min(kc.size(0), vc.size(0)), bt.size(1), scale, stream);
+                             std::min(kc.size(0), vc.size(0)), bt.size(1), scale, bytes > 0 ? ws.mutable_data_ptr() : nullptr, (size_t)bytes, stream);
   return result_of(rc, a[8], std::move(out));
 }
 

@@ -23,6 +23,8 @@ struct sa_args {
   int parts; uint32_t parts_recip;      // groups of sixteen keys a block
   int tail;
   float scale2;
+  int splits;                           // workgroups that share a tile's keys
+  float* part; float2* part_ml;         // of splits > 1, [T][QH][splits]: sums of D coordinates; largest score, sum of weights
 };
 
 #define SA_FRAME 8.f
@@ -31,14 +33,15 @@ template <int DT> constexpr float SA_LIFT = DT == AKV_BF16 ? 0.f : 5.f;
 
 // Of a wavefront in LDS, behind bitmaps (or in their place) and before lists: 32 keys, then in their place 32 values, then 64 coordinates of its sums.
 // Rows lie apart so that the operands' reads meet no bank twice: sixteen bytes more for keys, 32 for transposing reads of values.
-template <int D, int W> struct sa_lds {
+template <int D> struct sa_lds {
+  static constexpr int W = 4;           // wavefronts
   static constexpr int K_ROW = 2 * D + 16, V_ROW = 2 * D + 32, WAVE = 32 * V_ROW, AREA = W * (WAVE > 8192 ? WAVE : 8192) + 32 * K_ROW;
 };
 
-template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 : D == 256 ? 1 : D == 128 ? 3 : 4) void sa_kernel(sa_args a) {
-  typedef sa_lds<D, W> P;
+template <int D, int DT> __global__ __launch_bounds__(256, D == 256 ? 1 : D == 128 ? 3 : 4) void sa_kernel(sa_args a) {
+  typedef sa_lds<D> P;
   typedef ab_math<DT> M;
-  constexpr int KS = D / 16, OT = D / 32, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, THREADS = 64 * W;
+  constexpr int KS = D / 16, OT = D / 32, LPR = D / 8, RPI = 64 / LPR, VI = 32 / RPI, W = P::W, THREADS = 64 * W;
   extern __shared__ __align__(1024) unsigned char lds[];
   __shared__ int wave_sum[W];
   __shared__ float2 ml[W][32];
@@ -50,7 +53,7 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 :
 
   // rows before the first sequence, by all workgroups
   const int front = a.tail ? ab_start(a.b, 0) : 0;
-  if (front > 0) {
+  if (front > 0 && blockIdx.y == 0) {
     const int64_t per = (int64_t)a.QH * (D / 4);
     for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < front * per; i += (int64_t)gridDim.x * THREADS) {
       const int64_t token = i / per, rest = i - token * per, hd = rest / (D / 4);
@@ -181,15 +184,16 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 :
     ab_u4 x[VI];             // keys or values on their way
     unit now = {};
     entry ahead = {};
-    if (wave < units) {
-      now = find(look(wave));
-      ahead = look(wave + W);
+    const int mine0 = (int)blockIdx.y * W + wave, stride = a.splits * W;
+    if (mine0 < units) {
+      now = find(look(mine0));
+      ahead = look(mine0 + stride);
       request(x, now.k, now.left, k_off, k_pos);
     }
-    for (int p = wave; p < units; p += W) {
-      const bool more = p + W < units;
+    for (int p = mine0; p < units; p += stride) {
+      const bool more = p + stride < units;
       const unit next = find(ahead);
-      ahead = look(p + 2 * W);
+      ahead = look(p + 2 * stride);
       akv_wave_sync();                   // (the values before have been read)
 #pragma unroll
       for (int i = 0; i < VI; ++i) *(lds_u4*)(uintptr_t)(at + (RPI * i + lane / LPR) * P::K_ROW + 16 * (lane % LPR)) = x[i];
@@ -276,6 +280,8 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 :
     uint32_t most = 0u;      // of the sums' bits without the sign: 0x7f800000 or more where one is not finite
     uint16_t* const to = (uint16_t*)a.out + (int64_t)(first + t_row) * a.os_tok + (int64_t)(kvh * a.G + g_row) * a.os_head + 4 * half;
     float4* const part = (float4*)lds;
+    const int64_t place = ((int64_t)(first + t_row) * a.QH + kvh * a.G + g_row) * a.splits + blockIdx.y;
+    if (a.splits > 1 && wave == 0 && half == 0 && valid && (only < 0 || t_row == only)) a.part_ml[place] = make_float2(top, sum);
 #pragma unroll
     for (int d0 = 0; d0 < OT; d0 += 2) {
       // 64 coordinates at a time; of their eight groups of 4 + 4 (a lane of each half four) a wavefront adds 8 / W
@@ -297,7 +303,9 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 :
         }
         if (valid) {
           most = max(max(most, max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu)), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
-          if (only < 0 || t_row == only) *(ab_u2*)(to + 32 * d0 + 8 * i) = (ab_u2){M::pair(y.x * inv, y.y * inv), M::pair(y.z * inv, y.w * inv)};
+          if (only >= 0 && t_row != only) continue;
+          if (a.splits == 1) *(ab_u2*)(to + 32 * d0 + 8 * i) = (ab_u2){M::pair(y.x * inv, y.y * inv), M::pair(y.z * inv, y.w * inv)};
+          else *(float4*)(a.part + place * D + 4 * half + 32 * d0 + 8 * i) = y;
         }
       }
     }
@@ -308,11 +316,40 @@ template <int D, int DT, int W> __global__ __launch_bounds__(64 * W, W > 4 ? 2 :
   }
 }
 
+// The sums of the workgroups that share a tile's keys: a wavefront a row
+template <int D, int DT> __global__ __launch_bounds__(256) void sa_join_kernel(sa_args a) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), token = row / a.QH;
+  if (token >= a.b.T || token < ab_start(a.b, 0) || (!a.tail && token >= ab_start(a.b, a.b.S))) return;
+  const float2* const ml = a.part_ml + row * a.splits;
+  const float* const from = a.part + row * a.splits * D + N * lane;
+  float top = -INFINITY, sum = 0.f, y[N] = {};
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s].x);
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[s].x - top);
+    sum = fmaf(ml[s].y, f, sum);
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = fmaf(from[(int64_t)s * D + i], f, y[i]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* const to = (uint16_t*)a.out + token * a.os_tok + (row - token * a.QH) * a.os_head + N * lane;
+  if constexpr (N == 1) *to = (uint16_t)ab_math<DT>::pair(y[0] * inv, 0.f);
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *(uint32_t*)(to + i) = ab_math<DT>::pair(y[i] * inv, y[i + 1] * inv);
+}
+
 #define SA_LDS (150 << 10)
 #define SA_MOST_SELECTED 4096
+#define SA_SPLITS 8
 #define SA_MOST_STRIDE ((1ll << 27) - 1)          // of a block's tokens: sixteen of them within 2^32 bytes
-template <int D, int DT, int W> static int sa_run(sa_args a, hipStream_t stream) {
-  typedef sa_lds<D, W> P;
+template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
+  typedef sa_lds<D> P;
+  a.parts = (a.b.block_size + 15) / 16;
+  a.parts_recip = (uint32_t)(0xffffffffull / (uint32_t)a.parts);
+  a.words = (int)((a.b.max_blocks + 31) / 32);
+  if (a.words < 1) a.words = 1;
   int64_t bytes = 0;
   for (a.TG = 32 / a.GC;; a.TG = (a.TG + 1) / 2) {
     const int64_t bits = ((int64_t)a.TG * a.words * 4 + 15) & ~15ll, all = (int64_t)a.words * 32;
@@ -326,30 +363,39 @@ template <int D, int DT, int W> static int sa_run(sa_args a, hipStream_t stream)
   int dev = 0;
   AKV_HIP(hipGetDevice(&dev));
   static akv_device_once once;
-  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)sa_kernel<D, DT, W>, SA_LDS); })) return rc;
-  sa_kernel<D, DT, W><<<(uint32_t)units, 64 * W, bytes, stream>>>(a);
+  if (const int rc = once(dev, [&]() -> int { return ab_lds((const void*)sa_kernel<D, DT>, SA_LDS); })) return rc;
+  sa_kernel<D, DT><<<dim3((uint32_t)units, (uint32_t)a.splits), 64 * P::W, bytes, stream>>>(a);
   AKV_LAUNCH_CHECK("sa_kernel");
+  if (a.splits > 1) {
+    sa_join_kernel<D, DT><<<(uint32_t)(((int64_t)a.b.T * a.QH + 3) / 4), 256, 0, stream>>>(a);
+    AKV_LAUNCH_CHECK("sa_join_kernel");
+  }
   return AKV_OK;
 }
-template <int D, int DT> static int sa_launch(sa_args a, hipStream_t stream) {
-  a.HS = (a.G + 31) / 32;
-  a.GC = (a.G + a.HS - 1) / a.HS;
-  a.parts = (a.b.block_size + 15) / 16;
-  a.parts_recip = (uint32_t)(0xffffffffull / (uint32_t)a.parts);
-  a.words = (int)((a.b.max_blocks + 31) / 32);
-  if (a.words < 1) a.words = 1;
-  // one token after another, and not a tile for every other CU: eight wavefronts share its keys
-  const int64_t tokens = a.b.T < a.b.S ? a.b.T : a.b.S;
-  if constexpr (D < 256)
-    if (a.b.T <= a.b.S && 2 * tokens * a.KVH * a.HS <= ab_cus()) return sa_run<D, DT, 8>(a, stream);
-  return sa_run<D, DT, 4>(a, stream);
+// Query heads of a kv head in groups of at most 32 rows
+static inline int sa_groups(int G) { return (G + 31) / 32; }
+// Workgroups that share the keys of a tile: one token a sequence, and few of them, leave most CUs without a tile, and a CU takes in some 36 bytes a clock.
+// Joining takes 4 us, so that it has to be for 1024 keys or more, and half of the CUs take in what memory gives.  32 heads on 8, blocks of 16, us with one
+// workgroup and with 8 / units of 128: one token and 64 blocks 18.3 and 13.5, 128 blocks 28.4 and 14.7, 32 blocks 13.1 and 13.5; four tokens, 64 blocks, 18.7
+// and 16.1; eight 20.8 and 19.4 (four workgroups a tile 21.0); sixteen 23.9 and, with two, 28.4.
+static inline int sa_splits(int64_t T, int S, int QH, int KVH, int block_size, int k_sel) {
+  if (T <= 0 || T > S || QH <= 0 || KVH <= 0 || block_size <= 0 || (int64_t)k_sel * ((block_size + 15) / 16) < 64) return 1;
+  const int64_t units = T * KVH * sa_groups(QH / KVH);
+  int splits = 1;
+  while (splits < SA_SPLITS && 4 * splits * units <= ab_cus()) splits *= 2;
+  return splits;
+}
+static inline size_t sa_sums(int64_t rows, int splits) { return akv_align256((size_t)rows * splits * 8); }
+extern "C" size_t akv_sparse_attn_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int block_size, int num_selected) {
+  const int splits = sa_splits(num_tokens, num_seqs, num_q_heads, num_kv_heads, block_size, num_selected);
+  return splits == 1 || !ab_head_size(d) ? 0 : sa_sums(num_tokens * num_q_heads, splits) + (size_t)(num_tokens * num_q_heads) * splits * d * 4;
 }
 
 extern "C" int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head, const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head, const void* value_cache,
                                int64_t vs_blk, int64_t vs_pos, int64_t vs_head, const void* block_tables, int bt_itype, int64_t bt_stride, const void* context_lens, int cl_itype,
                                const void* query_starts, int qs_itype, const int32_t* selected, int64_t ss_tok, int64_t ss_head, int num_selected, void* out, int64_t os_tok, int64_t os_head,
                                int zero_tail, int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size, int64_t num_blocks, int64_t max_blocks_per_seq,
-                               float scale, void* stream) {
+                               float scale, void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "akv_sparse_attn";
   AKV_REQUIRE(akv_valid_dtype(dtype), "%s: bad dtype %d", name, dtype);
   const int rc = ab_check(name, block_tables, bt_itype, context_lens, cl_itype, query_starts, qs_itype, num_seqs, num_tokens, num_kv_heads, block_size, num_blocks, max_blocks_per_seq);
@@ -368,6 +414,8 @@ extern "C" int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int
     return akv_fail(AKV_ERR_UNSUPPORTED, "%s: rows must lie at multiples of 16 bytes (outputs of 8)", name);
   if (block_size == 1) ks_pos = vs_pos = 0;
   if (ks_pos < 0 || vs_pos < 0 || ks_pos > SA_MOST_STRIDE || vs_pos > SA_MOST_STRIDE) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: tokens of a block 2^27 elements apart", name);
+  const size_t need = akv_sparse_attn_workspace_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, block_size, num_selected);
+  if (need && (!workspace || workspace_bytes < need || !ab_aligned(workspace, 256))) return akv_fail(AKV_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", name, need);
   sa_args a = {};
   a.b = ab_make(block_tables, bt_itype, bt_stride, context_lens, cl_itype, query_starts, qs_itype, num_seqs, num_tokens, block_size, num_blocks, max_blocks_per_seq);
   a.q = query; a.qs_tok = qs_tok; a.qs_head = qs_head;
@@ -376,6 +424,11 @@ extern "C" int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int
   a.selected = selected; a.ss_tok = ss_tok; a.ss_head = ss_head; a.k_sel = num_selected;
   a.out = out; a.os_tok = os_tok; a.os_head = os_head;
   a.KVH = num_kv_heads; a.QH = num_q_heads; a.G = num_q_heads / num_kv_heads;
+  a.HS = sa_groups(a.G);
+  a.GC = (a.G + a.HS - 1) / a.HS;
+  a.splits = sa_splits(num_tokens, num_seqs, num_q_heads, num_kv_heads, block_size, num_selected);
+  a.part_ml = (float2*)workspace;
+  a.part = (float*)((char*)workspace + sa_sums(num_tokens * num_q_heads, a.splits));
   a.tail = zero_tail; a.scale2 = scale * 1.44269504088896341f;
   const hipStream_t s = (hipStream_t)stream;
 #define SA_CASE(DIM) if (d == DIM) return dtype == AKV_F16 ? sa_launch<DIM, AKV_F16>(a, s) : sa_launch<DIM, AKV_BF16>(a, s);

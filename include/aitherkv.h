@@ -605,6 +605,7 @@ int akv_block_index_select(const void* query, int dtype, int64_t qs_tok, int64_t
                            int64_t num_blocks, int64_t max_blocks_per_seq,
                            int num_selected, int num_sink_blocks, int num_recent_blocks,
                            void* workspace, size_t workspace_bytes, void* stream);
+size_t akv_sparse_attn_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int block_size, int num_selected);
 int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
                     const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
                     const void* value_cache, int64_t vs_blk, int64_t vs_pos, int64_t vs_head,
@@ -612,7 +613,7 @@ int akv_sparse_attn(const void* query, int dtype, int64_t qs_tok, int64_t qs_hea
                     const void* query_starts, int qs_itype, const int32_t* selected, int64_t ss_tok, int64_t ss_head, int num_selected,
                     void* out, int64_t os_tok, int64_t os_head, int zero_tail,
                     int num_seqs, int64_t num_tokens, int num_q_heads, int num_kv_heads, int d, int block_size,
-                    int64_t num_blocks, int64_t max_blocks_per_seq, float scale, void* stream);
+                    int64_t num_blocks, int64_t max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes, void* stream);
 size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length);
 int akv_key_weights(const void* query, int dtype, int64_t qs_tok, int64_t qs_head,
                     const void* key_cache, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,

@@ -420,3 +420,34 @@ def test_shared_blocks_are_cut_to_blocks_of_their_own(dev):
             assert torch.equal(cache[to[i].long()].flatten(0, 1)[:40, h], want)
             assert torch.equal(kept[i, h].cpu(), torch.from_numpy(kept_reference(w[i, h].cpu().numpy(), int(ctx[i]), 40, 1, 5)).int())
     assert torch.equal(cache[:int(to.min())], before[:int(to.min())])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d,heads,kvh,block", [(128, 32, 8, 16), (64, 6, 1, 32), (256, 8, 2, 7), (128, 64, 1, 16), (64, 16, 16, 1)])
+def test_few_tokens(dev, d, heads, kvh, block, dtype):
+    """About one token a sequence, so that workgroups share the keys of a token: with gaps, two tokens at once, odd values, rows of no sequence."""
+    gen = torch.Generator().manual_seed(d + heads)
+    b = Batch([(1, 700), (0, 30), (1, 5), (2, 900), (0, 0), (1, 64), (0, 3), (1, 2000), (1, 1)], block, dev, seed=16)
+    q, k, v = inputs(gen, b, dtype, dev, heads, kvh, d)
+    b.unused(math.nan, k, v)
+    sel = some_columns(gen, b, kvh, 64)
+    sel[3] = -1
+    sel = sel.to(dev)
+    got = akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel)
+    assert_attention(got, b, q, k, v, sel)
+    for _ in range(3):
+        assert torch.equal(got, akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel))
+    into = torch.full_like(q, 3.0)
+    akv.paged_sparse_attention(q, k, v, b.tables[2:6], b.ctx[2:6], b.starts[2:7], sel, out=into)
+    few = akv.paged_sparse_attention(q, k, v, b.tables[2:6], b.ctx[2:6], b.starts[2:7], sel)
+    assert (into[:1] == 3).all() and (into[5:] == 3).all() and (few[:1] == 0).all() and (few[5:] == 0).all() and torch.equal(few[1:5], into[1:5])
+    assert_attention(torch.cat([got[:1], few[1:5], got[5:]]), b, q, k, v, sel)
+    # the first of two tokens does not see what the second does
+    v[b.host[3, 899 // block], 899 % block] = math.inf
+    sel[2:4, :, 0] = 899 // block
+    got = akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel)
+    assert torch.isfinite(got[2]).all() and not torch.isfinite(got[3]).any()
+    v[b.host[3, 899 // block], 899 % block] = 0
+    sel[3] = -1
+    got[3] = 0
+    assert_attention(got, b, q, k, v, sel)

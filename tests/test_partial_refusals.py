@@ -252,8 +252,8 @@ def library_select(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sinks=1, recent=2, ws=P
     return status("akv_block_index_select", q, dtype, 512, 64, P, P, P, 0, 2, P, 0, P, 0, P, 2, T, qh, kvh, d, block, 3, cols, k, sinks, recent, ws, size, None)
 
 
-def library_sparse(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sel=P, block=16, scale=0.1, cols=2, out=P, T=5, ks_pos=128, vs_pos=128):
-    return status("akv_sparse_attn", q, dtype, 512, 64, P, 2048, ks_pos, 64, P, 2048, vs_pos, 64, P, 0, 2, P, 0, P, 0, sel, 8, 4, k, out, 512, 64, 1, 2, T, qh, kvh, d, block, 3, cols, scale, None)
+def library_sparse(d=64, dtype=0, q=P, qh=8, kvh=2, k=4, sel=P, block=16, scale=0.1, cols=2, out=P, T=5, ks_pos=128, vs_pos=128, ws=P, size=1 << 30):
+    return status("akv_sparse_attn", q, dtype, 512, 64, P, 2048, ks_pos, 64, P, 2048, vs_pos, 64, P, 0, 2, P, 0, P, 0, sel, 8, 4, k, out, 512, 64, 1, 2, T, qh, kvh, d, block, 3, cols, scale, ws, size, None)
 
 
 def library_weights(d=64, dtype=0, q=P, qh=8, kvh=2, length=32, ws=P, size=1 << 30, scale=0.1, out=P, S=2):
@@ -292,7 +292,8 @@ INVALID, UNSUPPORTED, WORKSPACE = _lib.AKV_ERR_INVALID, _lib.AKV_ERR_UNSUPPORTED
     (library_sparse, INVALID, dict(k=-1)), (library_sparse, INVALID, dict(qh=7)), (library_sparse, INVALID, dict(scale=0.0)), (library_sparse, INVALID, dict(scale=float("inf"))),
     (library_sparse, INVALID, dict(scale=float("nan"))), (library_sparse, UNSUPPORTED, dict(d=96)), (library_sparse, UNSUPPORTED, dict(dtype=2)),
     (library_sparse, UNSUPPORTED, dict(k=4097)), (library_sparse, UNSUPPORTED, dict(block=4097)), (library_sparse, UNSUPPORTED, dict(q=P + 8)),
-    (library_sparse, UNSUPPORTED, dict(ks_pos=1 << 27)), (library_sparse, UNSUPPORTED, dict(vs_pos=1 << 27)), (library_sparse, UNSUPPORTED, dict(vs_pos=-128)), (library_sparse, 0, dict(T=0)),
+    (library_sparse, UNSUPPORTED, dict(ks_pos=1 << 27)), (library_sparse, UNSUPPORTED, dict(vs_pos=1 << 27)), (library_sparse, UNSUPPORTED, dict(vs_pos=-128)),
+    (library_sparse, WORKSPACE, dict(T=2, k=64, ws=None)), (library_sparse, WORKSPACE, dict(T=2, k=64, size=100)), (library_sparse, WORKSPACE, dict(T=2, k=64, ws=P + 16)), (library_sparse, 0, dict(T=0)),
     (library_weights, INVALID, dict(dtype=7)), (library_weights, INVALID, dict(q=None)), (library_weights, INVALID, dict(out=None)), (library_weights, INVALID, dict(qh=7)),
     (library_weights, INVALID, dict(length=31)), (library_weights, INVALID, dict(scale=-1.0)), (library_weights, UNSUPPORTED, dict(d=32)), (library_weights, UNSUPPORTED, dict(dtype=2)),
     (library_weights, UNSUPPORTED, dict(S=70000)), (library_weights, WORKSPACE, dict(ws=None)), (library_weights, WORKSPACE, dict(size=100)), (library_weights, 0, dict(S=0)),
