@@ -28,7 +28,8 @@ __device__ __forceinline__ uint32_t ev_order(float x) {
 //
 // Few workgroups have much to do here, so that each waits for its code too: the loops are short.  Weights are alike in their upper bits, so that counters have
 // copies; when few share the known bits they are listed, and later levels read the list alone.  8 heads of 32768 positions take 32 us: a bit at a time with
-// orders in registers 42, one copy of a counter and no list 36.  16 sequences of 8 heads of 8192 take 16 us, and took 57 with registers.
+// orders in registers 42, one copy of a counter and no list 36.  (Counters take some 2.5 lanes a clock; eleven bits at a time with two
+// copies took as long.)  16 sequences of 8 heads, up to 9000 positions, take 15 us.
 #define EV_THREADS 1024
 #define EV_HELD 32768                   // orders in LDS
 #define EV_COPIES 16                    // of a counter: weights are alike, and lanes that add to one word wait for each other
@@ -320,7 +321,9 @@ __device__ __forceinline__ void ev_store(const ev_piece& x, uint8_t* p, int log,
 }
 
 // To blocks that nobody reads: a thread a piece of a row, heads of a token side by side, as the rows lie where they go to.
-// (With four bytes a thread and a division of 64 bits for it, 16 sequences of 2048 tokens of 4 bits took 68 us.)
+// 16 sequences of 2048 tokens of 4 bits take 34 us: 125 MB read, since most lines of 128 bytes hold a row of another head or token as well, and 40 MB written,
+// 4.8 TB/s, what a large copy reaches.  (With four bytes a thread and a division of 64 bits for it 68 us; four tokens a thread, all loads on their way
+// together, 38: neighbouring tokens share lines.)
 __global__ __launch_bounds__(256) void ev_copy_kernel(ev_move_args a) {
   const int seq = blockIdx.y;
   const int n = min(ab_clamp(akv_load_index(a.b.lens, a.b.lens_it, seq), AB_MOST_TOKENS), a.keep);

@@ -239,7 +239,7 @@ template <int D, int KIND> struct kw_keys {
   }
 };
 
-// ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows
+// ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows.  4096 rows of 128 take 10 us: a row of the rotation after the other.
 template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a) {
   constexpr int PER = 256 / D > 0 ? 256 / D : 1, LANES = D < 256 ? D : 256, R = 8 / PER;      // threads of a row; rows of a thread
   __shared__ __align__(16) float x[8][D];
@@ -328,6 +328,8 @@ template <int KT> __device__ __forceinline__ void kw_row_stats(const ab_f16 (&s)
 
 // ---- many rows over plain keys: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
 // has one barrier.  Workgroups of `splits` take steps in turn.
+// 1024 tokens after 7000, 16 heads on 4, heads of 256: 78 us, and 79 for kw_sum below, 800 TFLOP/s each (matrix cores 37 % of clocks, LDS 37 %, vector unit
+// 29 %): a step's operands come from LDS, its maxima are taken, and the next step waits for both.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
   constexpr int ROWS = P::ROWS, RT = P::RT;
@@ -546,6 +548,8 @@ __global__ __launch_bounds__(256) void kw_add_kernel(kw_args a) {
 
 // ---- many rows over packed keys: a block of rows stays in LDS while the wavefronts walk through `runs` x N keys, each by itself, the next codes on their
 // way: codes are a quarter of the keys' bytes and cost more to turn into levels than to read again for the next block of rows.
+// The last 32 tokens of four prompts of up to 16352 keys, 32 heads on 8, 4 bits: 41 us, and 44 for the sum below (vector unit 36 % of clocks, matrix cores 29 %, LDS
+// 25 %): three products a score, and codes turned into levels twice.
 template <int D> struct kw_block { static constexpr int ROWS = D == 256 ? 64 : 128; };
 // rows r0 .. into LDS, those past the last as zeros
 template <int D, int KIND> __device__ __forceinline__ void kw_put_block(const kw_args& a, const kw_rows& R, int r0, int kvh, unsigned char* rows) {
@@ -709,6 +713,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
 // ---- few rows a sequence: keys are read once, as long as a sequence and kv head has no more rows than a tile; scores are kept, four bytes a row and
 // key, and read back by kw_few_sum with the statistics of the rows.  A workgroup of four wavefronts takes `runs` x N keys, the next ones on
 // their way while the ones before are multiplied.
+// One token of 16 sequences, 1024 to 41000 keys each, 8 heads of 128: 120 us, 4.3 TB/s of what is read; kw_few_sum 15.
 #define KW_FEW 32
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
@@ -851,17 +856,18 @@ __global__ __launch_bounds__(256) void kw_few_sum_kernel(kw_args a, int keys) {
 struct kw_scratch { int64_t tokens; size_t stat, part, turned, by, scores, few_part, sums, bytes; int parts, few_parts, runs, splits; int64_t stride; bool few; };
 // Scratch of a call, its tokens in slabs of what KW_SCRATCH holds (a multiple of 32, or all).  Scores are kept where the batch has no more than a
 // tile of rows a sequence and kv head on average: a key of 128 coordinates that is read again costs 256 bytes, the scores of 4 rows written and
-// read 32.
+// read 32.  (One token of 16 sequences of up to 41000 keys 135 us against 229, four tokens 197 against 243.)
 static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, bool packed, int keys, int64_t length) {
   kw_scratch w = {};
   w.few = T * (QH / KVH) <= (int64_t)KW_FEW * S;
   w.stride = (length + keys * 4 - 1) / (keys * 4) * (keys * 4);
-  // runs of keys a workgroup: as many as leave forty workgroups a CU, over packed keys, whose rows have to come to LDS first, four
+  // runs of keys a workgroup: as many as leave forty workgroups a CU (48 sequences 509 us against 517 with one run; two sequences 25 with one against 31 with
+  // four); over packed keys, whose rows have to come to LDS first, four (the last 32 tokens of four prompts 105 us against 110, 128 tokens 342 against 353)
   w.runs = 4;
   while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < (w.few ? 40 : 4) * ab_cus()) w.runs /= 2;
   w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
   w.parts = w.few ? 0 : packed ? (int)(w.stride / (keys * w.runs)) : (int)((length + keys - 1) / keys);
-  // workgroups that share the rows of a part: as many as give every CU two
+  // workgroups that share the rows of a part: as many as give every CU two (1024 tokens after 7000, heads of 256, 172 us against 229; after 1000, 62 against 228)
   w.splits = 1;
   while (!w.few && !packed && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
   const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
