@@ -451,3 +451,62 @@ def test_few_tokens(dev, d, heads, kvh, block, dtype):
     sel[3] = -1
     got[3] = 0
     assert_attention(got, b, q, k, v, sel)
+
+
+def test_few_tokens_captured(dev):
+    """A decode step in a graph, with the second launch that joins what workgroups share; lengths and selections change between replays."""
+    b = Batch([(1, 1500), (1, 900), (1, 700)], 16, dev, seed=17)
+    gen = torch.Generator().manual_seed(11)
+    q, k, v = inputs(gen, b, BF, dev, 16, 4, 128)
+    index = akv.BlockIndex(b.blocks, 4, 128, dev)
+    index.update(k, b.tables, b.ctx)
+    ctx = b.ctx.clone()
+
+    def step():
+        sel = index.select(q, b.tables, ctx, b.starts, 16, 80)
+        return sel, akv.paged_sparse_attention(q, k, v, b.tables, ctx, b.starts, sel)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for lens in ((1500, 900, 700), (17, 1, 0), (1400, 16, 699), (0, 900, 300)):
+        ctx.copy_(torch.tensor(lens, device=dev))
+        q.copy_(vectors(gen, BF, dev, *q.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        for x, y in zip(kept, step()):
+            assert torch.equal(x, y)
+        b.lens = [(1, c) for c in lens]
+        assert_attention(kept[1], b, q, k, v, kept[0])
+
+
+def test_starts_that_go_back_and_lengths_out_of_range(dev):
+    """Starts that go back, lengths below zero or past the tables: rows of such sequences are undefined, the others' are right, and nothing else is touched."""
+    b = Batch([(4, 100), (6, 80), (5, 300)], 16, dev, seed=18)
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = inputs(gen, b, BF, dev, 8, 2, 64)
+    index = akv.BlockIndex(b.blocks, 2, 64, dev)
+    index.update(k, b.tables, b.ctx)
+    sel = index.select(q, b.tables, b.ctx, b.starts, 16, 5)
+    want = akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, b.starts, sel)
+    w = akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts)
+    for starts in ([0, 4, 4, 0], [9, 4, 10, 15], [0, -5, 10, 99], [7, 3, 2, 1]):
+        s = torch.tensor(starts, dtype=torch.int32, device=dev)
+        index.select(q, b.tables, b.ctx, s, 16, 5)
+        akv.paged_sparse_attention(q, k, v, b.tables, b.ctx, s, sel)
+        akv.paged_key_weights(q, k, b.tables, b.ctx, s)
+        index.update(k, b.tables, b.ctx, s)
+    ctx = b.ctx.clone()
+    ctx[0], ctx[2] = -7, 1 << 30
+    tables = b.tables.clamp(0, b.blocks - 1)
+    s2 = index.select(q, tables, ctx, b.starts, 16, 5)
+    assert (s2[:4] == -1).all() and torch.equal(s2[4:10], sel[4:10])
+    out = akv.paged_sparse_attention(q, k, v, tables, ctx, b.starts, s2)
+    assert (out[:4] == 0).all() and torch.equal(out[4:10], want[4:10])
+    w2 = akv.paged_key_weights(q, k, tables, ctx, b.starts)
+    assert (w2[0] == 0).all() and torch.equal(w2[1], w[1])
+    kept, now, _ = akv.evict_tokens(w, tables[:2], ctx[:2], [k, v], 40, 2, 8)
+    assert now.tolist() == [0, 40] and (kept[0] == -1).all()
