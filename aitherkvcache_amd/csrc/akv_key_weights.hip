@@ -239,7 +239,8 @@ template <int D, int KIND> struct kw_keys {
   }
 };
 
-// ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows.  4096 rows of 128 take 10 us: a row of the rotation after the other.
+// ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows.  4096 rows of 128 take
+// 9 us (10.5 with eight rows of the rotation on their way, and waited for): LDS, eight clocks for four numbers that all lanes read.
 template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a) {
   constexpr int PER = 256 / D > 0 ? 256 / D : 1, LANES = D < 256 ? D : 256, R = 8 / PER;      // threads of a row; rows of a thread
   __shared__ __align__(16) float x[8][D];
@@ -257,20 +258,28 @@ template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a
   __syncthreads();
   const int d = threadIdx.x % LANES, who = threadIdx.x / LANES;
   float y[R][2] = {};
-  // (short loops: the first workgroups wait for the code as well, and unrolled it was 11 KB and cost 19 us)
+  // (a short loop: the first workgroups wait for the code as well, and unrolled it was 11 KB and cost 19 us)
+  constexpr int STEP = 16;
+  float p[STEP];                        // (a step's on their way together, while the step before is added)
+  const float* turn = a.turn + d;
+#pragma unroll
+  for (int e = 0; e < STEP; ++e) p[e] = turn[e * D];
 #pragma unroll 1
-  for (int j = 0; j < D; j += 8) {
-    float p[8];                         // (on their way together)
+  for (int j = 0; j < D; j += STEP) {
+    if (j + STEP < D) turn += STEP * D;
+    float next[STEP];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = a.turn[(size_t)(j + e) * D + d];
+    for (int e = 0; e < STEP; ++e) next[e] = turn[e * D];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float4 u = *(const float4*)&x[who * R + i][j], v = *(const float4*)&x[who * R + i][j + 4];
-      y[i][0] = fmaf(p[0], u.x, y[i][0]); y[i][1] = fmaf(p[1], u.y, y[i][1]);
-      y[i][0] = fmaf(p[2], u.z, y[i][0]); y[i][1] = fmaf(p[3], u.w, y[i][1]);
-      y[i][0] = fmaf(p[4], v.x, y[i][0]); y[i][1] = fmaf(p[5], v.y, y[i][1]);
-      y[i][0] = fmaf(p[6], v.z, y[i][0]); y[i][1] = fmaf(p[7], v.w, y[i][1]);
-    }
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int e = 0; e < STEP; e += 4) {
+        const float4 u = *(const float4*)&x[who * R + i][j + e];
+        y[i][0] = fmaf(p[e], u.x, y[i][0]); y[i][1] = fmaf(p[e + 1], u.y, y[i][1]);
+        y[i][0] = fmaf(p[e + 2], u.z, y[i][0]); y[i][1] = fmaf(p[e + 3], u.w, y[i][1]);
+      }
+#pragma unroll
+    for (int e = 0; e < STEP; ++e) p[e] = next[e];
   }
   __syncthreads();
 #pragma unroll
