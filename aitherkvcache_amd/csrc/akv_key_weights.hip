@@ -578,7 +578,8 @@ __global__ __launch_bounds__(256) void kw_add_kernel(kw_args a) {
 }
 
 // ---- many rows over packed keys: a block of rows stays in LDS while the wavefronts walk through `runs` x N keys, each by itself, the next codes on their
-// way: codes are a quarter of the keys' bytes and cost more to turn into levels than to read again for the next block of rows.
+// way: codes are a quarter of the keys' bytes and cost more to turn into levels than to read again for the next block of rows.  Workgroups of
+// `splits` take blocks in turn.
 // The last 32 tokens of four prompts of up to 16352 keys, 32 heads on 8, 4 bits: 41 us, and 44 for the sum below (vector unit 36 % of clocks, matrix cores 29 %, LDS
 // 25 %): three products a score, and codes turned into levels twice.
 template <int D> struct kw_block { static constexpr int ROWS = D == 256 ? 64 : 128; };
@@ -606,7 +607,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
   __shared__ float by[ROWS];
   __shared__ __align__(16) float norms[P::N];
   __shared__ kw_levels<KIND> levels;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t from64 = (int64_t)part * P::N * a.runs;
   if (from64 >= ctx) return;
@@ -617,7 +618,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
   const float unit = kw_fill(levels, a.centroids);
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
   float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
-  for (int r0 = 0; r0 < R.rows; r0 += ROWS) {
+  for (int r0 = ROWS * split; r0 < R.rows; r0 += ROWS * a.splits) {
     const int count = min(ROWS, R.rows - r0), last = kw_pos(a, R, r0 + count - 1), end = min(from + P::N * a.runs, last + 1);
     if (last < from) continue;
     kw_keys<D, KIND> K;
@@ -682,21 +683,23 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
   extern __shared__ __align__(16) unsigned char rows[];          // [ROWS][ROW]
   __shared__ __align__(16) float ref[ROWS], inv[ROWS], by[ROWS];
   __shared__ kw_levels<KIND> levels;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x / a.splits, split = blockIdx.x % a.splits, kvh = blockIdx.y, seq = blockIdx.z;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t from = (int64_t)part * P::N * a.runs;
   const kw_rows R = kw_rows_of(a, seq, ctx);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
-  float* to = a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head;
+  float* to = a.splits == 1 ? a.out + (int64_t)seq * a.os_seq + (int64_t)kvh * a.os_head : a.sums + (((int64_t)split * a.b.S + seq) * a.KVH + kvh) * a.length;
+  bool add = a.add && a.splits == 1;    // (the first block that sees something of the keys writes, the others add)
+  auto zeros = [&]() {
+    for (int64_t i = from + tid; i < from + P::N * a.runs && i < a.length; i += 256) to[i] = 0.f;
+  };
   if (from >= ctx || R.rows == 0 || kw_pos(a, R, R.rows - 1) < from) {
-    if (!a.add)
-      for (int64_t i = from + tid; i < from + P::N * a.runs && i < a.length; i += 256) to[i] = 0.f;
+    if (!add) zeros();
     return;
   }
   const float unit = kw_fill(levels, a.centroids);
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
-  bool add = a.add;                     // (the first block that sees something of the keys writes, the others add)
-  for (int r0 = 0; r0 < R.rows; r0 += ROWS) {
+  for (int r0 = ROWS * split; r0 < R.rows; r0 += ROWS * a.splits) {
     const int count = min(ROWS, R.rows - r0), last = kw_pos(a, R, r0 + count - 1);
     if (last < from) continue;
     kw_keys<D, KIND> K;
@@ -739,6 +742,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
     }
     add = true;
   }
+  if (!add) zeros();                    // (none of the workgroup's blocks does)
 }
 
 // ---- few rows a sequence: keys are read once, as long as a sequence and kv head has no more rows than a tile; scores are kept, four bytes a row and
@@ -898,9 +902,10 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < (w.few ? 40 : 4) * ab_cus()) w.runs /= 2;
   w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
   w.parts = w.few ? 0 : packed ? (int)(w.stride / (keys * w.runs)) : (int)((length + keys - 1) / keys);
-  // workgroups that share the rows of a part: as many as give every CU two (1024 tokens after 7000, heads of 256, 172 us against 229; after 1000, 62 against 228)
+  // workgroups that share the rows of a part: as many as give every CU two (1024 tokens after 7000, heads of 256, 172 us against 229; after 1000, 62 against 228;
+  // 4 bits, 1469 tokens of 8 heads on 2 after 3884, 184 against 616)
   w.splits = 1;
-  while (!w.few && !packed && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
+  while (!w.few && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
   const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
   w.tokens = KW_SCRATCH / per / 32 * 32;
   if (w.tokens < 32) w.tokens = 32;
