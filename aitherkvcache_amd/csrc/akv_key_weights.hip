@@ -239,73 +239,83 @@ template <int D, int KIND> struct kw_keys {
   }
 };
 
-// ---- queries of packed rows: turned, scaled and as two terms; a workgroup takes 8 rows.  4096 rows of 128 take
-// 9 us (10.5 with eight rows of the rotation on their way, and waited for): LDS, eight clocks for four numbers that all lanes read.
-template <int D> __global__ __launch_bounds__(256) void kw_turn_kernel(kw_args a) {
-  constexpr int PER = 256 / D > 0 ? 256 / D : 1, LANES = D < 256 ? D : 256, R = 8 / PER;      // threads of a row; rows of a thread
-  __shared__ __align__(16) float x[8][D];
-  const uint32_t rows = (uint32_t)(a.t1 - a.t0) * (uint32_t)a.QH, r0 = blockIdx.x * 8u, QH = (uint32_t)a.QH, G = (uint32_t)a.G;
-  for (int i = threadIdx.x; i < 8 * D; i += 256) {
-    const uint32_t r = r0 + i / D;
-    float v = 0.f;
-    if (r < rows) {
-      const uint32_t token = r / QH;
-      const int64_t at = (int64_t)(token + (uint32_t)a.t0) * a.qs_tok + (int64_t)(r - token * QH) * a.qs_head + i % D;
-      v = a.dtype == AKV_F16 ? akv_elem<AKV_F16>::load(a.q, at) : akv_elem<AKV_BF16>::load(a.q, at);
-    }
-    x[i / D][i % D] = v;
-  }
-  __syncthreads();
-  const int d = threadIdx.x % LANES, who = threadIdx.x / LANES;
-  float y[R][2] = {};
-  // (a short loop: the first workgroups wait for the code as well, and unrolled it was 11 KB and cost 19 us)
-  constexpr int STEP = 16;
-  float p[STEP];                        // (a step's on their way together, while the step before is added)
-  const float* turn = a.turn + d;
+// ---- queries of packed rows: turned, scaled and as two terms.  32 rows a tile and 32 coordinates a wavefront: queries are 16-bit numbers as they are, an entry of the
+// rotation three of their type, so that products and sums are float32 like those of one number after the other.  A workgroup's part of the rotation
+// stays in registers for all of its tiles.  4096 rows of 128 take 7 us and 47000 18, where a row of the rotation after the other, for eight rows a
+// workgroup, took 9 and 43.
+template <int D, int DT> __global__ __launch_bounds__(2 * D) void kw_turn_kernel(kw_args a) {
+  typedef ab_math<DT> M;
+  constexpr int KS = D / 16, LANES = D / 16;         // LANES: threads of a row, in the end
+  __shared__ __align__(16) float x[32][D + 4];
+  const uint32_t rows = (uint32_t)(a.t1 - a.t0) * (uint32_t)a.QH, QH = (uint32_t)a.QH;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
+  // an entry times 2^12 in float16 (a rotation's are 1 at most), so that its third term is a normal number
+  constexpr float UP = DT == AKV_F16 ? 4096.f : 1.f;
+  ab_u4 pi[3][KS];
+  const float* const turn = a.turn + 32 * wave + col;
 #pragma unroll
-  for (int e = 0; e < STEP; ++e) p[e] = turn[e * D];
-#pragma unroll 1
-  for (int j = 0; j < D; j += STEP) {
-    if (j + STEP < D) turn += STEP * D;
-    float next[STEP];
+  for (int k = 0; k < KS; ++k)
 #pragma unroll
-    for (int e = 0; e < STEP; ++e) next[e] = turn[e * D];
+    for (int e = 0; e < 4; ++e) {
+      float u = turn[(16 * k + 8 * h + 2 * e) * D] * UP, v = turn[(16 * k + 8 * h + 2 * e + 1) * D] * UP;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int e = 0; e < STEP; e += 4) {
-        const float4 u = *(const float4*)&x[who * R + i][j + e];
-        y[i][0] = fmaf(p[e], u.x, y[i][0]); y[i][1] = fmaf(p[e + 1], u.y, y[i][1]);
-        y[i][0] = fmaf(p[e + 2], u.z, y[i][0]); y[i][1] = fmaf(p[e + 3], u.w, y[i][1]);
+      for (int part = 0; part < 3; ++part) {
+        const uint32_t two = M::pair(u, v);
+        pi[part][k][e] = two;
+        u -= M::low(two);
+        v -= M::high(two);
       }
-#pragma unroll
-    for (int e = 0; e < STEP; ++e) p[e] = next[e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < R; ++i) x[who * R + i][d] = y[i][0] + y[i][1];
-  __syncthreads();
-  // a wavefront a row: scaled so that the largest lies in [2^13, 2^14), and as two terms
-  const int lane = threadIdx.x & 63;
-#pragma unroll 1
-  for (uint32_t i = threadIdx.x >> 6; i < 8 && r0 + i < rows; i += 4) {
-    float v[D / 64], t = 0.f;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      v[e] = x[i][64 * e + lane];
-      t = fmaxf(t, fabsf(v[e]));
     }
-    const uint32_t exponent = akv_row_exponent(akv_wave_max(t)), token = (r0 + i) / QH, head = r0 + i - token * QH, kvh = head / G;
-    const int64_t to = (int64_t)kvh * (a.t1 - a.t0) * a.G + (int64_t)token * a.G + (head - kvh * G);
-    const float scale = akv_row_scale(exponent) * 8192.f;
+  for (uint32_t r0 = 32 * blockIdx.x; r0 < rows; r0 += 32 * gridDim.x) {
+    const uint32_t r = min(r0 + col, rows - 1), token = r / QH;
+    const uint16_t* q = (const uint16_t*)a.q + (int64_t)(token + (uint32_t)a.t0) * a.qs_tok + (int64_t)(r - token * QH) * a.qs_head + 8 * h;
+    ab_u4 y[KS];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      const float u = v[e] * scale;
-      const _Float16 hi = (_Float16)u, lo = (_Float16)(u - (float)hi);
-      a.turned[to * (2 * D) + 64 * e + lane] = __builtin_bit_cast(uint16_t, hi);
-      a.turned[to * (2 * D) + D + 64 * e + lane] = __builtin_bit_cast(uint16_t, lo);
+    for (int k = 0; k < KS; ++k) y[k] = *(const ab_u4*)(q + 16 * k);
+    ab_f16 s[3];
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[part][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s[part] = M::mfma32(y[k], pi[part][k], s[part]);
     }
-    if (lane == 0) a.turned_by[to] = akv_row_unscale(exponent) * (1.f / 8192.f) * a.scale2;
+    __syncthreads();                   // (the tile before has been read)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[8 * (i / 4) + 4 * h + i % 4][32 * wave + col] = (s[0][i] + (s[1][i] + s[2][i])) * (1.f / UP);
+    __syncthreads();
+    // sixteen numbers of a row a thread: scaled so that the largest lies in [2^13, 2^14), and as two terms
+    const uint32_t i = tid / LANES, part = tid % LANES;
+    ab_f4 v[4];
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = *(const ab_f4*)&x[i][4 * (part + LANES * j)];
+      t = fmaxf(fmaxf(fmaxf(t, fabsf(v[j][0])), fmaxf(fabsf(v[j][1]), fabsf(v[j][2]))), fabsf(v[j][3]));
+    }
+    t = fmaxf(t, akv_lane_xor<1>(t));
+    t = fmaxf(t, akv_lane_xor<2>(t));
+    if constexpr (LANES > 4) t = fmaxf(t, akv_lane_xor<4>(t));
+    if constexpr (LANES > 8) t = fmaxf(t, akv_lane_xor<8>(t));
+    if (r0 + i < rows) {
+      const uint32_t exponent = akv_row_exponent(t), token = (r0 + i) / QH, head = r0 + i - token * QH, kvh = kw_div(a, head);
+      const int64_t to = (int64_t)kvh * (a.t1 - a.t0) * a.G + (int64_t)token * a.G + (head - kvh * a.G);
+      const float scale = akv_row_scale(exponent) * 8192.f;
+      typedef _Float16 four __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        four hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = v[j][e] * scale;
+          hi[e] = (_Float16)u;
+          lo[e] = (_Float16)(u - (float)hi[e]);
+        }
+        *(four*)(a.turned + to * (2 * D) + 4 * (part + LANES * j)) = hi;
+        *(four*)(a.turned + to * (2 * D) + D + 4 * (part + LANES * j)) = lo;
+      }
+      if (part == 0) a.turned_by[to] = akv_row_unscale(exponent) * (1.f / 8192.f) * a.scale2;
+    }
   }
 }
 
@@ -966,7 +976,10 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
     const int64_t rows = (int64_t)(a.t1 - a.t0) * a.QH;
     if (rows > 0) {
       if constexpr (P::PACKED) {
-        kw_turn_kernel<D><<<(uint32_t)((rows + 7) / 8), 256, 0, stream>>>(a);
+        const int64_t tiles = (rows + 31) / 32, most = 8 * 32 / D * ab_cus();
+        const uint32_t groups = (uint32_t)(tiles < most ? tiles : most);
+        if (a.dtype == AKV_F16) kw_turn_kernel<D, AKV_F16><<<groups, 2 * D, 0, stream>>>(a);
+        else kw_turn_kernel<D, AKV_BF16><<<groups, 2 * D, 0, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_turn_kernel");
       }
       if (w.few) {
