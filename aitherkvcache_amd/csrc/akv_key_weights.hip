@@ -345,6 +345,10 @@ template <int KT> __device__ __forceinline__ void kw_row_stats(const ab_f16 (&s)
   if (m != m || m == -INFINITY) m = -INFINITY, l = 0.f;      // (-inf times 0: a row that is none)
 }
 
+// what is left of a row over a part: maximum and sum for kw_join, or, of the only part, what kw_join would make of them
+__device__ __forceinline__ float2 kw_stat(const kw_args& a, float top, float sum) {
+  return a.parts > 1 ? make_float2(top, sum) : sum > 0.f ? make_float2(top, 1.f / sum) : make_float2(0.f, 0.f);
+}
 // ---- many rows over plain keys: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
 // has one barrier.  Workgroups of `splits` take steps in turn.
 // 1024 tokens after 7000, 16 heads on 4, heads of 256: 78 us, and 79 for kw_sum below, 800 TFLOP/s each (matrix cores 37 % of clocks, LDS 37 %, vector unit
@@ -369,7 +373,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
   const bool any = base < ctx;
   if (any) K.request(a, seq, kvh, base, ctx);
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
-  float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
+  float2* to = (a.parts == 1 ? a.stat : a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G)) + slab;
   // what the wavefronts have of a step's rows, together: four lanes a row, every wavefront a quarter
   auto join = [&](int r0, int buf) {
     const int r = ROWS / 4 * wave + (lane >> 2);
@@ -380,7 +384,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_ke
       float sum = e.x == -INFINITY ? 0.f : e.y * __builtin_amdgcn_exp2f(e.x - top);
       sum += akv_lane_xor<1>(sum);
       sum += akv_lane_xor<2>(sum);
-      if ((lane & 3) == 0 && r0 + r < R.rows) to[r0 + r] = make_float2(top, sum);
+      if ((lane & 3) == 0 && r0 + r < R.rows) to[r0 + r] = kw_stat(a, top, sum);
     }
   };
   next.put(rows);
@@ -627,7 +631,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
   const float unit = kw_fill(levels, a.centroids);
   const int64_t slab = kw_slab_row(a, R, kvh, 0);
-  float2* to = a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G) + slab;
+  float2* to = (a.parts == 1 ? a.stat : a.part + (int64_t)part * a.KVH * ((int64_t)(a.t1 - a.t0) * a.G)) + slab;
   for (int r0 = ROWS * split; r0 < R.rows; r0 += ROWS * a.splits) {
     const int count = min(ROWS, R.rows - r0), last = kw_pos(a, R, r0 + count - 1), end = min(from + P::N * a.runs, last + 1);
     if (last < from) continue;
@@ -682,7 +686,7 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
       for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][tid].x);
 #pragma unroll
       for (int w = 0; w < 4; ++w) sum += ml[w][tid].x == -INFINITY ? 0.f : ml[w][tid].y * __builtin_amdgcn_exp2f(ml[w][tid].x - top);
-      to[r0 + tid] = make_float2(top, sum);
+      to[r0 + tid] = kw_stat(a, top, sum);
     }
   }
 }
@@ -911,11 +915,13 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   w.runs = 4;
   while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < (w.few ? 40 : 4) * ab_cus()) w.runs /= 2;
   w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
-  w.parts = w.few ? 0 : packed ? (int)(w.stride / (keys * w.runs)) : (int)((length + keys - 1) / keys);
+  w.parts = w.few ? 0 : packed ? (int)((length + keys * w.runs - 1) / (keys * w.runs)) : (int)((length + keys - 1) / keys);
   // workgroups that share the rows of a part: as many as give every CU two (1024 tokens after 7000, heads of 256, 172 us against 229; after 1000, 62 against 228;
-  // 4 bits, 1469 tokens of 8 heads on 2 after 3884, 184 against 616)
+  // 4 bits, 1469 tokens of 8 heads on 2 after 3884, 184 against 616), and no more than an average sequence has steps (blocks) of rows: 30 prompts of 10 to 21
+  // tokens, 64 heads on 8, 4 bits, 44 us against 61 with four
   w.splits = 1;
-  while (!w.few && w.splits < 8 && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
+  const int64_t step = packed && D < 256 ? 128 : 64;
+  while (!w.few && w.splits < 8 && T * (QH / KVH) > step * w.splits * S && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
   const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
   w.tokens = KW_SCRATCH / per / 32 * 32;
   if (w.tokens < 32) w.tokens = 32;
@@ -966,7 +972,7 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
       }))
     return rc;
   const int add = a.add;
-  const int keys = P::PACKED ? P::N * w.runs : P::N;
+  const int keys = P::PACKED ? P::N * w.runs : P::N;      // of a part
   const dim3 grid((uint32_t)((a.length + keys - 1) / keys * w.splits), (uint32_t)a.KVH, (uint32_t)a.b.S);
   int64_t t = 0;
   do {                                  // (without a token: zeros)
@@ -989,8 +995,10 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
         if constexpr (P::PACKED) kw_packed_stats_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
         else kw_stats_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_stats_kernel");
-        kw_join_kernel<<<dim3((uint32_t)(((int64_t)(a.t1 - a.t0) * a.G + 63) / 64), (uint32_t)a.KVH), 256, 0, stream>>>(a, keys);
-        AKV_LAUNCH_CHECK("kw_join_kernel");
+        if (w.parts > 1) {
+          kw_join_kernel<<<dim3((uint32_t)(((int64_t)(a.t1 - a.t0) * a.G + 63) / 64), (uint32_t)a.KVH), 256, 0, stream>>>(a, keys);
+          AKV_LAUNCH_CHECK("kw_join_kernel");
+        }
       }
     }
     if (w.few) {
