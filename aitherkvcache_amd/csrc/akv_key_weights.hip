@@ -351,7 +351,7 @@ __device__ __forceinline__ float2 kw_stat(const kw_args& a, float top, float sum
 }
 // ---- many rows over plain keys: maxima and sums of the rows over a part of the keys, 32 KT of them a wavefront.  Rows are requested a step of ROWS ahead, and a step
 // has one barrier.  Workgroups of `splits` take steps in turn.
-// 1024 tokens after 7000, 16 heads on 4, heads of 256: 78 us, and 79 for kw_sum below, 800 TFLOP/s each (matrix cores 37 % of clocks, LDS 37 %, vector unit
+// 1024 tokens after 7000, 16 heads on 4, heads of 256: 79 us, and 80 for kw_sum below, 790 TFLOP/s each (matrix cores 37 % of clocks, LDS 37 %, vector unit
 // 29 %): a step's operands come from LDS, its maxima are taken, and the next step waits for both.
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_stats_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(256) void kw_add_kernel(kw_args a) {
 // ---- many rows over packed keys: a block of rows stays in LDS while the wavefronts walk through `runs` x N keys, each by itself, the next codes on their
 // way: codes are a quarter of the keys' bytes and cost more to turn into levels than to read again for the next block of rows.  Workgroups of
 // `splits` take blocks in turn.
-// The last 32 tokens of four prompts of up to 16352 keys, 32 heads on 8, 4 bits: 41 us, and 44 for the sum below (vector unit 36 % of clocks, matrix cores 29 %, LDS
+// The last 32 tokens of four prompts of up to 16352 keys, 32 heads on 8, 4 bits: 42 us, and 40 for the sum below (vector unit 36 % of clocks, matrix cores 29 %, LDS
 // 25 %): three products a score, and codes turned into levels twice.
 template <int D> struct kw_block { static constexpr int ROWS = D == 256 ? 64 : 128; };
 // rows r0 .. into LDS, those past the last as zeros
@@ -911,7 +911,7 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   w.few = T * (QH / KVH) <= (int64_t)KW_FEW * S;
   w.stride = (length + keys * 4 - 1) / (keys * 4) * (keys * 4);
   // runs of keys a workgroup: as many as leave forty workgroups a CU (48 sequences 509 us against 517 with one run; two sequences 25 with one against 31 with
-  // four); over packed keys, whose rows have to come to LDS first, four (the last 32 tokens of four prompts 105 us against 110, 128 tokens 342 against 353)
+  // four); over packed keys, whose rows have to come to LDS first, four (the last 32 tokens of four prompts 105 us then against 110, 128 tokens 342 against 353)
   w.runs = 4;
   while (w.runs > 1 && w.stride / (keys * w.runs) * S * KVH < (w.few ? 40 : 4) * ab_cus()) w.runs /= 2;
   w.few_parts = w.few ? (int)(w.stride / (keys * w.runs)) : 0;
