@@ -402,6 +402,13 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
     const akv_evict_cache& x = caches[i];
     AKV_REQUIRE(x.data && x.row_bytes > 0, "%s: cache %d: null pointer or rows of %lld bytes", name, i, (long long)x.row_bytes);
     if (x.row_bytes > 1 << 20) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: rows of more than 2^20 bytes", name);
+    // (rows in two caches would be moved twice at the same time)
+    for (int j = 0; j < i; ++j) {
+      const akv_evict_cache& y = caches[j];
+      const bool alike = x.s_blk == y.s_blk && x.s_pos == y.s_pos && x.s_head == y.s_head;
+      const int64_t apart = (int64_t)((intptr_t)x.data - (intptr_t)y.data);
+      AKV_REQUIRE(apart != 0 && !(alike && apart < y.row_bytes && -apart < x.row_bytes), "%s: caches %d and %d share rows", name, j, i);
+    }
     ev_cache& c = a.c[i];
     c.p = (uint8_t*)x.data; c.blk = x.s_blk; c.pos = x.s_pos; c.head = x.s_head;
     // units as wide as rows, their places and their ends allow

@@ -85,11 +85,11 @@ def evict_tokens(weights: torch.Tensor, block_tables: torch.Tensor, context_lens
     weights       [num_seqs, num_kv_heads, length] float32, as paged_key_weights adds them up (length at least that of the tables)
     block_tables  [num_seqs, blocks] int32 / int64;  context_lens [num_seqs]
     caches        up to 8 tensors [num_blocks, block_size, num_kv_heads, ...] of any type: keys, values, packed rows, norms; strides are
-                  honoured, rows must be contiguous.  Position kept[j] of a sequence and head goes to position j of each
+                  honoured, rows must be contiguous and none a part of two caches.  Position kept[j] of a sequence and head goes to position j of each
     keep          tokens that stay (of a shorter sequence all), among them the first num_sink and the last num_recent; equal weights: the
                   earlier token; a NaN counts as -infinity
     out_tables    [num_seqs, blocks of `keep` tokens or more]: blocks that the rows move to and that no sequence of the call reads, for
-                  sequences that share blocks.  None: in place, and no block may belong to two sequences
+                  sequences that share blocks.  None: in place, and no block may belong to two sequences or stand twice in a table
 
     Returns (kept [num_seqs, num_kv_heads, keep] int32: positions in ascending order, -1 behind the last; the sequences' lengths now, in
     the type of context_lens; weights of the tokens that stayed, at their new positions, zeros behind, in a new tensor).  Rows behind the

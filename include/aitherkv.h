@@ -588,7 +588,7 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  *   type of context_lens (another tensor).  Lengths are clamped to `length`.
  * akv_evict_move: rows of up to AKV_EVICT_CACHES caches [num_blocks][block_size][num_kv_heads][row_bytes] (byte strides): position kept[j] to position
  *   j, in the blocks of out_tables, which no sequence of the call may read, or in place (out_tables NULL; no two sequences may
- *   share a block then).  caches is a host pointer.
+ *   share a block then).  caches is a host pointer; no row may be part of two of them.
  * akv_evict: akv_evict_select, then akv_evict_move by what it chose.
  * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must not overlap in time.
  * ------------------------------------------------------------------------------- */

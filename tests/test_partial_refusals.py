@@ -303,7 +303,8 @@ INVALID, UNSUPPORTED, WORKSPACE = _lib.AKV_ERR_INVALID, _lib.AKV_ERR_UNSUPPORTED
     (library_evict, INVALID, dict(sinks=-1)), (library_evict, INVALID, dict(length=-1)), (library_evict, INVALID, dict(kvh=0)), (library_evict, UNSUPPORTED, dict(length=1 << 31)),
     (library_evict, UNSUPPORTED, dict(S=70000)), (library_evict, 0, dict(S=0)),
     (library_move, INVALID, dict(caches=[(None, 4096, 256, 128, 128)])), (library_move, INVALID, dict(caches=[(P, 4096, 256, 128, 0)])), (library_move, INVALID, dict(keep=0)),
-    (library_move, INVALID, dict(n=-1)), (library_move, INVALID, dict(kept=None)), (library_move, INVALID, dict(ot=P, ot_it=3)), (library_move, UNSUPPORTED, dict(n=9)),
+    (library_move, INVALID, dict(n=-1)), (library_move, INVALID, dict(caches=[(P, 4096, 256, 128, 128), (P, 4096, 256, 128, 128)])),
+    (library_move, INVALID, dict(caches=[(P, 4096, 256, 128, 64), (P + 256, 4096, 256, 128, 64), (P + 32, 4096, 256, 128, 96)])), (library_move, INVALID, dict(caches=[(P, 4096, 256, 128, 64), (P, 8192, 256, 128, 64)])), (library_move, INVALID, dict(kept=None)), (library_move, INVALID, dict(ot=P, ot_it=3)), (library_move, UNSUPPORTED, dict(n=9)),
     (library_move, UNSUPPORTED, dict(caches=[(P, 4096, 256, 128, 1 << 21)])), (library_move, UNSUPPORTED, dict(S=70000)), (library_move, 0, dict(S=0)), (library_move, 0, dict(caches=[])),
 ])
 def test_library_refuses(call, want, change):
