@@ -241,12 +241,14 @@ template <int D, int KIND> struct kw_keys {
 
 // ---- queries of packed rows: turned, scaled and as two terms.  32 rows a tile and 32 coordinates a wavefront: queries are 16-bit numbers as they are, an entry of the
 // rotation three of their type, so that products and sums are float32 like those of one number after the other.  A workgroup's part of the rotation
-// stays in registers for all of its tiles.  4096 rows of 128 take 7 us and 47000 18, where a row of the rotation after the other, for eight rows a
-// workgroup, took 9 and 43.
+// stays in registers for all of its tiles, queries go through LDS, the next tile's on their way.  4096 rows of 128 take 6.4 us and 47000 15, where a row of the
+// rotation after the other, for eight rows a workgroup, took 9 and 43; queries in the operand's order straight from memory 7 and 18.  213000 rows of 256 take
+// 117: one workgroup a CU, whose registers hold the rotation's part, multiplies and writes in turn.
 template <int D, int DT> __global__ __launch_bounds__(2 * D) void kw_turn_kernel(kw_args a) {
   typedef ab_math<DT> M;
   constexpr int KS = D / 16, LANES = D / 16;         // LANES: threads of a row, in the end
   __shared__ __align__(16) float x[32][D + 4];
+  __shared__ __align__(16) uint16_t in[32][D + 8];   // queries: rows arrive in the order in which they lie
   const uint32_t rows = (uint32_t)(a.t1 - a.t0) * (uint32_t)a.QH, QH = (uint32_t)a.QH;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
   // an entry times 2^12 in float16 (a rotation's are 1 at most), so that its third term is a normal number
@@ -266,19 +268,33 @@ template <int D, int DT> __global__ __launch_bounds__(2 * D) void kw_turn_kernel
         v -= M::high(two);
       }
     }
-  for (uint32_t r0 = 32 * blockIdx.x; r0 < rows; r0 += 32 * gridDim.x) {
-    const uint32_t r = min(r0 + col, rows - 1), token = r / QH;
-    const uint16_t* q = (const uint16_t*)a.q + (int64_t)(token + (uint32_t)a.t0) * a.qs_tok + (int64_t)(r - token * QH) * a.qs_head + 8 * h;
-    ab_u4 y[KS];
+  ab_u4 next[2];
+  auto request = [&](uint32_t r0) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) y[k] = *(const ab_u4*)(q + 16 * k);
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t p = tid + j * 2 * D, r = min(r0 + p / (D / 8), rows - 1), token = r / QH;
+      next[j] = *(const ab_u4*)((const uint16_t*)a.q + (int64_t)(token + (uint32_t)a.t0) * a.qs_tok + (int64_t)(r - token * QH) * a.qs_head + 8 * (p % (D / 8)));
+    }
+  };
+  request(32 * blockIdx.x);
+  for (uint32_t r0 = 32 * blockIdx.x; r0 < rows; r0 += 32 * gridDim.x) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t p = tid + j * 2 * D;
+      *(ab_u4*)&in[p / (D / 8)][8 * (p % (D / 8))] = next[j];
+    }
+    __syncthreads();
+    if (r0 + 32 * gridDim.x < rows) request(r0 + 32 * gridDim.x);
     ab_f16 s[3];
 #pragma unroll
-    for (int part = 0; part < 3; ++part) {
+    for (int part = 0; part < 3; ++part)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[part][i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s[part] = M::mfma32(y[k], pi[part][k], s[part]);
+    for (int k = 0; k < KS; ++k) {
+      const ab_u4 y = *(const ab_u4*)&in[col][16 * k + 8 * h];
+#pragma unroll
+      for (int part = 0; part < 3; ++part) s[part] = M::mfma32(y, pi[part][k], s[part]);
     }
     __syncthreads();                   // (the tile before has been read)
 #pragma unroll
