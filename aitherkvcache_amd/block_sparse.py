@@ -51,8 +51,8 @@ class BlockIndex:
 
         key_cache       [num_blocks, block_size, num_kv_heads, head_dim] float16 / bfloat16 (strides honoured)
         block_tables    [num_seqs, blocks] int32 / int64;  context_lens [num_seqs] tokens of a sequence, the newest included
-        query_start_loc [num_seqs + 1]: sequence i has query_start_loc[i + 1] - query_start_loc[i] new tokens; None: the means of all
-                        blocks of every sequence (the cache was filled or rearranged by other means)
+        query_start_loc [num_seqs + 1]: sequence i has query_start_loc[i + 1] - query_start_loc[i] new tokens (the first start may be any:
+                        a part of a batch); None: the means of all blocks of every sequence (the cache was filled or rearranged by other means)
 
         A last block that is not full has the mean of the keys in it; a mean that is not finite is kept as zeros.  Sums are 64 bits."""
         result = _lib.calls().index_update(key_cache, block_tables, context_lens, query_start_loc, self.codes, self.scales, self.num_blocks,
@@ -68,8 +68,8 @@ class BlockIndex:
         self._check()
         dev = _lib.require_gpu(key_cache, block_tables, context_lens, query_start_loc, self.codes, self.scales)
         num_seqs, bt, lens, starts = check_sequences(block_tables, context_lens, query_start_loc)
-        # a sequence has no more new tokens than its table has places
-        tokens = 0 if starts is None else min(num_seqs * bt.shape[1] * block_size, (1 << 30) - 1)
+        # (starts may lie behind the rows of sequences that are not of this call: as many tokens as a batch can have)
+        tokens = 0 if starts is None else (1 << 30) - 1
         with _lib.on_device(dev):
             _lib.check(_lib.lib().akv_block_index_update(
                 key_cache.data_ptr(), _lib.dtype_code(key_cache), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),

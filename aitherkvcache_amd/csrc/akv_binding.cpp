@@ -444,9 +444,7 @@ PyObject* index_update(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (some && (qs.dim() != 1 || qs.numel() < 1 || !qs.is_contiguous() || index_code(qs) < 0)) Py_RETURN_NONE;
   const int64_t seqs = some ? qs.numel() - 1 : cl.numel();
   if (seqs < 1 || !fits_int(seqs) || bt.size(0) < seqs || cl.numel() < seqs) Py_RETURN_NONE;
-  // (a sequence has no more new tokens than its table has places)
-  const int64_t most = (1 << 30) - 1, places = std::min(bt.size(1), most) * std::min(kc.size(1), most);
-  const int64_t tokens = !some ? 0 : places > most / seqs ? most : seqs * places;
+  const int64_t tokens = some ? (1 << 30) - 1 : 0;     // (starts may lie behind rows of other sequences: as many tokens as a batch can have)
   void* stream;
   if (!stream_of(ts.device(), stream)) return nullptr;
   return status(without_gil(g_lib.index_update, kc.const_data_ptr(), float_code(kc), kc.stride(0), kc.stride(1), kc.stride(2), bt.const_data_ptr(), index_code(bt), bt.stride(0),

@@ -569,7 +569,8 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  * akv_block_index_update: of every block that the sequences' new tokens came to (query_starts NULL: of every
  *   block of theirs), per kv head the mean of the keys it holds, in 8 bits: codes [num_blocks][num_kv_heads][d] int8, scales
  *   [num_blocks][num_kv_heads] float32, contiguous.  scale = max |mean| (1 / 127), code = rint(mean (1 / max |mean| 127)), every operation
- *   on the mean rounded to float32; zeros where the mean is not finite.
+ *   on the mean rounded to float32; zeros where the mean is not finite.  No row of a token is read: num_tokens is
+ *   what starts are clamped to, and has to be no less than the last of them.
  * akv_block_index_select: selected [num_tokens][num_kv_heads][num_selected] int32, table columns in ascending order, -1 behind the
  *   last: of the blocks up to the token's own the first num_sink_blocks, the last num_recent_blocks (at least 1) and the best others
  *   by (c_q . code) scale, c_q the sum of the group's queries in 8 bits like a mean; equal scores: the lower column.  Tokens
