@@ -314,7 +314,8 @@ template <int D, int DT> __global__ __launch_bounds__(2 * D) void kw_turn_kernel
     if constexpr (LANES > 4) t = fmaxf(t, akv_lane_xor<4>(t));
     if constexpr (LANES > 8) t = fmaxf(t, akv_lane_xor<8>(t));
     if (r0 + i < rows) {
-      const uint32_t exponent = akv_row_exponent(t), token = (r0 + i) / QH, head = r0 + i - token * QH, kvh = kw_div(a, head);
+      // (no exponent below 14: the scale of a row of zeros, or next to it, is a number, 2^126 at most)
+      const uint32_t exponent = max(akv_row_exponent(t), 14u), token = (r0 + i) / QH, head = r0 + i - token * QH, kvh = kw_div(a, head);
       const int64_t to = (int64_t)kvh * (a.t1 - a.t0) * a.G + (int64_t)token * a.G + (head - kvh * a.G);
       const float scale = akv_row_scale(exponent) * 8192.f;
       typedef _Float16 four __attribute__((ext_vector_type(4)));
@@ -330,7 +331,8 @@ template <int D, int DT> __global__ __launch_bounds__(2 * D) void kw_turn_kernel
         *(four*)(a.turned + to * (2 * D) + 4 * (part + LANES * j)) = hi;
         *(four*)(a.turned + to * (2 * D) + D + 4 * (part + LANES * j)) = lo;
       }
-      if (part == 0) a.turned_by[to] = akv_row_unscale(exponent) * (1.f / 8192.f) * a.scale2;
+      // (above zero, whatever the scale of the scores: what is masked is -infinity times it.  A score of such a row is below 2^-96 of the key's norm)
+      if (part == 0) a.turned_by[to] = fmaxf(akv_row_unscale(exponent) * (1.f / 8192.f) * a.scale2, 0x1p-126f);
     }
   }
 }
