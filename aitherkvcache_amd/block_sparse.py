@@ -86,7 +86,8 @@ class BlockIndex:
         block_tables, context_lens, query_start_loc as in paged_chunk_attention
         num_selected     blocks a list, among them the first num_sink_blocks of the context and the last num_recent_blocks up to the
                          token's own (at least 1: its own block is always read); the others are those of largest (c_q . codes) scale with
-                         c_q the sum of the group's queries in 8 bits; equal scores: the lower column
+                         c_q the sum of the group's queries in 8 bits, a float32 number (infinite past the largest); equal scores: the
+                         lower column
         out              where the result goes (that shape, int32, contiguous)
 
         Products are of whole numbers: the result does not hang on the order of a sum."""

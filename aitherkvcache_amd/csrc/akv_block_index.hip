@@ -270,7 +270,8 @@ __global__ __launch_bounds__(256) void bi_select_kernel(bi_rank_args a) {
 // Sixteen tokens of a sequence and a kv head by one workgroup, scores and all: nothing goes to memory but the lists.
 //
 // A lane holds the scores of one column of every sixteen and four of the tokens, in registers where tables have no more than W x HELD tiles;
-// HELD = 0: made anew for each of the passes.  The k-th largest score of a token is found by a histogram over equal parts of the range of its scores (a part's
+// HELD = 0: made anew for each of the passes.  A column that is not free to be chosen has a NaN in its place, since a score may be any other number: one past the
+// largest float32 number is infinite.  The k-th largest score of a token is found by a histogram over equal parts of the range of its scores (a part's
 // number does not fall as the score rises, so whatever is rounded on the way the parts are in order), then among the scores of the one part in
 // which the count passes k; where these are more than fit (scores that are alike), by halving the range of all scores bit by
 // bit.  Columns above it, and those that equal it, are marked in two bitmaps a token, from which the lists are written in order.
@@ -397,7 +398,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
       for (int e = 0; e < 4; ++e) {
         const bool free = cc >= a.sinks && cc < free_to[e];
         lo[e] = fminf(lo[e], free ? x[e] : INFINITY);
-        x[e] = free ? x[e] : -INFINITY;
+        x[e] = free ? x[e] : NAN;
       }
     } else {
 #pragma unroll
@@ -425,8 +426,8 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
     request(blk[0], 0, c[0]);
 #pragma unroll
     for (int i = 0; i < HELD; i += STAGED) {
-      held[i] = (ab_f4)(-INFINITY);
-      if (STAGED == 2) held[i + 1] = (ab_f4)(-INFINITY);
+      held[i] = (ab_f4)(NAN);
+      if (STAGED == 2) held[i + 1] = (ab_f4)(NAN);
       if (wave + W * i >= tiles) continue;
       const int next = i + STAGED < HELD ? i + STAGED : i;
       if (next > i) request(blk[next / BATCH], next % BATCH, c[next / STAGED & 1]);
@@ -440,6 +441,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
   enum { RANGE, PARTS, CANDIDATES, BITS, MARKS };
   float scale[4], shift[4];
   int part[4], bit = 31;
+  // (the median of a NaN and two numbers is the lesser one: what is not free has the lowest part, and so has an infinite score, whose token has a scale of 0 and one part)
   auto part_of = [&](float s, int e) { return (int)__builtin_amdgcn_fmed3f(fmaf(s, scale[e], shift[e]), 0.f, BI_PARTS - 1.f); };
   int row0 = 4 * hq, my_col = col;      // the lane's first token, its column of a tile
   // sixteen columns of token 4 hq + e: a lane of the token writes their marks
@@ -459,7 +461,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
       for (int e = 0; e < 4; ++e) {
         const int p = part_of(s[e], e);
         above[e] = __ballot(p > part[e]);
-        if (p == part[e] && s[e] != -INFINITY) {
+        if (p == part[e] && s[e] == s[e]) {
           const int at = atomicAdd(&rows[row0 + e].candidates, 1);
           if (at < BI_CANDIDATES) cand[(row0 + e) * BI_CANDIDATES + at] = make_float2(s[e], __int_as_float(16 * tile + my_col));
         }
@@ -472,7 +474,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
     } else if (pass == BITS) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (s[e] != -INFINITY && bi_order(s[e]) >= (rows[row0 + e].order | 1u << bit)) atomicAdd(hist + row0 + e, 1);
+        if (s[e] == s[e] && bi_order(s[e]) >= (rows[row0 + e].order | 1u << bit)) atomicAdd(hist + row0 + e, 1);
     } else if (pass == MARKS) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -507,7 +509,7 @@ template <int D, int DT, int W, int HELD> __global__ __launch_bounds__(64 * W, 4
           h = fmaxf(h, range[1][w][tid]);
         }
         const float f = BI_PARTS / (h - l);
-        const bool fine = f < INFINITY && fabsf(l * f) < INFINITY;      // (scores that are all alike, or nearly: one part; and none where h < l)
+        const bool fine = f < INFINITY && fabsf(l * f) < INFINITY;      // (scores that are all alike, or nearly, or infinite: one part; and none where h < l)
         rows[tid].scale = fine ? f : 0.f;
         rows[tid].shift = fine ? -l * f : 0.f;
         rows[tid].candidates = rows[tid].tied = 0;
