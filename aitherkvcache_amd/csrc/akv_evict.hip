@@ -380,9 +380,52 @@ __global__ __launch_bounds__(256) void ev_compact_kernel(ev_move_args a) {
   }
 }
 
-extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_head, const void* kept_lens, int kl_itype, int keep, const void* block_tables, int bt_itype, int64_t bt_stride,
-                              int64_t max_blocks_per_seq, const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq, const akv_evict_cache* caches, int num_caches,
-                              int num_seqs, int num_kv_heads, int block_size, int64_t num_blocks, void* stream) {
+// Whether a row of cache x and one of cache y share a byte (or two rows of one cache), over `counts` blocks, positions and heads.  A dimension of the same stride in both
+// moves the one against the other by multiples of it, the widest first; what has unlike strides is taken as one piece from end to end.
+static bool ev_meet(const __int128* stride, const int64_t* reach, int dims, __int128 lo, __int128 hi, bool other) {
+  if (dims == 0) return other && lo <= 0 && 0 <= hi;
+  __int128 rest = 0;                    // what the dimensions behind move
+  for (int i = 1; i < dims; ++i) rest += stride[i] * reach[i];
+  auto floor = [](__int128 a, __int128 b) { return a / b - (a % b < 0); };
+  __int128 from = -floor(rest - lo, *stride), to = floor(hi + rest, *stride);
+  if (from < -*reach) from = -*reach;
+  if (to > *reach) to = *reach;
+  if (to - from > 64) return true;      // (of strides that are no layout of rows side by side)
+  for (__int128 d = from; d <= to; ++d)
+    if (ev_meet(stride + 1, reach + 1, dims - 1, lo - d * *stride, hi - d * *stride, other || d != 0)) return true;
+  return false;
+}
+static bool ev_share(const akv_evict_cache& x, const akv_evict_cache& y, bool same, const int64_t* counts) {
+  const int64_t xs[3] = {x.s_blk, x.s_pos, x.s_head}, ys[3] = {y.s_blk, y.s_pos, y.s_head};
+  __int128 stride[3], x0 = (intptr_t)x.data, x1 = x0 + x.row_bytes, y0 = (intptr_t)y.data, y1 = y0 + y.row_bytes, ways = 0;
+  int64_t reach[3];
+  int dims = 0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t n = counts[i] - 1;
+    if (n == 0) continue;
+    if (xs[i] != ys[i]) {
+      (xs[i] < 0 ? x0 : x1) += (__int128)xs[i] * n;
+      (ys[i] < 0 ? y0 : y1) += (__int128)ys[i] * n;
+    } else if (xs[i] != 0) {
+      const __int128 s = xs[i] < 0 ? -(__int128)xs[i] : xs[i];
+      int at = dims++;
+      for (; at > 0 && stride[at - 1] < s; --at) stride[at] = stride[at - 1], reach[at] = reach[at - 1];
+      stride[at] = s;
+      reach[at] = n;
+      ways += s * n;
+    } else if (same) return true;
+  }
+  if (x0 - ways >= y1 || y0 - ways >= x1) return false;
+  return ev_meet(stride, reach, dims, y0 - x1 + 1, y1 - x0 - 1, !same);
+}
+
+// The launch of a move: `groups` workgroups (0: nothing to do)
+struct ev_plan { ev_move_args a; dim3 groups; bool in_place; };
+static int ev_prepare(ev_plan& plan, const int32_t* kept, int64_t ks_seq, int64_t ks_head, const void* kept_lens, int kl_itype, int keep, const void* block_tables, int bt_itype,
+                      int64_t bt_stride, int64_t max_blocks_per_seq, const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq, const akv_evict_cache* caches,
+                      int num_caches, int num_seqs, int num_kv_heads, int block_size, int64_t num_blocks) {
+  plan.groups = dim3(0);
+  plan.in_place = !out_tables;
   const char* name = "akv_evict_move";
   const int rc = ab_check(name, block_tables, bt_itype, kept_lens, kl_itype, nullptr, AKV_I32, num_seqs, 0, num_kv_heads, block_size, num_blocks, max_blocks_per_seq);
   if (rc) return rc;
@@ -392,7 +435,8 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
   if (num_seqs == 0 || num_caches == 0 || num_blocks == 0 || max_blocks_per_seq == 0) return AKV_OK;
   AKV_REQUIRE(kept, "%s: null pointer", name);
   if (num_seqs > 65535 || num_kv_heads > 65535) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 65535 sequences or kv heads", name);
-  ev_move_args a = {};
+  ev_move_args& a = plan.a;
+  a = ev_move_args{};
   a.b = ab_make(block_tables, bt_itype, bt_stride, kept_lens, kl_itype, nullptr, AKV_I32, num_seqs, 0, block_size, num_blocks, max_blocks_per_seq);
   a.to_tables = out_tables ? out_tables : block_tables; a.to_it = out_tables ? ot_itype : bt_itype;
   a.to_stride = out_tables ? ot_stride : bt_stride; a.to_blocks = out_tables ? out_blocks_per_seq : max_blocks_per_seq;
@@ -402,13 +446,10 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
     const akv_evict_cache& x = caches[i];
     AKV_REQUIRE(x.data && x.row_bytes > 0, "%s: cache %d: null pointer or rows of %lld bytes", name, i, (long long)x.row_bytes);
     if (x.row_bytes > 1 << 20) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: rows of more than 2^20 bytes", name);
-    // (rows in two caches would be moved twice at the same time)
-    for (int j = 0; j < i; ++j) {
-      const akv_evict_cache& y = caches[j];
-      const bool alike = x.s_blk == y.s_blk && x.s_pos == y.s_pos && x.s_head == y.s_head;
-      const int64_t apart = (int64_t)((intptr_t)x.data - (intptr_t)y.data);
-      AKV_REQUIRE(apart != 0 && !(alike && apart < y.row_bytes && -apart < x.row_bytes), "%s: caches %d and %d share rows", name, j, i);
-    }
+    // (a row in two places would be moved twice at the same time)
+    const int64_t counts[3] = {num_blocks, block_size, num_kv_heads};
+    AKV_REQUIRE(!ev_share(x, x, true, counts), "%s: rows of cache %d share memory", name, i);
+    for (int j = 0; j < i; ++j) AKV_REQUIRE(!ev_share(x, caches[j], false, counts), "%s: caches %d and %d share rows", name, j, i);
     ev_cache& c = a.c[i];
     c.p = (uint8_t*)x.data; c.blk = x.s_blk; c.pos = x.s_pos; c.head = x.s_head;
     // units as wide as rows, their places and their ends allow
@@ -423,27 +464,42 @@ extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_he
     pieces += c.pieces;
   }
   a.pieces = (int)pieces; a.heads = num_kv_heads;
-  const hipStream_t s = (hipStream_t)stream;
   if (out_tables) {
     const int64_t most = out_blocks_per_seq * block_size < keep ? out_blocks_per_seq * block_size : keep, all = most * pieces * num_kv_heads;
     if (all > 0xffffff00ll) return akv_fail(AKV_ERR_UNSUPPORTED, "%s: more than 2^32 pieces a sequence", name);
-    if (all == 0) return AKV_OK;
-    ev_copy_kernel<<<dim3((uint32_t)((all + 255) / 256), (uint32_t)num_seqs), 256, 0, s>>>(a);
-    AKV_LAUNCH_CHECK("ev_copy_kernel");
+    plan.groups = dim3((uint32_t)((all + 255) / 256), (uint32_t)num_seqs);
   } else {
-    ev_compact_kernel<<<dim3((uint32_t)slices, (uint32_t)num_kv_heads, (uint32_t)num_seqs), 256, 0, s>>>(a);
-    AKV_LAUNCH_CHECK("ev_compact_kernel");
+    plan.groups = dim3((uint32_t)slices, (uint32_t)num_kv_heads, (uint32_t)num_seqs);
   }
   return AKV_OK;
+}
+static int ev_move(const ev_plan& plan, void* stream) {
+  if (plan.groups.x == 0) return AKV_OK;
+  if (plan.in_place) ev_compact_kernel<<<plan.groups, 256, 0, (hipStream_t)stream>>>(plan.a);
+  else ev_copy_kernel<<<plan.groups, 256, 0, (hipStream_t)stream>>>(plan.a);
+  AKV_LAUNCH_CHECK(plan.in_place ? "ev_compact_kernel" : "ev_copy_kernel");
+  return AKV_OK;
+}
+
+extern "C" int akv_evict_move(const int32_t* kept, int64_t ks_seq, int64_t ks_head, const void* kept_lens, int kl_itype, int keep, const void* block_tables, int bt_itype, int64_t bt_stride,
+                              int64_t max_blocks_per_seq, const void* out_tables, int ot_itype, int64_t ot_stride, int64_t out_blocks_per_seq, const akv_evict_cache* caches, int num_caches,
+                              int num_seqs, int num_kv_heads, int block_size, int64_t num_blocks, void* stream) {
+  ev_plan plan;
+  const int rc = ev_prepare(plan, kept, ks_seq, ks_head, kept_lens, kl_itype, keep, block_tables, bt_itype, bt_stride, max_blocks_per_seq, out_tables, ot_itype, ot_stride,
+                            out_blocks_per_seq, caches, num_caches, num_seqs, num_kv_heads, block_size, num_blocks);
+  return rc ? rc : ev_move(plan, stream);
 }
 
 extern "C" int akv_evict(const float* weights, int64_t ws_seq, int64_t ws_head, int64_t length, const void* context_lens, int cl_itype, int num_seqs, int num_kv_heads, int keep,
                          int num_sink, int num_recent, int32_t* kept, int64_t ks_seq, int64_t ks_head, float* kept_weights, int64_t os_seq, int64_t os_head, void* kept_lens,
                          const void* block_tables, int bt_itype, int64_t bt_stride, int64_t max_blocks_per_seq, const void* out_tables, int ot_itype, int64_t ot_stride,
                          int64_t out_blocks_per_seq, const akv_evict_cache* caches, int num_caches, int block_size, int64_t num_blocks, void* stream) {
-  if (const int rc = akv_evict_select(weights, ws_seq, ws_head, length, context_lens, cl_itype, num_seqs, num_kv_heads, keep, num_sink, num_recent, kept, ks_seq, ks_head, kept_weights,
-                                      os_seq, os_head, kept_lens, stream))
-    return rc;
-  return akv_evict_move(kept, ks_seq, ks_head, kept_lens, cl_itype, keep, block_tables, bt_itype, bt_stride, max_blocks_per_seq, out_tables, ot_itype, ot_stride, out_blocks_per_seq, caches,
-                        num_caches, num_seqs, num_kv_heads, block_size, num_blocks, stream);
+  // (what is refused is refused before anything runs)
+  ev_plan plan;
+  int rc = ev_prepare(plan, kept, ks_seq, ks_head, kept_lens, cl_itype, keep, block_tables, bt_itype, bt_stride, max_blocks_per_seq, out_tables, ot_itype, ot_stride, out_blocks_per_seq,
+                      caches, num_caches, num_seqs, num_kv_heads, block_size, num_blocks);
+  if (rc == AKV_OK)
+    rc = akv_evict_select(weights, ws_seq, ws_head, length, context_lens, cl_itype, num_seqs, num_kv_heads, keep, num_sink, num_recent, kept, ks_seq, ks_head, kept_weights, os_seq, os_head,
+                          kept_lens, stream);
+  return rc ? rc : ev_move(plan, stream);
 }

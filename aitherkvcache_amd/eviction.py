@@ -85,7 +85,7 @@ def evict_tokens(weights: torch.Tensor, block_tables: torch.Tensor, context_lens
     weights       [num_seqs, num_kv_heads, length] float32, as paged_key_weights adds them up (length at least that of the tables)
     block_tables  [num_seqs, blocks] int32 / int64;  context_lens [num_seqs]
     caches        up to 8 tensors [num_blocks, block_size, num_kv_heads, ...] of any type: keys, values, packed rows, norms; strides are
-                  honoured, rows must be contiguous and none a part of two caches.  Position kept[j] of a sequence and head goes to position j of each
+                  honoured, rows must be contiguous and share no memory with others.  Position kept[j] of a sequence and head goes to position j of each
     keep          tokens that stay (of a shorter sequence all), among them the first num_sink and the last num_recent; equal weights: the
                   earlier token; a NaN counts as -infinity
     out_tables    [num_seqs, blocks of `keep` tokens or more]: blocks that the rows move to and that no sequence of the call reads, for
@@ -129,13 +129,14 @@ def evict_tokens(weights: torch.Tensor, block_tables: torch.Tensor, context_lens
     if length < left.shape[2]:
         left.zero_()
     L = _lib.lib()
+    chosen = (weights.data_ptr(), weights.stride(0), weights.stride(1), length, lens.data_ptr(), itype, num_seqs, kv_heads, keep, num_sink, num_recent,
+              kept.data_ptr(), kept.stride(0), kept.stride(1), left.data_ptr(), left.stride(0), left.stride(1), now.data_ptr())
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
-        _lib.check(L.akv_evict_select(weights.data_ptr(), weights.stride(0), weights.stride(1), length, lens.data_ptr(), itype, num_seqs, kv_heads, keep, num_sink,
-                                      num_recent, kept.data_ptr(), kept.stride(0), kept.stride(1), left.data_ptr(), left.stride(0), left.stride(1), now.data_ptr(), stream))
-        held = (_lib.EvictCache * len(caches))(*(_lib.EvictCache(t.data_ptr(), *strides, size) for t, (strides, size) in zip(caches, rows)))
-        if blocks and all(size for _, size in rows):
-            _lib.check(L.akv_evict_move(kept.data_ptr(), kept.stride(0), kept.stride(1), now.data_ptr(), itype, keep, bt.data_ptr(), bt_itype, bt.stride(0),
-                                        bt.shape[1], None if ot is None else ot.data_ptr(), ot_itype, 0 if ot is None else ot.stride(0),
-                                        0 if ot is None else ot.shape[1], held, len(caches), num_seqs, kv_heads, block_size, blocks, stream))
+        if not blocks or not all(size for _, size in rows):
+            _lib.check(L.akv_evict_select(*chosen, stream))
+        else:
+            held = (_lib.EvictCache * len(caches))(*(_lib.EvictCache(t.data_ptr(), *strides, size) for t, (strides, size) in zip(caches, rows)))
+            _lib.check(L.akv_evict(*chosen, bt.data_ptr(), bt_itype, bt.stride(0), bt.shape[1], None if ot is None else ot.data_ptr(), ot_itype,
+                                   0 if ot is None else ot.stride(0), 0 if ot is None else ot.shape[1], held, len(caches), block_size, blocks, stream))
     return kept, now, left

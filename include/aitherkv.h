@@ -589,8 +589,9 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  *   type of context_lens (another tensor).  Lengths are clamped to `length`.
  * akv_evict_move: rows of up to AKV_EVICT_CACHES caches [num_blocks][block_size][num_kv_heads][row_bytes] (byte strides): position kept[j] to position
  *   j, in the blocks of out_tables, which no sequence of the call may read, or in place (out_tables NULL; no two sequences may
- *   share a block then).  caches is a host pointer; no row may be part of two of them.
- * akv_evict: akv_evict_select, then akv_evict_move by what it chose.
+ *   share a block then).  caches is a host pointer; rows that share memory, of two caches or of one, are refused, and so are caches
+ *   whose rows lie between each other with unlike strides so that it cannot be told.
+ * akv_evict: akv_evict_select, then akv_evict_move by what it chose; a call that is refused runs neither.
  * Workspaces: device memory at a multiple of 256 bytes, contents of no meaning between calls; calls that share one must not overlap in time.
  * ------------------------------------------------------------------------------- */
 int akv_block_index_update(const void* key_cache, int dtype, int64_t ks_blk, int64_t ks_pos, int64_t ks_head,
