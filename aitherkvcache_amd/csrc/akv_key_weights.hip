@@ -35,6 +35,7 @@ struct kw_args {
   float* scores; int64_t stride;        // few rows: [token - t0][QH][stride]
   float2* few_part; int few_parts;      // [token - t0][QH][few_parts]
   int runs;
+  bool by_token;                        // few rows: workgroups are numbered by the slab's tokens, not by the sequences
   float scale2;
 };
 
@@ -782,13 +783,21 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_packed_s
 // their way while the ones before are multiplied.
 // One token of 16 sequences, 1024 to 41000 keys each, 8 heads of 128: 120 us, 4.3 TB/s of what is read; kw_few_sum 15.
 #define KW_FEW 32
+// The sequence of a workgroup, or -1.  Where a slab has half as many tokens as there are sequences, or fewer, workgroups are numbered by its tokens: the first one that a
+// sequence has in the slab stands for the sequence.
+__device__ __forceinline__ int kw_few_seq(const kw_args& a) {
+  if (!a.by_token) return blockIdx.z;
+  const int token = a.t0 + (int)blockIdx.z, seq = ab_last(a.b.S, token, [&](int i) { return (int64_t)ab_start(a.b, i); });
+  return seq >= 0 && token == max(ab_start(a.b, seq), a.t0) && token < ab_start(a.b, seq + 1) ? seq : -1;
+}
 template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kernel(kw_args a) {
   typedef kw_plan<D, KIND> P;
   __shared__ __align__(16) unsigned char rows[32 * P::ROW];
   __shared__ float2 ml[4][32];
   __shared__ __align__(16) float norms[P::PACKED ? P::N : 4];
   __shared__ kw_levels<P::PACKED ? KIND : 4> levels;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = kw_few_seq(a);
+  if (seq < 0) return;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t from64 = (int64_t)part * P::N * a.runs;
   if (from64 >= ctx) return;
@@ -871,7 +880,8 @@ template <int D, int KIND> __global__ __launch_bounds__(256, 2) void kw_few_kern
 #define KW_FEW_KEYS 1024
 __global__ __launch_bounds__(256) void kw_few_sum_kernel(kw_args a, int keys) {
   __shared__ float2 stat[KW_FEW];
-  const int kvh = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int kvh = blockIdx.y, seq = kw_few_seq(a), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (seq < 0) return;
   const int ctx = ab_ctx(a.b, seq);
   const int64_t key0 = (int64_t)blockIdx.x * KW_FEW_KEYS, key = key0 + 4 * tid;
   const kw_rows R = kw_rows_of(a, seq, ctx);
@@ -921,12 +931,17 @@ __global__ __launch_bounds__(256) void kw_few_sum_kernel(kw_args a, int keys) {
 // ---- launches
 #define KW_SCRATCH (256ll << 20)
 struct kw_scratch { int64_t tokens; size_t stat, part, turned, by, scores, few_part, sums, bytes; int parts, few_parts, runs, splits; int64_t stride; bool few; };
-// Scratch of a call, its tokens in slabs of what KW_SCRATCH holds (a multiple of 32, or all).  Scores are kept where the batch has no more than a
-// tile of rows a sequence and kv head on average: a key of 128 coordinates that is read again costs 256 bytes, the scores of 4 rows written and
-// read 32.  (One token of 16 sequences of up to 41000 keys 135 us against 229, four tokens 197 against 243.)
-static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, bool packed, int keys, int64_t length) {
+// Scratch of a call, its tokens in slabs of what KW_SCRATCH holds, or of one where it does not hold that (and the sums of workgroups that share a part besides, 2 MB at
+// most).  Scores are kept where the batch has no more than a tile of rows a sequence and kv head on average: a key of 128 coordinates that is read again
+// costs 256 bytes, the scores of 4 rows written and read 32.  (One token of 16 sequences of up to 41000 keys 135 us against 229, four tokens 197 against 243.)
+// Kept scores take four bytes for every query head and place of the tables, whatever the contexts are, and every slab reads and adds anew: with fewer than KW_FEW_LEAST
+// tokens a slab they are made twice.  Tables of 131072, us kept and made twice: 16 sequences of up to 40000 keys, 32 heads on 8, fifteen tokens a slab, 297 and 384 (4
+// bits 232 and 395); 64 of up to 8000 870 and 644 (608 and 904); 64 heads, seven tokens a slab, 1092 and 638 (742 and 908).  In tables of 2^18 four tokens of 32
+// sequences, seven a slab, 1379 and 490 (1188 and 576).
+#define KW_FEW_LEAST 8
+static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, bool packed, int keys, int64_t length, bool few) {
   kw_scratch w = {};
-  w.few = T * (QH / KVH) <= (int64_t)KW_FEW * S;
+  w.few = few;
   w.stride = (length + keys * 4 - 1) / (keys * 4) * (keys * 4);
   // runs of keys a workgroup: as many as leave forty workgroups a CU (48 sequences 509 us against 517 with one run; two sequences 25 with one against 31 with
   // four); over packed keys, whose rows have to come to LDS first, four (the last 32 tokens of four prompts 105 us then against 110, 128 tokens 342 against 353)
@@ -941,8 +956,10 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
   const int64_t step = packed && D < 256 ? 128 : 64;
   while (!w.few && w.splits < 8 && T * (QH / KVH) > step * w.splits * S && (int64_t)w.parts * S * KVH * w.splits < 2 * ab_cus()) w.splits *= 2;
   const int64_t per = (int64_t)QH * (8 + 8 * (int64_t)w.parts + (packed ? 4 * D + 4 : 0) + (w.few ? 4 * w.stride + 8 * w.few_parts : 0));
-  w.tokens = KW_SCRATCH / per / 32 * 32;
-  if (w.tokens < 32) w.tokens = 32;
+  w.tokens = KW_SCRATCH / per;
+  if (few && w.tokens < (T < KW_FEW_LEAST ? T : KW_FEW_LEAST)) return kw_layout(T, S, QH, KVH, D, packed, keys, length, false);
+  if (w.tokens > 32) w.tokens = w.tokens / 32 * 32;
+  if (w.tokens < 1) w.tokens = 1;
   if (w.tokens > T) w.tokens = T;
   const size_t rows = (size_t)(w.tokens * QH);
   w.stat = 0;
@@ -957,7 +974,7 @@ static inline kw_scratch kw_layout(int64_t T, int S, int QH, int KVH, int D, boo
 }
 static inline int kw_part(int D, bool packed) { return !packed && D <= 128 ? 256 : 128; }
 static inline size_t kw_bytes(int64_t T, int S, int QH, int KVH, int D, bool packed, int64_t length) {
-  return T <= 0 || S <= 0 || QH <= 0 || KVH <= 0 || length <= 0 || !ab_head_size(D) ? 0 : kw_layout(T, S, QH, KVH, D, packed, kw_part(D, packed), length).bytes;
+  return T <= 0 || S <= 0 || QH <= 0 || KVH <= 0 || length <= 0 || !ab_head_size(D) ? 0 : kw_layout(T, S, QH, KVH, D, packed, kw_part(D, packed), length, T * (QH / KVH) <= (int64_t)KW_FEW * S).bytes;
 }
 extern "C" size_t akv_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, false, length); }
 extern "C" size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int d, int64_t length) { return kw_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads, d, true, length); }
@@ -965,7 +982,7 @@ extern "C" size_t akv_packed_key_weights_workspace_bytes(int64_t num_tokens, int
 template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scratch, hipStream_t stream) {
   typedef kw_plan<D, KIND> P;
   static_assert(P::N == (!P::PACKED && D <= 128 ? 256 : 128), "kw_part");
-  const kw_scratch w = kw_layout(T, a.b.S, a.QH, a.KVH, D, P::PACKED, P::N, a.length);
+  const kw_scratch w = kw_layout(T, a.b.S, a.QH, a.KVH, D, P::PACKED, P::N, a.length, T * (a.QH / a.KVH) <= (int64_t)KW_FEW * a.b.S);
   char* const at = (char*)scratch;
   a.stat = (float2*)(at + w.stat);
   a.part = (float2*)(at + w.part);
@@ -1007,7 +1024,8 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
         AKV_LAUNCH_CHECK("kw_turn_kernel");
       }
       if (w.few) {
-        kw_few_kernel<D, KIND><<<dim3((uint32_t)w.few_parts, (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a);
+        a.by_token = w.tokens < T && 2 * w.tokens <= a.b.S;
+        kw_few_kernel<D, KIND><<<dim3((uint32_t)w.few_parts, (uint32_t)a.KVH, (uint32_t)(a.by_token ? a.t1 - a.t0 : a.b.S)), 256, 0, stream>>>(a);
         AKV_LAUNCH_CHECK("kw_few_kernel");
       } else {
         if constexpr (P::PACKED) kw_packed_stats_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
@@ -1020,7 +1038,8 @@ template <int D, int KIND> static int kw_launch(kw_args a, int64_t T, void* scra
       }
     }
     if (w.few) {
-      kw_few_sum_kernel<<<dim3((uint32_t)((a.length + KW_FEW_KEYS - 1) / KW_FEW_KEYS), (uint32_t)a.KVH, (uint32_t)a.b.S), 256, 0, stream>>>(a, P::N * w.runs);
+      a.by_token = a.by_token && a.add;          // (what is not added to is written for every sequence)
+      kw_few_sum_kernel<<<dim3((uint32_t)((a.length + KW_FEW_KEYS - 1) / KW_FEW_KEYS), (uint32_t)a.KVH, (uint32_t)(a.by_token ? a.t1 - a.t0 : a.b.S)), 256, 0, stream>>>(a, P::N * w.runs);
       AKV_LAUNCH_CHECK("kw_few_sum_kernel");
     } else {
       if constexpr (P::PACKED) kw_packed_sum_kernel<D, KIND><<<grid, 256, LDS, stream>>>(a);
