@@ -509,11 +509,21 @@ PyObject* sparse_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return result_of(rc, a[8], std::move(out));
 }
 
+// whether rows lie apart, as eviction.py's weights_for asks
+bool rows_apart(const at::Tensor& w) {
+  const bool first = w.stride(0) < w.stride(1) || (w.stride(0) == w.stride(1) && w.size(0) < w.size(1));
+  int64_t end = w.size(2);
+  for (const int64_t i : {first ? 0 : 1, first ? 1 : 0}) {
+    if (w.size(i) > 1 && w.stride(i) < end) return false;
+    end += w.stride(i) * (w.size(i) - 1);
+  }
+  return true;
+}
 // where weights go: `given`, or a new tensor
 bool weights_result(Tensors& ts, PyObject* given, int64_t seqs, int64_t heads, int64_t places, at::Tensor& w) {
   if (given == Py_None) return true;
   w = ts.take(given);
-  return ts.ok() && w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) >= seqs && w.size(1) == heads && w.size(2) >= places && w.stride(2) == 1 && w.stride(1) != 0 && w.stride(0) != 0;
+  return ts.ok() && w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) >= seqs && w.size(1) == heads && w.size(2) >= places && w.stride(2) == 1 && rows_apart(w);
 }
 
 // (query, key cache, block_tables, context_lens, query_start_loc, accumulated or None, scale or None)

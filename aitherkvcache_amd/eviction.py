@@ -19,6 +19,12 @@ def weights_for(accumulated: Optional[torch.Tensor], num_seqs: int, kv_heads: in
     if accumulated is None:
         return torch.empty(num_seqs, kv_heads, length, dtype=torch.float32, device=device)
     check_weights("accumulated", accumulated, num_seqs, kv_heads, length)
+    # (weights are added row by row, by workgroups of their own)
+    end = accumulated.shape[2]
+    for stride, count in sorted(zip(accumulated.stride()[:2], accumulated.shape[:2])):
+        if count > 1 and stride < end:
+            raise ValueError("accumulated has rows that share memory")
+        end += stride * (count - 1)
     return accumulated
 
 

@@ -62,3 +62,39 @@ def test_caches_over_each_other(dev, monkeypatch, view, take):
         with pytest.raises(ValueError, match="share"):
             akv.evict_tokens(w, b.tables, b.ctx, [cache, view(cache)], 60, 2, 8)
     assert torch.equal(cache, before)
+
+
+@pytest.mark.parametrize("take", [True, False])
+@pytest.mark.parametrize("strides,fine", [((64, 32, 1), True), ((32, 96, 1), True), ((200, 40, 1), True), ((64, 31, 1), False), ((33, 33, 1), False), ((0, 32, 1), False)])
+def test_accumulated_weights_apart_and_over_each_other(dev, monkeypatch, strides, fine, take):
+    b = Batch([(3, 20), (1, 30)], BLOCK, dev, seed=35, pad_cols=0)
+    q, k = torch.randn(4, 4, 64, device=dev).to(BF), torch.randn(b.blocks, BLOCK, HEADS, 64, device=dev).to(BF)
+    want = akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts)
+    acc = torch.zeros(1024, device=dev).as_strided((2, HEADS, 32), strides)
+    with binding(monkeypatch, take) as c:
+        if fine:
+            akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts, accumulated=acc)
+            assert torch.equal(acc, want) and c.taken == (1 if take else 0)
+        else:
+            with pytest.raises(ValueError, match="share memory"):
+                akv.paged_key_weights(q, k, b.tables, b.ctx, b.starts, accumulated=acc)
+            assert not acc.any()
+
+
+def test_chosen_and_moved_by_two_calls(dev):
+    """akv_evict_select, then akv_evict_move: what akv_evict does."""
+    from aitherkvcache_amd import _lib
+    b = Batch([(0, 200), (0, 90), (0, 17)], BLOCK, dev, seed=36)
+    w = torch.rand(3, HEADS, b.tables.shape[1] * BLOCK, device=dev)
+    cache, other = torch.randn(b.blocks, BLOCK, HEADS, 5, device=dev), torch.randn(b.blocks, BLOCK, HEADS, device=dev).half()
+    mine = [cache.clone(), other.clone()]
+    want = akv.evict_tokens(w, b.tables, b.ctx, [cache, other], 60, 2, 8)
+    kept, left, now = torch.empty(3, HEADS, 60, dtype=torch.int32, device=dev), torch.empty_like(w), torch.empty(3, dtype=torch.int32, device=dev)
+    L, stream = _lib.lib(), _lib.stream_ptr(dev)
+    held = (_lib.EvictCache * 2)(*(_lib.EvictCache(c.data_ptr(), *(s * c.element_size() for s in c.stride()[:3]), c[0, 0, 0].numel() * c.element_size()) for c in mine))
+    _lib.check(L.akv_evict_select(w.data_ptr(), w.stride(0), w.stride(1), w.shape[2], b.ctx.data_ptr(), 0, 3, HEADS, 60, 2, 8, kept.data_ptr(), kept.stride(0), kept.stride(1), left.data_ptr(),
+                                  left.stride(0), left.stride(1), now.data_ptr(), stream))
+    _lib.check(L.akv_evict_move(kept.data_ptr(), kept.stride(0), kept.stride(1), now.data_ptr(), 0, 60, b.tables.data_ptr(), 0, b.tables.stride(0), b.tables.shape[1], None, 0, 0, 0, held, 2, 3,
+                                HEADS, BLOCK, b.blocks, stream))
+    for x, y in zip([kept, now, left, *mine], [*want, cache, other]):
+        assert torch.equal(x, y)
