@@ -142,7 +142,7 @@ def paged_sparse_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
 
     A token sees the keys of its selected blocks up to its own position; one without a key gets zeros.  head_dim is 64, 128 or 256.
     Past a context, and in blocks that are not selected, the caches may hold anything; a value that is not finite reaches only tokens that
-    see it.  A block has at most 4096 tokens, less than 256 MB apart.  Scores and sums are float32; a key's weight is rounded to the query's type before it meets its value
+    see it.  A block has at most 4096 tokens, less than 256 MB apart, and a table at most some 800000 columns.  Scores and sums are float32; a key's weight is rounded to the query's type before it meets its value
     (in float16 also by 2^-30 of the row's largest), and so is the result."""
     result = _lib.calls().sparse_attention(query, key_cache, value_cache, block_tables, context_lens, query_start_loc, selected, scale, out)
     if result is not None:

@@ -345,6 +345,8 @@ __global__ __launch_bounds__(256) void ev_copy_kernel(ev_move_args a) {
 // In place.  A token never moves back, so what a tile of tokens writes lies before everything that later tiles read, and a workgroup that walks
 // the tiles in order needs only to have read a tile before it writes it.  Slices of the rows are independent of each other, and
 // so are heads and sequences: a workgroup each.
+// 16 sequences of 2048 tokens of 4 bits take 52 us and one of 4096 tokens of 8 heads of 128 62, where ev_copy_kernel takes 31 and 9.4: few workgroups (512 and 64), each of
+// which waits for a tile's positions, table entries and rows one after the other.
 #define EV_PIECES 8
 __global__ __launch_bounds__(256) void ev_compact_kernel(ev_move_args a) {
   const int head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;

@@ -43,12 +43,12 @@ def paged_key_weights(query: torch.Tensor, key_cache: torch.Tensor, block_tables
     summed over these tokens and over the query heads of a kv head: [num_seqs, num_kv_heads, length] float32, a key at its position.
 
     query, key_cache, block_tables, context_lens, query_start_loc, scale as in paged_chunk_attention
-    accumulated  [num_seqs, num_kv_heads, length] float32: the weights are added to what is there, and it is returned; its length is at
-                 least that of the tables, and positions past a context are left as they are.  Without it a new tensor as long as the tables,
+    accumulated  [num_seqs, num_kv_heads, length] float32, rows apart in memory: the weights are added to what is there, and it is returned; its
+                 length is at least that of the tables, and positions past a context are left as they are.  Without it a new tensor as long as the tables,
                  zero past a context
 
-    To weigh a prompt by its last tokens pass those tokens only.  head_dim is 64, 128 or 256.  Keys of a context must be finite; past it the
-    cache may hold anything.  Scores, weights and sums are float32."""
+    To weigh a prompt by its last tokens pass those tokens only.  head_dim is 64, 128 or 256, sequences and kv heads at most 65535.  Keys of a
+    context and queries must be finite; past it the cache may hold anything.  Scores, weights and sums are float32."""
     result = _lib.calls().key_weights(query, key_cache, block_tables, context_lens, query_start_loc, accumulated, scale)
     if result is not None:
         return result if type(result) is not int else _lib.check(result)

@@ -230,7 +230,7 @@ class TQPagedAttention:
         query, k_packed, k_norms, block_tables, context_lens, query_start_loc as in forward_chunk
         accumulated  as in paged_key_weights: float32, added to and returned; without it a new tensor as long as the tables
 
-        head_dim 64, 128 or 256, rows at multiples of 4 bytes; norms of the sequences' tokens must be finite.  Scores, weights and sums
+        head_dim 64, 128 or 256, rows at multiples of 4 bytes, at most 65535 sequences; queries and norms of the sequences' tokens must be finite.  Scores, weights and sums
         are float32, levels and rotated queries two float16 terms each (2^-22)."""
         from .chunk_attention import check_chunk, check_query
         from .eviction import weights_for

@@ -578,10 +578,12 @@ int akv_block_select(const float* scores, const void* block_tables, int bt_itype
  * akv_sparse_attn: attention of every new token over the keys at its position and before in the blocks its kv head has
  *   selected (a set: order and repetition do not matter; entries below 0 or past the token's own block are skipped); a row without a key
  *   is zero.  selected has strides ss_tok / ss_head, at most 4096 entries a list.  zero_tail as above.  A value
- *   that is not finite reaches only tokens that see it.  Blocks of at most 4096 tokens, less than 2^27 elements apart.
+ *   that is not finite reaches only tokens that see it.  Blocks of at most 4096 tokens, less than 2^27 elements apart; tables of
+ *   more than some 800000 columns may be refused (the bits of a token's columns and its list have to fit 150 KB).
  * akv_key_weights: weights [num_seqs][num_kv_heads][length] float32 (strides ws_seq / ws_head, length >= max_blocks_per_seq x block_size): the
  *   softmax weight of every key summed over the sequence's new tokens and the group's heads; accumulate: added to what is there (only
- *   keys of the context are touched), otherwise written, zeros elsewhere.
+ *   keys of the context are touched), otherwise written, zeros elsewhere.  At most
+ *   65535 sequences and kv heads.  Rows of weights lie apart in memory.  Scratch is 258 MB at most, but where one token needs more.
  * akv_packed_key_weights: the same over packed rows and norms as in akv_paged_attn.
  * akv_evict_select: per sequence and kv head min(ctx, keep) positions in ascending order (kept [num_seqs][num_kv_heads][keep] int32, -1 behind
  *   the last): the first num_sink, the last num_recent and the heaviest others; equal weights: the lower position; a NaN counts
