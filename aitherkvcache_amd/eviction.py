@@ -135,14 +135,15 @@ def evict_tokens(weights: torch.Tensor, block_tables: torch.Tensor, context_lens
     if length < left.shape[2]:
         left.zero_()
     L = _lib.lib()
+    moved = [_lib.EvictCache(t.data_ptr(), *strides, size) for t, (strides, size) in zip(caches, rows) if size]      # (a row of nothing stays where it is)
     chosen = (weights.data_ptr(), weights.stride(0), weights.stride(1), length, lens.data_ptr(), itype, num_seqs, kv_heads, keep, num_sink, num_recent,
               kept.data_ptr(), kept.stride(0), kept.stride(1), left.data_ptr(), left.stride(0), left.stride(1), now.data_ptr())
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
-        if not blocks or not all(size for _, size in rows):
+        if not blocks or not moved:
             _lib.check(L.akv_evict_select(*chosen, stream))
         else:
-            held = (_lib.EvictCache * len(caches))(*(_lib.EvictCache(t.data_ptr(), *strides, size) for t, (strides, size) in zip(caches, rows)))
+            held = (_lib.EvictCache * len(moved))(*moved)
             _lib.check(L.akv_evict(*chosen, bt.data_ptr(), bt_itype, bt.stride(0), bt.shape[1], None if ot is None else ot.data_ptr(), ot_itype,
-                                   0 if ot is None else ot.stride(0), 0 if ot is None else ot.shape[1], held, len(caches), block_size, blocks, stream))
+                                   0 if ot is None else ot.stride(0), 0 if ot is None else ot.shape[1], held, len(moved), block_size, blocks, stream))
     return kept, now, left

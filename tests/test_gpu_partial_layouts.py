@@ -98,3 +98,18 @@ def test_chosen_and_moved_by_two_calls(dev):
                                 HEADS, BLOCK, b.blocks, stream))
     for x, y in zip([kept, now, left, *mine], [*want, cache, other]):
         assert torch.equal(x, y)
+
+
+def test_rows_of_nothing(dev):
+    """A cache whose rows hold nothing does not keep the others from being moved."""
+    b = Batch([(0, 200), (0, 90)], BLOCK, dev, seed=37)
+    w = torch.rand(2, HEADS, b.tables.shape[1] * BLOCK, device=dev)
+    cache = torch.randn(b.blocks, BLOCK, HEADS, 4, device=dev)
+    alone = cache.clone()
+    empty = torch.zeros(b.blocks, BLOCK, HEADS, 0, device=dev)
+    got, want = akv.evict_tokens(w, b.tables, b.ctx, [empty, cache], 60, 2, 8), akv.evict_tokens(w, b.tables, b.ctx, [alone], 60, 2, 8)
+    for x, y in zip([*got, cache], [*want, alone]):
+        assert torch.equal(x, y)
+    got = akv.evict_tokens(w, b.tables, b.ctx, [empty], 60, 2, 8)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
